@@ -549,6 +549,55 @@ int usaf_hip_loss_scale_update(int32_t* scale_state, const int32_t* finite, cons
 int usaf_hip_overlay_scatter(void* base, int32_t dtype, int64_t numel, const int64_t* idx, const float* vals,
                              int64_t n, int32_t* bad_flag, void* stream);
 
+/*
+ * 8-bit block-scaled format: e4m3 codes, one scale 2^e (E8M0 byte e + 127) for each
+ * 1 x 128 block of an activation row and each 128 x 128 block of a weight, e the
+ * smallest integer with max|x| 2^-e <= 448, in [-120, 120].  Values that are not
+ * finite become the NaN code and take no part in the maximum.  Rows of codes are padded with zeros to
+ * kp = 128 ceil(cols / 128); a row's scale bytes take
+ * usaf_hip_fp8_scale_stride(cols) bytes (a multiple of 4, the bytes behind the last
+ * block unused).  No counterpart in the reference, whose experts are 4-bit or dense.
+ *
+ * usaf_hip_fp8_quantize_rows: x [rows, cols] fp16 / bf16, row stride ld -> q [rows, kp],
+ * s [rows, stride].  n_rows (device, may be NULL): rows from *n_rows on are left alone.
+ * usaf_hip_fp8_quantize_weight: w [E, R, C] of any float dtype -> q [E, R, kp],
+ * s [E, ceil(R/128), kp/128].  usaf_hip_fp8_dequantize: its values (rounded to out_dtype).
+ * usaf_hip_fp8_transpose: the same weight as [E, C, R]: exact, since blocks are square.
+ * q 16-byte aligned everywhere.
+ */
+int64_t usaf_hip_fp8_scale_stride(int64_t cols);
+int usaf_hip_fp8_quantize_rows(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld,
+                               const int32_t* n_rows, uint8_t* q, uint8_t* s, void* stream);
+int usaf_hip_fp8_quantize_weight(const void* w, int32_t dtype, int64_t E, int64_t R, int64_t C, uint8_t* q,
+                                 uint8_t* s, void* stream);
+int usaf_hip_fp8_dequantize(const uint8_t* q, const uint8_t* s, int64_t E, int64_t R, int64_t C, void* out,
+                            int32_t out_dtype, void* stream);
+int usaf_hip_fp8_transpose(const uint8_t* q, const uint8_t* s, int64_t E, int64_t R, int64_t C, uint8_t* qt,
+                           uint8_t* st, void* stream);
+
+/*
+ * out[m, n] = dtype( sum_k a[row(m), k] w_e[n, k] ), fp32 sums, for the slots m of
+ * expert e (offsets int32 [E + 1] on the device; NULL: E = 1 and all M slots).
+ * a, a_scale: usaf_hip_fp8_quantize_rows' layout; row(m) = a_rows[m], or m for NULL.
+ * w, w_scale: [E, N, K] in usaf_hip_fp8_quantize_weight's layout.  out [M, N] fp16 /
+ * bf16, 8-byte aligned.  Slots from offsets[E] on are left as they are.  E <= 255.
+ */
+int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, const int32_t* a_rows, int64_t M, const uint8_t* w,
+                      const uint8_t* w_scale, const int32_t* offsets, int64_t E, int64_t N, int64_t K, int32_t dtype,
+                      void* out, void* stream);
+
+/*
+ * Between the products of an 8-bit expert layer (the SwiGLU of qwen3moe_dml.py:58-62
+ * and its backward, with the layer's 16-bit roundings), for slots below *n_slots:
+ * usaf_hip_fp8_swiglu: gu [S, 2I] -> act [S, I], with its codes and scale bytes.
+ * usaf_hip_fp8_swiglu_bwd: gu, dact [S, I] -> dgu [S, 2I], with codes and scale bytes.
+ * I % 128 == 0; 16-byte aligned operands.
+ */
+int usaf_hip_fp8_swiglu(const void* gu, int64_t S, int64_t I, int32_t dtype, const int32_t* n_slots, void* act,
+                        uint8_t* q, uint8_t* s, void* stream);
+int usaf_hip_fp8_swiglu_bwd(const void* gu, const void* dact, int64_t S, int64_t I, int32_t dtype,
+                            const int32_t* n_slots, void* dgu, uint8_t* q, uint8_t* s, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,383 @@
+"""8-bit block format on the GPU against the 64-bit oracle: codec, product, grad-input, routed experts."""
+import pytest
+import torch
+
+import fp8_oracle as O
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+def _ids(d):
+    return str(d).replace("torch.", "")
+
+
+@pytest.fixture(scope="module")
+def F():
+    from usaf_amd import fp8
+    return fp8
+
+
+def _rand(*shape, dtype=torch.bfloat16, seed=0, scale=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype)
+
+
+def _within(got, ref, bound):
+    got = got.detach().double().cpu()
+    assert got.shape == ref.shape
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    fine = torch.isfinite(ref)
+    off = ((got - ref).abs() - bound)[fine]
+    assert off.numel() == 0 or float(off.max()) <= 0, f"{float(off.max())} past the bound"
+
+
+# ---- codec ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=_ids)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 127), (5, 128), (2, 129), (17, 640), (4, 2027)])
+def test_quantize_rows_is_the_oracles(F, rows, cols, dtype):
+    # magnitudes over the type's whole range, a row of zeros, a block border of every kind
+    x = _rand(rows, cols, dtype=torch.float32, seed=rows + cols)
+    x = (x * torch.exp2(torch.randint(-20, 12, (rows, cols), generator=torch.Generator().manual_seed(1)).float())).to(dtype)
+    x[rows // 2] = 0
+    r = F.quantize_rows(x.cuda())
+    ref, e = O.quantized_rows(x)
+    nb = -(-cols // 128)
+    assert r.q.shape == (rows, nb * 128)
+    s = r.s[:, :nb].cpu()
+    live = ref.new_tensor(0) != torch.nn.functional.pad(ref, (0, -cols % 128)).view(rows, nb, 128).abs().amax(-1)
+    assert torch.equal(s[live].int(), e[live].int())
+    got = r.q.cpu().view(torch.float8_e4m3fn).double().view(rows, nb, 128) * torch.exp2(s.double() - 127)[..., None]
+    got = got.view(rows, -1)
+    assert torch.equal(got[:, :cols], ref) and not got[:, cols:].any()
+
+
+@pytest.mark.parametrize("amax", [448.0, 449.0, 447.0, 896.0, 900.0, 1.75, 1.7578125, 2.0 ** -100, 3.0e38])
+def test_scale_at_the_borders(F, amax):
+    x = torch.zeros(1, 128, dtype=torch.bfloat16)
+    x[0, 3], x[0, 77] = amax, -amax / 3
+    r = F.quantize_rows(x.cuda())
+    ref, e = O.quantized_rows(x)
+    assert int(r.s[0, 0]) == int(e[0, 0])
+    assert torch.equal(O.values(r.q.cpu(), r.s[:, :1].cpu(), (1, 128)), ref)
+    assert float(x.abs().max()) * 2.0 ** (127 - int(r.s[0, 0])) <= 448
+
+
+def test_rows_behind_the_given_count_are_left(F):
+    x = _rand(6, 256).cuda()
+    n = torch.tensor([4], dtype=torch.int32, device="cuda")
+    rows = F.empty_rows(6, 256, x.device)
+    rows.q.fill_(17)
+    from usaf_amd import _native as N
+    N.call("usaf_hip_fp8_quantize_rows", x.data_ptr(), N.BF16, 6, 256, 256, n.data_ptr(), rows.q.data_ptr(),
+           rows.s.data_ptr(), N.stream_ptr(x.device))
+    assert bool((rows.q[4:] == 17).all()) and torch.equal(rows.q[:4], F.quantize_rows(x[:4]).q)
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (128, 128), (130, 257), (3, 96, 200), (2, 256, 128)])
+@pytest.mark.parametrize("dtype", [torch.float32] + DTYPES, ids=_ids)
+def test_weight_codec_and_transpose(F, shape, dtype):
+    w = _rand(*shape, dtype=dtype, seed=len(shape), scale=0.02)
+    t = F.Fp8Tensor.quantize(w.cuda())
+    ref, e = O.quantized_weight(w)
+    assert torch.equal(t.s.cpu().int(), e.int())
+    assert torch.equal(O.values(t.q.cpu(), t.s.cpu(), shape), ref)
+    assert torch.equal(t.dequantize().cpu().double(), ref)
+    assert torch.equal(t.dequantize(torch.bfloat16).cpu().double(), ref)
+    tt = t.transposed()
+    assert tt.shape == (*shape[:-2], shape[-1], shape[-2]) and tt is t.transposed()
+    assert torch.equal(O.values(tt.q.cpu(), tt.s.cpu(), tt.shape), ref.transpose(-1, -2))
+    assert not tt.q[..., shape[-2]:].any() and not t.q[..., shape[-1]:].any()
+
+
+def test_values_that_are_not_finite(F):
+    x = _rand(4, 300)
+    x[1, 5], x[2, 200], x[3, 299] = float("inf"), float("nan"), float("-inf")
+    w = F.Fp8Tensor.quantize(_rand(65, 300, seed=3, scale=0.1).cuda())
+    y = F.fp8_linear(x.cuda(), w)
+    assert bool(torch.isnan(y[1:]).all())
+    assert torch.equal(y[:1], F.fp8_linear(x[:1].cuda(), w)) and bool(torch.isfinite(y[0]).all())
+    v = _rand(130, 140)
+    v[129, 139] = float("inf")
+    t = F.Fp8Tensor.quantize(v.cuda())
+    assert int(torch.isnan(t.dequantize()).sum()) == 1
+
+
+# ---- product -------------------------------------------------------------------
+
+SIZES = [(1, 1, 1), (1, 64, 128), (2, 5, 127), (7, 130, 129), (31, 257, 640), (33, 128, 256), (64, 96, 384), (65, 1411, 300),
+         (129, 255, 1024), (300, 384, 512), (257, 640, 2027), (513, 300, 896)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=_ids)
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_linear(F, M, N, K, dtype):
+    x, w = _rand(M, K, dtype=dtype, seed=M), _rand(N, K, dtype=torch.float32, seed=N, scale=0.05)
+    t = F.Fp8Tensor.quantize(w.cuda())
+    xv = x.cuda().requires_grad_(True)
+    y = F.fp8_linear(xv, t)
+    assert y.dtype == dtype
+    a, wq = O.quantized_rows(x)[0], O.quantized_weight(w)[0]
+    ref = a @ wq.t()
+    _within(y, ref, O.product_bound(a, wq, ref, dtype))
+    dy = _rand(M, N, dtype=dtype, seed=K)
+    y.backward(dy.cuda())
+    b = O.quantized_rows(dy)[0]
+    ref = b @ wq
+    _within(xv.grad, ref, O.product_bound(b, wq.t(), ref, dtype))
+    assert torch.equal(F.fp8_linear(x.cuda(), t), y.detach())  # the same bits again, without a graph
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=_ids)
+def test_linear_sums_whole_numbers_exactly(F, dtype):
+    """Codes and scales that make every product and sum a whole number: no rounding anywhere, so a code at a wrong
+    place cannot hide in a tolerance."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.randint(-2, 3, (70, 512), generator=g).to(dtype)
+    w = torch.randint(-1, 2, (200, 512), generator=g).float()
+    ref = x.double() @ w.double().t()
+    assert float(ref.abs().max()) <= 256  # whole numbers that bf16 holds
+    assert torch.equal(F.fp8_linear(x.cuda(), F.Fp8Tensor.quantize(w.cuda())).double().cpu(), ref)
+
+
+def test_scales_of_every_block_reach_the_product(F):
+    """Blocks that differ by powers of two in every place of the exponent's range a sum in fp32 can hold."""
+    x = torch.zeros(40, 1024, dtype=torch.bfloat16)
+    w = torch.zeros(300, 1024)
+    for kb in range(8):
+        x[:, kb * 128 + 3 * kb] = 2.0 ** (kb - 4)
+        w[:, kb * 128 + 3 * kb] = 2.0 ** (-2 * kb)
+    x[::2] *= 4
+    w[128:256] *= 0.5
+    ref = x.double() @ w.double().t()
+    assert torch.equal(F.fp8_linear(x.cuda(), F.Fp8Tensor.quantize(w.cuda())).double().cpu(), ref.bfloat16().double())
+
+
+def test_gradient_against_differences(F):
+    """The product is linear in x wherever x and x + h are codes: differences are exact there."""
+    g = torch.Generator().manual_seed(7)
+    M, N, K = 3, 140, 130
+    x = torch.randint(-4, 5, (M, K), generator=g).to(torch.bfloat16)
+    w = torch.randint(-2, 3, (N, K), generator=g).float()
+    dy = torch.randint(-3, 4, (M, N), generator=g).to(torch.bfloat16)
+    t = F.Fp8Tensor.quantize(w.cuda())
+    xv = x.cuda().requires_grad_(True)
+    F.fp8_linear(xv, t).backward(dy.cuda())
+    for m, k in [(0, 0), (1, 64), (2, 127), (0, 128), (2, 129)]:
+        up, down = x.clone(), x.clone()
+        up[m, k] += 1
+        down[m, k] -= 1
+        d = (F.fp8_linear(up.cuda(), t).double() - F.fp8_linear(down.cuda(), t).double()) / 2
+        assert float((d.cpu() * dy.double()).sum()) == float(xv.grad[m, k])
+
+
+def test_linear_strides_shapes_and_streams(F):
+    t = F.Fp8Tensor.quantize(_rand(72, 136, seed=2, scale=0.1).cuda())
+    base = _rand(6, 5, 280, seed=4).cuda()
+    for x in (base[:, :, 3:139], base[:, ::2, :136], base[:, :, :272:2], base[0, :1, :136].expand(4, 136),
+              base[:3, 0, 1:137], base.permute(1, 0, 2)[:, :, 8:144], base[0, 0, :136]):
+        want = F.fp8_linear(x.contiguous(), t)
+        assert torch.equal(F.fp8_linear(x, t), want) and want.shape == (*x.shape[:-1], 72)
+    assert F.fp8_linear(base[:0, 0, :136], t).shape == (0, 72)
+    z = base[:0, 0, :136].clone().requires_grad_(True)
+    F.fp8_linear(z, t).sum().backward()
+    assert z.grad.shape == (0, 136)
+    want = F.fp8_linear(base[:, :, :136], t)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = F.fp8_linear(base[:, :, :136], t)
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_linear_in_a_graph(F):
+    t = F.Fp8Tensor.quantize(_rand(200, 384, seed=2, scale=0.1).cuda())
+    x = _rand(50, 384, seed=1).cuda()
+    with torch.no_grad():
+        F.fp8_linear(x, t)
+        graphs = []
+        for _ in range(2):  # two graphs of the same call: neither has the other's buffers
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                out = F.fp8_linear(x, t)
+            graphs.append((g, out))
+        for i in range(4):
+            x.copy_(_rand(50, 384, seed=10 + i))
+            for g, out in graphs:
+                g.replay()
+                torch.cuda.synchronize()
+                want = F.fp8_linear(x, t)
+                torch.cuda.synchronize()
+                assert torch.equal(out, want)
+
+
+# ---- routed experts --------------------------------------------------------------
+
+def _experts(F, E, H, I, seed=0):
+    from usaf_amd.moe import ExpertWeights
+    gu, dn = _rand(E, 2 * I, H, seed=seed, scale=0.05), _rand(E, H, I, seed=seed + 1, scale=0.05)
+    return ExpertWeights(F.Fp8Tensor.quantize(gu.cuda()), F.Fp8Tensor.quantize(dn.cuda()))
+
+
+def _routing(T, E, k, dtype, seed=0, only=None):
+    g = torch.Generator().manual_seed(seed)
+    p = torch.softmax(torch.randn(T, E, generator=g), -1)
+    if only is not None:
+        p[:, [e for e in range(E) if e not in only]] = 0
+    top = p.topk(k, -1)
+    return torch.zeros_like(p).scatter_(1, top.indices, top.values / top.values.sum(-1, keepdim=True)).to(dtype)
+
+
+# few and many slots for an expert, experts without one, an uneven routing, one token
+@pytest.mark.parametrize("dtype", DTYPES, ids=_ids)
+@pytest.mark.parametrize("T,E,k,H,I,only", [(1, 4, 2, 128, 128, None), (40, 5, 2, 256, 384, None), (70, 3, 1, 384, 128, [1]),
+                                            (300, 4, 2, 256, 256, None), (33, 200, 3, 128, 128, None),
+                                            (700, 2, 2, 128, 256, None)])
+def test_experts_step_by_step(F, T, E, k, H, I, only, dtype):
+    """Every step of the forward and backward against 64 bits of what that step was given: a code that falls
+    to the other side of a border in one step is the next one's input, not its error."""
+    from usaf_amd import moe as G
+    ew = _experts(F, E, H, I)
+    hs, w = _rand(T, H, dtype=dtype, seed=9), _routing(T, E, k, dtype, seed=3, only=only)
+    dout = _rand(T, H, dtype=dtype, seed=11)
+    hv, wv = hs.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    out = G.routed_experts(hv, wv, ew)
+    saved = out.grad_fn
+    _, gu, act, y = saved.saved_tensors
+    b = saved.b
+    offs, tok = b.offsets.tolist(), b.token_idx.long().cpu()
+    wgu, wd = ew.gate_up.dequantize().double().cpu(), ew.down.dequantize().double().cpu()
+    h = O.half_step(dtype)
+    a, q_act = O.quantized_rows(hs)[0], O.quantized_rows(act.cpu())[0]
+    g64, u64 = gu.double().cpu().split(I, 1)
+    sig = torch.sigmoid(g64)
+    silu = g64 * sig
+    # silu and its product are rounded one behind the other; silu_fast's exp2 and reciprocal are good to about 2^-22
+    _within(act, silu * u64, (silu * u64).abs() * (2.01 * h + 2.0 ** -20) + O.tiny(dtype) * (1 + u64.abs()))
+    for e in range(E):
+        s = slice(offs[e], offs[e + 1])
+        if offs[e] == offs[e + 1]:
+            continue
+        ref = a[tok[s]] @ wgu[e].t()
+        _within(gu[s], ref, O.product_bound(a[tok[s]], wgu[e], ref, dtype))
+        ref = q_act[s] @ wd[e].t()
+        _within(y[s], ref, O.product_bound(q_act[s], wd[e], ref, dtype))
+    y64, gu = y.double().cpu(), gu.clone()
+    ref, mags = torch.zeros(T, H, dtype=torch.float64), torch.zeros(T, H, dtype=torch.float64)
+    slot_e = torch.repeat_interleave(torch.arange(E), torch.tensor(offs[1:]) - torch.tensor(offs[:-1]))
+    pw = w[tok, slot_e].double()[:, None]
+    ref.index_add_(0, tok, pw * y64)
+    mags.index_add_(0, tok, (pw * y64).abs())
+    _within(out, ref, ref.abs() * h + O.tiny(dtype) + (E + 1) * 2.0 ** -24 * mags)
+    out.backward(dout.cuda())
+    # the backward's own steps again, on its inputs
+    dcur64 = pw * dout[tok].double()
+    dcur = dcur64.to(dtype).cuda()
+    dgu = torch.empty_like(gu)
+    F.experts_down_bwd(dcur, gu, ew, b, dgu)
+    qc = O.quantized_rows(dcur.cpu())[0]
+    dgu64 = dgu.double().cpu()
+    q_dgu = O.quantized_rows(dgu.cpu())[0]
+    dx, dmags = torch.zeros(T, H, dtype=torch.float64), torch.zeros(T, H, dtype=torch.float64)
+    for e in range(E):
+        s = slice(offs[e], offs[e + 1])
+        if offs[e] == offs[e + 1]:
+            continue
+        da = qc[s] @ wd[e]
+        db = O.product_bound(qc[s], wd[e].t(), da, dtype)  # how far the kernel's d(act) may be
+        dsig = sig[s] * (1 + g64[s] * (1 - sig[s]))
+        ref = torch.cat([da * u64[s] * dsig, da * silu[s]], 1)
+        grow = torch.cat([db * (u64[s] * dsig).abs(), db * silu[s].abs()], 1) * (1 + 4 * h)
+        # at most three roundings, and the hardware exp2 / reciprocal times the conditioning of 1 + g (1 - s)
+        cond = torch.cat([(da * u64[s] * sig[s]).abs() * (1 + g64[s].abs()), (da * silu[s]).abs()], 1)
+        tiny = O.tiny(dtype) * torch.cat([1 + dsig.abs() * 2, 1 + da.abs()], 1)
+        _within(dgu[s], ref, grow + ref.abs() * 3.1 * h + cond * 2.0 ** -19 + tiny)
+        r = (q_dgu[s] @ wgu[e])
+        rb = O.product_bound(q_dgu[s], wgu[e].t(), r, dtype)
+        dx.index_add_(0, tok[s], r)
+        dmags.index_add_(0, tok[s], rb + r.abs() * (E * 2.0 ** -24))
+    _within(hv.grad, dx, dmags + dx.abs() * h + O.tiny(dtype))
+    dw = torch.zeros(T, E, dtype=torch.float64)
+    dw[tok, slot_e] = (dout[tok].double() * y64).sum(1)
+    dm = torch.zeros(T, E, dtype=torch.float64)
+    dm[tok, slot_e] = (dout[tok].double() * y64).abs().sum(1)
+    _within(wv.grad, dw, dw.abs() * h + O.tiny(dtype) + H * 2.0 ** -24 * dm)
+    assert dgu64.shape == (offs[-1], 2 * I)
+
+
+def test_moe_block_on_8_bit_experts(F):
+    """The whole block, with and without a host read, forward and backward: the same bits."""
+    from usaf_amd import moe as G
+    T, E, H, I, k = 50, 16, 256, 128, 2
+    ew = _experts(F, E, H, I)
+    hs, router = _rand(T, H, seed=1).cuda(), (_rand(E, H, seed=2) / 16).cuda()
+    dout = _rand(T, H, seed=3).cuda()
+    res = []
+    for flag in (None, torch.zeros(1, dtype=torch.int32, device="cuda")):
+        x, r = hs.clone().requires_grad_(True), router.clone().requires_grad_(True)
+        out = G.moe_block(x, r, k, True, ew, overflow=flag)
+        out.backward(dout)
+        assert flag is None or int(flag) == 0
+        res.append((out.detach(), x.grad, r.grad))
+    for a, b in zip(*res):
+        assert torch.equal(a, b) and bool(torch.isfinite(a).all()) and float(a.abs().max()) > 0
+
+
+def test_experts_without_a_pair(F):
+    from usaf_amd import moe as G
+    ew = _experts(F, 4, 128, 128)
+    x = _rand(3, 128).cuda().requires_grad_(True)
+    w = torch.zeros(3, 4, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    out = G.routed_experts(x, w, ew)
+    out.backward(torch.ones_like(out))
+    assert not out.any() and not x.grad.any() and not w.grad.any()
+
+
+def test_sampled_gradient_on_8_bit_experts(F):
+    """A SparseGradStore gets the sampled weight gradient of 8-bit experts: positions of dgu^T hs and dcur^T act."""
+    from usaf_amd import moe as G
+    from usaf_amd.moe_loader import SparseGradStore
+    T, E, H, I, k = 60, 4, 256, 128, 2
+    ew = _experts(F, E, H, I)
+    idx = {"L.gate_up_proj": torch.arange(0, E * 2 * I * H, 97), "L.down_proj": torch.arange(5, E * H * I, 101)}
+    store = SparseGradStore(idx, {"L.gate_up_proj": (E, 2 * I, H), "L.down_proj": (E, H, I)}, device="cuda")
+    hs, w = _rand(T, H, seed=9), _routing(T, E, k, torch.bfloat16, seed=3)
+    dout = _rand(T, H, seed=11)
+    x = hs.cuda().requires_grad_(True)
+    out = G.routed_experts(x, w.cuda(), ew, capture=(store, "L"))
+    _, gu, act, _ = out.grad_fn.saved_tensors
+    b = out.grad_fn.b
+    gu, act = gu.clone(), act.double().cpu()
+    out.backward(dout.cuda())
+    offs, tok = b.offsets.tolist(), b.token_idx.long().cpu()
+    slot_e = torch.repeat_interleave(torch.arange(E), torch.tensor(offs[1:]) - torch.tensor(offs[:-1]))
+    dcur = (w[tok, slot_e].double()[:, None] * dout[tok].double()).bfloat16()
+    dgu = torch.empty_like(gu)
+    F.experts_down_bwd(dcur.cuda(), gu, ew, b, dgu)
+    for name, left, right in (("L.gate_up_proj", dgu.double().cpu(), hs.double()[tok]), ("L.down_proj", dcur.double(), act)):
+        ref = torch.stack([left[offs[e]:offs[e + 1]].t() @ right[offs[e]:offs[e + 1]] for e in range(E)]).reshape(-1)
+        mag = torch.stack([left[offs[e]:offs[e + 1]].t().abs() @ right[offs[e]:offs[e + 1]].abs() for e in range(E)]).reshape(-1)
+        ref, mag = ref[idx[name]], mag[idx[name]]
+        # fp32 sums over at most T slots, rounded to the activations' dtype once
+        _within(store.compact[name], ref, ref.abs() * O.half_step(torch.bfloat16) + 2 * T * 2.0 ** -23 * mag)
+
+
+def test_refusals_on_the_gpu(F):
+    from usaf_amd.moe import ExpertWeights, routed_experts
+    t = F.Fp8Tensor.quantize(_rand(64, 128).cuda())
+    x = _rand(2, 128).cuda()
+    with pytest.raises(ValueError, match="on one GPU"):
+        F.fp8_linear(x.cpu(), t)
+    with pytest.raises(ValueError, match="do not fit"):
+        F.fp8_linear(x[:, :127], t)
+    with pytest.raises(TypeError, match="fp16 or bf16"):
+        F.fp8_linear(x.float(), t)
+    ew = _experts(F, 2, 128, 128)
+    with pytest.raises(ValueError):
+        routed_experts(_rand(2, 256).cuda(), torch.ones(2, 2, dtype=torch.bfloat16, device="cuda"), ew)
+    with pytest.raises(NotImplementedError):
+        ew.set_overlay("gate_up", torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(1, device="cuda"),
+                       torch.bfloat16)
+    with pytest.raises(TypeError, match="both"):
+        ExpertWeights(ew.gate_up, torch.empty(2, 128, 128, dtype=torch.bfloat16, device="cuda"))

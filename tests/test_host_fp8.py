@@ -1,0 +1,91 @@
+"""Argument checks of the 8-bit block format: no GPU work."""
+import ctypes
+
+import pytest
+import torch
+
+from usaf_amd import _native as N
+from usaf_amd import fp8
+from usaf_amd.moe import ExpertWeights
+
+
+def _t(*shape):
+    *lead, r, c = shape
+    return fp8.Fp8Tensor(torch.zeros(*lead, r, -(-c // 128) * 128, dtype=torch.uint8),
+                         torch.zeros(*lead, -(-r // 128), -(-c // 128), dtype=torch.uint8), shape)
+
+
+def test_tensor_shapes():
+    assert _t(5, 130).numel() == 650 and _t(2, 5, 130).nbytes() == 2 * (5 * 256 + 2)
+    q, s = torch.zeros(5, 256, dtype=torch.uint8), torch.zeros(1, 2, dtype=torch.uint8)
+    for bad in [(5, 129, 1), (5,), (0, 130), (5, 300), (6, 130)]:
+        with pytest.raises(ValueError):
+            fp8.Fp8Tensor(q, s, bad)
+    with pytest.raises(TypeError):
+        fp8.Fp8Tensor(q.float(), s, (5, 130))
+    with pytest.raises(ValueError):
+        fp8.Fp8Tensor(q.t().contiguous().t(), s, (5, 130))
+    with pytest.raises(ValueError):
+        fp8.Fp8Tensor(torch.zeros(5 * 256 + 1, dtype=torch.uint8)[1:].view(5, 256), s, (5, 130))
+    assert fp8.Fp8Tensor(q.view(torch.float8_e4m3fn), s, (5, 130)).q.dtype == torch.uint8
+
+
+def test_linear_refuses():
+    w = _t(64, 128)
+    x = torch.zeros(3, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="GPU"):
+        fp8.fp8_linear(x, w)
+    with pytest.raises(ValueError, match="fit"):
+        fp8.fp8_linear(x[:, :100], w)
+    with pytest.raises(ValueError):
+        fp8.fp8_linear(x, _t(2, 64, 128))
+    with pytest.raises(TypeError):
+        fp8.fp8_linear(x.float(), w)
+    with pytest.raises(ValueError):
+        fp8.Fp8Tensor.quantize(torch.zeros(3))
+    with pytest.raises(ValueError):
+        fp8.Fp8Tensor.quantize(torch.zeros(0, 3))
+
+
+def test_expert_weights_refuse():
+    ExpertWeights(_t(3, 256, 256), _t(3, 256, 128))
+    with pytest.raises(NotImplementedError):
+        ExpertWeights(_t(3, 192, 256), _t(3, 256, 96))
+    with pytest.raises(NotImplementedError):
+        ExpertWeights(_t(256, 256, 128), _t(256, 128, 128))
+    with pytest.raises(TypeError):
+        ExpertWeights(torch.zeros(3, 256, 256), _t(3, 256, 128))
+    with pytest.raises(ValueError):
+        ExpertWeights(_t(3, 256, 256), _t(3, 128, 256))
+
+
+def test_entry_points_check_their_arguments():
+    lib, p, odd = N.load(), ctypes.c_void_p(4096), ctypes.c_void_p(4097)
+    inval, ok = N.USAF_ERR_INVALID, N.USAF_OK
+    rows = lib.usaf_hip_fp8_quantize_rows
+    assert rows(None, N.BF16, 0, 8, 8, None, None, None, None) == ok
+    assert rows(None, N.BF16, 1, 8, 8, None, p, p, None) == inval
+    assert rows(p, N.BF16, 1, 8, 7, None, p, p, None) == inval
+    assert rows(p, N.F32, 1, 8, 8, None, p, p, None) == inval
+    assert rows(p, N.BF16, 1, 8, 8, None, odd, p, None) == inval
+    assert rows(p, N.BF16, -1, 8, 8, None, p, p, None) == inval
+    assert rows(p, N.BF16, 1 << 62, 8, 8, None, p, p, None) == inval
+    gemm = lib.usaf_hip_fp8_gemm
+    assert gemm(None, None, None, 0, None, None, None, 1, 8, 8, N.BF16, None, None) == ok
+    assert gemm(p, p, None, 1, p, p, None, 2, 8, 8, N.BF16, p, None) == inval
+    assert gemm(p, p, None, 1, p, p, None, 1, 8, 0, N.BF16, p, None) == inval
+    assert gemm(p, p, None, 1, p, p, None, 1, 8, 8, N.F32, p, None) == inval
+    assert gemm(odd, p, None, 1, p, p, None, 1, 8, 8, N.BF16, p, None) == inval
+    assert gemm(p, odd, None, 1, p, p, None, 1, 8, 8, N.BF16, p, None) == inval
+    assert gemm(p, p, None, 1, p, p, None, 1, 8, 8, N.BF16, odd, None) == inval
+    assert gemm(p, p, None, 1 << 40, p, p, None, 1, 8, 8, N.BF16, p, None) == inval
+    assert gemm(p, p, None, 1, p, p, p, 256, 8, 8, N.BF16, p, None) == N.USAF_ERR_UNSUPPORTED
+    assert lib.usaf_hip_fp8_swiglu(p, 1, 100, N.BF16, p, p, p, p, None) == inval
+    assert lib.usaf_hip_fp8_swiglu(p, 1, 128, N.BF16, None, p, p, p, None) == inval
+    assert lib.usaf_hip_fp8_swiglu(None, 0, 128, N.BF16, None, None, None, None, None) == ok
+    assert lib.usaf_hip_fp8_swiglu_bwd(p, odd, 1, 128, N.BF16, p, p, p, p, None) == inval
+    assert lib.usaf_hip_fp8_quantize_weight(p, N.F32, 1, 1 << 25, 8, p, p, None) == inval
+    assert lib.usaf_hip_fp8_quantize_weight(p, 7, 1, 8, 8, p, p, None) == inval
+    assert lib.usaf_hip_fp8_dequantize(None, p, 1, 8, 8, p, N.F32, None) == inval
+    assert lib.usaf_hip_fp8_transpose(odd, p, 1, 8, 8, p, p, None) == inval
+    assert [lib.usaf_hip_fp8_scale_stride(c) for c in (0, 1, 512, 513, -1)] == [0, 4, 4, 8, -1]

@@ -1,0 +1,222 @@
+"""8-bit block-scaled weights: the codec, the product and its grad-input.
+
+Codes are e4m3; every block of 128 values (activations: 1 x 128 along the row,
+weights: 128 x 128) has one power-of-two scale, held as the E8M0 byte e + 127
+with e the smallest integer that brings the block's largest magnitude to 448 or
+below.  The matrix instruction applies such scales itself, so a product reads
+the codes as they are, where the 4-bit format's weights are first dequantized
+by vector instructions.  A weight takes 1.00006 bytes an element.
+
+``Fp8Tensor`` stands beside ``moe.Q4Tensor``: ``ExpertWeights(Fp8Tensor, Fp8Tensor)``
+makes ``routed_experts`` and ``moe_block`` run on 8-bit experts, forward and
+grad-input, and ``fp8_linear`` is the product for one weight.  Activations are
+quantized in the call.  The weights are frozen: gradients go to the activations,
+and to the positions a ``SparseGradStore`` samples.
+
+The reference has no 8-bit format; its frozen weights are 4-bit
+(usaf/quantization.py:21-132) or dense.
+"""
+from __future__ import annotations
+
+import contextlib
+from typing import NamedTuple, Optional, Sequence, Tuple
+
+import torch
+
+from . import _native as N
+
+BLOCK = 128
+_ACT = (torch.float16, torch.bfloat16)
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def on(device: torch.device):
+    """The device made current for a call's launches (nothing to do where it is)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+class Fp8Tensor:
+    """An HBM-resident weight [R, C] or [E, R, C] in the 8-bit block format.
+
+    q: e4m3 codes (uint8 or float8_e4m3fn), [.., R, 128 * ceil(C / 128)], zeros behind
+    column C; s: E8M0 bytes (uint8), [.., ceil(R / 128), ceil(C / 128)].  The tensors
+    are used as they are; a code behind column C that is not zero gives wrong products."""
+
+    def __init__(self, q: torch.Tensor, s: torch.Tensor, shape: Sequence[int]):
+        shape = torch.Size(int(d) for d in shape)
+        if len(shape) not in (2, 3) or any(d < 1 for d in shape):
+            raise ValueError(f"Fp8Tensor: shape must be [R, C] or [E, R, C] with no empty dimension, got {tuple(shape)}")
+        if q.dtype == torch.float8_e4m3fn:
+            q = q.view(torch.uint8)
+        if q.dtype != torch.uint8 or s.dtype != torch.uint8:
+            raise TypeError(f"Fp8Tensor: codes are e4m3 or uint8 and scales uint8 (E8M0), got {q.dtype}, {s.dtype}")
+        *lead, rows, cols = shape
+        if tuple(q.shape) != (*lead, rows, _blocks(cols) * BLOCK) or tuple(s.shape) != (*lead, _blocks(rows), _blocks(cols)):
+            raise ValueError(f"Fp8Tensor: codes {tuple(q.shape)} and scales {tuple(s.shape)} do not fit {tuple(shape)}: "
+                             f"need {(*lead, rows, _blocks(cols) * BLOCK)} and {(*lead, _blocks(rows), _blocks(cols))}")
+        if not q.is_contiguous() or not s.is_contiguous() or q.device != s.device or q.data_ptr() % 16:
+            raise ValueError("Fp8Tensor: codes and scales must be contiguous, on one device, the codes 16-byte aligned")
+        self.q, self.s, self.shape = q, s, shape
+        self._t: Optional["Fp8Tensor"] = None
+
+    @classmethod
+    def quantize(cls, tensor: torch.Tensor, device=None) -> "Fp8Tensor":
+        """From a float weight [R, C] or [E, R, C] (copied to the GPU first where it is on the CPU)."""
+        if tensor.dim() not in (2, 3) or tensor.numel() == 0:
+            raise ValueError(f"Fp8Tensor.quantize: need a non-empty [R, C] or [E, R, C] tensor, got {tuple(tensor.shape)}")
+        dev = torch.device(device) if device is not None else (tensor.device if tensor.is_cuda else N.default_device())
+        if dev.index is None:
+            dev = torch.device(dev.type, torch.cuda.current_device())
+        w = tensor.detach()
+        if w.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            w = w.float()
+        w = N.on_device(w, dev)
+        *lead, rows, cols = w.shape
+        q = torch.empty(*lead, rows, _blocks(cols) * BLOCK, dtype=torch.uint8, device=dev)
+        s = torch.empty(*lead, _blocks(rows), _blocks(cols), dtype=torch.uint8, device=dev)
+        with on(dev):
+            N.call("usaf_hip_fp8_quantize_weight", w.data_ptr(), N.dtype_code(w.dtype), lead[0] if lead else 1, rows, cols,
+                   q.data_ptr(), s.data_ptr(), N.stream_ptr(dev))
+        return cls(q, s, w.shape)
+
+    def dequantize(self, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values, exact in fp32 and bf16 and rounded in fp16, which lacks the smallest."""
+        out = torch.empty(self.shape, dtype=out_dtype, device=self.device)
+        with on(self.device):
+            N.call("usaf_hip_fp8_dequantize", self.q.data_ptr(), self.s.data_ptr(), *self._erc(), out.data_ptr(),
+                   N.dtype_code(out_dtype), N.stream_ptr(self.device))
+        return out
+
+    def transposed(self) -> "Fp8Tensor":
+        """The transpose (of each matrix), which the grad-input product reads: exact, built
+        at the first call and kept (as many bytes again)."""
+        if self._t is None:
+            *lead, rows, cols = self.shape
+            q = torch.empty(*lead, cols, _blocks(rows) * BLOCK, dtype=torch.uint8, device=self.device)
+            s = torch.empty(*lead, _blocks(cols), _blocks(rows), dtype=torch.uint8, device=self.device)
+            with on(self.device):
+                N.call("usaf_hip_fp8_transpose", self.q.data_ptr(), self.s.data_ptr(), *self._erc(), q.data_ptr(),
+                       s.data_ptr(), N.stream_ptr(self.device))
+            self._t = Fp8Tensor(q, s, (*lead, cols, rows))
+        return self._t
+
+    def _erc(self) -> Tuple[int, int, int]:
+        return (1, *self.shape) if len(self.shape) == 2 else tuple(self.shape)
+
+    @property
+    def device(self) -> torch.device:
+        return self.q.device
+
+    def numel(self) -> int:
+        return self.shape.numel()
+
+    def nbytes(self) -> int:
+        return self.q.numel() + self.s.numel()
+
+
+class Rows(NamedTuple):
+    """Quantized activation rows: codes [rows, 128 * ceil(cols / 128)], scale bytes, columns."""
+    q: torch.Tensor
+    s: torch.Tensor
+    cols: int
+
+
+def empty_rows(rows: int, cols: int, device: torch.device) -> Rows:
+    q = torch.empty(rows, _blocks(cols) * BLOCK, dtype=torch.uint8, device=device)
+    return Rows(q, torch.empty(rows, -(-_blocks(cols) // 4) * 4, dtype=torch.uint8, device=device), cols)
+
+
+def quantize_rows(x: torch.Tensor, n_rows: Optional[torch.Tensor] = None) -> Rows:
+    """Rows of fp16 / bf16 activations [M, K] in blocks of 128 along the row.  n_rows:
+    optional int32 device value; rows from there on are left undefined."""
+    if x.dim() != 2 or x.dtype not in _ACT:
+        raise TypeError(f"quantize_rows: need fp16 or bf16 rows [M, K], got {x.dtype} {tuple(x.shape)}")
+    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    rows = empty_rows(x.shape[0], x.shape[1], x.device)
+    N.call("usaf_hip_fp8_quantize_rows", x.data_ptr(), N.dtype_code(x.dtype), x.shape[0], x.shape[1],
+           max(x.stride(0), x.shape[1]), N.ptr(n_rows), rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(x.device))
+    return rows
+
+
+def product(x: Rows, w: Fp8Tensor, out: torch.Tensor, offsets: Optional[torch.Tensor] = None,
+            row_of: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[m] = x[row_of[m] or m] @ w_e^T for the slots m of expert e (offsets; one expert without)."""
+    E, n, k = w._erc()
+    if x.cols != k or out.shape[1] != n:
+        raise ValueError(f"fp8 product: rows of {x.cols} and output {tuple(out.shape)} do not fit the weight {tuple(w.shape)}")
+    N.call("usaf_hip_fp8_gemm", x.q.data_ptr(), x.s.data_ptr(), N.ptr(row_of), out.shape[0], w.q.data_ptr(),
+           w.s.data_ptr(), N.ptr(offsets), E, n, k, N.dtype_code(out.dtype), out.data_ptr(), N.stream_ptr(out.device))
+    return out
+
+
+class Fp8LinearFn(torch.autograd.Function):
+    """y = Q(x) W^T; dx = Q(dy) W."""
+
+    @staticmethod
+    def forward(ctx, x: torch.Tensor, w: Fp8Tensor):
+        ctx.w, ctx.dtype = w, x.dtype
+        return _linear(x, w)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy: torch.Tensor):
+        return _linear(dy.to(ctx.dtype), ctx.w.transposed()), None
+
+
+def _linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
+    n, k = w.shape
+    rows = x.reshape(-1, k) if x.numel() else x.new_empty(0, k)
+    out = torch.empty(rows.shape[0], n, dtype=x.dtype, device=x.device)
+    if rows.shape[0]:
+        with on(x.device):
+            product(quantize_rows(rows), w, out)
+    return out.view(*x.shape[:-1], n)
+
+
+def fp8_linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
+    """F.linear with an 8-bit block-scaled weight: x [..., K] fp16 / bf16, w [N, K] ->
+    [..., N] in x's dtype, summed in fp32.  Differentiable in x (the weight is frozen);
+    the first backward builds ``w.transposed()``.  A value of x that is not finite makes
+    its output row NaN."""
+    if len(w.shape) != 2:
+        raise ValueError(f"fp8_linear: need a weight [N, K], got {tuple(w.shape)}")
+    if x.dtype not in _ACT:
+        raise TypeError(f"fp8_linear: activations must be fp16 or bf16, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"fp8_linear: activations {tuple(x.shape)} do not fit the weight {tuple(w.shape)}")
+    if x.device != w.device or not x.is_cuda:
+        raise ValueError(f"fp8_linear: activations on {x.device}, weight on {w.device}: both on one GPU")
+    if torch.is_grad_enabled() and x.requires_grad:
+        return Fp8LinearFn.apply(x, w)
+    return _linear(x, w)
+
+
+# ---------------------------------------------------------------------------
+# the routed experts (moe.RoutedExpertsFn)
+# ---------------------------------------------------------------------------
+
+def experts_forward(hs: torch.Tensor, ew, b, gu: torch.Tensor, act: torch.Tensor, y: torch.Tensor) -> None:
+    """gu, act, y of the slots of bucketing b, for 8-bit experts ew.  Each step's output is
+    rounded to the activations' dtype, as on the layer's other kernels."""
+    S, I = act.shape
+    product(quantize_rows(hs), ew.gate_up, gu, b.offsets, b.token_idx)
+    rows = empty_rows(S, I, hs.device)
+    N.call("usaf_hip_fp8_swiglu", gu.data_ptr(), S, I, N.dtype_code(gu.dtype), b.offsets[-1:].data_ptr(), act.data_ptr(),
+           rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(hs.device))
+    product(rows, ew.down, y, b.offsets)
+
+
+def experts_down_bwd(dcur: torch.Tensor, gu: torch.Tensor, ew, b, dgu: torch.Tensor) -> Rows:
+    """dgu from the gradient dcur of the down projection's outputs; returns dgu quantized."""
+    S, I = gu.shape[0], gu.shape[1] // 2
+    n_slots = b.offsets[-1:]
+    dact = product(quantize_rows(dcur, n_slots), ew.down.transposed(), torch.empty(S, I, dtype=gu.dtype, device=gu.device),
+                   b.offsets)
+    rows = empty_rows(S, 2 * I, gu.device)
+    N.call("usaf_hip_fp8_swiglu_bwd", gu.data_ptr(), dact.data_ptr(), S, I, N.dtype_code(gu.dtype), n_slots.data_ptr(),
+           dgu.data_ptr(), rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(gu.device))
+    return rows

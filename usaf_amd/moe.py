@@ -16,6 +16,8 @@ from typing import Any, Optional, Tuple
 import torch
 
 from . import _native as N
+from . import fp8
+from .fp8 import Fp8Tensor
 
 
 # ---------------------------------------------------------------------------
@@ -258,8 +260,8 @@ class Q4Overlay:
 
 
 class ExpertWeights:
-    """The two fused expert tensors of one MoE layer, either 4-bit (Q4Tensor)
-    or dense 16-bit tensors of the activation dtype:
+    """The two fused expert tensors of one MoE layer, either 4-bit (Q4Tensor),
+    8-bit (fp8.Fp8Tensor) or dense 16-bit tensors of the activation dtype:
     gate_up [E, 2I, H] and down [E, H, I] (transformers' fused layout)."""
 
     def __init__(self, gate_up, down):
@@ -271,6 +273,15 @@ class ExpertWeights:
             raise ValueError(f"expert shapes do not form gate_up [E,2I,H] / down [E,H,I]: {tuple(gs)}, {tuple(ds)}")
         self.E, self.H, self.I = int(gs[0]), int(gs[2]), int(ds[2])
         self.overlays: dict = {}  # "gate_up" / "down" -> Q4Overlay
+        if isinstance(gate_up, Fp8Tensor) != isinstance(down, Fp8Tensor):
+            raise TypeError("8-bit experts: gate_up and down must both be Fp8Tensor")
+        if self.is_fp8 and (self.H % fp8.BLOCK or self.I % fp8.BLOCK or self.E > _T_MAX_E or gate_up.device != down.device):
+            raise NotImplementedError(f"8-bit experts need H and I in multiples of 128, at most {_T_MAX_E} experts and one "
+                                      f"device (E={self.E}, H={self.H}, I={self.I})")
+
+    @property
+    def is_fp8(self) -> bool:
+        return isinstance(self.gate_up, Fp8Tensor)
 
     @property
     def is_q4(self) -> bool:
@@ -500,6 +511,8 @@ class RoutedExpertsFn(torch.autograd.Function):
             raise ValueError(f"shape mismatch: hs {tuple(hs.shape)}, weights {tuple(weights.shape)}, "
                              f"experts E={E} H={ew.H} I={I}")
         dev = hs.device
+        if ew.is_fp8 and ew.gate_up.device != dev:
+            raise ValueError(f"activations on {dev}, 8-bit experts on {ew.gate_up.device}")
         st = N.stream_ptr(dev)
         code = N.dtype_code(dt)
         b = bucket_by_expert(weights) if slots is None else bucket_by_expert(weights, *slots)
@@ -508,14 +521,16 @@ class RoutedExpertsFn(torch.autograd.Function):
         act = torch.empty(S, I, dtype=dt, device=dev)
         y = torch.empty(S, H, dtype=dt, device=dev)
         act_blk = None
-        if S > 0 and _sampled_blocked(capture, b):
+        if S > 0 and not ew.is_fp8 and _sampled_blocked(capture, b):
             # the down projection's sampled gradient reads act blocked slot-major:
             # written by the gate_up epilogue, with act
             if b.blk_table is None:
                 b.blk_table = blocked_layout(b.offsets, S)
             n_blk = max(1, int(N.load().usaf_hip_blocked_elems(S, E, I)))
             act_blk = BlockedSlots(torch.empty(n_blk, dtype=dt, device=dev), I, b.offsets, b.blk_table)
-        if S > 0:
+        if S > 0 and ew.is_fp8:
+            fp8.experts_forward(hs, ew, b, gu, act, y)
+        elif S > 0:
             q, sz, w16 = ew._ptrs("gate_up", dt)
             timed_call("usaf_hip_moe_gate_up_fwd", hs.data_ptr(), T, H, b.token_idx.data_ptr(), b.offsets.data_ptr(),
                        S, E, I, q, sz, w16, code, gu.data_ptr(), act.data_ptr(),
@@ -572,7 +587,9 @@ class RoutedExpertsFn(torch.autograd.Function):
                    b.slot_w.data_ptr(), b.offsets.data_ptr(), S, E, H, code, dcur.data_ptr(), dweights.data_ptr(), st)
         dgu = torch.empty(S, 2 * I, dtype=dt, device=dev)
         tq = ew._ptrs_t("down")
-        if tq is not None:
+        if ew.is_fp8:
+            dgu_rows = fp8.experts_down_bwd(dcur, gu, ew, b, dgu)
+        elif tq is not None:
             timed_call("usaf_hip_moe_down_bwd_t", dcur.data_ptr(), H, gu.data_ptr(), b.offsets.data_ptr(), S, E, I,
                        *tq, code, dgu.data_ptr(), *ew._ovl("down_bwd", dt), st)
         else:
@@ -587,7 +604,9 @@ class RoutedExpertsFn(torch.autograd.Function):
             d_wdn = _dense_weight_grad(dcur, act, None, b, ctx.wdt[1])
         dx_slots = torch.empty(S, H, dtype=dt, device=dev)
         tq = ew._ptrs_t("gate_up")
-        if tq is not None:
+        if ew.is_fp8:
+            fp8.product(dgu_rows, ew.gate_up.transposed(), dx_slots, b.offsets)
+        elif tq is not None:
             timed_call("usaf_hip_moe_gate_up_bwd_t", dgu.data_ptr(), I, b.offsets.data_ptr(), S, E, H, *tq,
                        code, dx_slots.data_ptr(), *ew._ovl("gate_up_bwd", dt), st)
         else:
