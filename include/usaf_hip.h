@@ -598,6 +598,26 @@ int usaf_hip_fp8_swiglu(const void* gu, int64_t S, int64_t I, int32_t dtype, con
 int usaf_hip_fp8_swiglu_bwd(const void* gu, const void* dact, int64_t S, int64_t I, int32_t dtype,
                             const int32_t* n_slots, void* dgu, uint8_t* q, uint8_t* s, void* stream);
 
+/*
+ * A whole MoE layer for T <= 32 tokens (qwen3moe_dml.py:24-86 without the
+ * intermediate 16-bit roundings of logits, gate, up and the experts' outputs):
+ *   l = x router^T, the top_k largest l (ties: the lowest expert), w = softmax(l) of
+ *   those, divided by their sum if norm_topk_prob; a_e = dtype(silu(g) u), (g, u) =
+ *   gate_up_e x; out = dtype(sum_e w_e down_e a_e).
+ * x [T, H], router [E, H], out [T, H] of dtype (fp16 / bf16).  eight_bit == 0: 4-bit
+ * codes with group size 128 along whole rows and scales as usaf_hip_pack_scale_zero
+ * writes them; a weight is the real number code * scale + zero.  eight_bit != 0: codes
+ * and scale bytes as usaf_hip_fp8_quantize_weight writes them.
+ * ws: usaf_hip_moe_few_ws_bytes bytes, 16-byte aligned, nothing in them matters before the
+ * call; calls that may overlap need workspaces of their own.  E <= 256, top_k <= 16, H
+ * and I multiples of 128, H <= 16384, I <= 65536.  Three launches; no host read.
+ */
+int64_t usaf_hip_moe_few_ws_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I);
+int usaf_hip_moe_few(const void* x, int64_t T, int64_t H, const void* router, int64_t E, int64_t top_k,
+                     int32_t norm_topk_prob, int32_t dtype, int64_t I, int32_t eight_bit, const uint8_t* gate_up,
+                     const void* gate_up_scale, const uint8_t* down, const void* down_scale, void* out, void* ws,
+                     int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

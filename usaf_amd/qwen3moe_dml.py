@@ -19,11 +19,17 @@ at the active positions for ``usaf_amd.moe_loader.SparseGradStore``, as dense
 per-expert tensors (``store.add(name, ei, g)`` or a dict of fp16 buffers) for
 other stores.  The expert weights themselves receive no ``.grad``, as in the
 reference (it detaches every per-expert slice).
+
+Decoding: with ``block._usaf_few_tokens = n`` (up to 32) a block's passes of at most
+n tokens that want no gradient run as ``few.few_token_block``, router and experts in
+three launches, where the experts are 4-bit or 8-bit and carry no trained values.
+Its numerics (``few.py``) differ from this path's in what is rounded to 16 bits, so it is off by default.
 """
 from __future__ import annotations
 
 import torch
 
+from .few import few_token_block, few_token_ok
 from .moe import ExpertWeights, RouteTopKFn, routed_experts
 
 
@@ -72,12 +78,31 @@ def dml_qwen3_experts_forward(self, hidden_states: torch.Tensor, weights: torch.
     return routed_experts(hidden_states, weights, _expert_weights(self), capture)
 
 
+def _few_weights(block, hs: torch.Tensor):
+    """The experts of a pass that few_token_block takes for this block, or None."""
+    limit = getattr(block, "_usaf_few_tokens", 0)
+    if not 0 < hs.shape[0] <= limit:
+        return None
+    experts, router = block.experts, block.gate
+    if torch.is_grad_enabled() and (hs.requires_grad or router.weight.requires_grad
+                                    or getattr(experts, "_grad_capture", None) is not None):
+        return None
+    if not getattr(experts, "_usaf_q4", None) or router.weight.dtype != hs.dtype:
+        return None
+    ew = _expert_weights(experts)
+    return ew if few_token_ok(hs.shape[0], int(router.top_k), ew) else None
+
+
 def dml_qwen3_moe_block_forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
     """qwen3moe_dml.py:67-86: router linear, fp32 softmax, >=-threshold top-k
     mask, optional renormalisation, routed experts."""
     batch_size, sequence_length, hidden_dim = hidden_states.shape
     hs = hidden_states.view(-1, hidden_dim)
     router = self.gate
+    ew = _few_weights(self, hs)
+    if ew is not None:
+        out = few_token_block(hs, router.weight, int(router.top_k), bool(getattr(router, "norm_topk_prob", False)), ew)
+        return out.view(batch_size, sequence_length, hidden_dim)
     router_logits = torch.nn.functional.linear(hs, router.weight)
     weights = RouteTopKFn.apply(router_logits, int(router.top_k), bool(getattr(router, "norm_topk_prob", False)),
                                 hs.dtype)
