@@ -3,31 +3,31 @@
 //   l = x Wr^T, the k largest l (ties: the lowest expert), w = softmax(l) there (renormalised or not)
 //   a_e = dt(silu(g) u),  (g, u) = Wgu_e x;   out = dt(sum_e w_e Wd_e a_e)
 //
-// Three launches, nothing read back to the host, no slot lists: an expert takes the
-// tokens in place.  At most 32 tokens, so one 32-row MFMA operand holds them all
-// whatever their experts; a lane whose token the expert does not serve loads nothing,
-// and its rows of the result are not used.
+// Four launches, nothing read back to the host, no slot lists:
 //
-//   few_route    a block a token: logits, selection by rank, weights
-//   few_gate_up  a block an (expert in use, 32 columns of a): four waves split the contraction
-//   few_down     a block (32 columns of out, a part of the experts in use): its waves take
-//                (expert, part of the contraction) items and keep a weighted sum; the last
+//   few_logits   a wave an expert of the router and up to four tokens
+//   few_route    a block a token: selection by rank, weights, a bit of the token in its experts' masks
+//   few_gate_up  a block an (expert in use, 32 columns of a): its waves split the contraction
+//   few_down     a block (64 columns of out, a part of the experts in use): its waves take
+//                (expert, part of the contraction) items and add them up by token; the last
 //                block of a column tile adds the parts in order
 //
-// Weights are the MFMA's second operand, a lane's accumulators 16 tokens of one weight
-// row: the row's scale and zero are one register each.  A group of 128 is multiplied as
-// codes, D = sum_k x_k (c_k + offset) with exact small whole numbers as operands, and
+// An expert's tokens are the rows of a 16-row MFMA operand (more than 16: a second
+// round), weights its columns: a lane has one weight row and four tokens, so a row's scale
+// and zero are one register each.  A group of 128 is multiplied as codes, D = sum_k x_k
+// (c_k + offset) with exact small whole numbers as operands, and
 //   y += s D + (z - offset s) sum_k x_k           (4-bit; the sum by an MFMA against ones)
 //   y += 2^e D                                    (8-bit)
-// which takes 7 vector instructions for 8 codes and 64 for a group of a 32 x 32 tile,
-// where dequantizing each weight takes 32 for 8 codes.  The weight is the real number
-// s q + z: nothing rounds it.
+// which takes 7 vector instructions for 8 codes and 8 for a group of 16 rows, where
+// dequantizing each weight takes 32 for 8 codes.  The weight is the real number s q + z: nothing
+// rounds it.
 #include "fp8.h"
 
 namespace usaf {
 namespace {
 
 constexpr int FT = 32;        // tokens at most
+constexpr int FR = 16;        // tokens of one operand
 constexpr int F_MAX_E = 256;  // experts
 constexpr int F_MAX_K = 16;   // experts of a token
 enum { FMT_Q4 = 0, FMT_FP8 = 1 };
@@ -43,12 +43,13 @@ struct FewArgs {
   const void* dn_s;
   uint16_t* out;            // [T, H]
   // workspace
-  int32_t* sel;             // [T, k] experts
-  float* wt;                // [T, k] weights
+  double* logits;           // [T, E]
+  uint32_t* mask;           // [F_MAX_E] tokens of each expert
+  float* wt;                // [E, FT] their weights
   uint16_t* xp;             // [T, H] x in the fragments' order (4-bit)
   uint16_t* act;            // [experts in use, T, I] in the fragments' order
   float* part;              // [P, T, H] partial sums
-  int32_t* done;            // [H / 32] parts of a column tile that have arrived
+  int32_t* done;            // [H / 64] parts of a column tile that have arrived
   int P, KS;                // few_down: parts of the experts, of the contraction
 };
 
@@ -75,60 +76,68 @@ __device__ __forceinline__ int64_t order_key(double v) {
   return b < 0 ? -(b & INT64_MAX) : b;  // -0 with 0
 }
 
-// Logits in fp32 products of 8, added in 64 bits: which expert is the k-th hangs on
-// differences near fp32's own rounding.  1024 threads read the router's weight once
-// for a token; a wave has its experts' rows four at a time in flight.
-template <int DT, int FMT>
+// logits[t, e], products of 8 in fp32 and their sums in 64 bits: which expert is the
+// k-th hangs on differences near fp32's own rounding.  Wave: one expert, TB tokens.
+// The router's weight (0.5 MB for 128 experts of 2,048) is read by as many CUs as
+// there are fours of experts: by one block for each token it took 13 us.
+template <int DT, int FMT, int TB>
+__global__ __launch_bounds__(256) void few_logits_kernel(const FewArgs g) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n_eb = (g.E + 3) / 4, tb = blockIdx.x / n_eb, e = (blockIdx.x - tb * n_eb) * 4 + wave, t0 = tb * TB;
+  // what the later launches start from
+  const int id = blockIdx.x * 256 + tid, threads = gridDim.x * 256;
+  for (int i = id; i < F_MAX_E; i += threads) g.mask[i] = 0;
+  for (int i = id; i < g.H / 64; i += threads) g.done[i] = 0;
+  if constexpr (FMT == FMT_Q4) {
+    for (int i = id; i < g.T * (g.H / 8); i += threads) {
+      const uint4 v = *reinterpret_cast<const uint4*>(g.x + 8 * (int64_t)i);
+      const uint4 o = {__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
+                       __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u)};
+      *reinterpret_cast<uint4*>(g.xp + 8 * (int64_t)i) = o;
+    }
+  }
+  if (e >= g.E) return;
+  const uint16_t* const wr = g.router + (int64_t)e * g.H;
+  const uint16_t* xr[TB];
+#pragma unroll
+  for (int i = 0; i < TB; ++i) xr[i] = g.x + (int64_t)(t0 + i < g.T ? t0 + i : g.T - 1) * g.H;
+  double acc[TB];
+#pragma unroll
+  for (int i = 0; i < TB; ++i) acc[i] = 0;
+#pragma unroll 4
+  for (int h = 8 * lane; h < g.H; h += 512) {
+    const uint4 w = *reinterpret_cast<const uint4*>(wr + h);
+    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < TB; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(xr[i] + h);
+      const uint32_t xw[4] = {v.x, v.y, v.z, v.w};
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x2 a = unpack2<DT>(xw[q]), b = unpack2<DT>(ww[q]);
+        s = fmaf(a.x, b.x, s);
+        s = fmaf(a.y, b.y, s);
+      }
+      acc[i] += (double)s;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TB; ++i) {
+    const double l = wave_sum_d(acc[i]);
+    if (lane == 0 && t0 + i < g.T) g.logits[(int64_t)(t0 + i) * g.E + e] = l;
+  }
+}
+
 __global__ __launch_bounds__(1024) void few_route_kernel(const FewArgs g) {
-  extern __shared__ __attribute__((aligned(16))) uint16_t s_x[];
   __shared__ double s_l[F_MAX_E];
   __shared__ int64_t s_key[F_MAX_E];
   __shared__ float s_p[F_MAX_K];
-  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (t == 0)
-    for (int i = tid; i < g.H / 32; i += 1024) g.done[i] = 0;
-  for (int i = tid; i < g.H / 8; i += 1024) {
-    const uint4 v = *reinterpret_cast<const uint4*>(g.x + (int64_t)t * g.H + 8 * i);
-    *reinterpret_cast<uint4*>(s_x + 8 * i) = v;
-    if constexpr (FMT == FMT_Q4) {
-      const uint4 o = {__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
-                       __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u)};
-      *reinterpret_cast<uint4*>(g.xp + (int64_t)t * g.H + 8 * i) = o;
-    }
-  }
-  __syncthreads();
-  for (int e0 = wave; e0 < g.E; e0 += 64) {
-    double acc[4] = {0, 0, 0, 0};
-    for (int h = 8 * lane; h < g.H; h += 512) {
-      uint4 w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int e = e0 + 16 * j < g.E ? e0 + 16 * j : g.E - 1;
-        w[j] = *reinterpret_cast<const uint4*>(g.router + (int64_t)e * g.H + h);
-      }
-      const uint4 xv = *reinterpret_cast<const uint4*>(s_x + h);
-      const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t ww[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
-        float s = 0.f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x2 a = unpack2<DT>(xw[q]), b = unpack2<DT>(ww[q]);
-          s = fmaf(a.x, b.x, s);
-          s = fmaf(a.y, b.y, s);
-        }
-        acc[j] += (double)s;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const double l = wave_sum_d(acc[j]);
-      if (lane == 0 && e0 + 16 * j < g.E) {
-        s_l[e0 + 16 * j] = l;
-        s_key[e0 + 16 * j] = order_key(l);
-      }
-    }
+  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  if (tid < g.E) {
+    const double l = g.logits[(int64_t)t * g.E + tid];
+    s_l[tid] = l;
+    s_key[tid] = order_key(l);
   }
   __syncthreads();
   // rank of expert tid / 4: how many come before it; its four threads look at a quarter each
@@ -155,38 +164,78 @@ __global__ __launch_bounds__(1024) void few_route_kernel(const FewArgs g) {
   for (int o = lane; o < g.E; o += 64) sum += expf((float)(s_l[o] - m));
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
-  const bool chosen = e < g.E && rank < g.k;
+  const bool chosen = e < g.E && rank < g.k && (tid & 3) == 0;
   const float p = chosen ? expf((float)(s_l[e] - m)) : 0.f;
-  if (chosen && (tid & 3) == 0) s_p[rank] = p;
+  if (chosen) s_p[rank] = p;
   __syncthreads();
-  if (chosen && (tid & 3) == 0) {
+  if (chosen) {
     float total = sum;
     if (g.norm) {
       total = 0.f;
       for (int i = 0; i < g.k; ++i) total += s_p[i];
       if (sum != sum) total = sum;  // a NaN anywhere in the row
     }
-    g.sel[t * g.k + rank] = e;
-    g.wt[t * g.k + rank] = p / total;
+    g.wt[e * FT + t] = p / total;
+    atomicOr(&g.mask[e], 1u << t);  // bits of different blocks: any order gives the same mask
   }
 }
 
 // ---- products --------------------------------------------------------------------
 
-// Which tokens each expert serves, from the selections (ends with a barrier).
-__device__ __forceinline__ void token_masks(const FewArgs& g, uint32_t* s_mask, int tid, int threads) {
-  for (int i = tid; i < F_MAX_E; i += threads) s_mask[i] = 0;
-  __syncthreads();
-  for (int i = tid; i < g.T * g.k; i += threads) atomicOr(&s_mask[g.sel[i]], 1u << (i / g.k));
-  __syncthreads();
+// Place of the n-th set bit.
+__device__ __forceinline__ int nth_bit(uint64_t m, int n) {
+  int at = 0;
+#pragma unroll
+  for (int w = 32; w > 0; w >>= 1) {
+    const int c = __popcll((m >> at) & ((1ull << w) - 1));
+    if (n >= c) {
+      n -= c;
+      at += w;
+    }
+  }
+  return at;
 }
 
-// A wave's operands of one group of 128: NU units of 32 weight rows, and the tokens.
+// The experts in use, held by a wave: 256 bits and the lane's four masks.
+struct InUse {
+  uint64_t bits[F_MAX_E / 64];
+  uint32_t mask[F_MAX_E / 64];
+  int count;
+  __device__ __forceinline__ void load(const uint32_t* m, int lane) {
+    count = 0;
+#pragma unroll
+    for (int i = 0; i < F_MAX_E / 64; ++i) mask[i] = m[64 * i + lane];
+#pragma unroll
+    for (int i = 0; i < F_MAX_E / 64; ++i) {
+      bits[i] = __ballot(mask[i] != 0);
+      count += __popcll(bits[i]);
+    }
+  }
+  // The u-th expert in use (u < count) and its tokens.
+  __device__ __forceinline__ int expert(int u, uint32_t& tokens) const {
+    int e = 0;
+    tokens = 0;
+#pragma unroll
+    for (int i = 0; i < F_MAX_E / 64; ++i) {
+      const int c = __popcll(bits[i]);
+      if (u >= 0 && u < c) {
+        const int b = nth_bit(bits[i], u);
+        e = 64 * i + b;
+        tokens = (uint32_t)__builtin_amdgcn_readlane((int)mask[i], __builtin_amdgcn_readfirstlane(b));
+      }
+      u -= c;
+    }
+    return __builtin_amdgcn_readfirstlane(e);
+  }
+};
+
+// A wave's operands of one group of 128: NU units of 16 weight rows, and the tokens.
+// Lane (r, q) = (lane % 16, lane / 16) has k = 32 q + [0, 32) of weight row r and token r.
 template <int NU, int FMT>
 struct Group {
-  u32x4 c[NU][FMT == FMT_Q4 ? 2 : 4];  // codes: lane (row, half) has k = 64 s + 32 half + [0, 32) of its row
+  u32x4 c[NU][FMT == FMT_Q4 ? 1 : 2];  // codes
   uint32_t z[NU];                      // scale | zero, or the E8M0 byte
-  u32x4 x[8];                          // tokens: lane (token, half), register 4 s + j: k = 64 s + 32 half + 8 j + [0, 8)
+  u32x4 x[4];                          // register j: k = 32 q + 8 j + [0, 8)
 };
 
 template <int FMT>
@@ -194,28 +243,51 @@ __device__ __forceinline__ int64_t row_bytes(int K) {
   return FMT == FMT_Q4 ? K / 2 : K;
 }
 
+// Where a wave's operands come from: for each unit the first weight row's codes and scales,
+// and the tokens, all wave-uniform; the lane's place in them as 32-bit byte offsets.
+template <int NU>
+struct Source {
+  const uint8_t* w[NU];
+  const uint8_t* s[NU];
+  const uint8_t* x;
+  uint32_t w_off, s_off, x_off;
+
+  // Units of rows row[v] + [0, 16) of expert e's [R, K] matrix.
+  template <int FMT>
+  __device__ __forceinline__ void weights(const uint8_t* codes, const void* scales, int e, int R, int K,
+                                          const int (&row)[NU], int lane) {
+    const int r = lane & 15, q = lane >> 4, ng = K / 128;
+    const int64_t rb = row_bytes<FMT>(K);
+#pragma unroll
+    for (int v = 0; v < NU; ++v) {
+      w[v] = codes + ((int64_t)e * R + row[v]) * rb;
+      if constexpr (FMT == FMT_Q4) s[v] = reinterpret_cast<const uint8_t*>(scales) + ((int64_t)e * R + row[v]) * ng * 4;
+      else s[v] = reinterpret_cast<const uint8_t*>(scales) + ((int64_t)e * ((R + 127) / 128) + row[v] / 128) * ng;
+    }
+    w_off = (uint32_t)(r * rb + (FMT == FMT_Q4 ? 16 : 32) * q);
+    s_off = (uint32_t)(r * ng * 4);
+  }
+};
+
 template <int NU, int FMT>
-__device__ __forceinline__ void load_group(Group<NU, FMT>& b, const uint8_t* const (&w)[NU], const void* const (&s)[NU],
-                                           const uint16_t* x, bool live, int gr) {
+__device__ __forceinline__ void load_group(Group<NU, FMT>& b, const Source<NU>& src, bool live, int gr) {
 #pragma unroll
   for (int u = 0; u < NU; ++u) {
     if constexpr (FMT == FMT_Q4) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) b.c[u][i] = *reinterpret_cast<const u32x4*>(w[u] + gr * 64 + 32 * i);
-      b.z[u] = reinterpret_cast<const uint32_t*>(s[u])[gr];
+      b.c[u][0] = *reinterpret_cast<const u32x4*>(src.w[u] + gr * 64 + src.w_off);
+      b.z[u] = *reinterpret_cast<const uint32_t*>(src.s[u] + gr * 4 + src.s_off);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) b.c[u][i] = *reinterpret_cast<const u32x4*>(w[u] + gr * 128 + 64 * (i >> 1) + 16 * (i & 1));
-      b.z[u] = reinterpret_cast<const uint8_t*>(s[u])[gr];
+      for (int i = 0; i < 2; ++i) b.c[u][i] = *reinterpret_cast<const u32x4*>(src.w[u] + gr * 128 + 16 * i + src.w_off);
+      b.z[u] = src.s[u][gr];
     }
   }
   if (live) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      b.x[i] = *reinterpret_cast<const u32x4*>(x + gr * 128 + 64 * (i >> 2) + 8 * (i & 3));
+    for (int i = 0; i < 4; ++i) b.x[i] = *reinterpret_cast<const u32x4*>(src.x + gr * 256 + 16 * i + src.x_off);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b.x[i] = u32x4{0, 0, 0, 0};
+    for (int i = 0; i < 4; ++i) b.x[i] = u32x4{0, 0, 0, 0};
   }
 }
 
@@ -253,203 +325,181 @@ __device__ __forceinline__ u32x4 frag8(uint32_t a, uint32_t b) {
   return o;
 }
 
-// acc[u] += the group's product: rows are tokens, columns the unit's weight rows.
+template <int DT>
+__device__ __forceinline__ f32x4 mfma16(const u32x4 a, const u32x4 b, f32x4 c) {
+  if constexpr (DT == USAF_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// acc[u] += the group's product: value i of lane (r, q) is token row 4 q + i, weight row r.
 template <int NU, int FMT, int DT>
-__device__ __forceinline__ void mul_group(const Group<NU, FMT>& b, f32x16 (&acc)[NU]) {
-  f32x16 xs = f32x16{};
+__device__ __forceinline__ void mul_group(const Group<NU, FMT>& b, f32x4 (&acc)[NU]) {
+  f32x4 xs = {0.f, 0.f, 0.f, 0.f};
   if constexpr (FMT == FMT_Q4) {
     const uint32_t one = DT == USAF_BF16 ? 0x3F803F80u : 0x3C003C00u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) xs = mfma32<DT>(b.x[i], u32x4{one, one, one, one}, xs);
+    for (int i = 0; i < 4; ++i) xs = mfma16<DT>(b.x[i], u32x4{one, one, one, one}, xs);
   }
 #pragma unroll
   for (int u = 0; u < NU; ++u) {
-    f32x16 d = f32x16{};
+    f32x4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (FMT == FMT_Q4) d = mfma32<DT>(b.x[i], frag4<DT>(b.c[u][i >> 2][i & 3]), d);
-      else d = mfma32<DT>(b.x[i], frag8<DT>(b.c[u][i >> 1][2 * (i & 1)], b.c[u][i >> 1][2 * (i & 1) + 1]), d);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (FMT == FMT_Q4) d = mfma16<DT>(b.x[i], frag4<DT>(b.c[u][0][i]), d);
+      else d = mfma16<DT>(b.x[i], frag8<DT>(b.c[u][i >> 1][2 * (i & 1)], b.c[u][i >> 1][2 * (i & 1) + 1]), d);
     }
     if constexpr (FMT == FMT_Q4) {
       const float s = f16_bits_to_f32((uint16_t)b.z[u]), z = f16_bits_to_f32((uint16_t)(b.z[u] >> 16));
       const float zo = DT == USAF_BF16 ? fmaf(-128.0f, s, z) : fmaf(8.0f, s, z);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[u][i] = fmaf(zo, xs[i], fmaf(s, d[i], acc[u][i]));
+      for (int i = 0; i < 4; ++i) acc[u][i] = fmaf(zo, xs[i], fmaf(s, d[i], acc[u][i]));
     } else {
       const float s = __uint_as_float(b.z[u] == 0 ? 0x00400000u : b.z[u] << 23);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[u][i] = fmaf(s, d[i], acc[u][i]);
+      for (int i = 0; i < 4; ++i) acc[u][i] = fmaf(s, d[i], acc[u][i]);
     }
   }
 }
 
 // Groups [g0, g1) of the contraction, the next one's loads in flight.
 template <int NU, int FMT, int DT>
-__device__ __forceinline__ void mul_range(const uint8_t* const (&w)[NU], const void* const (&s)[NU], const uint16_t* x,
-                                          bool live, int g0, int g1, f32x16 (&acc)[NU]) {
+__device__ __forceinline__ void mul_range(const Source<NU>& src, bool live, int g0, int g1, f32x4 (&acc)[NU]) {
   if (g0 >= g1) return;
   Group<NU, FMT> a, b;
-  load_group<NU, FMT>(a, w, s, x, live, g0);
+  load_group<NU, FMT>(a, src, live, g0);
   for (int gr = g0;;) {
-    if (gr + 1 < g1) load_group<NU, FMT>(b, w, s, x, live, gr + 1);
+    if (gr + 1 < g1) load_group<NU, FMT>(b, src, live, gr + 1);
     __builtin_amdgcn_sched_barrier(0);
     mul_group<NU, FMT, DT>(a, acc);
     if (++gr >= g1) break;
-    if (gr + 1 < g1) load_group<NU, FMT>(a, w, s, x, live, gr + 1);
+    if (gr + 1 < g1) load_group<NU, FMT>(a, src, live, gr + 1);
     __builtin_amdgcn_sched_barrier(0);
     mul_group<NU, FMT, DT>(b, acc);
     if (++gr >= g1) break;
   }
 }
 
-// Scales of weight row `row` (of an expert with R rows): the first group's.
-template <int FMT>
-__device__ __forceinline__ const void* row_scales(const void* s, int e, int R, int row, int ng) {
-  if constexpr (FMT == FMT_Q4) return reinterpret_cast<const uint32_t*>(s) + ((int64_t)e * R + row) * ng;
-  else return reinterpret_cast<const uint8_t*>(s) + ((int64_t)e * ((R + 127) / 128) + row / 128) * ng;
-}
+// The tokens of one operand: rows [16 b, 16 b + 16) of the list of set bits.
+struct Tokens {
+  int count;     // rows in use
+  int mine;      // lane's operand row's token (lane % 16; 0 past the end)
+  bool live;
+  int own[4];    // tokens of the lane's result rows 4 q + i
+  __device__ __forceinline__ Tokens(uint32_t tokens, int b, int lane) {
+    const int r = lane & 15;
+    count = __popc(tokens) - FR * b;
+    count = count > FR ? FR : count;
+    live = r < count;
+    mine = live ? nth_bit(tokens, FR * b + r) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) own[i] = __shfl(mine, 4 * (lane >> 4) + i, 64);
+  }
+};
 
-constexpr int GU_WAVES = 4, GU_THREADS = 64 * GU_WAVES;
+constexpr int GU_NU = 4;  // 32 gate rows, 32 up rows
 
-template <int DT, int FMT>
-__global__ __launch_bounds__(GU_THREADS, 2) void few_gate_up_kernel(const FewArgs g) {
-  __shared__ uint32_t s_mask[F_MAX_E];
-  __shared__ int s_cnt[F_MAX_E / 64], s_e;
-  __shared__ f32x4 s_red[GU_WAVES][8][64];
+template <int DT, int FMT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void few_gate_up_kernel(const FewArgs g) {
+  __shared__ f32x4 s_red[WAVES][GU_NU][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l32 = lane & 31, half = lane >> 5;
+  const int r = lane & 15, q = lane >> 4;
   const int n_nt = g.I / 32, u = blockIdx.x / n_nt, n0 = (blockIdx.x - u * n_nt) * 32;
-  if (tid == 0) s_e = -1;
-  token_masks(g, s_mask, tid, GU_THREADS);
-  {  // the u-th expert in use
-    const bool used = s_mask[tid] != 0;
-    const uint64_t bal = __ballot(used);
-    if (lane == 0) s_cnt[wave] = __popcll(bal);
-    __syncthreads();
-    int rank = __popcll(bal & ((1ull << lane) - 1));
-    for (int i = 0; i < wave; ++i) rank += s_cnt[i];
-    if (used && rank == u) s_e = tid;
-    __syncthreads();
-  }
-  const int e = __builtin_amdgcn_readfirstlane(s_e);
-  if (e < 0) return;  // block-uniform
-  const uint32_t mask = s_mask[e];
+  InUse in;
+  in.load(g.mask, lane);
+  if (u >= in.count) return;  // block-uniform
+  uint32_t tokens;
+  const int e = in.expert(u, tokens);
   const int ng = g.H / 128;
-  const int64_t rb = row_bytes<FMT>(g.H);
-  const int rows[2] = {n0 + l32, g.I + n0 + l32};
-  const int lane_off = FMT == FMT_Q4 ? 16 * half : 32 * half;
-  const uint8_t* const w[2] = {g.gu + ((int64_t)e * 2 * g.I + rows[0]) * rb + lane_off,
-                               g.gu + ((int64_t)e * 2 * g.I + rows[1]) * rb + lane_off};
-  const void* const s[2] = {row_scales<FMT>(g.gu_s, e, 2 * g.I, rows[0], ng), row_scales<FMT>(g.gu_s, e, 2 * g.I, rows[1], ng)};
-  const uint16_t* const x = (FMT == FMT_Q4 ? g.xp : g.x) + (int64_t)(l32 < g.T ? l32 : 0) * g.H + 32 * half;
-  f32x16 acc[2] = {f32x16{}, f32x16{}};
-  mul_range<2, FMT, DT>(w, s, x, (mask >> l32) & 1, ng * wave / GU_WAVES, ng * (wave + 1) / GU_WAVES, acc);
+  Source<GU_NU> src;
+  src.weights<FMT>(g.gu, g.gu_s, e, 2 * g.I, g.H, {n0, n0 + 16, g.I + n0, g.I + n0 + 16}, lane);
+  src.x = reinterpret_cast<const uint8_t*>(FMT == FMT_Q4 ? g.xp : g.x);
+  for (int b = 0; FR * b < __popc(tokens); ++b) {
+    const Tokens tk(tokens, b, lane);
+    src.x_off = (uint32_t)((tk.mine * g.H + 32 * q) * 2);
+    f32x4 acc[GU_NU];
 #pragma unroll
-  for (int v = 0; v < 2; ++v)
+    for (int v = 0; v < GU_NU; ++v) acc[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+    mul_range<GU_NU, FMT, DT>(src, tk.live, ng * wave / WAVES, ng * (wave + 1) / WAVES, acc);
+    if (b) __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      s_red[wave][4 * v + q][lane] = f32x4{acc[v][4 * q], acc[v][4 * q + 1], acc[v][4 * q + 2], acc[v][4 * q + 3]};
-  __syncthreads();
-  // wave q finishes tokens 8 q + 4 half + [0, 4) of column n0 + l32
-  f32x4 gt = s_red[0][wave][lane], up = s_red[0][4 + wave][lane];
+    for (int v = 0; v < GU_NU; ++v) s_red[wave][v][lane] = acc[v];
+    __syncthreads();
+    if (wave < 2) {  // wave v finishes columns n0 + 16 v + [0, 16)
+      f32x4 gt = s_red[0][wave][lane], up = s_red[0][2 + wave][lane];
 #pragma unroll
-  for (int i = 1; i < GU_WAVES; ++i) {
-    const f32x4 a = s_red[i][wave][lane], b = s_red[i][4 + wave][lane];
+      for (int i = 1; i < WAVES; ++i) {
+        const f32x4 a = s_red[i][wave][lane], c = s_red[i][2 + wave][lane];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      gt[j] += a[j];
-      up[j] += b[j];
+        for (int j = 0; j < 4; ++j) {
+          gt[j] += a[j];
+          up[j] += c[j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (4 * q + j < tk.count)
+          store_from_f32<DT>(g.act, ((int64_t)u * g.T + tk.own[j]) * g.I + frag_pos<FMT>(n0 + 16 * wave + r),
+                             silu_fast(gt[j]) * up[j]);
     }
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int t = 8 * wave + 4 * half + j;
-    if ((mask >> t) & 1)
-      store_from_f32<DT>(g.act, ((int64_t)u * g.T + t) * g.I + frag_pos<FMT>(n0 + l32), silu_fast(gt[j]) * up[j]);
   }
 }
 
-constexpr int DN_WAVES = 8, DN_THREADS = 64 * DN_WAVES;
+constexpr int DN_WAVES = 8, DN_THREADS = 64 * DN_WAVES, DN_NU = 4, DN_COLS = 16 * DN_NU;
 
 template <int DT, int FMT>
-__global__ __launch_bounds__(DN_THREADS, 2) void few_down_kernel(const FewArgs g) {
-  __shared__ uint32_t s_mask[F_MAX_E];
-  __shared__ uint16_t s_used[F_MAX_E];
-  __shared__ int s_cnt[F_MAX_E / 64], s_last;
-  __shared__ __attribute__((aligned(16))) float s_w[F_MAX_E * FT];  // weight of (expert, token); later the partial sums
-  static_assert(F_MAX_E * FT * 4 >= DN_WAVES * 4 * 64 * 16, "the waves' sums fit the weights' place");
+__global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
+  extern __shared__ __attribute__((aligned(16))) float s_sum[];  // [waves][T][64]
+  int* const s_last = reinterpret_cast<int*>(s_sum);  // once the sums have been read
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l32 = lane & 31, half = lane >> 5;
-  const int nt = blockIdx.x / g.P, p = blockIdx.x - nt * g.P, n0 = 32 * nt;
-  token_masks(g, s_mask, tid, DN_THREADS);
-  for (int i = tid; i < g.T * g.k; i += DN_THREADS) s_w[g.sel[i] * FT + i / g.k] = g.wt[i];
-  bool used = false;
-  uint64_t bal = 0;
-  if (tid < F_MAX_E) {
-    used = s_mask[tid] != 0;
-    bal = __ballot(used);
-    if (lane == 0) s_cnt[wave] = __popcll(bal);
-  }
-  __syncthreads();
-  int total = 0;
-  {
-    int before = 0;
-#pragma unroll
-    for (int i = 0; i < F_MAX_E / 64; ++i) {
-      if (i == wave) before = total;
-      total += s_cnt[i];
-    }
-    if (used) s_used[before + __popcll(bal & ((1ull << lane) - 1))] = (uint16_t)tid;
-  }
-  __syncthreads();
-  const int u0 = total * p / g.P, u1 = total * (p + 1) / g.P;
+  const int r = lane & 15, q = lane >> 4;
+  const int nt = blockIdx.x / g.P, p = blockIdx.x - nt * g.P, n0 = DN_COLS * nt;
+  float* const sum = s_sum + wave * g.T * DN_COLS;  // the wave's own: its LDS operations complete in order
+  for (int i = lane; i < g.T * DN_COLS / 4; i += 64) reinterpret_cast<f32x4*>(sum)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  InUse in;
+  in.load(g.mask, lane);
+  const int u0 = in.count * p / g.P, u1 = in.count * (p + 1) / g.P;
   const int ng = g.I / 128, n_items = (u1 - u0) * g.KS;
-  const int64_t rb = row_bytes<FMT>(g.I);
-  const int lane_off = FMT == FMT_Q4 ? 16 * half : 32 * half;
-  f32x16 sum = f32x16{};
   for (int it = wave; it < n_items; it += DN_WAVES) {
     const int u = __builtin_amdgcn_readfirstlane(u0 + it / g.KS), ks = it % g.KS;
-    const int e = __builtin_amdgcn_readfirstlane((int)s_used[u]);
-    const uint32_t mask = (uint32_t)__builtin_amdgcn_readfirstlane((int)s_mask[e]);
-    const uint8_t* const w[1] = {g.dn + ((int64_t)e * g.H + n0 + l32) * rb + lane_off};
-    const void* const s[1] = {row_scales<FMT>(g.dn_s, e, g.H, n0 + l32, ng)};
-    const bool live = (mask >> l32) & 1;
-    const uint16_t* const x = g.act + ((int64_t)u * g.T + (live ? l32 : 0)) * g.I + 32 * half;
-    f32x16 y[1] = {f32x16{}};
-    mul_range<1, FMT, DT>(w, s, x, live, ng * ks / g.KS, ng * (ks + 1) / g.KS, y);
+    uint32_t tokens;
+    const int e = in.expert(u, tokens);
+    Source<DN_NU> src;
+    src.weights<FMT>(g.dn, g.dn_s, e, g.H, g.I, {n0, n0 + 16, n0 + 32, n0 + 48}, lane);
+    src.x = reinterpret_cast<const uint8_t*>(g.act + (int64_t)u * g.T * g.I);
+    for (int b = 0; FR * b < __popc(tokens); ++b) {
+      const Tokens tk(tokens, b, lane);
+      src.x_off = (uint32_t)((tk.mine * g.I + 32 * q) * 2);
+      float wt[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4 wv = *reinterpret_cast<const f32x4*>(&s_w[e * FT + 8 * q + 4 * half]);
-      const uint32_t m4 = mask >> (8 * q + 4 * half);
+      for (int i = 0; i < 4; ++i) wt[i] = 4 * q + i < tk.count ? g.wt[e * FT + tk.own[i]] : 0.f;
+      f32x4 y[DN_NU];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)  // a row of another token's is not added, not even as 0 times something
-        if ((m4 >> j) & 1) sum[4 * q + j] = fmaf(wv[j], y[0][4 * q + j], sum[4 * q + j]);
+      for (int v = 0; v < DN_NU; ++v) y[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+      mul_range<DN_NU, FMT, DT>(src, tk.live, ng * ks / g.KS, ng * (ks + 1) / g.KS, y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (4 * q + i < tk.count) {
+#pragma unroll
+          for (int v = 0; v < DN_NU; ++v) {
+            float* const at = sum + tk.own[i] * DN_COLS + 16 * v + r;
+            *at = fmaf(wt[i], y[v][i], *at);
+          }
+        }
+      __builtin_amdgcn_wave_barrier();
     }
   }
   __syncthreads();
-  f32x4* const red = reinterpret_cast<f32x4*>(s_w);
+  for (int i = tid; i < g.T * DN_COLS; i += DN_THREADS) {
+    const int t = i / DN_COLS;
+    const int64_t at = (int64_t)t * g.H + n0 + i % DN_COLS;
+    float v = s_sum[i];
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
-    red[(wave * 4 + q) * 64 + lane] = f32x4{sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]};
-  __syncthreads();
-  float v[4];
-  if (wave < 4) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = 0.f;
-#pragma unroll
-    for (int i = 0; i < DN_WAVES; ++i) {
-      const f32x4 a = red[(i * 4 + wave) * 64 + lane];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += a[j];
-    }
-    // tokens 8 wave + 4 half + [0, 4) of column n0 + l32
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = 8 * wave + 4 * half + j;
-      if (t >= g.T) continue;
-      if (g.P == 1) store_from_f32<DT>(g.out, (int64_t)t * g.H + n0 + l32, v[j]);
-      else __hip_atomic_store(&g.part[((int64_t)p * g.T + t) * g.H + n0 + l32], v[j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    for (int j = 1; j < DN_WAVES; ++j) v += s_sum[j * g.T * DN_COLS + i];
+    if (g.P == 1) store_from_f32<DT>(g.out, at, v);
+    else __hip_atomic_store(&g.part[(int64_t)p * g.T * g.H + at], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (g.P == 1) return;
   // The parts of a column tile meet at the device's coherence point: stored and loaded at
@@ -458,21 +508,20 @@ __global__ __launch_bounds__(DN_THREADS, 2) void few_down_kernel(const FewArgs g
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0)
-    s_last = __hip_atomic_fetch_add(&g.done[nt], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == g.P - 1;
+    *s_last = __hip_atomic_fetch_add(&g.done[nt], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == g.P - 1;
   __syncthreads();
-  if (!s_last) return;
-  for (int i = tid; i < g.T * 32; i += DN_THREADS) {
-    const int t = i >> 5;
-    const int64_t at = (int64_t)t * g.H + n0 + (i & 31);
+  if (!*s_last) return;
+  for (int i = tid; i < g.T * DN_COLS; i += DN_THREADS) {
+    const int64_t at = (int64_t)(i / DN_COLS) * g.H + n0 + i % DN_COLS;
     float o = 0.f;
-    for (int q = 0; q < g.P; ++q)
-      o += __hip_atomic_load(&g.part[(int64_t)q * g.T * g.H + at], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int j = 0; j < g.P; ++j)
+      o += __hip_atomic_load(&g.part[(int64_t)j * g.T * g.H + at], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     store_from_f32<DT>(g.out, at, o);
   }
 }
 
 struct FewPlan {
-  int64_t in_use, sel, wt, xp, act, part, done, bytes;
+  int64_t in_use, logits, mask, wt, xp, act, part, done, bytes;
   int P, KS;
 };
 
@@ -480,17 +529,18 @@ struct FewPlan {
 FewPlan few_plan(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
   FewPlan p;
   p.in_use = E < T * k ? E : T * k;
-  const int64_t tiles = H / 32, groups = I / 128;
+  const int64_t tiles = H / DN_COLS, groups = I / 128;
   int64_t parts = 512 / tiles;
   parts = parts < 1 ? 1 : parts > p.in_use ? p.in_use : parts;
   const int64_t per = (p.in_use + parts - 1) / parts;
-  int64_t ks = (DN_WAVES + per - 1) / per;
+  int64_t ks = (2 * DN_WAVES + per - 1) / per;
   p.P = (int)parts;
   p.KS = (int)(ks > groups ? groups : ks);
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t b = at; at += (bytes + 15) / 16 * 16; return b; };
-  p.sel = take(T * k * 4);
-  p.wt = take(T * k * 4);
+  p.logits = take(T * E * 8);
+  p.mask = take(F_MAX_E * 4);
+  p.wt = take(E * FT * 4);
   p.done = take(tiles * 4);
   p.xp = take(T * H * 2);
   p.act = take(p.in_use * T * I * 2);
@@ -501,11 +551,16 @@ FewPlan few_plan(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
 
 template <int DT, int FMT>
 int launch_few_layer(const FewArgs& g, int64_t in_use, hipStream_t st) {
-  few_route_kernel<DT, FMT><<<(unsigned)g.T, 1024, (size_t)g.H * 2, st>>>(g);
+  const int eb = (g.E + 3) / 4;
+  if (g.T == 1) few_logits_kernel<DT, FMT, 1><<<(unsigned)eb, 256, 0, st>>>(g);
+  else few_logits_kernel<DT, FMT, 4><<<(unsigned)(eb * ((g.T + 3) / 4)), 256, 0, st>>>(g);
+  if (int rc = check_launch("moe_few/logits")) return rc;
+  few_route_kernel<<<(unsigned)g.T, 1024, 0, st>>>(g);
   if (int rc = check_launch("moe_few/route")) return rc;
-  few_gate_up_kernel<DT, FMT><<<(unsigned)(in_use * (g.I / 32)), GU_THREADS, 0, st>>>(g);
+  few_gate_up_kernel<DT, FMT, 4><<<(unsigned)(in_use * (g.I / 32)), 256, 0, st>>>(g);
   if (int rc = check_launch("moe_few/gate_up")) return rc;
-  few_down_kernel<DT, FMT><<<(unsigned)(g.H / 32 * g.P), DN_THREADS, 0, st>>>(g);
+  few_down_kernel<DT, FMT>
+      <<<(unsigned)(g.H / DN_COLS * g.P), DN_THREADS, (size_t)DN_WAVES * g.T * DN_COLS * 4, st>>>(g);
   return check_launch("moe_few/down");
 }
 
@@ -560,7 +615,8 @@ extern "C" int usaf_hip_moe_few(const void* x, int64_t T, int64_t H, const void*
   g.dn_s = down_scale;
   g.out = reinterpret_cast<uint16_t*>(out);
   uint8_t* const b = reinterpret_cast<uint8_t*>(ws);
-  g.sel = reinterpret_cast<int32_t*>(b + p.sel);
+  g.logits = reinterpret_cast<double*>(b + p.logits);
+  g.mask = reinterpret_cast<uint32_t*>(b + p.mask);
   g.wt = reinterpret_cast<float*>(b + p.wt);
   g.done = reinterpret_cast<int32_t*>(b + p.done);
   g.xp = reinterpret_cast<uint16_t*>(b + p.xp);
