@@ -7,10 +7,9 @@
 //
 //   few_logits   a wave an expert of the router and up to four tokens
 //   few_route    a block a token: selection by rank, weights, a bit of the token in its experts' masks
-//   few_gate_up  a block an (expert in use, 32 columns of a): its waves split the contraction
-//   few_down     a block (64 columns of out, a part of the experts in use): its waves take
-//                (expert, part of the contraction) items and add them up by token; the last
-//                block of a column tile adds the parts in order
+//   few_gate_up  a block takes (expert in use, 32 columns of a) tiles; its waves split the contraction
+//   few_down     a block has 64 columns of out; the waves of a column tile share its (expert,
+//                group of 128) pairs evenly and add them up by token; the tile's last block adds the parts in order
 //
 // An expert's tokens are the rows of a 16-row MFMA operand (more than 16: a second
 // round), weights its columns: a lane has one weight row and four tokens, so a row's scale
@@ -50,7 +49,7 @@ struct FewArgs {
   uint16_t* act;            // [experts in use, T, I] in the fragments' order
   float* part;              // [P, T, H] partial sums
   int32_t* done;            // [H / 64] parts of a column tile that have arrived
-  int P, KS;                // few_down: parts of the experts, of the contraction
+  int P;                    // few_down: blocks of a column tile
 };
 
 // Order of 8 neighbouring values in a fragment of 4-bit codes: a code word's nibbles
@@ -196,36 +195,54 @@ __device__ __forceinline__ int nth_bit(uint64_t m, int n) {
   return at;
 }
 
-// The experts in use, held by a wave: 256 bits and the lane's four masks.
+// An expert and up to 16 of its tokens: what one pass over its weights multiplies.
+struct Item {
+  int e, u;         // the expert, its place among those in use
+  uint32_t tokens;  // all its tokens
+  int b;            // which 16 of them
+};
+
+// The experts in use, held by a wave: their bits, those of experts with more than 16
+// tokens (which come again behind all others), and the lane's four masks.
 struct InUse {
-  uint64_t bits[F_MAX_E / 64];
-  uint32_t mask[F_MAX_E / 64];
-  int count;
+  static constexpr int N = F_MAX_E / 64;
+  uint64_t bits[N], more[N];
+  uint32_t mask[N];
+  int count, items;
   __device__ __forceinline__ void load(const uint32_t* m, int lane) {
-    count = 0;
 #pragma unroll
-    for (int i = 0; i < F_MAX_E / 64; ++i) mask[i] = m[64 * i + lane];
+    for (int i = 0; i < N; ++i) mask[i] = m[64 * i + lane];
+    count = items = 0;
 #pragma unroll
-    for (int i = 0; i < F_MAX_E / 64; ++i) {
+    for (int i = 0; i < N; ++i) {
       bits[i] = __ballot(mask[i] != 0);
+      more[i] = __ballot(__popc(mask[i]) > FR);
       count += __popcll(bits[i]);
+      items += __popcll(more[i]);
     }
+    items += count;
   }
-  // The u-th expert in use (u < count) and its tokens.
-  __device__ __forceinline__ int expert(int u, uint32_t& tokens) const {
-    int e = 0;
-    tokens = 0;
+  // Item i < items; everything uniform.
+  __device__ __forceinline__ Item item(int i) const {
+    Item t;
+    t.b = i >= count;
+    int n = t.b ? i - count : i, before = 0;
+    t.e = t.u = 0;
+    t.tokens = 0;
 #pragma unroll
-    for (int i = 0; i < F_MAX_E / 64; ++i) {
-      const int c = __popcll(bits[i]);
-      if (u >= 0 && u < c) {
-        const int b = nth_bit(bits[i], u);
-        e = 64 * i + b;
-        tokens = (uint32_t)__builtin_amdgcn_readlane((int)mask[i], __builtin_amdgcn_readfirstlane(b));
+    for (int k = 0; k < N; ++k) {
+      const uint64_t from = t.b ? more[k] : bits[k];
+      const int c = __popcll(from);
+      if (n >= 0 && n < c) {
+        const int at = __builtin_amdgcn_readfirstlane(nth_bit(from, n));
+        t.e = 64 * k + at;
+        t.u = before + __popcll(bits[k] & ((1ull << at) - 1));
+        t.tokens = (uint32_t)__builtin_amdgcn_readlane((int)mask[k], at);
       }
-      u -= c;
+      n -= c;
+      before += __popcll(bits[k]);
     }
-    return __builtin_amdgcn_readfirstlane(e);
+    return t;
   }
 };
 
@@ -270,7 +287,7 @@ struct Source {
 };
 
 template <int NU, int FMT>
-__device__ __forceinline__ void load_group(Group<NU, FMT>& b, const Source<NU>& src, bool live, int gr) {
+__device__ __forceinline__ void load_group(Group<NU, FMT>& b, const Source<NU>& src, int gr) {
 #pragma unroll
   for (int u = 0; u < NU; ++u) {
     if constexpr (FMT == FMT_Q4) {
@@ -282,13 +299,8 @@ __device__ __forceinline__ void load_group(Group<NU, FMT>& b, const Source<NU>& 
       b.z[u] = src.s[u][gr];
     }
   }
-  if (live) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) b.x[i] = *reinterpret_cast<const u32x4*>(src.x + gr * 256 + 16 * i + src.x_off);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b.x[i] = u32x4{0, 0, 0, 0};
-  }
+  for (int i = 0; i < 4; ++i) b.x[i] = *reinterpret_cast<const u32x4*>(src.x + gr * 256 + 16 * i + src.x_off);
 }
 
 // Eight 4-bit codes -> a fragment register: bf16 128 + q, or fp16 q - 8.
@@ -364,86 +376,114 @@ __device__ __forceinline__ void mul_group(const Group<NU, FMT>& b, f32x4 (&acc)[
   }
 }
 
-// Groups [g0, g1) of the contraction, the next one's loads in flight.
-template <int NU, int FMT, int DT>
-__device__ __forceinline__ void mul_range(const Source<NU>& src, bool live, int g0, int g1, f32x4 (&acc)[NU]) {
-  if (g0 >= g1) return;
-  Group<NU, FMT> a, b;
-  load_group<NU, FMT>(a, src, live, g0);
-  for (int gr = g0;;) {
-    if (gr + 1 < g1) load_group<NU, FMT>(b, src, live, gr + 1);
-    __builtin_amdgcn_sched_barrier(0);
-    mul_group<NU, FMT, DT>(a, acc);
-    if (++gr >= g1) break;
-    if (gr + 1 < g1) load_group<NU, FMT>(a, src, live, gr + 1);
-    __builtin_amdgcn_sched_barrier(0);
-    mul_group<NU, FMT, DT>(b, acc);
-    if (++gr >= g1) break;
-  }
-}
-
-// The tokens of one operand: rows [16 b, 16 b + 16) of the list of set bits.
+// An item's tokens as rows of the operand.  Rows past the last repeat it; their results are not used.
 struct Tokens {
-  int count;     // rows in use
-  int mine;      // lane's operand row's token (lane % 16; 0 past the end)
-  bool live;
-  int own[4];    // tokens of the lane's result rows 4 q + i
-  __device__ __forceinline__ Tokens(uint32_t tokens, int b, int lane) {
-    const int r = lane & 15;
-    count = __popc(tokens) - FR * b;
-    count = count > FR ? FR : count;
-    live = r < count;
-    mine = live ? nth_bit(tokens, FR * b + r) : 0;
+  int count;   // rows in use
+  int own[4];  // tokens of the lane's result rows 4 q + i
+  // Returns the token of the lane's operand row.
+  __device__ __forceinline__ int set(const Item& t, int lane) {
+    const int r = lane & 15, left = __popc(t.tokens) - FR * t.b;
+    count = left > FR ? FR : left;
+    const int mine = nth_bit(t.tokens, FR * t.b + (r < count ? r : count - 1));
 #pragma unroll
     for (int i = 0; i < 4; ++i) own[i] = __shfl(mine, 4 * (lane >> 4) + i, 64);
+    return mine;
   }
 };
 
-constexpr int GU_NU = 4;  // 32 gate rows, 32 up rows
+// Both products walk a list of (item, group) pairs with the next pair's loads in flight
+// behind the present one's arithmetic, across the items' ends: a wave has only four to
+// sixteen groups of an item, and a first load takes as long as three groups' arithmetic.
+// The loads carry no condition (the last pair is loaded once more), or the compiler
+// would have to wait for all of them at every use.
 
-template <int DT, int FMT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void few_gate_up_kernel(const FewArgs g) {
-  __shared__ f32x4 s_red[WAVES][GU_NU][64];
+constexpr int GU_NU = 4, GU_WAVES = 4, GU_THREADS = 64 * GU_WAVES;  // 32 gate rows and their 32 up rows
+
+template <int DT, int FMT>
+__global__ __launch_bounds__(GU_THREADS, 3) void few_gate_up_kernel(const FewArgs g) {
+  __shared__ f32x4 s_red[2][GU_WAVES][GU_NU][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int n_nt = g.I / 32, u = blockIdx.x / n_nt, n0 = (blockIdx.x - u * n_nt) * 32;
+  const int n_nt = g.I / 32, ng = g.H / 128;
+  const int g0 = ng * wave / GU_WAVES, some = ng * (wave + 1) / GU_WAVES - g0;
+  const int n = some > 0 ? some : 1;  // a wave without a group of its own multiplies one and adds nothing
   InUse in;
   in.load(g.mask, lane);
-  if (u >= in.count) return;  // block-uniform
-  uint32_t tokens;
-  const int e = in.expert(u, tokens);
-  const int ng = g.H / 128;
+  const int work = in.items * n_nt;
+  int at = blockIdx.x, gr = 0;  // the pair being loaded
+  if (at >= work) return;       // block-uniform
   Source<GU_NU> src;
-  src.weights<FMT>(g.gu, g.gu_s, e, 2 * g.I, g.H, {n0, n0 + 16, g.I + n0, g.I + n0 + 16}, lane);
   src.x = reinterpret_cast<const uint8_t*>(FMT == FMT_Q4 ? g.xp : g.x);
-  for (int b = 0; FR * b < __popc(tokens); ++b) {
-    const Tokens tk(tokens, b, lane);
-    src.x_off = (uint32_t)((tk.mine * g.H + 32 * q) * 2);
-    f32x4 acc[GU_NU];
+  auto source = [&]() {
+    const Item t = in.item(at / n_nt);
+    const int n0 = at % n_nt * 32;
+    src.template weights<FMT>(g.gu, g.gu_s, t.e, 2 * g.I, g.H, {n0, n0 + 16, g.I + n0, g.I + n0 + 16}, lane);
+    Tokens tk;
+    src.x_off = (uint32_t)((tk.set(t, lane) * g.H + 32 * q) * 2);
+  };
+  f32x4 acc[GU_NU];
+  int par = 0;
+  auto finish = [&](int done) {
+    f32x4(&red)[GU_WAVES][GU_NU][64] = s_red[par];  // two in turn: one barrier an item
+    par ^= 1;
+#pragma unroll
+    for (int v = 0; v < GU_NU; ++v) red[wave][v][lane] = some > 0 ? acc[v] : f32x4{0.f, 0.f, 0.f, 0.f};
+    lds_barrier();
+    const Item t = in.item(done / n_nt);
+    Tokens tk;
+    tk.set(t, lane);
+    // wave: columns n0 + 16 (wave % 2) + [0, 16), two of the lane's four rows
+    const int v = wave & 1, j0 = wave & 2;
+    const int col = frag_pos<FMT>(done % n_nt * 32 + 16 * v + r);
+    f32x4 gt = red[0][v][lane], up = red[0][2 + v][lane];
+#pragma unroll
+    for (int i = 1; i < GU_WAVES; ++i) {
+      const f32x4 a = red[i][v][lane], c = red[i][2 + v][lane];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        gt[j] += a[j];
+        up[j] += c[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float gv = j0 ? gt[2 + j] : gt[j], uv = j0 ? up[2 + j] : up[j];
+      const int tok = j0 ? tk.own[2 + j] : tk.own[j];
+      if (4 * q + j0 + j < tk.count)
+        store_from_f32<DT>(g.act, ((int64_t)t.u * g.T + tok) * g.I + col, silu_fast(gv) * uv);
+    }
+  };
+  auto clear = [&]() {
 #pragma unroll
     for (int v = 0; v < GU_NU; ++v) acc[v] = f32x4{0.f, 0.f, 0.f, 0.f};
-    mul_range<GU_NU, FMT, DT>(src, tk.live, ng * wave / WAVES, ng * (wave + 1) / WAVES, acc);
-    if (b) __syncthreads();
-#pragma unroll
-    for (int v = 0; v < GU_NU; ++v) s_red[wave][v][lane] = acc[v];
-    __syncthreads();
-    if (wave < 2) {  // wave v finishes columns n0 + 16 v + [0, 16)
-      f32x4 gt = s_red[0][wave][lane], up = s_red[0][2 + wave][lane];
-#pragma unroll
-      for (int i = 1; i < WAVES; ++i) {
-        const f32x4 a = s_red[i][wave][lane], c = s_red[i][2 + wave][lane];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          gt[j] += a[j];
-          up[j] += c[j];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (4 * q + j < tk.count)
-          store_from_f32<DT>(g.act, ((int64_t)u * g.T + tk.own[j]) * g.I + frag_pos<FMT>(n0 + 16 * wave + r),
-                             silu_fast(gt[j]) * up[j]);
+  };
+  Group<GU_NU, FMT> a, b;
+  int now = at, now_gr = 0;  // the pair being multiplied
+  auto step = [&](const Group<GU_NU, FMT>& cur, Group<GU_NU, FMT>& nxt) {  // false: the last pair is done
+    now = at;
+    now_gr = gr;
+    if (gr + 1 < n) {
+      ++gr;
+    } else if (at + (int)gridDim.x < work) {
+      at += gridDim.x;
+      gr = 0;
+      source();
     }
+    load_group<GU_NU, FMT>(nxt, src, g0 + gr < ng ? g0 + gr : ng - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    mul_group<GU_NU, FMT, DT>(cur, acc);
+    __builtin_amdgcn_sched_barrier(0);
+    if (now_gr == n - 1) {
+      finish(now);
+      clear();
+      return now + (int)gridDim.x < work;
+    }
+    return true;
+  };
+  source();
+  clear();
+  load_group<GU_NU, FMT>(a, src, g0 < ng ? g0 : ng - 1);
+  while (step(a, b) && step(b, a)) {
   }
 }
 
@@ -452,7 +492,7 @@ constexpr int DN_WAVES = 8, DN_THREADS = 64 * DN_WAVES, DN_NU = 4, DN_COLS = 16 
 template <int DT, int FMT>
 __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
   extern __shared__ __attribute__((aligned(16))) float s_sum[];  // [waves][T][64]
-  int* const s_last = reinterpret_cast<int*>(s_sum);  // once the sums have been read
+  int* const s_last = reinterpret_cast<int*>(s_sum);             // once the sums have been read
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int nt = blockIdx.x / g.P, p = blockIdx.x - nt * g.P, n0 = DN_COLS * nt;
@@ -460,35 +500,66 @@ __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
   for (int i = lane; i < g.T * DN_COLS / 4; i += 64) reinterpret_cast<f32x4*>(sum)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   InUse in;
   in.load(g.mask, lane);
-  const int u0 = in.count * p / g.P, u1 = in.count * (p + 1) / g.P;
-  const int ng = g.I / 128, n_items = (u1 - u0) * g.KS;
-  for (int it = wave; it < n_items; it += DN_WAVES) {
-    const int u = __builtin_amdgcn_readfirstlane(u0 + it / g.KS), ks = it % g.KS;
-    uint32_t tokens;
-    const int e = in.expert(u, tokens);
+  // the wave's pairs: an even share of all waves' of this column tile
+  const int ng = g.I / 128, work = in.items * ng, parts = g.P * DN_WAVES, part = p * DN_WAVES + wave;
+  const int f1 = (int)((int64_t)work * (part + 1) / parts);
+  int f = (int)((int64_t)work * part / parts);  // the pair being loaded
+  if (f < f1) {
+    int it = f / ng, gr = f - it * ng;
     Source<DN_NU> src;
-    src.weights<FMT>(g.dn, g.dn_s, e, g.H, g.I, {n0, n0 + 16, n0 + 32, n0 + 48}, lane);
-    src.x = reinterpret_cast<const uint8_t*>(g.act + (int64_t)u * g.T * g.I);
-    for (int b = 0; FR * b < __popc(tokens); ++b) {
-      const Tokens tk(tokens, b, lane);
-      src.x_off = (uint32_t)((tk.mine * g.I + 32 * q) * 2);
-      float wt[4];
+    Tokens tk, next_tk;
+    float wt[4], next_wt[4];
+    auto source = [&]() {
+      const Item t = in.item(it);
+      src.template weights<FMT>(g.dn, g.dn_s, t.e, g.H, g.I, {n0, n0 + 16, n0 + 32, n0 + 48}, lane);
+      src.x = reinterpret_cast<const uint8_t*>(g.act + (int64_t)t.u * g.T * g.I);
+      src.x_off = (uint32_t)((next_tk.set(t, lane) * g.I + 32 * q) * 2);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) wt[i] = 4 * q + i < tk.count ? g.wt[e * FT + tk.own[i]] : 0.f;
-      f32x4 y[DN_NU];
+      for (int i = 0; i < 4; ++i) next_wt[i] = g.wt[t.e * FT + next_tk.own[i]];
+    };
+    f32x4 y[DN_NU];
+    auto begin = [&]() {
+      tk = next_tk;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) wt[i] = next_wt[i];
 #pragma unroll
       for (int v = 0; v < DN_NU; ++v) y[v] = f32x4{0.f, 0.f, 0.f, 0.f};
-      mul_range<DN_NU, FMT, DT>(src, tk.live, ng * ks / g.KS, ng * (ks + 1) / g.KS, y);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (4 * q + i < tk.count) {
-#pragma unroll
-          for (int v = 0; v < DN_NU; ++v) {
-            float* const at = sum + tk.own[i] * DN_COLS + 16 * v + r;
-            *at = fmaf(wt[i], y[v][i], *at);
-          }
+    };
+    Group<DN_NU, FMT> a, b;
+    auto step = [&](const Group<DN_NU, FMT>& cur, Group<DN_NU, FMT>& nxt) {
+      bool ends = true;
+      if (++f < f1) {
+        if (++gr == ng) {
+          gr = 0;
+          ++it;
+          source();
+        } else {
+          ends = false;
         }
-      __builtin_amdgcn_wave_barrier();
+      }
+      load_group<DN_NU, FMT>(nxt, src, gr);
+      __builtin_amdgcn_sched_barrier(0);
+      mul_group<DN_NU, FMT, DT>(cur, y);
+      __builtin_amdgcn_sched_barrier(0);
+      if (ends) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (4 * q + i < tk.count) {
+#pragma unroll
+            for (int v = 0; v < DN_NU; ++v) {
+              float* const to = sum + tk.own[i] * DN_COLS + 16 * v + r;
+              *to = fmaf(wt[i], y[v][i], *to);
+            }
+          }
+        __builtin_amdgcn_wave_barrier();
+        begin();
+      }
+      return f < f1;
+    };
+    source();
+    begin();
+    load_group<DN_NU, FMT>(a, src, gr);
+    while (step(a, b) && step(b, a)) {
     }
   }
   __syncthreads();
@@ -522,20 +593,18 @@ __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
 
 struct FewPlan {
   int64_t in_use, logits, mask, wt, xp, act, part, done, bytes;
-  int P, KS;
+  int P;
 };
 
 // Sizes, and where each buffer sits in the workspace (16-byte steps).
 FewPlan few_plan(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
   FewPlan p;
   p.in_use = E < T * k ? E : T * k;
-  const int64_t tiles = H / DN_COLS, groups = I / 128;
-  int64_t parts = 512 / tiles;
-  parts = parts < 1 ? 1 : parts > p.in_use ? p.in_use : parts;
-  const int64_t per = (p.in_use + parts - 1) / parts;
-  int64_t ks = (2 * DN_WAVES + per - 1) / per;
-  p.P = (int)parts;
-  p.KS = (int)(ks > groups ? groups : ks);
+  // a block a CU for the column tiles together, and about four pairs a wave at least
+  const int64_t tiles = H / DN_COLS, cus = device_cu_count(), pairs = p.in_use * (I / 128);
+  int64_t parts = cus / tiles, most = pairs / (4 * DN_WAVES);
+  parts = parts > most ? most : parts;
+  p.P = (int)(parts < 1 ? 1 : parts);
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t b = at; at += (bytes + 15) / 16 * 16; return b; };
   p.logits = take(T * E * 8);
@@ -544,7 +613,7 @@ FewPlan few_plan(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
   p.done = take(tiles * 4);
   p.xp = take(T * H * 2);
   p.act = take(p.in_use * T * I * 2);
-  p.part = take(parts > 1 ? parts * T * H * 4 : 0);
+  p.part = take(p.P > 1 ? p.P * T * H * 4 : 0);
   p.bytes = at;
   return p;
 }
@@ -557,7 +626,8 @@ int launch_few_layer(const FewArgs& g, int64_t in_use, hipStream_t st) {
   if (int rc = check_launch("moe_few/logits")) return rc;
   few_route_kernel<<<(unsigned)g.T, 1024, 0, st>>>(g);
   if (int rc = check_launch("moe_few/route")) return rc;
-  few_gate_up_kernel<DT, FMT, 4><<<(unsigned)(in_use * (g.I / 32)), 256, 0, st>>>(g);
+  const int64_t most = 3 * (int64_t)device_cu_count(), work = (in_use + g.T * g.k / (FR + 1)) * (g.I / 32);
+  few_gate_up_kernel<DT, FMT><<<(unsigned)(work < most ? work : most), GU_THREADS, 0, st>>>(g);
   if (int rc = check_launch("moe_few/gate_up")) return rc;
   few_down_kernel<DT, FMT>
       <<<(unsigned)(g.H / DN_COLS * g.P), DN_THREADS, (size_t)DN_WAVES * g.T * DN_COLS * 4, st>>>(g);
@@ -623,7 +693,6 @@ extern "C" int usaf_hip_moe_few(const void* x, int64_t T, int64_t H, const void*
   g.act = reinterpret_cast<uint16_t*>(b + p.act);
   g.part = reinterpret_cast<float*>(b + p.part);
   g.P = p.P;
-  g.KS = p.KS;
   hipStream_t st = as_stream(stream);
   if (eight_bit)
     return dtype == USAF_BF16 ? launch_few_layer<USAF_BF16, FMT_FP8>(g, p.in_use, st)
