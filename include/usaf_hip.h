@@ -605,8 +605,8 @@ int usaf_hip_fp8_swiglu_bwd(const void* gu, const void* dact, int64_t S, int64_t
  *   those, divided by their sum if norm_topk_prob; a_e = dtype(silu(g) u), (g, u) =
  *   gate_up_e x; out = dtype(sum_e w_e down_e a_e).
  * x [T, H], router [E, H], out [T, H] of dtype (fp16 / bf16).  eight_bit == 0: 4-bit
- * codes with group size 128 along whole rows and scales as usaf_hip_pack_scale_zero
- * writes them; a weight is the real number code * scale + zero.  eight_bit != 0: codes
+ * codes with group size 128 along whole rows; scales: usaf_hip_pack_scale_zero's words
+ * with an expert's matrix transposed, [E, K / 128, rows]; a weight is the real number code * scale + zero.  eight_bit != 0: codes
  * and scale bytes as usaf_hip_fp8_quantize_weight writes them.
  * ws: usaf_hip_moe_few_ws_bytes bytes, 16-byte aligned, nothing in them matters before the
  * call; calls that may overlap need workspaces of their own.  E <= 256, top_k <= 16, H

@@ -191,7 +191,7 @@ def test_weights_that_are_not_finite_stay_with_their_expert(B, fmt):
     if fmt == "q4":  # expert 1's down scales: infinite
         n = ew.down.s.numel() // E
         ew.down.s[n:2 * n] = float("inf")
-        ew.down._sz = None
+        ew.down._sz = ew.down._szg = None
     else:
         ew.down.q[1] = 0x7F
     got = B.few_token_block(x.cuda(), router.cuda(), 1, True, ew)

@@ -37,7 +37,7 @@ struct FewArgs {
   int T, E, k, norm;
   int H, I;
   const uint8_t* gu;        // codes [E, 2I, H]
-  const void* gu_s;         // 4-bit: fp16 scale | zero << 16 for each group; 8-bit: E8M0 bytes
+  const void* gu_s;         // 4-bit: fp16 scale | zero << 16, [E, H / 128, 2I]; 8-bit: E8M0 bytes
   const uint8_t* dn;        // codes [E, H, I]
   const void* dn_s;
   uint16_t* out;            // [T, H]
@@ -247,12 +247,17 @@ struct InUse {
 };
 
 // A wave's operands of one group of 128: NU units of 16 weight rows, and the tokens.
-// Lane (r, q) = (lane % 16, lane / 16) has k = 32 q + [0, 32) of weight row r and token r.
+//
+// The codes come from memory as they lie there, neighbouring lanes at neighbouring 16
+// bytes, and reach the fragments through LDS: loaded straight into fragments (lanes 0
+// to 15 in 16 rows) each lane's 16 bytes are an access of their own to the address unit,
+// 48 a load on average by its counters, which bound gate_up of 24 tokens at 55 us.
 template <int NU, int FMT>
 struct Group {
-  u32x4 c[NU][FMT == FMT_Q4 ? 1 : 2];  // codes
-  uint32_t z[NU];                      // scale | zero, or the E8M0 byte
-  u32x4 x[4];                          // register j: k = 32 q + 8 j + [0, 8)
+  static constexpr int W = FMT == FMT_Q4 ? 1 : 2;  // 16-byte words of a lane and unit
+  u32x4 c[NU][W];  // codes: 4-bit, lane l has word l % 4 of row l / 4; 8-bit, word l % 8 of rows l / 8 and 8 + l / 8
+  uint32_t z[NU];  // scale | zero of row l % 16, or the E8M0 byte
+  u32x4 x[4];      // tokens: lane (r, q), register j: k = 32 q + 8 j + [0, 8) of token row r
 };
 
 template <int FMT>
@@ -260,47 +265,82 @@ __device__ __forceinline__ int64_t row_bytes(int K) {
   return FMT == FMT_Q4 ? K / 2 : K;
 }
 
+typedef __amdgpu_buffer_rsrc_t Buffer;
+// Loads past `bytes` give zeros and touch no memory: what lanes of unused token rows do.
+__device__ __forceinline__ Buffer buffer_of(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+}
+constexpr uint32_t NO_ROW = 0x80000000u;  // past any buffer here
+constexpr int DEVICE_SCOPE = 16;          // sc1 of a buffer instruction
+
 // Where a wave's operands come from: for each unit the first weight row's codes and scales,
-// and the tokens, all wave-uniform; the lane's place in them as 32-bit byte offsets.
+// wave-uniform, and the tokens; the lane's place in them as byte offsets.
 template <int NU>
 struct Source {
   const uint8_t* w[NU];
   const uint8_t* s[NU];
-  const uint8_t* x;
-  uint32_t w_off, s_off, x_off;
+  Buffer x;
+  uint32_t w_off, x_off;
+  int rb8;  // bytes of 8 weight rows
 
-  // Units of rows row[v] + [0, 16) of expert e's [R, K] matrix.
+  // Units of rows row[v] + [0, 16) of expert e's [R, K] matrix.  Scales: 4-bit [E, K / 128, R]
+  // words, 8-bit [E, ceil(R / 128), K / 128] bytes.
   template <int FMT>
   __device__ __forceinline__ void weights(const uint8_t* codes, const void* scales, int e, int R, int K,
                                           const int (&row)[NU], int lane) {
-    const int r = lane & 15, q = lane >> 4, ng = K / 128;
+    const int ng = K / 128;
     const int64_t rb = row_bytes<FMT>(K);
 #pragma unroll
     for (int v = 0; v < NU; ++v) {
       w[v] = codes + ((int64_t)e * R + row[v]) * rb;
-      if constexpr (FMT == FMT_Q4) s[v] = reinterpret_cast<const uint8_t*>(scales) + ((int64_t)e * R + row[v]) * ng * 4;
+      if constexpr (FMT == FMT_Q4) s[v] = reinterpret_cast<const uint8_t*>(scales) + ((int64_t)e * ng * R + row[v]) * 4;
       else s[v] = reinterpret_cast<const uint8_t*>(scales) + ((int64_t)e * ((R + 127) / 128) + row[v] / 128) * ng;
     }
-    w_off = (uint32_t)(r * rb + (FMT == FMT_Q4 ? 16 : 32) * q);
-    s_off = (uint32_t)(r * ng * 4);
+    w_off = FMT == FMT_Q4 ? (uint32_t)((lane >> 2) * rb + 16 * (lane & 3)) : (uint32_t)((lane >> 3) * rb + 16 * (lane & 7));
+    rb8 = (int)(8 * rb);
   }
 };
 
 template <int NU, int FMT>
-__device__ __forceinline__ void load_group(Group<NU, FMT>& b, const Source<NU>& src, int gr) {
+__device__ __forceinline__ void load_group(Group<NU, FMT>& b, const Source<NU>& src, int R, int gr, int lane) {
 #pragma unroll
   for (int u = 0; u < NU; ++u) {
     if constexpr (FMT == FMT_Q4) {
       b.c[u][0] = *reinterpret_cast<const u32x4*>(src.w[u] + gr * 64 + src.w_off);
-      b.z[u] = *reinterpret_cast<const uint32_t*>(src.s[u] + gr * 4 + src.s_off);
+      b.z[u] = *reinterpret_cast<const uint32_t*>(src.s[u] + (int64_t)gr * R * 4 + (uint32_t)(lane & 15) * 4);
     } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) b.c[u][i] = *reinterpret_cast<const u32x4*>(src.w[u] + gr * 128 + 16 * i + src.w_off);
+      for (int i = 0; i < 2; ++i) b.c[u][i] = *reinterpret_cast<const u32x4*>(src.w[u] + gr * 128 + (int64_t)i * src.rb8 + src.w_off);
       b.z[u] = src.s[u][gr];
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) b.x[i] = *reinterpret_cast<const u32x4*>(src.x + gr * 256 + 16 * i + src.x_off);
+  for (int i = 0; i < 4; ++i)
+    b.x[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(src.x, src.x_off + 16 * i, gr * 256, 0));
+}
+
+// The codes' way through a wave's LDS, 16-byte words of rows of 64 (128) bytes.  Word c of
+// row r sits at c ^ (r / 4) (c ^ (r / 2)): the 16 rows that a quarter of the fragment read takes
+// are then in different banks.
+template <int FMT>
+constexpr int UNIT_LDS = FMT == FMT_Q4 ? 1024 : 2048;
+template <int FMT>
+__device__ __forceinline__ int word_at(int r, int c) {
+  if constexpr (FMT == FMT_Q4) return r * 64 + 16 * (c ^ ((r >> 2) & 3));
+  else return r * 128 + 16 * (c ^ ((r >> 1) & 7));
+}
+template <int NU, int FMT>
+__device__ __forceinline__ void store_codes(uint8_t* lds, const Group<NU, FMT>& b, int lane) {
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+    if constexpr (FMT == FMT_Q4) {
+      *reinterpret_cast<u32x4*>(lds + u * 1024 + word_at<FMT>(lane >> 2, lane & 3)) = b.c[u][0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<u32x4*>(lds + u * 2048 + word_at<FMT>(8 * i + (lane >> 3), lane & 7)) = b.c[u][i];
+    }
+  }
 }
 
 // Eight 4-bit codes -> a fragment register: bf16 128 + q, or fp16 q - 8.
@@ -348,7 +388,18 @@ __device__ __forceinline__ f32x4 mfma16(const u32x4 a, const u32x4 b, f32x4 c) {
 
 // acc[u] += the group's product: value i of lane (r, q) is token row 4 q + i, weight row r.
 template <int NU, int FMT, int DT>
-__device__ __forceinline__ void mul_group(const Group<NU, FMT>& b, f32x4 (&acc)[NU]) {
+__device__ __forceinline__ void mul_group(const Group<NU, FMT>& b, uint8_t* lds, int lane, f32x4 (&acc)[NU]) {
+  // one wave's LDS operations complete in order: the next group's store is behind these reads
+  __builtin_amdgcn_wave_barrier();
+  store_codes<NU, FMT>(lds, b, lane);
+  __builtin_amdgcn_wave_barrier();
+  u32x4 c[NU][Group<NU, FMT>::W];
+#pragma unroll
+  for (int u = 0; u < NU; ++u)
+#pragma unroll
+    for (int i = 0; i < Group<NU, FMT>::W; ++i)
+      c[u][i] = *reinterpret_cast<const u32x4*>(lds + u * UNIT_LDS<FMT> +
+                                                word_at<FMT>(lane & 15, Group<NU, FMT>::W * (lane >> 4) + i));
   f32x4 xs = {0.f, 0.f, 0.f, 0.f};
   if constexpr (FMT == FMT_Q4) {
     const uint32_t one = DT == USAF_BF16 ? 0x3F803F80u : 0x3C003C00u;
@@ -360,8 +411,8 @@ __device__ __forceinline__ void mul_group(const Group<NU, FMT>& b, f32x4 (&acc)[
     f32x4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (FMT == FMT_Q4) d = mfma16<DT>(b.x[i], frag4<DT>(b.c[u][0][i]), d);
-      else d = mfma16<DT>(b.x[i], frag8<DT>(b.c[u][i >> 1][2 * (i & 1)], b.c[u][i >> 1][2 * (i & 1) + 1]), d);
+      if constexpr (FMT == FMT_Q4) d = mfma16<DT>(b.x[i], frag4<DT>(c[u][0][i]), d);
+      else d = mfma16<DT>(b.x[i], frag8<DT>(c[u][i >> 1][2 * (i & 1)], c[u][i >> 1][2 * (i & 1) + 1]), d);
     }
     if constexpr (FMT == FMT_Q4) {
       const float s = f16_bits_to_f32((uint16_t)b.z[u]), z = f16_bits_to_f32((uint16_t)(b.z[u] >> 16));
@@ -376,18 +427,18 @@ __device__ __forceinline__ void mul_group(const Group<NU, FMT>& b, f32x4 (&acc)[
   }
 }
 
-// An item's tokens as rows of the operand.  Rows past the last repeat it; their results are not used.
+// An item's tokens as rows of the operand.  Rows past the last are not loaded and their results not used.
 struct Tokens {
   int count;   // rows in use
   int own[4];  // tokens of the lane's result rows 4 q + i
-  // Returns the token of the lane's operand row.
-  __device__ __forceinline__ int set(const Item& t, int lane) {
+  // Returns the lane's operand row's place in a buffer of tokens of `row` bytes.
+  __device__ __forceinline__ uint32_t set(const Item& t, int row, int lane) {
     const int r = lane & 15, left = __popc(t.tokens) - FR * t.b;
     count = left > FR ? FR : left;
     const int mine = nth_bit(t.tokens, FR * t.b + (r < count ? r : count - 1));
 #pragma unroll
     for (int i = 0; i < 4; ++i) own[i] = __shfl(mine, 4 * (lane >> 4) + i, 64);
-    return mine;
+    return r < count ? (uint32_t)(mine * row + 64 * (lane >> 4)) : NO_ROW;
   }
 };
 
@@ -400,10 +451,12 @@ struct Tokens {
 constexpr int GU_NU = 4, GU_WAVES = 4, GU_THREADS = 64 * GU_WAVES;  // 32 gate rows and their 32 up rows
 
 template <int DT, int FMT>
-__global__ __launch_bounds__(GU_THREADS, 3) void few_gate_up_kernel(const FewArgs g) {
-  __shared__ f32x4 s_red[2][GU_WAVES][GU_NU][64];
+__global__ __launch_bounds__(GU_THREADS, FMT == FMT_Q4 ? 4 : 3) void few_gate_up_kernel(const FewArgs g) {
+  __shared__ f32x4 red[GU_WAVES][GU_NU][64];
+  __shared__ __attribute__((aligned(16))) uint8_t s_codes[GU_WAVES][GU_NU * UNIT_LDS<FMT>];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
+  uint8_t* const codes = s_codes[wave];
   const int n_nt = g.I / 32, ng = g.H / 128;
   const int g0 = ng * wave / GU_WAVES, some = ng * (wave + 1) / GU_WAVES - g0;
   const int n = some > 0 ? some : 1;  // a wave without a group of its own multiplies one and adds nothing
@@ -413,25 +466,23 @@ __global__ __launch_bounds__(GU_THREADS, 3) void few_gate_up_kernel(const FewArg
   int at = blockIdx.x, gr = 0;  // the pair being loaded
   if (at >= work) return;       // block-uniform
   Source<GU_NU> src;
-  src.x = reinterpret_cast<const uint8_t*>(FMT == FMT_Q4 ? g.xp : g.x);
+  src.x = buffer_of(FMT == FMT_Q4 ? g.xp : g.x, g.T * g.H * 2);
   auto source = [&]() {
     const Item t = in.item(at / n_nt);
     const int n0 = at % n_nt * 32;
     src.template weights<FMT>(g.gu, g.gu_s, t.e, 2 * g.I, g.H, {n0, n0 + 16, g.I + n0, g.I + n0 + 16}, lane);
     Tokens tk;
-    src.x_off = (uint32_t)((tk.set(t, lane) * g.H + 32 * q) * 2);
+    src.x_off = tk.set(t, 2 * g.H, lane);
   };
   f32x4 acc[GU_NU];
-  int par = 0;
   auto finish = [&](int done) {
-    f32x4(&red)[GU_WAVES][GU_NU][64] = s_red[par];  // two in turn: one barrier an item
-    par ^= 1;
+    lds_barrier();  // the last item's sums have been read
 #pragma unroll
     for (int v = 0; v < GU_NU; ++v) red[wave][v][lane] = some > 0 ? acc[v] : f32x4{0.f, 0.f, 0.f, 0.f};
     lds_barrier();
     const Item t = in.item(done / n_nt);
     Tokens tk;
-    tk.set(t, lane);
+    tk.set(t, 2 * g.H, lane);
     // wave: columns n0 + 16 (wave % 2) + [0, 16), two of the lane's four rows
     const int v = wave & 1, j0 = wave & 2;
     const int col = frag_pos<FMT>(done % n_nt * 32 + 16 * v + r);
@@ -469,9 +520,9 @@ __global__ __launch_bounds__(GU_THREADS, 3) void few_gate_up_kernel(const FewArg
       gr = 0;
       source();
     }
-    load_group<GU_NU, FMT>(nxt, src, g0 + gr < ng ? g0 + gr : ng - 1);
+    load_group<GU_NU, FMT>(nxt, src, 2 * g.I, g0 + gr < ng ? g0 + gr : ng - 1, lane);
     __builtin_amdgcn_sched_barrier(0);
-    mul_group<GU_NU, FMT, DT>(cur, acc);
+    mul_group<GU_NU, FMT, DT>(cur, codes, lane, acc);
     __builtin_amdgcn_sched_barrier(0);
     if (now_gr == n - 1) {
       finish(now);
@@ -482,21 +533,24 @@ __global__ __launch_bounds__(GU_THREADS, 3) void few_gate_up_kernel(const FewArg
   };
   source();
   clear();
-  load_group<GU_NU, FMT>(a, src, g0 < ng ? g0 : ng - 1);
+  load_group<GU_NU, FMT>(a, src, 2 * g.I, g0 < ng ? g0 : ng - 1, lane);
   while (step(a, b) && step(b, a)) {
   }
 }
 
-constexpr int DN_WAVES = 8, DN_THREADS = 64 * DN_WAVES, DN_NU = 4, DN_COLS = 16 * DN_NU;
+constexpr int DN_WAVES = 4, DN_THREADS = 64 * DN_WAVES, DN_NU = 4, DN_COLS = 16 * DN_NU;
 
 template <int DT, int FMT>
 __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
-  extern __shared__ __attribute__((aligned(16))) float s_sum[];  // [waves][T][64]
-  int* const s_last = reinterpret_cast<int*>(s_sum);             // once the sums have been read
+  // the waves' codes, and their sums [waves][T][64]: 64 KiB at most (32 tokens, 8-bit)
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_down[];
+  float* const s_sum = reinterpret_cast<float*>(s_down + DN_WAVES * DN_NU * UNIT_LDS<FMT>);
+  int* const s_last = reinterpret_cast<int*>(s_down);  // once the codes have been read
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int nt = blockIdx.x / g.P, p = blockIdx.x - nt * g.P, n0 = DN_COLS * nt;
   float* const sum = s_sum + wave * g.T * DN_COLS;  // the wave's own: its LDS operations complete in order
+  uint8_t* const codes = s_down + wave * DN_NU * UNIT_LDS<FMT>;
   for (int i = lane; i < g.T * DN_COLS / 4; i += 64) reinterpret_cast<f32x4*>(sum)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   InUse in;
   in.load(g.mask, lane);
@@ -512,8 +566,8 @@ __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
     auto source = [&]() {
       const Item t = in.item(it);
       src.template weights<FMT>(g.dn, g.dn_s, t.e, g.H, g.I, {n0, n0 + 16, n0 + 32, n0 + 48}, lane);
-      src.x = reinterpret_cast<const uint8_t*>(g.act + (int64_t)t.u * g.T * g.I);
-      src.x_off = (uint32_t)((next_tk.set(t, lane) * g.I + 32 * q) * 2);
+      src.x = buffer_of(g.act + (int64_t)t.u * g.T * g.I, g.T * g.I * 2);
+      src.x_off = next_tk.set(t, 2 * g.I, lane);
 #pragma unroll
       for (int i = 0; i < 4; ++i) next_wt[i] = g.wt[t.e * FT + next_tk.own[i]];
     };
@@ -537,9 +591,9 @@ __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
           ends = false;
         }
       }
-      load_group<DN_NU, FMT>(nxt, src, gr);
+      load_group<DN_NU, FMT>(nxt, src, g.H, gr, lane);
       __builtin_amdgcn_sched_barrier(0);
-      mul_group<DN_NU, FMT, DT>(cur, y);
+      mul_group<DN_NU, FMT, DT>(cur, codes, lane, y);
       __builtin_amdgcn_sched_barrier(0);
       if (ends) {
 #pragma unroll
@@ -558,23 +612,32 @@ __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
     };
     source();
     begin();
-    load_group<DN_NU, FMT>(a, src, gr);
+    load_group<DN_NU, FMT>(a, src, g.H, gr, lane);
     while (step(a, b) && step(b, a)) {
     }
   }
   __syncthreads();
-  for (int i = tid; i < g.T * DN_COLS; i += DN_THREADS) {
-    const int t = i / DN_COLS;
-    const int64_t at = (int64_t)t * g.H + n0 + i % DN_COLS;
-    float v = s_sum[i];
+  // four columns of a token at a time
+  const int quads = g.T * (DN_COLS / 4);
+  const Buffer part_buf = buffer_of(g.part + (int64_t)p * g.T * g.H, g.T * g.H * 4);
+  auto place = [&](int i) { return (i / (DN_COLS / 4)) * g.H + n0 + i % (DN_COLS / 4) * 4; };
+  auto store_out = [&](int at, f32x4 v) {
+    *reinterpret_cast<uint2*>(g.out + at) = uint2{pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
+  };
+  for (int i = tid; i < quads; i += DN_THREADS) {
+    f32x4 v = reinterpret_cast<const f32x4*>(s_sum)[i];
 #pragma unroll
-    for (int j = 1; j < DN_WAVES; ++j) v += s_sum[j * g.T * DN_COLS + i];
-    if (g.P == 1) store_from_f32<DT>(g.out, at, v);
-    else __hip_atomic_store(&g.part[(int64_t)p * g.T * g.H + at], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int j = 1; j < DN_WAVES; ++j) {
+      const f32x4 o = reinterpret_cast<const f32x4*>(s_sum)[j * quads + i];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] += o[c];
+    }
+    if (g.P == 1) store_out(place(i), v);
+    else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part_buf, place(i) * 4, 0, DEVICE_SCOPE);
   }
   if (g.P == 1) return;
   // The parts of a column tile meet at the device's coherence point: stored and loaded at
-  // agent scope, which passes the dies' L2s, and counted behind a wait for the stores.  The
+  // device scope, which passes the dies' L2s, and counted behind a wait for the stores.  The
   // last block adds them in order, so the sum does not hang on who came last; no block waits for another.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
@@ -582,12 +645,22 @@ __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
     *s_last = __hip_atomic_fetch_add(&g.done[nt], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == g.P - 1;
   __syncthreads();
   if (!*s_last) return;
-  for (int i = tid; i < g.T * DN_COLS; i += DN_THREADS) {
-    const int64_t at = (int64_t)(i / DN_COLS) * g.H + n0 + i % DN_COLS;
-    float o = 0.f;
-    for (int j = 0; j < g.P; ++j)
-      o += __hip_atomic_load(&g.part[(int64_t)j * g.T * g.H + at], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    store_from_f32<DT>(g.out, at, o);
+  const Buffer all = buffer_of(g.part, g.P * g.T * g.H * 4);
+  for (int i = tid; i < quads; i += DN_THREADS) {
+    const int at = place(i);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < g.P; j += 4) {
+      f32x4 v[4];  // parts past the last read as zeros
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        v[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(all, (uint32_t)(((j + k) * g.T * g.H + at) * 4),
+                                                                               0, DEVICE_SCOPE));
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] += v[k][c];
+    }
+    store_out(at, o);
   }
 }
 
@@ -600,9 +673,9 @@ struct FewPlan {
 FewPlan few_plan(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
   FewPlan p;
   p.in_use = E < T * k ? E : T * k;
-  // a block a CU for the column tiles together, and about four pairs a wave at least
+  // two blocks a CU for the column tiles together, and about four pairs a wave at least
   const int64_t tiles = H / DN_COLS, cus = device_cu_count(), pairs = p.in_use * (I / 128);
-  int64_t parts = cus / tiles, most = pairs / (4 * DN_WAVES);
+  int64_t parts = 2 * cus / tiles, most = pairs / (4 * DN_WAVES);
   parts = parts > most ? most : parts;
   p.P = (int)(parts < 1 ? 1 : parts);
   int64_t at = 0;
@@ -630,7 +703,8 @@ int launch_few_layer(const FewArgs& g, int64_t in_use, hipStream_t st) {
   few_gate_up_kernel<DT, FMT><<<(unsigned)(work < most ? work : most), GU_THREADS, 0, st>>>(g);
   if (int rc = check_launch("moe_few/gate_up")) return rc;
   few_down_kernel<DT, FMT>
-      <<<(unsigned)(g.H / DN_COLS * g.P), DN_THREADS, (size_t)DN_WAVES * g.T * DN_COLS * 4, st>>>(g);
+      <<<(unsigned)(g.H / DN_COLS * g.P), DN_THREADS,
+         (size_t)DN_WAVES * (DN_NU * UNIT_LDS<FMT> + g.T * DN_COLS * 4), st>>>(g);
   return check_launch("moe_few/down");
 }
 
@@ -665,8 +739,8 @@ extern "C" int usaf_hip_moe_few(const void* x, int64_t T, int64_t H, const void*
     return set_error(USAF_ERR_INVALID, "moe_few: null pointer");
   if (((uintptr_t)x | (uintptr_t)router | (uintptr_t)gate_up | (uintptr_t)down | (uintptr_t)ws) % 16)
     return set_error(USAF_ERR_INVALID, "moe_few: activations, router, codes and workspace must be 16-byte aligned");
-  if ((!eight_bit && ((uintptr_t)gate_up_scale | (uintptr_t)down_scale) % 4) || (uintptr_t)out % 2)
-    return set_error(USAF_ERR_INVALID, "moe_few: misaligned scales or output");
+  if ((!eight_bit && ((uintptr_t)gate_up_scale | (uintptr_t)down_scale) % 4) || (uintptr_t)out % 8)
+    return set_error(USAF_ERR_INVALID, "moe_few: misaligned scales or output (8 bytes)");
   const FewPlan p = few_plan(T, E, top_k, H, I);
   if (ws_bytes < p.bytes)
     return set_error(USAF_ERR_INVALID, "moe_few: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)p.bytes);

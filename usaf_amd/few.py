@@ -70,7 +70,7 @@ def few_token_block(hs: torch.Tensor, router_weight: torch.Tensor, top_k: int, n
     if tokens == 0:
         return out
     with on(dev):
-        gu_s, dn_s = (gu.s, dn.s) if experts.is_fp8 else (gu.scale_zero(), dn.scale_zero())
+        gu_s, dn_s = (gu.s, dn.s) if experts.is_fp8 else (gu.scale_zero_by_group(), dn.scale_zero_by_group())
         ws = torch.empty(N.load().usaf_hip_moe_few_ws_bytes(tokens, E, top_k, H, I), dtype=torch.uint8, device=dev)
         N.call("usaf_hip_moe_few", x.data_ptr(), tokens, H, router.data_ptr(), E, top_k, 1 if norm_topk_prob else 0,
                N.dtype_code(dt), I, 1 if experts.is_fp8 else 0, gu.q.data_ptr(), gu_s.data_ptr(), dn.q.data_ptr(),

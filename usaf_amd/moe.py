@@ -34,6 +34,7 @@ class Q4Tensor:
     group_size: int = 128
     _sz: Optional[torch.Tensor] = field(default=None, repr=False, compare=False)
     _t: Optional[Tuple[torch.Tensor, torch.Tensor]] = field(default=None, repr=False, compare=False)
+    _szg: Optional[torch.Tensor] = field(default=None, repr=False, compare=False)
 
     @classmethod
     def from_entry(cls, entry: Any, device=None, group_size: int = 128) -> "Q4Tensor":
@@ -86,6 +87,14 @@ class Q4Tensor:
                    N.stream_ptr(self.q.device))
             self._sz = sz
         return self._sz
+
+    def scale_zero_by_group(self) -> torch.Tensor:
+        """scale_zero() of [E, R, C] as int32 [E, C / 128, R]: neighbouring rows' words side by
+        side, as the few-token layer reads them (built once, on the tensor's device)."""
+        if self._szg is None or self._szg.device != self.q.device:
+            E, rows, cols = (int(d) for d in self.shape)
+            self._szg = self.scale_zero().view(E, rows, cols // 128).transpose(1, 2).contiguous()
+        return self._szg
 
     def transposed(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """(codes int8 [E, cols, rows/2], scale/zero int32 [E, cols/128, rows/2, 2]):
