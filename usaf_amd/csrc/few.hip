@@ -182,17 +182,20 @@ __global__ __launch_bounds__(1024) void few_route_kernel(const FewArgs g) {
 // ---- products --------------------------------------------------------------------
 
 // Place of the n-th set bit.
-__device__ __forceinline__ int nth_bit(uint64_t m, int n) {
+__device__ __forceinline__ int nth_bit(uint32_t m, int n) {
   int at = 0;
 #pragma unroll
-  for (int w = 32; w > 0; w >>= 1) {
-    const int c = __popcll((m >> at) & ((1ull << w) - 1));
-    if (n >= c) {
-      n -= c;
-      at += w;
-    }
+  for (int w = 16; w > 0; w >>= 1) {
+    const int c = __popc((m >> at) & ((1u << w) - 1));
+    const bool past = n >= c;
+    n -= past ? c : 0;
+    at += past ? w : 0;
   }
   return at;
+}
+__device__ __forceinline__ int nth_bit(uint64_t m, int n) {
+  const int low = __popc((uint32_t)m);
+  return n < low ? nth_bit((uint32_t)m, n) : 32 + nth_bit((uint32_t)(m >> 32), n - low);
 }
 
 // An expert and up to 16 of its tokens: what one pass over its weights multiplies.
@@ -343,22 +346,27 @@ __device__ __forceinline__ void store_codes(uint8_t* lds, const Group<NU, FMT>& 
   }
 }
 
-// Eight 4-bit codes -> a fragment register: bf16 128 + q, or fp16 q - 8.
+// Eight 4-bit codes -> a fragment register: bf16 128 + q, or fp16 q - 8.  The constants
+// sit in registers, which makes one v_and_or of the two operations (GFX9 takes no literal there).
 template <int DT>
-__device__ __forceinline__ u32x4 frag4(uint32_t w) {
-  u32x4 o;
+struct Nibbles {
+  uint32_t keep = 0x000F000Fu, top = DT == USAF_BF16 ? 0x43004300u : 0x64006400u;
+  __device__ __forceinline__ Nibbles() { asm("" : "+s"(keep), "+v"(top)); }
+  __device__ __forceinline__ u32x4 frag(uint32_t w) const {
+    u32x4 o;
 #pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    const uint32_t t = (w >> (4 * p)) & 0x000F000Fu;
-    if constexpr (DT == USAF_BF16) {
-      o[p] = t | 0x43004300u;
-    } else {
-      const f16x2 c = {(f16)-1032.0f, (f16)-1032.0f};
-      o[p] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, t | 0x64006400u) + c);
+    for (int p = 0; p < 4; ++p) {
+      const uint32_t t = ((w >> (4 * p)) & keep) | top;
+      if constexpr (DT == USAF_BF16) {
+        o[p] = t;
+      } else {
+        const f16x2 c = {(f16)-1032.0f, (f16)-1032.0f};
+        o[p] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, t) + c);
+      }
     }
+    return o;
   }
-  return o;
-}
+};
 // Eight 8-bit codes -> a fragment register (exact in both types).
 template <int DT>
 __device__ __forceinline__ u32x4 frag8(uint32_t a, uint32_t b) {
@@ -388,7 +396,8 @@ __device__ __forceinline__ f32x4 mfma16(const u32x4 a, const u32x4 b, f32x4 c) {
 
 // acc[u] += the group's product: value i of lane (r, q) is token row 4 q + i, weight row r.
 template <int NU, int FMT, int DT>
-__device__ __forceinline__ void mul_group(const Group<NU, FMT>& b, uint8_t* lds, int lane, f32x4 (&acc)[NU]) {
+__device__ __forceinline__ void mul_group(const Group<NU, FMT>& b, uint8_t* lds, int lane, const Nibbles<DT>& nib,
+                                          f32x4 (&acc)[NU]) {
   // one wave's LDS operations complete in order: the next group's store is behind these reads
   __builtin_amdgcn_wave_barrier();
   store_codes<NU, FMT>(lds, b, lane);
@@ -411,7 +420,7 @@ __device__ __forceinline__ void mul_group(const Group<NU, FMT>& b, uint8_t* lds,
     f32x4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (FMT == FMT_Q4) d = mfma16<DT>(b.x[i], frag4<DT>(c[u][0][i]), d);
+      if constexpr (FMT == FMT_Q4) d = mfma16<DT>(b.x[i], nib.frag(c[u][0][i]), d);
       else d = mfma16<DT>(b.x[i], frag8<DT>(c[u][i >> 1][2 * (i & 1)], c[u][i >> 1][2 * (i & 1) + 1]), d);
     }
     if constexpr (FMT == FMT_Q4) {
@@ -474,6 +483,7 @@ __global__ __launch_bounds__(GU_THREADS, FMT == FMT_Q4 ? 4 : 3) void few_gate_up
     Tokens tk;
     src.x_off = tk.set(t, 2 * g.H, lane);
   };
+  const Nibbles<DT> nib;
   f32x4 acc[GU_NU];
   auto finish = [&](int done) {
     lds_barrier();  // the last item's sums have been read
@@ -522,7 +532,7 @@ __global__ __launch_bounds__(GU_THREADS, FMT == FMT_Q4 ? 4 : 3) void few_gate_up
     }
     load_group<GU_NU, FMT>(nxt, src, 2 * g.I, g0 + gr < ng ? g0 + gr : ng - 1, lane);
     __builtin_amdgcn_sched_barrier(0);
-    mul_group<GU_NU, FMT, DT>(cur, codes, lane, acc);
+    mul_group<GU_NU, FMT, DT>(cur, codes, lane, nib, acc);
     __builtin_amdgcn_sched_barrier(0);
     if (now_gr == n - 1) {
       finish(now);
@@ -571,6 +581,7 @@ __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) next_wt[i] = g.wt[t.e * FT + next_tk.own[i]];
     };
+    const Nibbles<DT> nib;
     f32x4 y[DN_NU];
     auto begin = [&]() {
       tk = next_tk;
@@ -593,7 +604,7 @@ __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
       }
       load_group<DN_NU, FMT>(nxt, src, g.H, gr, lane);
       __builtin_amdgcn_sched_barrier(0);
-      mul_group<DN_NU, FMT, DT>(cur, codes, lane, y);
+      mul_group<DN_NU, FMT, DT>(cur, codes, lane, nib, y);
       __builtin_amdgcn_sched_barrier(0);
       if (ends) {
 #pragma unroll
