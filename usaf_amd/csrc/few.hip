@@ -249,24 +249,28 @@ struct InUse {
   }
 };
 
-// A wave's operands of one group of 128: NU units of 16 weight rows, and the tokens.
+// A wave multiplies in steps: 128 bytes of each of its weight rows, two groups of 4-bit
+// codes or one of 8-bit ones, by units of 16 rows.  As soon as the codes of a step have left
+// their registers for LDS, those of the next step are loaded there: a wave has a whole step's
+// weights in flight behind its arithmetic.
 //
-// The codes come from memory as they lie there, neighbouring lanes at neighbouring 16
-// bytes, and reach the fragments through LDS: loaded straight into fragments (lanes 0
-// to 15 in 16 rows) each lane's 16 bytes are an access of their own to the address unit,
-// 48 a load on average by its counters, which bound gate_up of 24 tokens at 55 us.
-template <int NU, int FMT>
-struct Group {
-  static constexpr int W = FMT == FMT_Q4 ? 1 : 2;  // 16-byte words of a lane and unit
-  u32x4 c[NU][W];  // codes: 4-bit, lane l has word l % 4 of row l / 4; 8-bit, word l % 8 of rows l / 8 and 8 + l / 8
-  uint32_t z[NU];  // scale | zero of row l % 16, or the E8M0 byte
-  u32x4 x[4];      // tokens: lane (r, q), register j: k = 32 q + 8 j + [0, 8) of token row r
-};
+// The codes come as they lie in memory, neighbouring lanes at neighbouring 16 bytes, whole
+// 128-byte lines, and reach the fragments through LDS.  Loaded straight into fragments
+// (lanes 0 to 15 in 16 rows) each lane's 16 bytes are an access of their own to the address
+// unit, 48 a load, and steps of half a line ask the memory for 64 bytes at a time: gate_up of
+// 24 tokens took 55 us, and 41 with the first of the two mended.
+template <int FMT>
+constexpr int STEP = FMT == FMT_Q4 ? 2 : 1;  // groups
+constexpr int UNIT_LDS = 2048;
 
 template <int FMT>
-__device__ __forceinline__ int64_t row_bytes(int K) {
-  return FMT == FMT_Q4 ? K / 2 : K;
-}
+struct Unit {
+  u32x4 c[2];             // codes: lane l has word l % 8 of rows l / 8 and 8 + l / 8
+  uint32_t z[STEP<FMT>];  // scale | zero of row l % 16, or the E8M0 byte
+};
+struct Values {           // tokens, one group: lane (r, q), register j: k = 32 q + 8 j + [0, 8) of token row r
+  u32x4 x[4];
+};
 
 typedef __amdgpu_buffer_rsrc_t Buffer;
 // Loads past `bytes` give zeros and touch no memory: what lanes of unused token rows do.
@@ -276,75 +280,71 @@ __device__ __forceinline__ Buffer buffer_of(const void* p, int bytes) {
 constexpr uint32_t NO_ROW = 0x80000000u;  // past any buffer here
 constexpr int DEVICE_SCOPE = 16;          // sc1 of a buffer instruction
 
-// Where a wave's operands come from: for each unit the first weight row's codes and scales,
-// wave-uniform, and the tokens; the lane's place in them as byte offsets.
+// Where a wave's operands of a step come from: for each unit the first weight row's codes
+// and scales, wave-uniform, and the tokens; the lane's place in them as byte offsets.
 template <int NU>
 struct Source {
   const uint8_t* w[NU];
   const uint8_t* s[NU];
   Buffer x;
-  uint32_t w_off, x_off;
-  int rb8;  // bytes of 8 weight rows
+  uint32_t x_off;
 
   // Units of rows row[v] + [0, 16) of expert e's [R, K] matrix.  Scales: 4-bit [E, K / 128, R]
   // words, 8-bit [E, ceil(R / 128), K / 128] bytes.
   template <int FMT>
   __device__ __forceinline__ void weights(const uint8_t* codes, const void* scales, int e, int R, int K,
-                                          const int (&row)[NU], int lane) {
+                                          const int (&row)[NU]) {
     const int ng = K / 128;
-    const int64_t rb = row_bytes<FMT>(K);
+    const int64_t rb = FMT == FMT_Q4 ? K / 2 : K;
 #pragma unroll
     for (int v = 0; v < NU; ++v) {
       w[v] = codes + ((int64_t)e * R + row[v]) * rb;
       if constexpr (FMT == FMT_Q4) s[v] = reinterpret_cast<const uint8_t*>(scales) + ((int64_t)e * ng * R + row[v]) * 4;
       else s[v] = reinterpret_cast<const uint8_t*>(scales) + ((int64_t)e * ((R + 127) / 128) + row[v] / 128) * ng;
     }
-    w_off = FMT == FMT_Q4 ? (uint32_t)((lane >> 2) * rb + 16 * (lane & 3)) : (uint32_t)((lane >> 3) * rb + 16 * (lane & 7));
-    rb8 = (int)(8 * rb);
+  }
+};
+
+// The lane's place in a step of a unit, as byte offsets (R rows of K).
+template <int FMT>
+struct Place {
+  uint32_t whole, last;  // codes; of a row's last group alone (4-bit, an odd number of groups): its words twice
+  uint32_t z;
+  int64_t rows8;         // bytes of 8 rows
+  int ng, R;
+  __device__ __forceinline__ Place(int R_, int K, int lane) : ng(K / 128), R(R_) {
+    const int rb = FMT == FMT_Q4 ? K / 2 : K;
+    whole = (uint32_t)((lane >> 3) * rb + 16 * (lane & 7));
+    last = (uint32_t)((lane >> 3) * rb + 16 * (lane & 3));
+    z = 4 * (lane & 15);
+    rows8 = 8 * rb;
   }
 };
 
 template <int NU, int FMT>
-__device__ __forceinline__ void load_group(Group<NU, FMT>& b, const Source<NU>& src, int R, int gr, int lane) {
+__device__ __forceinline__ void load_unit(Unit<FMT>& b, const Source<NU>& src, const Place<FMT>& at, int u, int gr) {
+  const bool alone = FMT == FMT_Q4 && gr + 1 == at.ng;
+  const uint8_t* const w = src.w[u] + (FMT == FMT_Q4 ? 64 : 128) * gr;
+  const uint32_t off = alone ? at.last : at.whole;
 #pragma unroll
-  for (int u = 0; u < NU; ++u) {
-    if constexpr (FMT == FMT_Q4) {
-      b.c[u][0] = *reinterpret_cast<const u32x4*>(src.w[u] + gr * 64 + src.w_off);
-      b.z[u] = *reinterpret_cast<const uint32_t*>(src.s[u] + (int64_t)gr * R * 4 + (uint32_t)(lane & 15) * 4);
-    } else {
+  for (int i = 0; i < 2; ++i) b.c[i] = *reinterpret_cast<const u32x4*>(w + i * at.rows8 + off);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) b.c[u][i] = *reinterpret_cast<const u32x4*>(src.w[u] + gr * 128 + (int64_t)i * src.rb8 + src.w_off);
-      b.z[u] = src.s[u][gr];
-    }
+  for (int h = 0; h < STEP<FMT>; ++h) {
+    if constexpr (FMT == FMT_Q4)
+      b.z[h] = *reinterpret_cast<const uint32_t*>(src.s[u] + (int64_t)(alone ? gr : gr + h) * at.R * 4 + at.z);
+    else b.z[h] = src.s[u][gr];
   }
+}
+template <int NU>
+__device__ __forceinline__ void load_values(Values& b, const Source<NU>& src, int gr) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     b.x[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(src.x, src.x_off + 16 * i, gr * 256, 0));
 }
 
-// The codes' way through a wave's LDS, 16-byte words of rows of 64 (128) bytes.  Word c of
-// row r sits at c ^ (r / 4) (c ^ (r / 2)): the 16 rows that a quarter of the fragment read takes
-// are then in different banks.
-template <int FMT>
-constexpr int UNIT_LDS = FMT == FMT_Q4 ? 1024 : 2048;
-template <int FMT>
-__device__ __forceinline__ int word_at(int r, int c) {
-  if constexpr (FMT == FMT_Q4) return r * 64 + 16 * (c ^ ((r >> 2) & 3));
-  else return r * 128 + 16 * (c ^ ((r >> 1) & 7));
-}
-template <int NU, int FMT>
-__device__ __forceinline__ void store_codes(uint8_t* lds, const Group<NU, FMT>& b, int lane) {
-#pragma unroll
-  for (int u = 0; u < NU; ++u) {
-    if constexpr (FMT == FMT_Q4) {
-      *reinterpret_cast<u32x4*>(lds + u * 1024 + word_at<FMT>(lane >> 2, lane & 3)) = b.c[u][0];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<u32x4*>(lds + u * 2048 + word_at<FMT>(8 * i + (lane >> 3), lane & 7)) = b.c[u][i];
-    }
-  }
-}
+// The codes' way through a wave's LDS: 16 rows of 128 bytes, 16-byte word c of row r at
+// c ^ (r / 2), so that the 16 rows which a quarter of the fragment read takes are in different banks.
+__device__ __forceinline__ int word_at(int r, int c) { return r * 128 + 16 * (c ^ ((r >> 1) & 7)); }
 
 // Eight 4-bit codes -> a fragment register: bf16 128 + q, or fp16 q - 8.  The constants
 // sit in registers, which makes one v_and_or of the two operations (GFX9 takes no literal there).
@@ -394,46 +394,72 @@ __device__ __forceinline__ f32x4 mfma16(const u32x4 a, const u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// acc[u] += the group's product: value i of lane (r, q) is token row 4 q + i, weight row r.
+// One step of NU units: acc[u] += the product of their rows and the tokens; value i of
+// lane (r, q) is token row 4 q + i, weight row r.  Meanwhile b's weights are loaded from src,
+// groups gr on, and the tokens' values there: 4-bit, v0 and v1 are a step's two groups (`two`:
+// it has the second), each loaded behind its last use; 8-bit, v0 is this step's and v1 the
+// next one's.  No load carries a condition, or the compiler would have to wait for all of them at every use.
 template <int NU, int FMT, int DT>
-__device__ __forceinline__ void mul_group(const Group<NU, FMT>& b, uint8_t* lds, int lane, const Nibbles<DT>& nib,
-                                          f32x4 (&acc)[NU]) {
-  // one wave's LDS operations complete in order: the next group's store is behind these reads
-  __builtin_amdgcn_wave_barrier();
-  store_codes<NU, FMT>(lds, b, lane);
-  __builtin_amdgcn_wave_barrier();
-  u32x4 c[NU][Group<NU, FMT>::W];
-#pragma unroll
-  for (int u = 0; u < NU; ++u)
-#pragma unroll
-    for (int i = 0; i < Group<NU, FMT>::W; ++i)
-      c[u][i] = *reinterpret_cast<const u32x4*>(lds + u * UNIT_LDS<FMT> +
-                                                word_at<FMT>(lane & 15, Group<NU, FMT>::W * (lane >> 4) + i));
-  f32x4 xs = {0.f, 0.f, 0.f, 0.f};
-  if constexpr (FMT == FMT_Q4) {
-    const uint32_t one = DT == USAF_BF16 ? 0x3F803F80u : 0x3C003C00u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) xs = mfma16<DT>(b.x[i], u32x4{one, one, one, one}, xs);
-  }
+__device__ __forceinline__ void mul_step(Unit<FMT> (&b)[NU], Values& v0, Values& v1, bool two, const Source<NU>& src,
+                                         const Place<FMT>& at, int gr, uint8_t* lds, int lane, const Nibbles<DT>& nib,
+                                         f32x4 (&acc)[NU]) {
+  const int r = lane & 15, q = lane >> 4;
+  uint32_t z[NU][STEP<FMT>];
+  __builtin_amdgcn_wave_barrier();  // one wave's LDS operations complete in order
 #pragma unroll
   for (int u = 0; u < NU; ++u) {
-    f32x4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (FMT == FMT_Q4) d = mfma16<DT>(b.x[i], nib.frag(c[u][0][i]), d);
-      else d = mfma16<DT>(b.x[i], frag8<DT>(c[u][i >> 1][2 * (i & 1)], c[u][i >> 1][2 * (i & 1) + 1]), d);
-    }
-    if constexpr (FMT == FMT_Q4) {
-      const float s = f16_bits_to_f32((uint16_t)b.z[u]), z = f16_bits_to_f32((uint16_t)(b.z[u] >> 16));
-      const float zo = DT == USAF_BF16 ? fmaf(-128.0f, s, z) : fmaf(8.0f, s, z);
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<u32x4*>(lds + u * UNIT_LDS + word_at(8 * i + (lane >> 3), lane & 7)) = b[u].c[i];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[u][i] = fmaf(zo, xs[i], fmaf(s, d[i], acc[u][i]));
-    } else {
-      const float s = __uint_as_float(b.z[u] == 0 ? 0x00400000u : b.z[u] << 23);
+    for (int h = 0; h < STEP<FMT>; ++h) z[u][h] = b[u].z[h];
+  }
+  __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[u][i] = fmaf(s, d[i], acc[u][i]);
+  for (int u = 0; u < NU; ++u) load_unit<NU, FMT>(b[u], src, at, u, gr);
+  if constexpr (FMT == FMT_FP8) load_values<NU>(v1, src, gr);
+  __builtin_amdgcn_sched_barrier(0);
+  auto word = [&](int u, int c) { return *reinterpret_cast<const u32x4*>(lds + u * UNIT_LDS + word_at(r, c)); };
+  if constexpr (FMT == FMT_Q4) {
+    const uint32_t one = DT == USAF_BF16 ? 0x3F803F80u : 0x3C003C00u;
+    auto group = [&](int h, const Values& v) {
+      f32x4 xs = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xs = mfma16<DT>(v.x[i], u32x4{one, one, one, one}, xs);
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const u32x4 c = word(u, 4 * h + q);
+        f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d = mfma16<DT>(v.x[i], nib.frag(c[i]), d);
+        const float sc = f16_bits_to_f32((uint16_t)z[u][h]);
+        const float zo = fmaf(DT == USAF_BF16 ? -128.0f : 8.0f, sc, f16_bits_to_f32((uint16_t)(z[u][h] >> 16)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[u][i] = fmaf(zo, xs[i], fmaf(sc, d[i], acc[u][i]));
+      }
+    };
+    group(0, v0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_values<NU>(v0, src, gr);
+    __builtin_amdgcn_sched_barrier(0);
+    if (two) group(1, v1);
+    __builtin_amdgcn_sched_barrier(0);
+    load_values<NU>(v1, src, gr + 1);
+  } else {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const u32x4 c0 = word(u, 2 * q), c1 = word(u, 2 * q + 1);
+      f32x4 d = {0.f, 0.f, 0.f, 0.f};
+      d = mfma16<DT>(v0.x[0], frag8<DT>(c0.x, c0.y), d);
+      d = mfma16<DT>(v0.x[1], frag8<DT>(c0.z, c0.w), d);
+      d = mfma16<DT>(v0.x[2], frag8<DT>(c1.x, c1.y), d);
+      d = mfma16<DT>(v0.x[3], frag8<DT>(c1.z, c1.w), d);
+      const float sc = __uint_as_float(z[u][0] == 0 ? 0x00400000u : z[u][0] << 23);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[u][i] = fmaf(sc, d[i], acc[u][i]);
     }
   }
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // An item's tokens as rows of the operand.  Rows past the last are not loaded and their results not used.
@@ -451,35 +477,34 @@ struct Tokens {
   }
 };
 
-// Both products walk a list of (item, group) pairs with the next pair's loads in flight
-// behind the present one's arithmetic, across the items' ends: a wave has only four to
-// sixteen groups of an item, and a first load takes as long as three groups' arithmetic.
-// The loads carry no condition (the last pair is loaded once more), or the compiler
-// would have to wait for all of them at every use.
+// Both products walk a list of (item, step) pairs, across the items' ends: a wave has only
+// one to eight steps of an item, and a first load takes as long as several steps' arithmetic.
+// The last pair's weights are loaded once more.
 
 constexpr int GU_NU = 4, GU_WAVES = 4, GU_THREADS = 64 * GU_WAVES;  // 32 gate rows and their 32 up rows
 
 template <int DT, int FMT>
-__global__ __launch_bounds__(GU_THREADS, FMT == FMT_Q4 ? 4 : 3) void few_gate_up_kernel(const FewArgs g) {
+__global__ __launch_bounds__(GU_THREADS, 3) void few_gate_up_kernel(const FewArgs g) {
   __shared__ f32x4 red[GU_WAVES][GU_NU][64];
-  __shared__ __attribute__((aligned(16))) uint8_t s_codes[GU_WAVES][GU_NU * UNIT_LDS<FMT>];
+  __shared__ __attribute__((aligned(16))) uint8_t s_codes[GU_WAVES][GU_NU * UNIT_LDS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
-  uint8_t* const codes = s_codes[wave];
-  const int n_nt = g.I / 32, ng = g.H / 128;
-  const int g0 = ng * wave / GU_WAVES, some = ng * (wave + 1) / GU_WAVES - g0;
-  const int n = some > 0 ? some : 1;  // a wave without a group of its own multiplies one and adds nothing
+  const int n_nt = g.I / 32, ng = g.H / 128, ns = (ng + STEP<FMT> - 1) / STEP<FMT>;
+  const int s0 = ns * wave / GU_WAVES, some = ns * (wave + 1) / GU_WAVES - s0;  // the wave's steps
+  const int n = some > 0 ? some : 1;  // a wave without a step of its own multiplies one and adds nothing
+  const int first = STEP<FMT> * (s0 < ns ? s0 : ns - 1);
   InUse in;
   in.load(g.mask, lane);
   const int work = in.items * n_nt;
-  int at = blockIdx.x, gr = 0;  // the pair being loaded
+  int at = blockIdx.x, st = 0;  // the pair being loaded
   if (at >= work) return;       // block-uniform
+  const Place<FMT> place(2 * g.I, g.H, lane);
   Source<GU_NU> src;
   src.x = buffer_of(FMT == FMT_Q4 ? g.xp : g.x, g.T * g.H * 2);
   auto source = [&]() {
     const Item t = in.item(at / n_nt);
     const int n0 = at % n_nt * 32;
-    src.template weights<FMT>(g.gu, g.gu_s, t.e, 2 * g.I, g.H, {n0, n0 + 16, g.I + n0, g.I + n0 + 16}, lane);
+    src.template weights<FMT>(g.gu, g.gu_s, t.e, 2 * g.I, g.H, {n0, n0 + 16, g.I + n0, g.I + n0 + 16});
     Tokens tk;
     src.x_off = tk.set(t, 2 * g.H, lane);
   };
@@ -518,33 +543,38 @@ __global__ __launch_bounds__(GU_THREADS, FMT == FMT_Q4 ? 4 : 3) void few_gate_up
 #pragma unroll
     for (int v = 0; v < GU_NU; ++v) acc[v] = f32x4{0.f, 0.f, 0.f, 0.f};
   };
-  Group<GU_NU, FMT> a, b;
-  int now = at, now_gr = 0;  // the pair being multiplied
-  auto step = [&](const Group<GU_NU, FMT>& cur, Group<GU_NU, FMT>& nxt) {  // false: the last pair is done
-    now = at;
-    now_gr = gr;
-    if (gr + 1 < n) {
-      ++gr;
+  Unit<FMT> weights[GU_NU];
+  Values v0, v1;
+  auto step = [&](Values& v0, Values& v1) {  // false: it was the last
+    const int done = at, gr = first + STEP<FMT> * st;  // the pair being multiplied
+    const bool ends = st == n - 1;
+    if (!ends) {
+      ++st;
     } else if (at + (int)gridDim.x < work) {
       at += gridDim.x;
-      gr = 0;
+      st = 0;
       source();
     }
-    load_group<GU_NU, FMT>(nxt, src, 2 * g.I, g0 + gr < ng ? g0 + gr : ng - 1, lane);
-    __builtin_amdgcn_sched_barrier(0);
-    mul_group<GU_NU, FMT, DT>(cur, codes, lane, nib, acc);
-    __builtin_amdgcn_sched_barrier(0);
-    if (now_gr == n - 1) {
-      finish(now);
+    mul_step<GU_NU, FMT, DT>(weights, v0, v1, gr + 1 < ng, src, place, first + STEP<FMT> * st, s_codes[wave], lane, nib, acc);
+    if (ends) {
+      finish(done);
       clear();
-      return now + (int)gridDim.x < work;
+      return done + (int)gridDim.x < work;
     }
     return true;
   };
   source();
   clear();
-  load_group<GU_NU, FMT>(a, src, 2 * g.I, g0 < ng ? g0 : ng - 1, lane);
-  while (step(a, b) && step(b, a)) {
+#pragma unroll
+  for (int u = 0; u < GU_NU; ++u) load_unit<GU_NU, FMT>(weights[u], src, place, u, first);
+  load_values<GU_NU>(v0, src, first);
+  if constexpr (FMT == FMT_Q4) {
+    load_values<GU_NU>(v1, src, first + 1);
+    while (step(v0, v1)) {
+    }
+  } else {
+    while (step(v0, v1) && step(v1, v0)) {
+    }
   }
 }
 
@@ -552,30 +582,32 @@ constexpr int DN_WAVES = 4, DN_THREADS = 64 * DN_WAVES, DN_NU = 4, DN_COLS = 16 
 
 template <int DT, int FMT>
 __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
-  // the waves' codes, and their sums [waves][T][64]: 64 KiB at most (32 tokens, 8-bit)
+  // the waves' codes, and their sums [waves][T][64]: 64 KiB at most
   extern __shared__ __attribute__((aligned(16))) uint8_t s_down[];
-  float* const s_sum = reinterpret_cast<float*>(s_down + DN_WAVES * DN_NU * UNIT_LDS<FMT>);
+  float* const s_sum = reinterpret_cast<float*>(s_down + DN_WAVES * DN_NU * UNIT_LDS);
   int* const s_last = reinterpret_cast<int*>(s_down);  // once the codes have been read
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int nt = blockIdx.x / g.P, p = blockIdx.x - nt * g.P, n0 = DN_COLS * nt;
   float* const sum = s_sum + wave * g.T * DN_COLS;  // the wave's own: its LDS operations complete in order
-  uint8_t* const codes = s_down + wave * DN_NU * UNIT_LDS<FMT>;
+  uint8_t* const codes = s_down + wave * DN_NU * UNIT_LDS;
   for (int i = lane; i < g.T * DN_COLS / 4; i += 64) reinterpret_cast<f32x4*>(sum)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   InUse in;
   in.load(g.mask, lane);
   // the wave's pairs: an even share of all waves' of this column tile
-  const int ng = g.I / 128, work = in.items * ng, parts = g.P * DN_WAVES, part = p * DN_WAVES + wave;
+  const int ng = g.I / 128, ns = (ng + STEP<FMT> - 1) / STEP<FMT>, work = in.items * ns, parts = g.P * DN_WAVES;
+  const int part = p * DN_WAVES + wave;
   const int f1 = (int)((int64_t)work * (part + 1) / parts);
   int f = (int)((int64_t)work * part / parts);  // the pair being loaded
   if (f < f1) {
-    int it = f / ng, gr = f - it * ng;
+    int it = f / ns, st = f - it * ns;
+    const Place<FMT> place(g.H, g.I, lane);
     Source<DN_NU> src;
     Tokens tk, next_tk;
     float wt[4], next_wt[4];
     auto source = [&]() {
       const Item t = in.item(it);
-      src.template weights<FMT>(g.dn, g.dn_s, t.e, g.H, g.I, {n0, n0 + 16, n0 + 32, n0 + 48}, lane);
+      src.template weights<FMT>(g.dn, g.dn_s, t.e, g.H, g.I, {n0, n0 + 16, n0 + 32, n0 + 48});
       src.x = buffer_of(g.act + (int64_t)t.u * g.T * g.I, g.T * g.I * 2);
       src.x_off = next_tk.set(t, 2 * g.I, lane);
 #pragma unroll
@@ -590,22 +622,21 @@ __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
 #pragma unroll
       for (int v = 0; v < DN_NU; ++v) y[v] = f32x4{0.f, 0.f, 0.f, 0.f};
     };
-    Group<DN_NU, FMT> a, b;
-    auto step = [&](const Group<DN_NU, FMT>& cur, Group<DN_NU, FMT>& nxt) {
+    Unit<FMT> weights[DN_NU];
+    Values v0, v1;
+    auto step = [&](Values& v0, Values& v1) {
+      const int gr = STEP<FMT> * st;
       bool ends = true;
       if (++f < f1) {
-        if (++gr == ng) {
-          gr = 0;
+        if (++st == ns) {
+          st = 0;
           ++it;
           source();
         } else {
           ends = false;
         }
       }
-      load_group<DN_NU, FMT>(nxt, src, g.H, gr, lane);
-      __builtin_amdgcn_sched_barrier(0);
-      mul_group<DN_NU, FMT, DT>(cur, codes, lane, nib, y);
-      __builtin_amdgcn_sched_barrier(0);
+      mul_step<DN_NU, FMT, DT>(weights, v0, v1, gr + 1 < ng, src, place, STEP<FMT> * st, codes, lane, nib, y);
       if (ends) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -623,8 +654,16 @@ __global__ __launch_bounds__(DN_THREADS) void few_down_kernel(const FewArgs g) {
     };
     source();
     begin();
-    load_group<DN_NU, FMT>(a, src, g.H, gr, lane);
-    while (step(a, b) && step(b, a)) {
+#pragma unroll
+    for (int u = 0; u < DN_NU; ++u) load_unit<DN_NU, FMT>(weights[u], src, place, u, STEP<FMT> * st);
+    load_values<DN_NU>(v0, src, STEP<FMT> * st);
+    if constexpr (FMT == FMT_Q4) {
+      load_values<DN_NU>(v1, src, STEP<FMT> * st + 1);
+      while (step(v0, v1)) {
+      }
+    } else {
+      while (step(v0, v1) && step(v1, v0)) {
+      }
     }
   }
   __syncthreads();
@@ -681,12 +720,13 @@ struct FewPlan {
 };
 
 // Sizes, and where each buffer sits in the workspace (16-byte steps).
-FewPlan few_plan(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
+FewPlan few_plan(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I, bool eight_bit) {
   FewPlan p;
   p.in_use = E < T * k ? E : T * k;
-  // two blocks a CU for the column tiles together, and about four pairs a wave at least
-  const int64_t tiles = H / DN_COLS, cus = device_cu_count(), pairs = p.in_use * (I / 128);
-  int64_t parts = 2 * cus / tiles, most = pairs / (4 * DN_WAVES);
+  // two blocks a CU for the column tiles together, and about two pairs a wave at least (which 8-bit codes have
+  // more of: their plan never takes less of the workspace)
+  const int64_t tiles = H / DN_COLS, cus = device_cu_count(), pairs = p.in_use * (I / 128) / (eight_bit ? 1 : 2);
+  int64_t parts = 2 * cus / tiles, most = pairs / (2 * DN_WAVES);
   parts = parts > most ? most : parts;
   p.P = (int)(parts < 1 ? 1 : parts);
   int64_t at = 0;
@@ -715,7 +755,7 @@ int launch_few_layer(const FewArgs& g, int64_t in_use, hipStream_t st) {
   if (int rc = check_launch("moe_few/gate_up")) return rc;
   few_down_kernel<DT, FMT>
       <<<(unsigned)(g.H / DN_COLS * g.P), DN_THREADS,
-         (size_t)DN_WAVES * (DN_NU * UNIT_LDS<FMT> + g.T * DN_COLS * 4), st>>>(g);
+         (size_t)DN_WAVES * (DN_NU * UNIT_LDS + g.T * DN_COLS * 4), st>>>(g);
   return check_launch("moe_few/down");
 }
 
@@ -736,7 +776,7 @@ using namespace usaf;
 
 extern "C" int64_t usaf_hip_moe_few_ws_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I) {
   if (few_sizes(T, E, top_k, H, I) != USAF_OK) return -1;
-  return T == 0 ? 0 : few_plan(T, E, top_k, H, I).bytes;
+  return T == 0 ? 0 : few_plan(T, E, top_k, H, I, true).bytes;
 }
 
 extern "C" int usaf_hip_moe_few(const void* x, int64_t T, int64_t H, const void* router, int64_t E, int64_t top_k,
@@ -752,7 +792,7 @@ extern "C" int usaf_hip_moe_few(const void* x, int64_t T, int64_t H, const void*
     return set_error(USAF_ERR_INVALID, "moe_few: activations, router, codes and workspace must be 16-byte aligned");
   if ((!eight_bit && ((uintptr_t)gate_up_scale | (uintptr_t)down_scale) % 4) || (uintptr_t)out % 8)
     return set_error(USAF_ERR_INVALID, "moe_few: misaligned scales or output (8 bytes)");
-  const FewPlan p = few_plan(T, E, top_k, H, I);
+  const FewPlan p = few_plan(T, E, top_k, H, I, eight_bit != 0);
   if (ws_bytes < p.bytes)
     return set_error(USAF_ERR_INVALID, "moe_few: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)p.bytes);
   FewArgs g{};
