@@ -148,7 +148,7 @@ def product(x: Rows, w: Fp8Tensor, out: torch.Tensor, offsets: Optional[torch.Te
     E, n, k = w._erc()
     if x.cols != k or out.shape[1] != n:
         raise ValueError(f"fp8 product: rows of {x.cols} and output {tuple(out.shape)} do not fit the weight {tuple(w.shape)}")
-    N.call("usaf_hip_fp8_gemm", x.q.data_ptr(), x.s.data_ptr(), N.ptr(row_of), out.shape[0], w.q.data_ptr(),
+    N.call("usaf_hip_fp8_gemm", x.q.data_ptr(), x.s.data_ptr(), x.q.shape[0], N.ptr(row_of), out.shape[0], w.q.data_ptr(),
            w.s.data_ptr(), N.ptr(offsets), E, n, k, N.dtype_code(out.dtype), out.data_ptr(), N.stream_ptr(out.device))
     return out
 
