@@ -69,17 +69,17 @@ def test_entry_points_check_their_arguments():
     assert rows(p, N.BF16, -1, 8, 8, None, p, p, None) == inval
     assert rows(p, N.BF16, 1 << 62, 8, 8, None, p, p, None) == inval
     gemm = lib.usaf_hip_fp8_gemm
-    assert gemm(None, None, 0, None, 0, None, None, None, 1, 8, 8, N.BF16, None, None) == ok
-    assert gemm(p, p, 1, None, 1, p, p, None, 2, 8, 8, N.BF16, p, None) == inval
-    assert gemm(p, p, 1, None, 1, p, p, None, 1, 8, 0, N.BF16, p, None) == inval
-    assert gemm(p, p, 1, None, 1, p, p, None, 1, 8, 8, N.F32, p, None) == inval
-    assert gemm(odd, p, 1, None, 1, p, p, None, 1, 8, 8, N.BF16, p, None) == inval
-    assert gemm(p, odd, 1, None, 1, p, p, None, 1, 8, 8, N.BF16, p, None) == inval
-    assert gemm(p, p, 1, None, 1, p, p, None, 1, 8, 8, N.BF16, odd, None) == inval
-    assert gemm(p, p, 1, None, 2, p, p, None, 1, 8, 8, N.BF16, p, None) == inval
-    assert gemm(p, p, 1 << 33, p, 1, p, p, None, 1, 8, 8, N.BF16, p, None) == N.USAF_ERR_UNSUPPORTED
-    assert gemm(p, p, 1 << 40, None, 1 << 40, p, p, None, 1, 8, 8, N.BF16, p, None) == inval
-    assert gemm(p, p, 1, None, 1, p, p, p, 256, 8, 8, N.BF16, p, None) == N.USAF_ERR_UNSUPPORTED
+    assert gemm(None, None, 0, None, 0, None, None, None, 1, 8, 8, N.BF16, 0, None, None) == ok
+    assert gemm(p, p, 1, None, 1, p, p, None, 2, 8, 8, N.BF16, 0, p, None) == inval
+    assert gemm(p, p, 1, None, 1, p, p, None, 1, 8, 0, N.BF16, 0, p, None) == inval
+    assert gemm(p, p, 1, None, 1, p, p, None, 1, 8, 8, N.F32, 0, p, None) == inval
+    assert gemm(odd, p, 1, None, 1, p, p, None, 1, 8, 8, N.BF16, 0, p, None) == inval
+    assert gemm(p, odd, 1, None, 1, p, p, None, 1, 8, 8, N.BF16, 0, p, None) == inval
+    assert gemm(p, p, 1, None, 1, p, p, None, 1, 8, 8, N.BF16, 0, odd, None) == inval
+    assert gemm(p, p, 1, None, 2, p, p, None, 1, 8, 8, N.BF16, 0, p, None) == inval
+    assert gemm(p, p, 1 << 33, p, 1, p, p, None, 1, 8, 8, N.BF16, 0, p, None) == N.USAF_ERR_UNSUPPORTED
+    assert gemm(p, p, 1 << 40, None, 1 << 40, p, p, None, 1, 8, 8, N.BF16, 0, p, None) == inval
+    assert gemm(p, p, 1, None, 1, p, p, p, 256, 8, 8, N.BF16, 0, p, None) == N.USAF_ERR_UNSUPPORTED
     assert lib.usaf_hip_fp8_swiglu(p, 1, 100, N.BF16, p, p, p, p, None) == inval
     assert lib.usaf_hip_fp8_swiglu(p, 1, 128, N.BF16, None, p, p, p, None) == inval
     assert lib.usaf_hip_fp8_swiglu(None, 0, 128, N.BF16, None, None, None, None, None) == ok

@@ -9,11 +9,14 @@
 // holds 4 consecutive columns of one slot.  Codes are padded with zeros to whole
 // blocks along k; rows past the last slot or column repeat it and are not stored.
 //
-// A block of eight waves has a tile of 32 MW MI slots x 32 NW NI columns.  Both operands
-// come by LDS DMA, one 128-byte line of each row a step, into a ring of NS stages; at a
-// step's one barrier its stage has landed and the stage before it has been read, so the
-// DMAs of the step NS - 1 ahead go there.  16-byte chunks of a row are XOR-swizzled by
-// the row (by the DMA's source address), which makes the fragment reads free of bank conflicts.
+// A block of eight waves has tiles of 32 MW MI slots x 32 NW NI columns; KW of its waves
+// split the contraction's blocks.  Blocks stay (one a CU) and walk a die's run of the tile list.
+// Both operands come by LDS DMA, 128-byte lines of KW k-blocks a step, into a ring of NS
+// stages; at a step's one barrier its stage has landed and the stage before it has been
+// read, so the DMAs of the step NS - 1 ahead go there, straight across tile ends: a tile of 6
+// steps (a contraction of 768) would spend as long on its first lines as on its products.
+// 16-byte chunks of a row are XOR-swizzled by the row (by the DMA's source address), which
+// makes the fragment reads free of bank conflicts.
 #include "fp8.h"
 
 namespace usaf {
@@ -65,206 +68,348 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
   const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
   return reinterpret_cast<const uint8_t*>((uintptr_t)(((uint64_t)hi << 32) | (uint64_t)lo));
 }
+// 32 codes of a lane -> four bf16 fragment registers of their values, exact.
+__device__ __forceinline__ void values16(const u32x4 lo, const u32x4 hi, int e8m0, u32x4 (&o)[4]) {
+  const int b = e8m0 & 0xFF;
+  const float s = __uint_as_float(b == 0 ? 0x00400000u : (uint32_t)b << 23);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t w = j < 4 ? lo[j] : hi[j - 4];
+    o[j >> 1][2 * (j & 1)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
+    o[j >> 1][2 * (j & 1) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true));
+  }
+}
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// Tiles of all experts (one wave, offsets from global memory; E <= 255).
+// The list of m-tiles (experts in order, each in tiles of SLOTS), held by a wave: lane l
+// has experts 4 l .. 4 l + 3 (E <= 255).
 template <int SLOTS>
-__device__ __forceinline__ int all_tiles(const int32_t* offsets, int E, int lane) {
-  int n = 0;
+struct SlotTiles {
+  int off[5], c[4], incl, sum, total;
+  __device__ __forceinline__ void load(const int32_t* offsets, int E, int lane) {
+    sum = 0;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int i = 4 * lane + k;
-    if (i < E) n += (offsets[i + 1] - offsets[i] + SLOTS - 1) / SLOTS;
+    for (int k = 0; k < 5; ++k) off[k] = offsets[4 * lane + k < E ? 4 * lane + k : E];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      c[k] = (off[k + 1] - off[k] + SLOTS - 1) / SLOTS;
+      sum += c[k];
+    }
+    incl = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += o;
+    }
+    total = __builtin_amdgcn_readlane(incl, 63);
   }
+  // m-tile mt < total -> expert, first slot, slots
+  __device__ __forceinline__ void tile(int mt, int lane, int& e, int& beg, int& valid) const {
+    const int src = __builtin_ctzll(__ballot(incl > mt));
+    int j = mt - (incl - sum), ee = 4 * lane, b = off[0], end = off[1];
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d, 64);
-  return __builtin_amdgcn_readfirstlane(n);
-}
-
-template <int MW, int MI, int NI>
-struct Tile {
-  static constexpr int NW = G_WAVES / MW;
-  static constexpr int M = 32 * MW * MI, N = 32 * NW * NI;
-  static constexpr int A_BYTES = M * 128, W_BYTES = N * 128;
-  static constexpr int A_SCALES = M < 64 ? 256 : 4 * M;  // a word for each slot, 64 at a time
-  static constexpr int STAGE = A_BYTES + W_BYTES + A_SCALES + 256;  // and 64 words of the weight's
-  static constexpr int FIT = 160 * 1024 / STAGE, NS = FIT > 4 ? 4 : FIT;
-  static constexpr int LDS = NS * STAGE;
-  static constexpr int A_DMA = M >= 64 ? M / 64 : 1, W_DMA = N / 64, DMAS = A_DMA + W_DMA + 1;
-  static constexpr int OUT_ROW = 64 * NI;  // bytes of a wave's row of results
-  static_assert(NS >= 2 && M <= 256 && G_WAVES * 32 * MI * OUT_ROW <= LDS, "LDS");
+    for (int k = 0; k < 3; ++k) {
+      if (ee == 4 * lane + k && j >= c[k]) {  // past expert 4 l + k
+        j -= c[k];
+        ee = 4 * lane + k + 1;
+        b = off[k + 1];
+        end = off[k + 2];
+      }
+    }
+    e = __builtin_amdgcn_readlane(ee, src);
+    beg = __builtin_amdgcn_readlane(b + j * SLOTS, src);
+    const int rem = __builtin_amdgcn_readlane(end, src) - beg;
+    valid = rem < SLOTS ? rem : SLOTS;
+  }
 };
 
-template <int MW, int MI, int NI, int DT>
+template <int MW, int NW, int MI, int NI>
+struct Tile {
+  static constexpr int KW = G_WAVES / (MW * NW);
+  static constexpr int M = 32 * MW * MI, N = 32 * NW * NI;
+  static constexpr int A_BYTES = M * 128, W_BYTES = N * 128;         // of one k-block
+  static constexpr int SCALES = 4 * 64 * ((M + 63) / 64) + 256;      // a word for each slot, 64 words of the weight's
+  static constexpr int SLAB = A_BYTES + W_BYTES + SCALES, STAGE = KW * SLAB;
+  static constexpr int FIT = 160 * 1024 / STAGE, NS = FIT > 4 ? 4 : FIT, LDS = NS * STAGE;
+  // DMA instructions of a wave and step: the rows of its own k-block, shared by the MW NW waves that have it
+  static constexpr int SHARE = MW * NW;
+  static constexpr int A_DMA = (M / 8 + SHARE - 1) / SHARE, W_DMA = N / 8 / SHARE;
+  static constexpr int A_WORDS = (M + 63) / 64;                      // scale instructions of the slots
+  static constexpr int S_DMA = (A_WORDS + 1 + SHARE - 1) / SHARE, DMAS = A_DMA + W_DMA + S_DMA;
+  static constexpr int OUT_ROW = 64 * NI;                            // bytes of a wave's row of results
+  static_assert(NS >= 2 && MW * NW * KW == G_WAVES && N / 8 % SHARE == 0, "tile");
+  static_assert(KW > 1 ? G_WAVES * 4096 * NI <= STAGE : G_WAVES * 32 * OUT_ROW <= STAGE, "results go through a stage");
+};
+
+template <int MW, int NW, int MI, int NI, int DT, bool WIDE>
 __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
-  typedef Tile<MW, MI, NI> T;
+  typedef Tile<MW, NW, MI, NI> T;
+  constexpr int KW = T::KW;
   extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
   const uint32_t sm_lds = (uint32_t)(uintptr_t)(lds_void_ptr)sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, half = lane >> 5;
-  const int wm = wave % MW, wn = wave / MW;
+  const int kw = wave / T::SHARE, part = wave % T::SHARE, wm = part % MW, wn = part / MW;
 
-  // ---- the block's tile.  A die's blocks take a run of the list, so that what they share sits
-  //      in its L2: of one expert, or of one weight, eight slot tiles side by side
-  const int m_tiles = g.offsets ? all_tiles<T::M>(g.offsets, g.E, lane) : (int)((g.M + T::M - 1) / T::M);
-  const int tiles = m_tiles * g.n_nt, per = (tiles + G_XCDS - 1) / G_XCDS;
-  const int j = (int)blockIdx.x / G_XCDS, id = ((int)blockIdx.x % G_XCDS) * per + j;
-  if (j >= per || id >= tiles) return;  // block-uniform
-  int mt, nt, e = 0, valid;
-  int64_t m_beg;
+  // ---- the block's tiles: its die's run of the list, every blocks-of-a-die-th.  What a die's
+  //      blocks share at a time sits in its L2: an expert, or eight slot tiles of one weight
+  SlotTiles<T::M> slots;
+  int m_tiles = (int)((g.M + T::M - 1) / T::M);
   if (g.offsets) {
-    mt = id / g.n_nt;
-    nt = id - mt * g.n_nt;
-    GemmArgs o{};
-    o.offsets = g.offsets;
-    o.E = g.E;
-    int beg;
-    if (!slot_tile<T::M>(o, lane, mt, e, beg, valid)) return;
-    m_beg = beg;
-  } else {
-    constexpr int GROUP = 8;
-    const int band = id / (GROUP * g.n_nt), rest = id - band * GROUP * g.n_nt;
-    const int tall = m_tiles - band * GROUP < GROUP ? m_tiles - band * GROUP : GROUP;
-    nt = rest / tall;
-    mt = band * GROUP + rest - nt * tall;
-    m_beg = (int64_t)mt * T::M;
-    valid = g.M - m_beg < T::M ? (int)(g.M - m_beg) : T::M;
+    slots.load(g.offsets, g.E, lane);
+    m_tiles = slots.total;
   }
-  const int64_t n0 = (int64_t)nt * T::N;
-  const int nkb = (int)(g.Kp / 128);
-
-  // ---- DMA sources: uniform bases, 32-bit lane offsets.  Instruction i of wave w fills rows
-  //      8 (8 i + w) + [0, 8) of the stage, lane l chunk l % 8 of row l / 8
-  const uint8_t* a_base = uniform(g.a_rows ? g.A : g.A + m_beg * g.Kp);
-  const uint8_t* w_base = uniform(g.W + ((int64_t)e * g.N + n0) * g.Kp);
-  auto slot_row = [&](int r) -> int64_t {  // operand row of slot r of the tile, from a_base's
-    r = r < valid ? r : valid - 1;
-    return g.a_rows ? (int64_t)g.a_rows[m_beg + r] : r;
+  const int tiles = m_tiles * g.n_nt, per = (tiles + G_XCDS - 1) / G_XCDS, stride = (int)gridDim.x / G_XCDS;
+  const int xcd = (int)blockIdx.x % G_XCDS, run = xcd * per;
+  const int end = run + per < tiles ? run + per : tiles, id0 = run + (int)blockIdx.x / G_XCDS;
+  if (id0 >= end) return;  // block-uniform
+  struct Place {
+    int e, valid, nt;
+    int64_t m_beg;
   };
-  uint32_t a_off[T::A_DMA], w_off[T::W_DMA];
-#pragma unroll
-  for (int i = 0; i < T::A_DMA; ++i) {
-    const int r = (8 * (8 * i + wave) + (lane >> 3)) % T::M;  // (tiles of 32 slots: two waves fill each row)
-    a_off[i] = (uint32_t)(slot_row(r) * g.Kp) + 16 * ((lane & 7) ^ g_swz(r));
-  }
-#pragma unroll
-  for (int i = 0; i < T::W_DMA; ++i) {
-    const int r = 8 * (8 * i + wave) + (lane >> 3);
-    const int64_t n = n0 + r < g.N ? r : g.N - 1 - n0;
-    w_off[i] = (uint32_t)(n * g.Kp) + 16 * ((lane & 7) ^ g_swz(r));
-  }
-  // scales, a word for each row: waves below M / 64 those of 64 slots each, the others (all the
-  // same) those of the tile's blocks of 128 columns, the words around the byte
-  constexpr int A_SCALE_WAVES = (T::M + 63) / 64;
-  const bool a_scale = wave < A_SCALE_WAVES;
-  const uint8_t* const s_base = uniform(a_scale ? (g.a_rows ? g.as : g.as + m_beg * g.sp) : g.ws);
+  auto place = [&](int id) {
+    Place t;
+    t.e = 0;
+    if (g.offsets) {
+      const int mt = id / g.n_nt;
+      t.nt = id - mt * g.n_nt;
+      int beg;
+      slots.tile(mt, lane, t.e, beg, t.valid);
+      t.m_beg = beg;
+    } else {
+      constexpr int GROUP = 8;
+      const int band = id / (GROUP * g.n_nt), rest = id - band * GROUP * g.n_nt;
+      const int tall = m_tiles - band * GROUP < GROUP ? m_tiles - band * GROUP : GROUP;
+      t.nt = rest / tall;
+      t.m_beg = (int64_t)(band * GROUP + rest - t.nt * tall) * T::M;
+      t.valid = g.M - t.m_beg < T::M ? (int)(g.M - t.m_beg) : T::M;
+    }
+    return t;
+  };
+  const int nkb = (int)(g.Kp / 128), steps = (nkb + KW - 1) / KW;
   const int64_t nrb = (g.N + 127) / 128;
   const int ws_shift = (int)((uintptr_t)g.ws & 3);
-  int64_t ws_row = (n0 / 128 + (lane < 2 ? lane : 0));
-  ws_row = ((int64_t)e * nrb + (ws_row < nrb ? ws_row : nrb - 1)) * nkb + ws_shift;
-  const uint32_t s_off = a_scale ? (uint32_t)(slot_row((64 * wave + lane) % T::M) * g.sp) : 0;
-  const uint32_t s_lds = (uint32_t)(T::A_BYTES + T::W_BYTES + (a_scale ? 256 * wave : T::A_SCALES));
+  // byte of the scale of columns 128 b + [0, 128) of the tile, k-block 0, from the word that ws sits in
+  auto ws_at = [&](const Place& t, int b) {
+    int64_t at = (int64_t)t.nt * T::N / 128 + b;
+    return ((int64_t)t.e * nrb + (at < nrb ? at : nrb - 1)) * nkb + ws_shift;
+  };
 
-  auto issue = [&](int kb, int stage) {
-    kb = kb < nkb ? kb : nkb - 1;
-    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(sm_lds + stage * T::STAGE));
-    const uint8_t* const a = a_base + (int64_t)kb * 128;
-    const uint8_t* const w = w_base + (int64_t)kb * 128;
+  // ---- the DMA stream: uniform bases, 32-bit lane offsets.  Of a k-block's rows, instruction i
+  //      of wave `part` fills 8 (SHARE i + part) + [0, 8), lane l chunk l % 8 of row l / 8
+  int i_id = id0, i_step = 0, i_stage = 0;
+  const uint8_t *a_base, *w_base, *as_base;
+  uint32_t a_off[T::A_DMA], w_off[T::W_DMA], s_off[T::S_DMA];
+  int64_t ws_off = 0;
+  auto open = [&]() {
+    const Place t = place(i_id);
+    const int64_t n0 = (int64_t)t.nt * T::N;
+    a_base = uniform(g.a_rows ? g.A : g.A + t.m_beg * g.Kp);
+    as_base = uniform(g.a_rows ? g.as : g.as + t.m_beg * g.sp);
+    w_base = uniform(g.W + ((int64_t)t.e * g.N + n0) * g.Kp);
+    auto row = [&](int r) -> int64_t {  // operand row of slot r of the tile, from a_base's
+      r = r < t.valid ? r : t.valid - 1;
+      return g.a_rows ? (int64_t)g.a_rows[t.m_beg + r] : r;
+    };
 #pragma unroll
-    for (int i = 0; i < T::A_DMA; ++i) g_dma16(a, a_off[i], to + (8 * i + wave) * 1024 % T::A_BYTES);
+    for (int i = 0; i < T::A_DMA; ++i) {
+      const int r = (8 * (T::SHARE * i + part) + (lane >> 3)) % T::M;  // (of few rows, some twice)
+      a_off[i] = (uint32_t)(row(r) * g.Kp) + 16 * ((lane & 7) ^ g_swz(r));
+    }
 #pragma unroll
-    for (int i = 0; i < T::W_DMA; ++i) g_dma16(w, w_off[i], to + T::A_BYTES + (8 * i + wave) * 1024);
-    if (a_scale) g_dma4(s_base + (kb & ~3), s_off, to + s_lds);
-    else g_dma4(s_base - ws_shift, (uint32_t)((ws_row + kb) & ~(int64_t)3), to + s_lds);
+    for (int i = 0; i < T::W_DMA; ++i) {
+      const int r = 8 * (T::SHARE * i + part) + (lane >> 3);
+      const int64_t n = n0 + r < g.N ? r : g.N - 1 - n0;
+      w_off[i] = (uint32_t)(n * g.Kp) + 16 * ((lane & 7) ^ g_swz(r));
+    }
+    // scale words: instruction s < A_WORDS those of 64 slots, the others (all the same) the
+    // weight's, the words around the bytes of the tile's blocks of 128 columns
+#pragma unroll
+    for (int i = 0; i < T::S_DMA; ++i) {
+      const int w = T::SHARE * i + part;
+      s_off[i] = w < T::A_WORDS ? (uint32_t)(row((64 * w + lane) % T::M) * g.sp) : 0;
+    }
+    ws_off = ws_at(t, lane < T::N / 128 ? lane : 0);
+  };
+  auto issue = [&]() {
+    const int kb = i_step * KW + kw, k = kb < nkb ? kb : nkb - 1;
+    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(sm_lds + i_stage * T::STAGE + kw * T::SLAB));
+    const uint8_t* const a = a_base + (int64_t)k * 128;
+    const uint8_t* const w = w_base + (int64_t)k * 128;
+#pragma unroll
+    for (int i = 0; i < T::A_DMA; ++i) g_dma16(a, a_off[i], to + (T::SHARE * i + part) * 1024 % T::A_BYTES);
+#pragma unroll
+    for (int i = 0; i < T::W_DMA; ++i) g_dma16(w, w_off[i], to + T::A_BYTES + (T::SHARE * i + part) * 1024);
+#pragma unroll
+    for (int i = 0; i < T::S_DMA; ++i) {
+      const int s = T::SHARE * i + part;  // wave-uniform
+      const uint32_t at = to + T::A_BYTES + T::W_BYTES;
+      if (s < T::A_WORDS) g_dma4(as_base + (k & ~3), s_off[i], at + 256 * s);
+      else g_dma4(g.ws - ws_shift, (uint32_t)((ws_off + k) & ~(int64_t)3), at + 256 * T::A_WORDS);
+    }
+    i_stage = i_stage + 1 == T::NS ? 0 : i_stage + 1;
+    if (++i_step == steps) {
+      if (i_id + stride < end) {
+        i_id += stride;
+        i_step = 0;
+        open();
+      } else {
+        i_step = steps - 1;  // past the block's last step: that one again, which nobody reads
+      }
+    }
   };
 
   f32x16 acc[MI][NI];
-#pragma unroll
-  for (int i = 0; i < MI; ++i)
-#pragma unroll
-    for (int k = 0; k < NI; ++k) acc[i][k] = f32x16{};
-  const int mine = valid - 32 * MI * wm;  // slots of the wave's part
-  const int live = mine <= 0 ? 0 : mine >= 32 * MI ? MI : (mine + 31) >> 5;  // its blocks of 32 with any
-
-  for (int s = 0; s < T::NS - 1; ++s) issue(s, s);
   int stage = 0;
-  for (int kb = 0; kb < nkb; ++kb) {
-    wait_vmcnt<(T::NS - 2) * T::DMAS>();  // the wave's DMAs of this step
-    lds_barrier();                        // and everyone's; the stage before this one has been read
-    issue(kb + T::NS - 1, stage == 0 ? T::NS - 1 : stage - 1);
-    const uint8_t* const sa = sm + stage * T::STAGE;
-    const uint8_t* const sw = sa + T::A_BYTES;
-    const uint32_t* const sc = reinterpret_cast<const uint32_t*>(sw + T::W_BYTES);
-    auto word = [&](const uint8_t* rows, int r, int c) {
-      return *reinterpret_cast<const u32x4*>(rows + r * 128 + 16 * (c ^ g_swz(r)));
-    };
-    int s_a[MI], s_w[NI];
+  open();
+  for (int s = 0; s < T::NS - 1; ++s) issue();
+  for (int id = id0; id < end; id += stride) {
+    const Place t = place(id);
+    const int mine = t.valid - 32 * MI * wm;  // slots of the wave's part
+    const int live = mine <= 0 ? 0 : mine >= 32 * MI ? MI : (mine + 31) >> 5;  // its blocks of 32 with any
+    int64_t ws_byte[NI];
 #pragma unroll
-    for (int i = 0; i < MI; ++i) s_a[i] = (int)(sc[32 * (MI * wm + i) + l32] >> (8 * (kb & 3)));
+    for (int k = 0; k < NI; ++k) ws_byte[k] = ws_at(t, (32 * (NI * wn + k)) / 128);
 #pragma unroll
-    for (int k = 0; k < NI; ++k) {
-      const int b = (32 * (NI * wn + k)) / 128;  // which block of 128 columns
-      int64_t at = n0 / 128 + b;
-      at = ((int64_t)e * nrb + (at < nrb ? at : nrb - 1)) * nkb + ws_shift + kb;
-      s_w[k] = (int)(sc[T::A_SCALES / 4 + b] >> (8 * (int)(at & 3)));
-    }
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = 4 * h + 2 * half;
-      u32x4 w0[NI], w1[NI];
+      for (int k = 0; k < NI; ++k) acc[i][k] = f32x16{};
+    for (int step = 0; step < steps; ++step) {
+      wait_vmcnt<(T::NS - 2) * T::DMAS>();  // the wave's DMAs of this step (and what is older)
+      lds_barrier();                        // and everyone's; the stage before this one has been read
+      issue();
+      const int kb = step * KW + kw;
+      const uint8_t* const sa = sm + stage * T::STAGE + kw * T::SLAB;
+      const uint8_t* const sw = sa + T::A_BYTES;
+      const uint32_t* const sc = reinterpret_cast<const uint32_t*>(sw + T::W_BYTES);
+      stage = stage + 1 == T::NS ? 0 : stage + 1;
+      if (KW > 1 && kb >= nkb) continue;  // wave-uniform
+      auto word = [&](const uint8_t* rows, int r, int c) {
+        return *reinterpret_cast<const u32x4*>(rows + r * 128 + 16 * (c ^ g_swz(r)));
+      };
+      int s_a[MI], s_w[NI];
 #pragma unroll
-      for (int k = 0; k < NI; ++k) {
-        w0[k] = word(sw, 32 * (NI * wn + k) + l32, c);
-        w1[k] = word(sw, 32 * (NI * wn + k) + l32, c + 1);
+      for (int i = 0; i < MI; ++i) s_a[i] = (int)(sc[32 * (MI * wm + i) + l32] >> (8 * (kb & 3)));
+#pragma unroll
+      for (int k = 0; k < NI; ++k)
+        s_w[k] = (int)(sc[64 * T::A_WORDS + (32 * (NI * wn + k)) / 128] >> (8 * (int)((ws_byte[k] + kb) & 3)));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = 4 * h + 2 * half;
+        if constexpr (!WIDE) {
+          u32x4 w0[NI], w1[NI];
+#pragma unroll
+          for (int k = 0; k < NI; ++k) {
+            w0[k] = word(sw, 32 * (NI * wn + k) + l32, c);
+            w1[k] = word(sw, 32 * (NI * wn + k) + l32, c + 1);
+          }
+#pragma unroll
+          for (int i = 0; i < MI; ++i) {
+            if (i >= live) continue;  // wave-uniform
+            const u32x4 a0 = word(sa, 32 * (MI * wm + i) + l32, c), a1 = word(sa, 32 * (MI * wm + i) + l32, c + 1);
+#pragma unroll
+            for (int k = 0; k < NI; ++k) acc[i][k] = mfma8(w0[k], w1[k], a0, a1, acc[i][k], s_w[k], s_a[i]);
+          }
+        } else {
+          u32x4 wf[NI][4];
+#pragma unroll
+          for (int k = 0; k < NI; ++k)
+            values16(word(sw, 32 * (NI * wn + k) + l32, c), word(sw, 32 * (NI * wn + k) + l32, c + 1), s_w[k], wf[k]);
+#pragma unroll
+          for (int i = 0; i < MI; ++i) {
+            if (i >= live) continue;
+            u32x4 af[4];
+            values16(word(sa, 32 * (MI * wm + i) + l32, c), word(sa, 32 * (MI * wm + i) + l32, c + 1), s_a[i], af);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int k = 0; k < NI; ++k) acc[i][k] = mfma32<USAF_BF16>(wf[k][j], af[j], acc[i][k]);
+          }
+        }
       }
+    }
+    // ---- results, through the stage that was read last: nothing is sent there before the next
+    //      step's barrier.  A lane's values 4 q .. 4 q + 3 of a 32 x 32 block are columns 8 q +
+    //      4 half + [0, 4) of slot l32
+    lds_barrier();
+    uint8_t* const free = sm + (stage == 0 ? T::NS - 1 : stage - 1) * T::STAGE;
+    const int64_t nw = (int64_t)t.nt * T::N + 32 * NI * wn, mw = t.m_beg + 32 * MI * wm;
+    if constexpr (KW > 1) {
+      // the KW partial sums in order: wave kw finishes values VPW kw .. of each block's 16
+      constexpr int VPW = 16 / KW;
+      float* const red = reinterpret_cast<float*>(free);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
-        if (i >= live) continue;  // wave-uniform
-        const u32x4 a0 = word(sa, 32 * (MI * wm + i) + l32, c), a1 = word(sa, 32 * (MI * wm + i) + l32, c + 1);
+        if (i) lds_barrier();  // the last 32 slots' have been read
 #pragma unroll
-        for (int k = 0; k < NI; ++k) acc[i][k] = mfma8(w0[k], w1[k], a0, a1, acc[i][k], s_w[k], s_a[i]);
+        for (int k = 0; k < NI; ++k)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) red[((k * 16 + v) * G_WAVES + wave) * 64 + lane] = acc[i][k][v];
+        lds_barrier();
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+          float o[VPW];
+#pragma unroll
+          for (int v = 0; v < VPW; ++v) {
+            const int at = ((k * 16 + VPW * kw + v) * G_WAVES + part) * 64 + lane;
+            o[v] = red[at];
+#pragma unroll
+            for (int w = 1; w < KW; ++w) o[v] += red[at + w * T::SHARE * 64];
+          }
+          if (32 * i + l32 < mine) {
+#pragma unroll
+            for (int v = 0; v < VPW; v += 2) {
+              const int b = VPW * kw + v;
+              const int64_t n = nw + 32 * k + 8 * (b >> 2) + 4 * half + (b & 3);
+              uint16_t* const to = g.out + (mw + 32 * i + l32) * g.N + n;
+              const uint32_t two = pack2<DT>(o[v], o[v + 1]);
+              if (n + 1 < g.N && ((uintptr_t)to & 3) == 0) {
+                *reinterpret_cast<uint32_t*>(to) = two;
+              } else {
+                if (n < g.N) to[0] = (uint16_t)two;
+                if (n + 1 < g.N) to[1] = (uint16_t)(two >> 16);
+              }
+            }
+          }
+        }
       }
-    }
-    stage = stage + 1 == T::NS ? 0 : stage + 1;
-  }
-  wait_vmcnt<0>();
-  lds_barrier();  // no DMA is under way, nobody reads the ring
-
-  // ---- results: lane's values 4 q .. 4 q + 3 of a 32 x 32 block are columns 8 q + 4 half +
-  //      [0, 4) of slot l32.  Through the wave's part of LDS, for whole lines to memory
-  uint8_t* const so = sm + wave * (32 * MI * T::OUT_ROW);
-  constexpr int CH = T::OUT_ROW / 16;  // 16-byte chunks of a row
-#pragma unroll
-  for (int i = 0; i < MI; ++i)
-#pragma unroll
-    for (int k = 0; k < NI; ++k)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r = 32 * i + l32, c = 4 * k + q;
-        *reinterpret_cast<uint2*>(so + r * T::OUT_ROW + 16 * (c ^ (r & (CH - 1))) + 8 * half) =
-            uint2{pack2<DT>(acc[i][k][4 * q], acc[i][k][4 * q + 1]), pack2<DT>(acc[i][k][4 * q + 2], acc[i][k][4 * q + 3])};
-      }
-  __builtin_amdgcn_wave_barrier();
-  const bool wide = g.N % 8 == 0 && ((uintptr_t)g.out & 15) == 0;
-  const int64_t nw = n0 + 32 * NI * wn;
-#pragma unroll 4
-  for (int it = 0; it < 32 * MI * CH / 64; ++it) {
-    const int r = it * (64 / CH) + lane / CH, c = lane % CH;
-    const u32x4 v = *reinterpret_cast<const u32x4*>(so + r * T::OUT_ROW + 16 * (c ^ (r & (CH - 1))));
-    const int64_t n = nw + 8 * c;
-    if (r >= mine || n >= g.N) continue;
-    uint16_t* const to = g.out + (m_beg + 32 * MI * wm + r) * g.N + n;
-    if (wide) {
-      *reinterpret_cast<u32x4*>(to) = v;
     } else {
+      // 32 slots at a time through the wave's part, for whole lines to memory
+      uint8_t* const so = free + wave * (32 * T::OUT_ROW);
+      constexpr int CH = T::OUT_ROW / 16;  // 16-byte chunks of a row
+      const bool wide = g.N % 8 == 0 && ((uintptr_t)g.out & 15) == 0;
 #pragma unroll
-      for (int b = 0; b < 8; ++b)
-        if (n + b < g.N) to[b] = (uint16_t)(v[b >> 1] >> (16 * (b & 1)));
+      for (int i = 0; i < MI; ++i) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < NI; ++k)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint2*>(so + l32 * T::OUT_ROW + 16 * ((4 * k + q) ^ (l32 & (CH - 1))) + 8 * half) =
+                uint2{pack2<DT>(acc[i][k][4 * q], acc[i][k][4 * q + 1]), pack2<DT>(acc[i][k][4 * q + 2], acc[i][k][4 * q + 3])};
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int it = 0; it < 32 * CH / 64; ++it) {
+          const int r = it * (64 / CH) + lane / CH, c = lane % CH;
+          const u32x4 v = *reinterpret_cast<const u32x4*>(so + r * T::OUT_ROW + 16 * (c ^ (r & (CH - 1))));
+          const int64_t n = nw + 8 * c;
+          if (32 * i + r >= mine || n >= g.N) continue;
+          uint16_t* const to = g.out + (mw + 32 * i + r) * g.N + n;
+          if (wide) {
+            *reinterpret_cast<u32x4*>(to) = v;
+          } else {
+#pragma unroll
+            for (int b = 0; b < 8; ++b)
+              if (n + b < g.N) to[b] = (uint16_t)(v[b >> 1] >> (16 * (b & 1)));
+          }
+        }
+      }
     }
   }
+  wait_vmcnt<0>();  // no DMA lands in LDS that is someone else's by then
 }
 
 bool raise_fp8_lds(const void* kernel, size_t bytes) {
@@ -272,41 +417,75 @@ bool raise_fp8_lds(const void* kernel, size_t bytes) {
   (void)hipGetLastError();
   return true;
 }
-template <int MW, int MI, int NI, int DT>
+template <int MW, int NW, int MI, int NI, int DT, bool WIDE>
 void prepare_one() {
-  static const bool done = raise_fp8_lds(reinterpret_cast<const void*>(&fp8_gemm_kernel<MW, MI, NI, DT>),
-                                         Tile<MW, MI, NI>::LDS);
+  static const bool done = raise_fp8_lds(reinterpret_cast<const void*>(&fp8_gemm_kernel<MW, NW, MI, NI, DT, WIDE>),
+                                         Tile<MW, NW, MI, NI>::LDS);
   (void)done;
 }
 
-template <int MW, int MI, int NI>
-int launch(Fp8Args g, int dt, hipStream_t st) {
-  typedef Tile<MW, MI, NI> T;
-  const int64_t m_tiles = g.offsets ? (g.M < g.E ? g.M : g.E) + g.M / T::M : (g.M + T::M - 1) / T::M;
-  const int64_t n_nt = (g.N + T::N - 1) / T::N, blocks = (m_tiles * n_nt + G_XCDS - 1) / G_XCDS * G_XCDS;
-  if (blocks >= (int64_t)1 << 31) return set_error(USAF_ERR_INVALID, "fp8_gemm: too many tiles");
-  g.n_nt = (int)n_nt;
-  if (dt == USAF_BF16) {
-    prepare_one<MW, MI, NI, USAF_BF16>();
-    fp8_gemm_kernel<MW, MI, NI, USAF_BF16><<<(unsigned)blocks, G_THREADS, T::LDS, st>>>(g);
-  } else {
-    prepare_one<MW, MI, NI, USAF_F16>();
-    fp8_gemm_kernel<MW, MI, NI, USAF_F16><<<(unsigned)blocks, G_THREADS, T::LDS, st>>>(g);
-  }
+template <int MW, int NW, int MI, int NI, int DT, bool WIDE>
+int launch_dt(const Fp8Args& g, unsigned blocks, hipStream_t st) {
+  prepare_one<MW, NW, MI, NI, DT, WIDE>();
+  fp8_gemm_kernel<MW, NW, MI, NI, DT, WIDE><<<blocks, G_THREADS, Tile<MW, NW, MI, NI>::LDS, st>>>(g);
   return check_launch("fp8_gemm");
 }
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Each shape of tile: launch, one-time set-up, and what a call would take with it.
+template <int MW, int NW, int MI, int NI>
+struct Shape {
+  typedef Tile<MW, NW, MI, NI> T;
+  static int64_t tiles_at_most(const Fp8Args& g) {
+    return (g.offsets ? (g.M < g.E ? g.M : g.E) + g.M / T::M : ceil_div(g.M, T::M)) * ceil_div(g.N, T::N);
+  }
+  static int launch(Fp8Args g, int dt, bool wide, hipStream_t st) {
+    const int64_t tiles = tiles_at_most(g), cus = device_cu_count();
+    if (tiles >= (int64_t)1 << 31) return set_error(USAF_ERR_INVALID, "fp8_gemm: too many tiles");
+    g.n_nt = (int)ceil_div(g.N, T::N);
+    const unsigned blocks = (unsigned)(ceil_div(tiles < cus ? tiles : cus, G_XCDS) * G_XCDS);
+    if (dt == USAF_BF16)
+      return wide ? launch_dt<MW, NW, MI, NI, USAF_BF16, true>(g, blocks, st)
+                  : launch_dt<MW, NW, MI, NI, USAF_BF16, false>(g, blocks, st);
+    return wide ? launch_dt<MW, NW, MI, NI, USAF_F16, true>(g, blocks, st)
+                : launch_dt<MW, NW, MI, NI, USAF_F16, false>(g, blocks, st);
+  }
+  static void prepare() {
+    prepare_one<MW, NW, MI, NI, USAF_BF16, false>();
+    prepare_one<MW, NW, MI, NI, USAF_BF16, true>();
+    prepare_one<MW, NW, MI, NI, USAF_F16, false>();
+    prepare_one<MW, NW, MI, NI, USAF_F16, true>();
+  }
+  // Cycles of a CU, roughly: a step is bound by its matrix instructions or by its lines
+  static double cycles(const Fp8Args& g, bool wide) {
+    const double steps = (double)ceil_div(g.Kp / 128, T::KW);
+    const double mfma = 2.0 * MI * NI * 2 * (wide ? 128 : 64), lines = (double)T::KW * (T::M + T::N) * 128 / 24;
+    const double step = (mfma > lines ? mfma : lines) + 250, tile = steps * step + 1500;
+    // slots of an expert: full tiles and on average half a tile
+    const double m = g.offsets ? (double)(g.M < g.E ? g.M : g.E) * 0.5 + (double)g.M / T::M : (double)ceil_div(g.M, T::M);
+    const double rounds = m * (double)ceil_div(g.N, T::N) / device_cu_count();
+    return tile * (rounds < 1 ? 1 : g.offsets ? rounds + 0.5 : (double)(int64_t)(rounds + 0.999));
+  }
+};
+typedef Shape<2, 4, 4, 2> S256x256;
+typedef Shape<2, 4, 2, 2> S128x256;
+typedef Shape<2, 4, 2, 1> S128x128;
+typedef Shape<1, 4, 2, 1> S64x128;
+typedef Shape<1, 2, 2, 1> S64x64;
+typedef Shape<1, 4, 1, 1> S32x128;
+typedef Shape<1, 1, 1, 1> S32x32;
 
 }  // namespace
 
 void prepare_fp8_kernels() {
-  prepare_one<1, 1, 1, USAF_BF16>();
-  prepare_one<1, 1, 1, USAF_F16>();
-  prepare_one<1, 2, 1, USAF_BF16>();
-  prepare_one<1, 2, 1, USAF_F16>();
-  prepare_one<2, 2, 2, USAF_BF16>();
-  prepare_one<2, 2, 2, USAF_F16>();
-  prepare_one<2, 4, 2, USAF_BF16>();
-  prepare_one<2, 4, 2, USAF_F16>();
+  S256x256::prepare();
+  S128x256::prepare();
+  S128x128::prepare();
+  S64x128::prepare();
+  S64x64::prepare();
+  S32x128::prepare();
+  S32x32::prepare();
 }
 
 }  // namespace usaf
@@ -315,7 +494,7 @@ using namespace usaf;
 
 extern "C" int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, int64_t a_total, const int32_t* a_rows, int64_t M,
                                  const uint8_t* w, const uint8_t* w_scale, const int32_t* offsets, int64_t E, int64_t N,
-                                 int64_t K, int32_t dtype, void* out, void* stream) {
+                                 int64_t K, int32_t dtype, int32_t wide, void* out, void* stream) {
   if (M < 0 || N < 0 || K < 0 || E < 1 || N > 1 << 24 || K > 1 << 24 || M > 0x7FFFFFFF || a_total < 0)
     return set_error(USAF_ERR_INVALID, "fp8_gemm: bad size M=%lld N=%lld K=%lld E=%lld", (long long)M, (long long)N,
                      (long long)K, (long long)E);
@@ -346,9 +525,21 @@ extern "C" int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, int64
       E * ((N + 127) / 128) * (g.Kp / 128) >= (int64_t)1 << 31)
     return set_error(USAF_ERR_UNSUPPORTED, "fp8_gemm: operands past 4 GiB of gathered rows or 2 GiB of scales");
   hipStream_t st = as_stream(stream);
-  const int64_t per = M / E;  // slots of an expert on average
-  if (per <= 32) return launch<1, 1, 1>(g, dtype, st);
-  if (per <= 64) return launch<1, 2, 1>(g, dtype, st);
-  if (per <= 128) return launch<2, 2, 2>(g, dtype, st);
-  return launch<2, 4, 2>(g, dtype, st);
+  typedef int (*Launch)(Fp8Args, int, bool, hipStream_t);
+  const bool w16 = wide != 0;
+  Launch best = S256x256::launch;
+  double least = S256x256::cycles(g, w16);
+  auto consider = [&](Launch f, double c) {
+    if (c < least) {
+      least = c;
+      best = f;
+    }
+  };
+  consider(S128x256::launch, S128x256::cycles(g, w16));
+  consider(S128x128::launch, S128x128::cycles(g, w16));
+  consider(S64x128::launch, S64x128::cycles(g, w16));
+  consider(S64x64::launch, S64x64::cycles(g, w16));
+  consider(S32x128::launch, S32x128::cycles(g, w16));
+  consider(S32x32::launch, S32x32::cycles(g, w16));
+  return best(g, dtype, w16, st);
 }

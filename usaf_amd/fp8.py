@@ -143,13 +143,14 @@ def quantize_rows(x: torch.Tensor, n_rows: Optional[torch.Tensor] = None) -> Row
 
 
 def product(x: Rows, w: Fp8Tensor, out: torch.Tensor, offsets: Optional[torch.Tensor] = None,
-            row_of: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """out[m] = x[row_of[m] or m] @ w_e^T for the slots m of expert e (offsets; one expert without)."""
+            row_of: Optional[torch.Tensor] = None, wide: bool = False) -> torch.Tensor:
+    """out[m] = x[row_of[m] or m] @ w_e^T for the slots m of expert e (offsets; one expert without).
+    wide: sums to fp32's own precision, by the 16-bit matrix instruction (usaf_hip_fp8_gemm)."""
     E, n, k = w._erc()
     if x.cols != k or out.shape[1] != n:
         raise ValueError(f"fp8 product: rows of {x.cols} and output {tuple(out.shape)} do not fit the weight {tuple(w.shape)}")
     N.call("usaf_hip_fp8_gemm", x.q.data_ptr(), x.s.data_ptr(), x.q.shape[0], N.ptr(row_of), out.shape[0], w.q.data_ptr(),
-           w.s.data_ptr(), N.ptr(offsets), E, n, k, N.dtype_code(out.dtype), out.data_ptr(), N.stream_ptr(out.device))
+           w.s.data_ptr(), N.ptr(offsets), E, n, k, N.dtype_code(out.dtype), 1 if wide else 0, out.data_ptr(), N.stream_ptr(out.device))
     return out
 
 
@@ -199,15 +200,24 @@ def fp8_linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
 # the routed experts (moe.RoutedExpertsFn)
 # ---------------------------------------------------------------------------
 
+def _wide(dtype: torch.dtype) -> bool:
+    """Whether the experts' products take the 16-bit matrix instruction.  The 8-bit one is off by
+    1.5e-5 of the result, which alone neither type shows.  But here results are quantized again,
+    and values that fall to the other side of a code's border by it put an error of about
+    sqrt(1.5e-5 * 2^-4) = 1e-3 into the layer's output: less than bf16's own 1.7e-3,
+    six times fp16's 2.1e-4."""
+    return dtype == torch.float16
+
+
 def experts_forward(hs: torch.Tensor, ew, b, gu: torch.Tensor, act: torch.Tensor, y: torch.Tensor) -> None:
     """gu, act, y of the slots of bucketing b, for 8-bit experts ew.  Each step's output is
     rounded to the activations' dtype, as on the layer's other kernels."""
     S, I = act.shape
-    product(quantize_rows(hs), ew.gate_up, gu, b.offsets, b.token_idx)
+    product(quantize_rows(hs), ew.gate_up, gu, b.offsets, b.token_idx, wide=_wide(hs.dtype))
     rows = empty_rows(S, I, hs.device)
     N.call("usaf_hip_fp8_swiglu", gu.data_ptr(), S, I, N.dtype_code(gu.dtype), b.offsets[-1:].data_ptr(), act.data_ptr(),
            rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(hs.device))
-    product(rows, ew.down, y, b.offsets)
+    product(rows, ew.down, y, b.offsets, wide=_wide(hs.dtype))
 
 
 def experts_down_bwd(dcur: torch.Tensor, gu: torch.Tensor, ew, b, dgu: torch.Tensor) -> Rows:
@@ -215,8 +225,13 @@ def experts_down_bwd(dcur: torch.Tensor, gu: torch.Tensor, ew, b, dgu: torch.Ten
     S, I = gu.shape[0], gu.shape[1] // 2
     n_slots = b.offsets[-1:]
     dact = product(quantize_rows(dcur, n_slots), ew.down.transposed(), torch.empty(S, I, dtype=gu.dtype, device=gu.device),
-                   b.offsets)
+                   b.offsets, wide=_wide(gu.dtype))
     rows = empty_rows(S, 2 * I, gu.device)
     N.call("usaf_hip_fp8_swiglu_bwd", gu.data_ptr(), dact.data_ptr(), S, I, N.dtype_code(gu.dtype), n_slots.data_ptr(),
            dgu.data_ptr(), rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(gu.device))
     return rows
+
+
+def experts_gate_up_bwd(dgu: Rows, ew, b, dx_slots: torch.Tensor) -> None:
+    """The slots' gradient of the hidden states from dgu quantized (experts_down_bwd)."""
+    product(dgu, ew.gate_up.transposed(), dx_slots, b.offsets, wide=_wide(dx_slots.dtype))

@@ -614,7 +614,7 @@ class RoutedExpertsFn(torch.autograd.Function):
         dx_slots = torch.empty(S, H, dtype=dt, device=dev)
         tq = ew._ptrs_t("gate_up")
         if ew.is_fp8:
-            fp8.product(dgu_rows, ew.gate_up.transposed(), dx_slots, b.offsets)
+            fp8.experts_gate_up_bwd(dgu_rows, ew, b, dx_slots)
         elif tq is not None:
             timed_call("usaf_hip_moe_gate_up_bwd_t", dgu.data_ptr(), I, b.offsets.data_ptr(), S, E, H, *tq,
                        code, dx_slots.data_ptr(), *ew._ovl("gate_up_bwd", dt), st)
