@@ -594,12 +594,18 @@ int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, int64_t a_total,
  * and its backward, with the layer's 16-bit roundings), for slots below *n_slots:
  * usaf_hip_fp8_swiglu: gu [S, 2I] -> act [S, I], with its codes and scale bytes.
  * usaf_hip_fp8_swiglu_bwd: gu, dact [S, I] -> dgu [S, 2I], with codes and scale bytes.
- * I % 128 == 0; 16-byte aligned operands.
+ * usaf_hip_fp8_combine_bwd: usaf_hip_moe_combine_bwd with dcur [S, H] as codes and scale bytes.
+ * act, dgu and dcur may be NULL: their 16-bit values are then not stored.
+ * I % 128 == 0, H % 128 == 0; 16-byte aligned operands.
  */
 int usaf_hip_fp8_swiglu(const void* gu, int64_t S, int64_t I, int32_t dtype, const int32_t* n_slots, void* act,
                         uint8_t* q, uint8_t* s, void* stream);
 int usaf_hip_fp8_swiglu_bwd(const void* gu, const void* dact, int64_t S, int64_t I, int32_t dtype,
                             const int32_t* n_slots, void* dgu, uint8_t* q, uint8_t* s, void* stream);
+
+int usaf_hip_fp8_combine_bwd(const void* dout, const void* y, const int32_t* token_idx, const float* slot_w,
+                             const int32_t* offsets, int64_t S, int64_t E, int64_t H, int32_t dtype, void* dcur,
+                             uint8_t* q, uint8_t* s, void* dweights, void* stream);
 
 /*
  * A whole MoE layer for T <= 32 tokens (qwen3moe_dml.py:24-86 without the

@@ -246,6 +246,10 @@ def test_experts_step_by_step(F, T, E, k, H, I, only, dtype):
     saved = out.grad_fn
     _, gu, act, y = saved.saved_tensors
     b = saved.b
+    assert act is None  # no weight gradient is wanted
+    act, again = torch.empty(b.n_slots, I, dtype=dtype, device="cuda"), [torch.empty_like(gu), torch.empty_like(y)]
+    F.experts_forward(hs.cuda(), ew, b, again[0], act, again[1])
+    assert torch.equal(again[0], gu) and torch.equal(again[1], y)
     offs, tok = b.offsets.tolist(), b.token_idx.long().cpu()
     wgu, wd = ew.gate_up.dequantize().double().cpu(), ew.down.dequantize().double().cpu()
     h = O.half_step(dtype)
@@ -274,8 +278,11 @@ def test_experts_step_by_step(F, T, E, k, H, I, only, dtype):
     # the backward's own steps again, on its inputs
     dcur64 = pw * dout[tok].double()
     dcur = dcur64.to(dtype).cuda()
-    dgu = torch.empty_like(gu)
-    F.experts_down_bwd(dcur, gu, ew, b, dgu)
+    dgu, dx_slots, got_dcur = torch.empty_like(gu), torch.empty_like(y), torch.empty_like(y)
+    rows = F.experts_combine_bwd(dout.cuda(), y, b, got_dcur, torch.zeros(T, E, dtype=dtype, device="cuda"))
+    # (equal to the last bit but for the sign of zeros, which a code has too)
+    assert torch.equal(got_dcur, dcur) and torch.equal(rows.q, F.quantize_rows(got_dcur).q)
+    F.experts_bwd(rows, gu, ew, b, dgu, dx_slots)
     qc = O.quantized_rows(dcur.cpu())[0]
     dgu64 = dgu.double().cpu()
     q_dgu = O.quantized_rows(dgu.cpu())[0]
@@ -354,7 +361,7 @@ def test_sampled_gradient_on_8_bit_experts(F):
     slot_e = torch.repeat_interleave(torch.arange(E), torch.tensor(offs[1:]) - torch.tensor(offs[:-1]))
     dcur = (w[tok, slot_e].double()[:, None] * dout[tok].double()).bfloat16()
     dgu = torch.empty_like(gu)
-    F.experts_down_bwd(dcur.cuda(), gu, ew, b, dgu)
+    F.experts_bwd(F.quantize_rows(dcur.cuda()), gu, ew, b, dgu, torch.empty(gu.shape[0], H, dtype=gu.dtype, device="cuda"))
     for name, left, right in (("L.gate_up_proj", dgu.double().cpu(), hs.double()[tok]), ("L.down_proj", dcur.double(), act)):
         ref = torch.stack([left[offs[e]:offs[e + 1]].t() @ right[offs[e]:offs[e + 1]] for e in range(E)]).reshape(-1)
         mag = torch.stack([left[offs[e]:offs[e + 1]].t().abs() @ right[offs[e]:offs[e + 1]].abs() for e in range(E)]).reshape(-1)

@@ -51,6 +51,8 @@ _SIGNATURES: dict[str, list] = {
     "usaf_hip_fp8_gemm": [_c_p, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32,
                           _c_p, _c_p],
     "usaf_hip_fp8_swiglu": [_c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_p],
+    "usaf_hip_fp8_combine_bwd": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_p, _c_p,
+                                 _c_p],
     "usaf_hip_fp8_swiglu_bwd": [_c_p, _c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_p],
     "usaf_hip_moe_few": [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i32, _c_i32, _c_i64, _c_i32, _c_p, _c_p, _c_p,
                          _c_p, _c_p, _c_p, _c_i64, _c_p],

@@ -170,9 +170,8 @@ __global__ __launch_bounds__(256) void fp8_transpose_kernel(const uint8_t* __res
   if (threadIdx.x == 0) st[(e * nkb + kb) * nrb + rb] = s[(e * nrb + rb) * nkb + kb];
 }
 
-// gu [S, 2I] -> act = dt(dt(silu(gate)) up) [S, I], its codes and scale bytes, for
-// the slots in use (offsets[E]).  16 lanes a block of 128 columns.  Between two
-// products of hundreds of us this reads and writes each value once.
+// gu [S, 2I] -> act = dt(dt(silu(gate)) up) [S, I] (null: not stored), its codes and scale
+// bytes, for the slots in use (offsets[E]).  16 lanes a block of 128 columns.
 template <int DT>
 __global__ __launch_bounds__(256) void fp8_swiglu_kernel(const uint16_t* __restrict__ gu, int64_t S, int64_t I,
                                                          const int32_t* __restrict__ n_slots, uint16_t* __restrict__ act,
@@ -196,12 +195,12 @@ __global__ __launch_bounds__(256) void fp8_swiglu_kernel(const uint16_t* __restr
     a[2 * j] = v.x;
     a[2 * j + 1] = v.y;
   }
-  *reinterpret_cast<uint4*>(act + m * I + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (act) *reinterpret_cast<uint4*>(act + m * I + c) = make_uint4(w[0], w[1], w[2], w[3]);
   store_block(a, lane16, q + m * I + c, s + m * sp + kb);
 }
 
-// gu, dact -> dgu [S, 2I] with the roundings of the layer's other grad-input
-// kernels, its codes and scale bytes.
+// gu, dact -> dgu [S, 2I] with the roundings of the layer's other grad-input kernels
+// (null: not stored), its codes and scale bytes.
 template <int DT>
 __global__ __launch_bounds__(256) void fp8_swiglu_bwd_kernel(const uint16_t* __restrict__ gu,
                                                              const uint16_t* __restrict__ dact, int64_t S, int64_t I,
@@ -238,10 +237,66 @@ __global__ __launch_bounds__(256) void fp8_swiglu_bwd_kernel(const uint16_t* __r
     du[2 * j] = b.x;
     du[2 * j + 1] = b.y;
   }
-  *reinterpret_cast<uint4*>(dgu + m * 2 * I + c) = make_uint4(wg[0], wg[1], wg[2], wg[3]);
-  *reinterpret_cast<uint4*>(dgu + m * 2 * I + I + c) = make_uint4(wu[0], wu[1], wu[2], wu[3]);
+  if (dgu) {
+    *reinterpret_cast<uint4*>(dgu + m * 2 * I + c) = make_uint4(wg[0], wg[1], wg[2], wg[3]);
+    *reinterpret_cast<uint4*>(dgu + m * 2 * I + I + c) = make_uint4(wu[0], wu[1], wu[2], wu[3]);
+  }
   store_block(dg, lane16, q + m * 2 * I + c, s + m * sp + kb);
   store_block(du, lane16, q + m * 2 * I + I + c, s + m * sp + nkb + kb);
+}
+
+// Backward of the weighted sum, slot m (token t, expert e): dcur = dt(w dout[t]) as codes and
+// scale bytes (and, where a sampled or dense weight gradient reads it, in 16 bits), and
+// dweights[t, e] = dt(<dout[t], y[m]>).  One block a slot, 16 lanes a block of 128
+// columns.  With the 16-bit dcur written and read again this took 59 + 47 us where a pass over
+// 32,768 slots of 2,048 reads 268 MB and writes 67.
+template <int DT>
+__global__ __launch_bounds__(256) void fp8_combine_bwd_kernel(const uint16_t* __restrict__ dout,
+                                                              const uint16_t* __restrict__ y,
+                                                              const int32_t* __restrict__ token_idx,
+                                                              const float* __restrict__ slot_w,
+                                                              const int32_t* __restrict__ offsets, int E, int64_t H,
+                                                              int sp, uint16_t* __restrict__ dcur,
+                                                              uint8_t* __restrict__ q, uint8_t* __restrict__ s,
+                                                              uint16_t* __restrict__ dweights) {
+#pragma clang fp contract(off)
+  __shared__ float s_part[4];
+  const int64_t m = blockIdx.x;
+  if (m >= offsets[E]) return;  // block-uniform
+  const int64_t t = token_idx[m];
+  const float wm = slot_w[m];
+  const int lane16 = threadIdx.x & 15;
+  float part = 0.f;
+  for (int64_t c = (int64_t)threadIdx.x * 8; c < H; c += 2048) {  // H % 128 == 0: 16 lanes go together
+    float g[8], v[8], d[8];
+    load8<DT>(dout + t * H + c, true, 8, g);
+    load8<DT>(y + m * H + c, true, 8, v);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = pack2<DT>(g[2 * j] * wm, g[2 * j + 1] * wm);
+      const f32x2 f = unpack2<DT>(w[j]);
+      d[2 * j] = f.x;
+      d[2 * j + 1] = f.y;
+      part += g[2 * j] * v[2 * j];
+      part += g[2 * j + 1] * v[2 * j + 1];
+    }
+    if (dcur) *reinterpret_cast<uint4*>(dcur + m * H + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    store_block(d, lane16, q + m * H + c, s + m * sp + c / FB);
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) part += __shfl_xor(part, k, 64);
+  if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = part;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int lo = 0, hi = E - 1;  // expert of slot m: the largest e with offsets[e] <= m
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (offsets[mid] <= m) lo = mid;
+      else hi = mid - 1;
+    }
+    store_from_f32<DT>(dweights, t * E + lo, s_part[0] + s_part[1] + s_part[2] + s_part[3]);
+  }
 }
 
 int blocks16(int64_t n, const char* what, unsigned* out) {  // 16 lane groups a block
@@ -337,7 +392,7 @@ static int swiglu_args(const char* what, int64_t S, int64_t I, const void* a, co
   if (S < 0 || I <= 0 || I % FP8_BLOCK || I > 1 << 24)
     return set_error(USAF_ERR_INVALID, "%s: need S >= 0 and I a positive multiple of 128", what);
   if (S > ((int64_t)1 << 40) / I) return set_error(USAF_ERR_INVALID, "%s: too many slots", what);
-  if (S > 0 && (!a || !b || !c || !n || !q || !s)) return set_error(USAF_ERR_INVALID, "%s: null pointer", what);
+  if (S > 0 && (!a || !b || !n || !q || !s)) return set_error(USAF_ERR_INVALID, "%s: null pointer", what);
   if (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)q) % 16)
     return set_error(USAF_ERR_INVALID, "%s: operands must be 16-byte aligned", what);
   return blocks16(S * (I / FP8_BLOCK), what, blocks);
@@ -346,7 +401,7 @@ static int swiglu_args(const char* what, int64_t S, int64_t I, const void* a, co
 extern "C" int usaf_hip_fp8_swiglu(const void* gu, int64_t S, int64_t I, int32_t dtype, const int32_t* n_slots, void* act,
                                    uint8_t* q, uint8_t* s, void* stream) {
   unsigned blocks;
-  if (int rc = swiglu_args("fp8_swiglu", S, I, gu, act, act, n_slots, q, s, &blocks)) return rc;
+  if (int rc = swiglu_args("fp8_swiglu", S, I, gu, gu, act, n_slots, q, s, &blocks)) return rc;
   if (S == 0) return clear_error();
   const int sp = (int)usaf_hip_fp8_scale_stride(I);
   const uint16_t* g = reinterpret_cast<const uint16_t*>(gu);
@@ -375,4 +430,28 @@ extern "C" int usaf_hip_fp8_swiglu_bwd(const void* gu, const void* dact, int64_t
   else
     return set_error(USAF_ERR_INVALID, "fp8_swiglu_bwd: dtype must be fp16 or bf16");
   return check_launch("fp8_swiglu_bwd");
+}
+
+extern "C" int usaf_hip_fp8_combine_bwd(const void* dout, const void* y, const int32_t* token_idx, const float* slot_w,
+                                        const int32_t* offsets, int64_t S, int64_t E, int64_t H, int32_t dtype, void* dcur,
+                                        uint8_t* q, uint8_t* s, void* dweights, void* stream) {
+  if (S < 0 || S > 0x7FFFFFFF || E < 1 || E > 1024 || H <= 0 || H % FP8_BLOCK || H > 1 << 24)
+    return set_error(USAF_ERR_INVALID, "fp8_combine_bwd: need 0 <= S < 2^31, 1 <= E <= 1024 and H a positive multiple of 128");
+  if (S == 0) return clear_error();
+  if (!dout || !y || !token_idx || !slot_w || !offsets || !q || !s || !dweights)
+    return set_error(USAF_ERR_INVALID, "fp8_combine_bwd: null pointer");
+  if (((uintptr_t)dout | (uintptr_t)y | (uintptr_t)dcur | (uintptr_t)q) % 16)
+    return set_error(USAF_ERR_INVALID, "fp8_combine_bwd: operands must be 16-byte aligned");
+  const int sp = (int)usaf_hip_fp8_scale_stride(H);
+  const uint16_t *d = reinterpret_cast<const uint16_t*>(dout), *yy = reinterpret_cast<const uint16_t*>(y);
+  uint16_t *o = reinterpret_cast<uint16_t*>(dcur), *dw = reinterpret_cast<uint16_t*>(dweights);
+  if (dtype == USAF_BF16)
+    fp8_combine_bwd_kernel<USAF_BF16><<<(unsigned)S, 256, 0, as_stream(stream)>>>(d, yy, token_idx, slot_w, offsets, (int)E, H,
+                                                                                  sp, o, q, s, dw);
+  else if (dtype == USAF_F16)
+    fp8_combine_bwd_kernel<USAF_F16><<<(unsigned)S, 256, 0, as_stream(stream)>>>(d, yy, token_idx, slot_w, offsets, (int)E, H,
+                                                                                 sp, o, q, s, dw);
+  else
+    return set_error(USAF_ERR_INVALID, "fp8_combine_bwd: dtype must be fp16 or bf16");
+  return check_launch("fp8_combine_bwd");
 }

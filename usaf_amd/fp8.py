@@ -209,29 +209,35 @@ def _wide(dtype: torch.dtype) -> bool:
     return dtype == torch.float16
 
 
-def experts_forward(hs: torch.Tensor, ew, b, gu: torch.Tensor, act: torch.Tensor, y: torch.Tensor) -> None:
-    """gu, act, y of the slots of bucketing b, for 8-bit experts ew.  Each step's output is
-    rounded to the activations' dtype, as on the layer's other kernels."""
-    S, I = act.shape
-    product(quantize_rows(hs), ew.gate_up, gu, b.offsets, b.token_idx, wide=_wide(hs.dtype))
-    rows = empty_rows(S, I, hs.device)
-    N.call("usaf_hip_fp8_swiglu", gu.data_ptr(), S, I, N.dtype_code(gu.dtype), b.offsets[-1:].data_ptr(), act.data_ptr(),
-           rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(hs.device))
-    product(rows, ew.down, y, b.offsets, wide=_wide(hs.dtype))
-
-
-def experts_down_bwd(dcur: torch.Tensor, gu: torch.Tensor, ew, b, dgu: torch.Tensor) -> Rows:
-    """dgu from the gradient dcur of the down projection's outputs; returns dgu quantized."""
+def experts_forward(hs: torch.Tensor, ew, b, gu: torch.Tensor, act: Optional[torch.Tensor], y: torch.Tensor) -> None:
+    """gu, act (None: not stored) and y of the slots of bucketing b, for 8-bit experts ew. Each step's
+    output is rounded to the activations' dtype, as on the layer's other kernels."""
     S, I = gu.shape[0], gu.shape[1] // 2
-    n_slots = b.offsets[-1:]
-    dact = product(quantize_rows(dcur, n_slots), ew.down.transposed(), torch.empty(S, I, dtype=gu.dtype, device=gu.device),
-                   b.offsets, wide=_wide(gu.dtype))
-    rows = empty_rows(S, 2 * I, gu.device)
-    N.call("usaf_hip_fp8_swiglu_bwd", gu.data_ptr(), dact.data_ptr(), S, I, N.dtype_code(gu.dtype), n_slots.data_ptr(),
-           dgu.data_ptr(), rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(gu.device))
+    wide = _wide(hs.dtype)
+    product(quantize_rows(hs), ew.gate_up, gu, b.offsets, b.token_idx, wide=wide)
+    rows = empty_rows(S, I, hs.device)
+    N.call("usaf_hip_fp8_swiglu", gu.data_ptr(), S, I, N.dtype_code(gu.dtype), b.offsets[-1:].data_ptr(), N.ptr(act),
+           rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(hs.device))
+    product(rows, ew.down, y, b.offsets, wide=wide)
+
+
+def experts_combine_bwd(dout: torch.Tensor, y: torch.Tensor, b, dcur: Optional[torch.Tensor],
+                        dweights: torch.Tensor) -> Rows:
+    """The gradient of the down projection's outputs, quantized (and in dcur where given), and of the routing weights."""
+    S, H = y.shape
+    rows = empty_rows(S, H, y.device)
+    N.call("usaf_hip_fp8_combine_bwd", dout.data_ptr(), y.data_ptr(), b.token_idx.data_ptr(), b.slot_w.data_ptr(),
+           b.offsets.data_ptr(), S, b.offsets.numel() - 1, H, N.dtype_code(y.dtype), N.ptr(dcur), rows.q.data_ptr(),
+           rows.s.data_ptr(), dweights.data_ptr(), N.stream_ptr(y.device))
     return rows
 
 
-def experts_gate_up_bwd(dgu: Rows, ew, b, dx_slots: torch.Tensor) -> None:
-    """The slots' gradient of the hidden states from dgu quantized (experts_down_bwd)."""
-    product(dgu, ew.gate_up.transposed(), dx_slots, b.offsets, wide=_wide(dx_slots.dtype))
+def experts_bwd(dcur: Rows, gu: torch.Tensor, ew, b, dgu: Optional[torch.Tensor], dx_slots: torch.Tensor) -> None:
+    """dgu (None: not stored) and the slots' gradient of the hidden states."""
+    S, I = gu.shape[0], gu.shape[1] // 2
+    wide = _wide(gu.dtype)
+    dact = product(dcur, ew.down.transposed(), torch.empty(S, I, dtype=gu.dtype, device=gu.device), b.offsets, wide=wide)
+    rows = empty_rows(S, 2 * I, gu.device)
+    N.call("usaf_hip_fp8_swiglu_bwd", gu.data_ptr(), dact.data_ptr(), S, I, N.dtype_code(gu.dtype), b.offsets[-1:].data_ptr(),
+           N.ptr(dgu), rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(gu.device))
+    product(rows, ew.gate_up.transposed(), dx_slots, b.offsets, wide=wide)

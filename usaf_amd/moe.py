@@ -527,7 +527,9 @@ class RoutedExpertsFn(torch.autograd.Function):
         b = bucket_by_expert(weights) if slots is None else bucket_by_expert(weights, *slots)
         S = b.n_slots
         gu = torch.empty(S, 2 * I, dtype=dt, device=dev)
-        act = torch.empty(S, I, dtype=dt, device=dev)
+        # the gated activations of 8-bit experts are kept where a weight gradient will read them
+        keep = not ew.is_fp8 or capture is not None or ctx.needs_input_grad[5]
+        act = torch.empty(S, I, dtype=dt, device=dev) if keep else None
         y = torch.empty(S, H, dtype=dt, device=dev)
         act_blk = None
         if S > 0 and not ew.is_fp8 and _sampled_blocked(capture, b):
@@ -577,6 +579,8 @@ class RoutedExpertsFn(torch.autograd.Function):
             d_wgu = torch.zeros(E, 2 * I, H, dtype=ctx.wdt[0], device=dev) if want_gu else None
             d_wdn = torch.zeros(E, H, I, dtype=ctx.wdt[1], device=dev) if want_dn else None
             return torch.zeros_like(hs), dweights, None, None, d_wgu, d_wdn, None, None
+        if ew.is_fp8:
+            return _fp8_experts_backward(ctx, dout, dweights)
         dcur = torch.empty(S, H, dtype=dt, device=dev)
         dcur_blk = None
         if _sampled_blocked(capture, b) and _blocked_ok(dout) and _blocked_ok(y):
@@ -596,9 +600,7 @@ class RoutedExpertsFn(torch.autograd.Function):
                    b.slot_w.data_ptr(), b.offsets.data_ptr(), S, E, H, code, dcur.data_ptr(), dweights.data_ptr(), st)
         dgu = torch.empty(S, 2 * I, dtype=dt, device=dev)
         tq = ew._ptrs_t("down")
-        if ew.is_fp8:
-            dgu_rows = fp8.experts_down_bwd(dcur, gu, ew, b, dgu)
-        elif tq is not None:
+        if tq is not None:
             timed_call("usaf_hip_moe_down_bwd_t", dcur.data_ptr(), H, gu.data_ptr(), b.offsets.data_ptr(), S, E, I,
                        *tq, code, dgu.data_ptr(), *ew._ovl("down_bwd", dt), st)
         else:
@@ -613,9 +615,7 @@ class RoutedExpertsFn(torch.autograd.Function):
             d_wdn = _dense_weight_grad(dcur, act, None, b, ctx.wdt[1])
         dx_slots = torch.empty(S, H, dtype=dt, device=dev)
         tq = ew._ptrs_t("gate_up")
-        if ew.is_fp8:
-            fp8.experts_gate_up_bwd(dgu_rows, ew, b, dx_slots)
-        elif tq is not None:
+        if tq is not None:
             timed_call("usaf_hip_moe_gate_up_bwd_t", dgu.data_ptr(), I, b.offsets.data_ptr(), S, E, H, *tq,
                        code, dx_slots.data_ptr(), *ew._ovl("gate_up_bwd", dt), st)
         else:
@@ -637,6 +637,29 @@ class RoutedExpertsFn(torch.autograd.Function):
             ctx.link.dx = dhs
             dhs = None
         return dhs, dweights, None, None, d_wgu, d_wdn, None, None
+
+
+def _fp8_experts_backward(ctx, dout: torch.Tensor, dweights: torch.Tensor):
+    """RoutedExpertsFn.backward on 8-bit experts.  The 16-bit gradients between the products
+    are stored only where a weight gradient reads them."""
+    hs, gu, act, y = ctx.saved_tensors
+    b, capture, dt, dev = ctx.b, ctx.capture, hs.dtype, hs.device
+    E, H, I, S = ctx.ew.E, ctx.ew.H, ctx.ew.I, b.n_slots
+    want_gu, want_dn = ctx.needs_input_grad[4], ctx.needs_input_grad[5]
+    dcur = torch.empty(S, H, dtype=dt, device=dev) if capture is not None or want_dn else None
+    dgu = torch.empty(S, 2 * I, dtype=dt, device=dev) if capture is not None or want_gu else None
+    dout = dout if dout.data_ptr() % 16 == 0 else dout.clone()
+    dx_slots = torch.empty(S, H, dtype=dt, device=dev)
+    fp8.experts_bwd(fp8.experts_combine_bwd(dout, y, b, dcur, dweights), gu, ctx.ew, b, dgu, dx_slots)
+    dhs = combine(dx_slots, None, b.pair_slot, dt)
+    if capture is not None:
+        _capture(capture, "down_proj", dcur, act, None, b, (E, H, I), dt)
+        _capture(capture, "gate_up_proj", dgu, hs, b.token_idx, b, (E, 2 * I, H), dt)
+    d_wdn = _dense_weight_grad(dcur, act, None, b, ctx.wdt[1]) if want_dn else None
+    d_wgu = _dense_weight_grad(dgu, hs, b.token_idx, b, ctx.wdt[0]) if want_gu else None
+    if ctx.link is not None:
+        ctx.link.dx, dhs = dhs, None
+    return dhs, dweights, None, None, d_wgu, d_wdn, None, None
 
 
 def _no_overlay(ew: ExpertWeights, which: str) -> None:
