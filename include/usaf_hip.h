@@ -590,6 +590,14 @@ int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, int64_t a_total,
                       int32_t dtype, int32_t wide, void* out, void* stream);
 
 /*
+ * usaf_hip_fp8_quantize_rows and usaf_hip_fp8_gemm of one weight [N, K] in one call:
+ * x [M, K], row stride ld -> out [M, N].  ws: usaf_hip_fp8_linear_ws_bytes, 16-byte aligned.
+ */
+int64_t usaf_hip_fp8_linear_ws_bytes(int64_t M, int64_t K);
+int usaf_hip_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* w,
+                        const uint8_t* w_scale, int64_t N, void* out, void* ws, int64_t ws_bytes, void* stream);
+
+/*
  * Between the products of an 8-bit expert layer (the SwiGLU of qwen3moe_dml.py:58-62
  * and its backward, with the layer's 16-bit roundings), for slots below *n_slots:
  * usaf_hip_fp8_swiglu: gu [S, 2I] -> act [S, I], with its codes and scale bytes.

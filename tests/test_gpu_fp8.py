@@ -191,6 +191,15 @@ def test_linear_strides_shapes_and_streams(F):
     assert torch.equal(got, want)
 
 
+def test_linear_has_no_second_derivative(F):
+    t = F.Fp8Tensor.quantize(_rand(64, 128).cuda())
+    x = _rand(2, 128).cuda().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(F.fp8_linear(x, t).sum(), x, create_graph=True)
+    (g,) = torch.autograd.grad(F.fp8_linear(x, t).sum(), x)
+    assert g.shape == x.shape
+
+
 def test_linear_in_a_graph(F):
     t = F.Fp8Tensor.quantize(_rand(200, 384, seed=2, scale=0.1).cuda())
     x = _rand(50, 384, seed=1).cuda()

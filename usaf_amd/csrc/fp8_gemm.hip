@@ -543,3 +543,21 @@ extern "C" int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, int64
   consider(S32x32::launch, S32x32::cycles(g, w16));
   return best(g, dtype, w16, st);
 }
+
+extern "C" int64_t usaf_hip_fp8_linear_ws_bytes(int64_t M, int64_t K) {
+  if (M < 0 || K < 0 || K > 1 << 24 || M > 0x7FFFFFFF) return -1;
+  return M * ((K + FP8_BLOCK - 1) / FP8_BLOCK * FP8_BLOCK + usaf_hip_fp8_scale_stride(K));
+}
+
+extern "C" int usaf_hip_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* w,
+                                   const uint8_t* w_scale, int64_t N, void* out, void* ws, int64_t ws_bytes, void* stream) {
+  const int64_t need = usaf_hip_fp8_linear_ws_bytes(M, K);
+  if (need < 0) return set_error(USAF_ERR_INVALID, "fp8_linear: bad size M=%lld K=%lld", (long long)M, (long long)K);
+  if (M == 0 || N == 0) return clear_error();
+  if (!ws || ws_bytes < need)
+    return set_error(USAF_ERR_INVALID, "fp8_linear: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)need);
+  uint8_t* const q = reinterpret_cast<uint8_t*>(ws);
+  uint8_t* const s = q + M * ((K + FP8_BLOCK - 1) / FP8_BLOCK * FP8_BLOCK);
+  if (int rc = usaf_hip_fp8_quantize_rows(x, dtype, M, K, ld, nullptr, q, s, stream)) return rc;
+  return usaf_hip_fp8_gemm(q, s, M, nullptr, M, w, w_scale, nullptr, 1, N, K, dtype, 0, out, stream);
+}

@@ -163,19 +163,27 @@ class Fp8LinearFn(torch.autograd.Function):
         return _linear(x, w)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy: torch.Tensor):
-        return _linear(dy.to(ctx.dtype), ctx.w.transposed()), None
+        if torch.is_grad_enabled():
+            raise RuntimeError("fp8_linear has no second derivative (create_graph=True)")
+        return _linear(dy if dy.dtype == ctx.dtype else dy.to(ctx.dtype), ctx.w.transposed()), None
 
 
 def _linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
     n, k = w.shape
-    rows = x.reshape(-1, k) if x.numel() else x.new_empty(0, k)
-    out = torch.empty(rows.shape[0], n, dtype=x.dtype, device=x.device)
-    if rows.shape[0]:
-        with on(x.device):
-            product(quantize_rows(rows), w, out)
-    return out.view(*x.shape[:-1], n)
+    dev = x.device
+    rows = x if x.dim() == 2 else x.reshape(-1, k) if x.numel() else x.new_empty(0, k)
+    m = rows.shape[0]
+    if rows.stride(1) != 1 or rows.stride(0) < k:
+        rows = rows.contiguous()
+    out = torch.empty(m, n, dtype=x.dtype, device=dev)
+    if m:
+        need = m * (_blocks(k) * BLOCK + -(-_blocks(k) // 4) * 4)  # usaf_hip_fp8_linear_ws_bytes
+        with on(dev):
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            N.call("usaf_hip_fp8_linear", rows.data_ptr(), N.dtype_code(x.dtype), m, k, max(rows.stride(0), k),
+                   w.q.data_ptr(), w.s.data_ptr(), n, out.data_ptr(), ws.data_ptr(), need, N.stream_ptr(dev))
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
 
 
 def fp8_linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
@@ -200,25 +208,23 @@ def fp8_linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
 # the routed experts (moe.RoutedExpertsFn)
 # ---------------------------------------------------------------------------
 
-def _wide(dtype: torch.dtype) -> bool:
-    """Whether the experts' products take the 16-bit matrix instruction.  The 8-bit one is off by
-    1.5e-5 of the result, which alone neither type shows.  But here results are quantized again,
-    and values that fall to the other side of a code's border by it put an error of about
-    sqrt(1.5e-5 * 2^-4) = 1e-3 into the layer's output: less than bf16's own 1.7e-3,
-    six times fp16's 2.1e-4."""
-    return dtype == torch.float16
+# The experts' products whose results are quantized again (gate and up, the gated activation's
+# gradient) take the 16-bit matrix instruction.  The 8-bit one is off by 1.5e-5 of a result, which
+# neither 16-bit type shows; but values that fall to the other side of a code's border by
+# it (a step of up to 2^-3) put an error of about sqrt(1.5e-5 * 2^-4) = 1e-3 into the layer's output, and
+# more into its gradients: 1.4 to 1.9 times bf16's own rounding in all, six times fp16's.  The
+# two last products, whose results are only rounded, take the 8-bit one.
 
 
 def experts_forward(hs: torch.Tensor, ew, b, gu: torch.Tensor, act: Optional[torch.Tensor], y: torch.Tensor) -> None:
     """gu, act (None: not stored) and y of the slots of bucketing b, for 8-bit experts ew. Each step's
     output is rounded to the activations' dtype, as on the layer's other kernels."""
     S, I = gu.shape[0], gu.shape[1] // 2
-    wide = _wide(hs.dtype)
-    product(quantize_rows(hs), ew.gate_up, gu, b.offsets, b.token_idx, wide=wide)
+    product(quantize_rows(hs), ew.gate_up, gu, b.offsets, b.token_idx, wide=True)
     rows = empty_rows(S, I, hs.device)
     N.call("usaf_hip_fp8_swiglu", gu.data_ptr(), S, I, N.dtype_code(gu.dtype), b.offsets[-1:].data_ptr(), N.ptr(act),
            rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(hs.device))
-    product(rows, ew.down, y, b.offsets, wide=wide)
+    product(rows, ew.down, y, b.offsets)
 
 
 def experts_combine_bwd(dout: torch.Tensor, y: torch.Tensor, b, dcur: Optional[torch.Tensor],
@@ -235,9 +241,8 @@ def experts_combine_bwd(dout: torch.Tensor, y: torch.Tensor, b, dcur: Optional[t
 def experts_bwd(dcur: Rows, gu: torch.Tensor, ew, b, dgu: Optional[torch.Tensor], dx_slots: torch.Tensor) -> None:
     """dgu (None: not stored) and the slots' gradient of the hidden states."""
     S, I = gu.shape[0], gu.shape[1] // 2
-    wide = _wide(gu.dtype)
-    dact = product(dcur, ew.down.transposed(), torch.empty(S, I, dtype=gu.dtype, device=gu.device), b.offsets, wide=wide)
+    dact = product(dcur, ew.down.transposed(), torch.empty(S, I, dtype=gu.dtype, device=gu.device), b.offsets, wide=True)
     rows = empty_rows(S, 2 * I, gu.device)
     N.call("usaf_hip_fp8_swiglu_bwd", gu.data_ptr(), dact.data_ptr(), S, I, N.dtype_code(gu.dtype), b.offsets[-1:].data_ptr(),
            N.ptr(dgu), rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(gu.device))
-    product(rows, ew.gate_up.transposed(), dx_slots, b.offsets, wide=wide)
+    product(rows, ew.gate_up.transposed(), dx_slots, b.offsets)
