@@ -234,22 +234,31 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
     }
     ws_off = ws_at(t, lane < T::N / 128 ? lane : 0);
   };
-  auto issue = [&]() {
-    const int kb = i_step * KW + kw, k = kb < nkb ? kb : nkb - 1;
-    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(sm_lds + i_stage * T::STAGE + kw * T::SLAB));
-    const uint8_t* const a = a_base + (int64_t)k * 128;
-    const uint8_t* const w = w_base + (int64_t)k * 128;
-#pragma unroll
-    for (int i = 0; i < T::A_DMA; ++i) g_dma16(a, a_off[i], to + (T::SHARE * i + part) * 1024 % T::A_BYTES);
-#pragma unroll
-    for (int i = 0; i < T::W_DMA; ++i) g_dma16(w, w_off[i], to + T::A_BYTES + (T::SHARE * i + part) * 1024);
-#pragma unroll
-    for (int i = 0; i < T::S_DMA; ++i) {
-      const int s = T::SHARE * i + part;  // wave-uniform
-      const uint32_t at = to + T::A_BYTES + T::W_BYTES;
-      if (s < T::A_WORDS) g_dma4(as_base + (k & ~3), s_off[i], at + 256 * s);
-      else g_dma4(g.ws - ws_shift, (uint32_t)((ws_off + k) & ~(int64_t)3), at + 256 * T::A_WORDS);
+  // One step's DMAs, in T::DMAS pieces: begin, the pieces, advance
+  uint32_t i_to = 0;
+  int i_k = 0;
+  const uint8_t *i_a = nullptr, *i_w = nullptr;
+  auto begin = [&]() {
+    const int kb = i_step * KW + kw;
+    i_k = kb < nkb ? kb : nkb - 1;
+    i_to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(sm_lds + i_stage * T::STAGE + kw * T::SLAB));
+    i_a = a_base + (int64_t)i_k * 128;
+    i_w = w_base + (int64_t)i_k * 128;
+  };
+  auto piece = [&](int p) {
+    if (p < T::W_DMA) {
+      g_dma16(i_w, w_off[p < T::W_DMA ? p : 0], i_to + T::A_BYTES + (T::SHARE * p + part) * 1024);
+    } else if (p < T::W_DMA + T::A_DMA) {
+      const int i = p - T::W_DMA;
+      g_dma16(i_a, a_off[i < T::A_DMA ? i : 0], i_to + (T::SHARE * i + part) * 1024 % T::A_BYTES);
+    } else if (p < T::DMAS) {
+      const int i = p - T::W_DMA - T::A_DMA, s = T::SHARE * i + part;  // wave-uniform
+      const uint32_t sc = i_to + T::A_BYTES + T::W_BYTES;
+      if (s < T::A_WORDS) g_dma4(as_base + (i_k & ~3), s_off[i < T::S_DMA ? i : 0], sc + 256 * s);
+      else g_dma4(g.ws - ws_shift, (uint32_t)((ws_off + i_k) & ~(int64_t)3), sc + 256 * T::A_WORDS);
     }
+  };
+  auto advance = [&]() {
     i_stage = i_stage + 1 == T::NS ? 0 : i_stage + 1;
     if (++i_step == steps) {
       if (i_id + stride < end) {
@@ -265,7 +274,12 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
   f32x16 acc[MI][NI];
   int stage = 0;
   open();
-  for (int s = 0; s < T::NS - 1; ++s) issue();
+  for (int s = 0; s < T::NS - 1; ++s) {
+    begin();
+#pragma unroll
+    for (int p = 0; p < T::DMAS; ++p) piece(p);
+    advance();
+  }
   for (int id = id0; id < end; id += stride) {
     const Place t = place(id);
     const int mine = t.valid - 32 * MI * wm;  // slots of the wave's part
@@ -280,13 +294,18 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
     for (int step = 0; step < steps; ++step) {
       wait_vmcnt<(T::NS - 2) * T::DMAS>();  // the wave's DMAs of this step (and what is older)
       lds_barrier();                        // and everyone's; the stage before this one has been read
-      issue();
+      begin();
       const int kb = step * KW + kw;
       const uint8_t* const sa = sm + stage * T::STAGE + kw * T::SLAB;
       const uint8_t* const sw = sa + T::A_BYTES;
       const uint32_t* const sc = reinterpret_cast<const uint32_t*>(sw + T::W_BYTES);
       stage = stage + 1 == T::NS ? 0 : stage + 1;
-      if (KW > 1 && kb >= nkb) continue;  // wave-uniform
+      if (KW > 1 && kb >= nkb) {  // wave-uniform
+#pragma unroll
+        for (int p = 0; p < T::DMAS; ++p) piece(p);
+        advance();
+        continue;
+      }
       auto word = [&](const uint8_t* rows, int r, int c) {
         return *reinterpret_cast<const u32x4*>(rows + r * 128 + 16 * (c ^ g_swz(r)));
       };
@@ -296,40 +315,69 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
 #pragma unroll
       for (int k = 0; k < NI; ++k)
         s_w[k] = (int)(sc[64 * T::A_WORDS + (32 * (NI * wn + k)) / 128] >> (8 * (int)((ws_byte[k] + kb) & 3)));
+      // A wave's DMAs go out PER at a time between its matrix instructions: eight waves sending all of
+      // theirs first wait for the address unit (16 cycles each, 1,200 in all) before they multiply
+      constexpr int PER = (T::DMAS + MI - 1) / MI > 2 ? (T::DMAS + MI - 1) / MI : 2;
+      u32x4 w0[NI], w1[NI], a0, a1;
+      auto load_w = [&](int h, u32x4(&x0)[NI], u32x4(&x1)[NI]) {
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+          x0[k] = word(sw, 32 * (NI * wn + k) + l32, 4 * h + 2 * half);
+          x1[k] = word(sw, 32 * (NI * wn + k) + l32, 4 * h + 2 * half + 1);
+        }
+      };
+      auto load_a = [&](int h, int i, u32x4& x0, u32x4& x1) {
+        x0 = word(sa, 32 * (MI * wm + i) + l32, 4 * h + 2 * half);
+        x1 = word(sa, 32 * (MI * wm + i) + l32, 4 * h + 2 * half + 1);
+      };
+      load_w(0, w0, w1);
+      load_a(0, 0, a0, a1);
+      u32x4 wf[WIDE ? NI : 1][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int c = 4 * h + 2 * half;
-        if constexpr (!WIDE) {
-          u32x4 w0[NI], w1[NI];
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int k = 0; k < NI; ++k) values16(w0[k], w1[k], s_w[k], wf[k]);
+        }
+        u32x4 v0[NI], v1[NI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          // the next fragments, while these are multiplied
+          u32x4 b0 = a0, b1 = a1;
+          if (i + 1 < MI) {
+            load_a(h, i + 1, b0, b1);
+          } else if (h == 0) {
+            load_w(1, v0, v1);
+            load_a(1, 0, b0, b1);
+          }
+#pragma unroll
+          for (int p = 0; p < PER; ++p) piece((h * MI + i) * PER + p);
+          if (i < live) {  // wave-uniform
+            if constexpr (!WIDE) {
+#pragma unroll
+              for (int k = 0; k < NI; ++k) acc[i][k] = mfma8(w0[k], w1[k], a0, a1, acc[i][k], s_w[k], s_a[i]);
+            } else {
+              u32x4 af[4];
+              values16(a0, a1, s_a[i], af);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int k = 0; k < NI; ++k) acc[i][k] = mfma32<USAF_BF16>(wf[k][j], af[j], acc[i][k]);
+            }
+          }
+          a0 = b0;
+          a1 = b1;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (h == 0) {
 #pragma unroll
           for (int k = 0; k < NI; ++k) {
-            w0[k] = word(sw, 32 * (NI * wn + k) + l32, c);
-            w1[k] = word(sw, 32 * (NI * wn + k) + l32, c + 1);
-          }
-#pragma unroll
-          for (int i = 0; i < MI; ++i) {
-            if (i >= live) continue;  // wave-uniform
-            const u32x4 a0 = word(sa, 32 * (MI * wm + i) + l32, c), a1 = word(sa, 32 * (MI * wm + i) + l32, c + 1);
-#pragma unroll
-            for (int k = 0; k < NI; ++k) acc[i][k] = mfma8(w0[k], w1[k], a0, a1, acc[i][k], s_w[k], s_a[i]);
-          }
-        } else {
-          u32x4 wf[NI][4];
-#pragma unroll
-          for (int k = 0; k < NI; ++k)
-            values16(word(sw, 32 * (NI * wn + k) + l32, c), word(sw, 32 * (NI * wn + k) + l32, c + 1), s_w[k], wf[k]);
-#pragma unroll
-          for (int i = 0; i < MI; ++i) {
-            if (i >= live) continue;
-            u32x4 af[4];
-            values16(word(sa, 32 * (MI * wm + i) + l32, c), word(sa, 32 * (MI * wm + i) + l32, c + 1), s_a[i], af);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int k = 0; k < NI; ++k) acc[i][k] = mfma32<USAF_BF16>(wf[k][j], af[j], acc[i][k]);
+            w0[k] = v0[k];
+            w1[k] = v1[k];
           }
         }
       }
+      advance();
     }
     // ---- results, through the stage that was read last: nothing is sent there before the next
     //      step's barrier.  A lane's values 4 q .. 4 q + 3 of a 32 x 32 block are columns 8 q +
