@@ -317,7 +317,8 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
         s_w[k] = (int)(sc[64 * T::A_WORDS + (32 * (NI * wn + k)) / 128] >> (8 * (int)((ws_byte[k] + kb) & 3)));
       // A wave's DMAs go out PER at a time between its matrix instructions: eight waves sending all of
       // theirs first wait for the address unit (16 cycles each, 1,200 in all) before they multiply
-      constexpr int PER = (T::DMAS + MI - 1) / MI > 2 ? (T::DMAS + MI - 1) / MI : 2;
+      constexpr int SLOTS = MI > 1 ? MI : 2 * MI - 1, PER = (T::DMAS + SLOTS - 1) / SLOTS > 2 ? (T::DMAS + SLOTS - 1) / SLOTS : 2;
+      static_assert((2 * MI - 1) * PER >= T::DMAS, "all pieces of a step go out");
       u32x4 w0[NI], w1[NI], a0, a1;
       auto load_w = [&](int h, u32x4(&x0)[NI], u32x4(&x1)[NI]) {
 #pragma unroll
@@ -351,7 +352,10 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
             load_a(1, 0, b0, b1);
           }
 #pragma unroll
-          for (int p = 0; p < PER; ++p) piece((h * MI + i) * PER + p);
+          for (int p = 0; p < PER; ++p) {
+            const int at = (h * MI + i - 1) * PER + p;  // none before the first matrix instructions
+            if (at >= 0) piece(at);
+          }
           if (i < live) {  // wave-uniform
             if constexpr (!WIDE) {
 #pragma unroll
