@@ -397,3 +397,110 @@ def test_refusals_on_the_gpu(F):
                        torch.bfloat16)
     with pytest.raises(TypeError, match="both"):
         ExpertWeights(ew.gate_up, torch.empty(2, 128, 128, dtype=torch.bfloat16, device="cuda"))
+
+# every tile of the product: few to many rows, narrow and wide outputs, short and long contractions, one expert and many
+TILES = [(None, 1, 33, 128), (None, 70, 33, 640), (None, 1, 2000, 1300), (None, 33, 4100, 640), (None, 4100, 200, 300),
+         (None, 1000, 4100, 128), (None, 2000, 4100, 300), (None, 513, 1030, 640), (1, 2000, 130, 640), (3, 33, 4100, 640),
+         (8, 200, 4100, 300), (8, 500, 4100, 128), (8, 1500, 4100, 300), (40, 33, 1030, 300), (40, 2000, 2000, 129),
+         (255, 300, 130, 256)]
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("E,M,N,K", TILES)
+def test_product_of_whole_numbers_on_every_tile(F, E, M, N, K, wide):
+    """Exact, as test_linear_sums_whole_numbers_exactly: gathered rows, experts without a slot, slots behind the last one left."""
+    dtype = DTYPES[(M + N) % 2]
+    g = torch.Generator().manual_seed(M + N + K)
+    n_rows = M if E is None else M // 2 + 1
+    x = torch.randint(-1, 2, (n_rows, K), generator=g).to(dtype).cuda()
+    w = torch.randint(-1, 2, ((E, N, K) if E else (N, K)), generator=g).float().cuda()
+    out = torch.full((M, N), 333.0, dtype=dtype, device="cuda")
+    rows, t = F.quantize_rows(x), F.Fp8Tensor.quantize(w)
+    if E is None:
+        F.product(rows, t, out, wide=wide)
+        assert torch.equal(out.float(), x.float() @ w.t())
+        return
+    ends = torch.randint(0, M - M // 8 + 1, (E,), generator=g).sort().values.tolist()
+    offs = [0] + ends[:-1] + [M - M // 8]
+    tok = torch.randint(0, n_rows, (M,), generator=g).to(torch.int32).cuda()
+    F.product(rows, t, out, torch.tensor(offs, dtype=torch.int32, device="cuda"), tok, wide=wide)
+    picked = x.float()[tok.long()]
+    for e in range(E):
+        lo, hi = offs[e], offs[e + 1]
+        assert torch.equal(out[lo:hi].float(), picked[lo:hi] @ w[e].t())
+    assert bool((out[offs[-1]:] == 333).all())
+
+
+def test_what_is_kept_is_built_once_for_all_streams(F):
+    """The transpose is built on one stream behind other work and read on another without a wait."""
+    from usaf_amd.moe import Q4Tensor
+    w = _rand(2048, 4096, seed=2, scale=0.1).cuda()
+    x = _rand(40, 4096, seed=1).cuda()
+    t, again = F.Fp8Tensor.quantize(w), F.Fp8Tensor.quantize(w)
+    q4 = Q4Tensor.quantize(w.half().view(4, 512, 4096))
+    dy = _rand(40, 2048, seed=3).cuda()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        busy = torch.ones(8192, 8192, device="cuda")
+        for _ in range(3):
+            busy = busy @ busy * 2.0 ** -13
+        t.transposed()
+        q4.scale_zero_by_group()
+    xv = x.requires_grad_(True)
+    (got,) = torch.autograd.grad(F.fp8_linear(xv, t), xv, dy)
+    words = q4.scale_zero_by_group().clone()
+    torch.cuda.synchronize()
+    (want,) = torch.autograd.grad(F.fp8_linear(xv, again), xv, dy)
+    assert torch.equal(got, want)
+    assert torch.equal(words, q4.scale_zero().view(4, 512, 32).transpose(1, 2))
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            F.fp8_linear(xv, t)
+
+
+def test_a_layer_tuned_and_served(F):
+    """8-bit experts as they are used: prompt and gradient on the routed path of a patched block, a step of its
+    norm's weight, then tokens one by one through the few-token layer, the output head in 8 bits."""
+    from types import SimpleNamespace
+    from usaf_amd import qwen3moe_dml as Q
+    E, H, I, k, V = 8, 256, 128, 2, 1000
+    ew = _experts(F, E, H, I, seed=20)
+    head = F.Fp8Tensor.quantize(_rand(V, H, seed=22, scale=0.05).cuda())
+    router = torch.zeros(E, H, dtype=torch.bfloat16, device="cuda")
+    router[torch.arange(E), torch.arange(E)] = 1
+
+    class Experts(torch.nn.Module):
+        forward = Q.dml_qwen3_experts_forward
+
+    class Block(torch.nn.Module):
+        forward = Q.dml_qwen3_moe_block_forward
+
+    ex, block = Experts(), Block()
+    ex._usaf_q4 = {"gate_up_proj": ew.gate_up, "down_proj": ew.down}
+    block.experts, block.gate = ex, SimpleNamespace(weight=router, top_k=k, norm_topk_prob=True)
+    block._usaf_few_tokens = 4
+    x = _rand(1, 48, H, seed=23).cuda()
+    # the router reads whole numbers, so both paths route alike (no ties at the threshold)
+    x[0, :, :E] = torch.stack([torch.randperm(E, generator=torch.Generator().manual_seed(i)) for i in range(48)]).to(x)
+    scale = torch.ones(H, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+
+    def model(x):
+        return F.fp8_linear(x * scale + block(x * scale), head)
+
+    logits = model(x)
+    assert logits.grad_fn is not None and logits.shape == (1, 48, V)
+    logits.float().logsumexp(-1).sum().backward()
+    assert bool(torch.isfinite(scale.grad).all()) and float(scale.grad.abs().max()) > 0
+    with torch.no_grad():
+        whole = model(x)
+        assert torch.equal(whole, logits.detach())
+        one = torch.cat([model(x[:, i:i + 1]) for i in range(48)], 1)
+        four = torch.cat([model(x[:, i:i + 4]) for i in range(0, 48, 4)], 1)
+    # The few-token path leaves the layer's activations unquantized.  On the routed path each of two products has operands off by
+    # half a step of e4m3 at most (2^-4): a share of about 2^-4 / sqrt(3) of each term's size at random signs, so a relative error of
+    # sqrt(2) * 2^-4 / sqrt(3) = 5 % of the layer's output; gate times up doubles that of its two factors.  The output head
+    # quantizes both sides' inputs again, another 2 * 2^-4 / sqrt(3) = 7 % between them.  Together less than 20 %.
+    ref = whole.double()
+    for got in (one, four):
+        assert float((got.double() - ref).norm() / ref.norm()) < 0.2

@@ -6,7 +6,7 @@ import torch
 
 from usaf_amd import _native as N
 from usaf_amd import fp8
-from usaf_amd.moe import ExpertWeights
+from usaf_amd.moe import ExpertWeights, Q4Tensor, routed_experts
 
 
 def _t(*shape):
@@ -95,3 +95,35 @@ def test_entry_points_check_their_arguments():
     assert lib.usaf_hip_fp8_dequantize(None, p, 1, 8, 8, p, N.F32, None) == inval
     assert lib.usaf_hip_fp8_transpose(odd, p, 1, 8, 8, p, p, None) == inval
     assert [lib.usaf_hip_fp8_scale_stride(c) for c in (0, 1, 512, 513, -1)] == [0, 4, 4, 8, -1]
+    few, need = lib.usaf_hip_moe_few, lib.usaf_hip_moe_few_ws_bytes
+    size = need(2, 4, 2, 128, 128)
+    assert size > 0 and need(0, 4, 2, 128, 128) == 0 and need(32, 256, 16, 16384, 65536) < 2 << 30
+    assert all(need(*a) == -1 for a in [(33, 4, 2, 128, 128), (-1, 4, 2, 128, 128), (2, 257, 2, 128, 128), (2, 4, 5, 128, 128),
+                                        (2, 4, 0, 128, 128), (2, 32, 17, 128, 128), (2, 4, 2, 100, 128), (2, 4, 2, 128, 100),
+                                        (2, 4, 2, 16512, 128), (2, 4, 2, 128, 65664), (2, 4, 2, 0, 128), (2, 0, 0, 128, 128)])
+    good = dict(x=p, T=2, H=128, router=p, E=4, k=2, norm=1, dt=N.BF16, I=128, eight=1, gu=p, gs=p, dn=p, ds=p, out=p, ws=p,
+                ws_bytes=size, stream=None)
+    assert few(*{**good, "T": 0, "x": None, "ws": None, "ws_bytes": 0}.values()) == ok
+    for bad in [{"x": None}, {"router": None}, {"gu": None}, {"gs": None}, {"dn": None}, {"ds": None}, {"out": None}, {"ws": None},
+                {"x": odd}, {"router": odd}, {"gu": odd}, {"dn": odd}, {"ws": odd}, {"out": odd}, {"ws_bytes": 64}, {"dt": N.F32},
+                {"eight": 0, "gs": odd}, {"eight": 0, "ds": odd}]:
+        assert few(*{**good, **bad}.values()) == inval, bad
+    for bad in [{"T": 33}, {"H": 130}, {"I": 64}, {"E": 300}, {"k": 5}]:
+        assert few(*{**good, **bad}.values()) != ok, bad
+
+
+def test_capture_refuses_what_is_kept_or_wants_a_gradient(monkeypatch):
+    """A tensor first built in a capture would hold nothing until the replay; captured training steps are switched off."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    w = _t(128, 128)
+    with pytest.raises(RuntimeError, match="captured"):
+        w.transposed()
+    assert w._t is None
+    q4 = Q4Tensor(torch.zeros(512, 64, dtype=torch.int8), torch.ones(512, dtype=torch.float16),
+                  torch.zeros(512, dtype=torch.float16), torch.Size((2, 256, 128)))
+    with pytest.raises(RuntimeError, match="captured"):
+        q4.scale_zero_by_group()
+    assert q4._szg is None
+    x = torch.zeros(3, 128, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(RuntimeError, match="captured"):
+        routed_experts(x, torch.zeros(3, 2, dtype=torch.bfloat16), ExpertWeights(_t(2, 256, 128), _t(2, 128, 128)))

@@ -204,6 +204,12 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def refuse_capture(what: str) -> None:
+    """Raise where the current stream is being captured into a graph."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} cannot be captured into a graph: make it before the capture, or without a gradient")
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

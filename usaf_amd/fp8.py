@@ -43,7 +43,9 @@ class Fp8Tensor:
 
     q: e4m3 codes (uint8 or float8_e4m3fn), [.., R, 128 * ceil(C / 128)], zeros behind
     column C; s: E8M0 bytes (uint8), [.., ceil(R / 128), ceil(C / 128)].  The tensors
-    are used as they are; a code behind column C that is not zero gives wrong products."""
+    are used as they are; a code behind column C that is not zero gives wrong products.
+    They are not written to once the weight has been used, and a weight is kept until the
+    work that reads it, on whichever streams, has ended."""
 
     def __init__(self, q: torch.Tensor, s: torch.Tensor, shape: Sequence[int]):
         shape = torch.Size(int(d) for d in shape)
@@ -92,14 +94,16 @@ class Fp8Tensor:
 
     def transposed(self) -> "Fp8Tensor":
         """The transpose (of each matrix), which the grad-input product reads: exact, built
-        at the first call and kept (as many bytes again)."""
+        at the first call (not in a stream capture) and kept (as many bytes again)."""
         if self._t is None:
+            N.refuse_capture("Fp8Tensor.transposed: the first call")
             *lead, rows, cols = self.shape
             q = torch.empty(*lead, cols, _blocks(rows) * BLOCK, dtype=torch.uint8, device=self.device)
             s = torch.empty(*lead, _blocks(cols), _blocks(rows), dtype=torch.uint8, device=self.device)
             with on(self.device):
                 N.call("usaf_hip_fp8_transpose", self.q.data_ptr(), self.s.data_ptr(), *self._erc(), q.data_ptr(),
                        s.data_ptr(), N.stream_ptr(self.device))
+            torch.cuda.current_stream(self.device).synchronize()  # any stream may read it from here on
             self._t = Fp8Tensor(q, s, (*lead, cols, rows))
         return self._t
 
@@ -137,8 +141,9 @@ def quantize_rows(x: torch.Tensor, n_rows: Optional[torch.Tensor] = None) -> Row
     if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
         x = x.contiguous()
     rows = empty_rows(x.shape[0], x.shape[1], x.device)
-    N.call("usaf_hip_fp8_quantize_rows", x.data_ptr(), N.dtype_code(x.dtype), x.shape[0], x.shape[1],
-           max(x.stride(0), x.shape[1]), N.ptr(n_rows), rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(x.device))
+    with on(x.device):
+        N.call("usaf_hip_fp8_quantize_rows", x.data_ptr(), N.dtype_code(x.dtype), x.shape[0], x.shape[1],
+               max(x.stride(0), x.shape[1]), N.ptr(n_rows), rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(x.device))
     return rows
 
 
@@ -149,8 +154,10 @@ def product(x: Rows, w: Fp8Tensor, out: torch.Tensor, offsets: Optional[torch.Te
     E, n, k = w._erc()
     if x.cols != k or out.shape[1] != n:
         raise ValueError(f"fp8 product: rows of {x.cols} and output {tuple(out.shape)} do not fit the weight {tuple(w.shape)}")
-    N.call("usaf_hip_fp8_gemm", x.q.data_ptr(), x.s.data_ptr(), x.q.shape[0], N.ptr(row_of), out.shape[0], w.q.data_ptr(),
-           w.s.data_ptr(), N.ptr(offsets), E, n, k, N.dtype_code(out.dtype), 1 if wide else 0, out.data_ptr(), N.stream_ptr(out.device))
+    with on(out.device):
+        N.call("usaf_hip_fp8_gemm", x.q.data_ptr(), x.s.data_ptr(), x.q.shape[0], N.ptr(row_of), out.shape[0],
+               w.q.data_ptr(), w.s.data_ptr(), N.ptr(offsets), E, n, k, N.dtype_code(out.dtype), 1 if wide else 0,
+               out.data_ptr(), N.stream_ptr(out.device))
     return out
 
 
@@ -190,7 +197,8 @@ def fp8_linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
     """F.linear with an 8-bit block-scaled weight: x [..., K] fp16 / bf16, w [N, K] ->
     [..., N] in x's dtype, summed in fp32.  Differentiable in x (the weight is frozen);
     the first backward builds ``w.transposed()``.  A value of x that is not finite makes
-    its output row NaN."""
+    its output row NaN.  A stream capture takes the call without a gradient only, as the
+    graph of a training step is switched off (graphs.py)."""
     if len(w.shape) != 2:
         raise ValueError(f"fp8_linear: need a weight [N, K], got {tuple(w.shape)}")
     if x.dtype not in _ACT:
@@ -200,6 +208,7 @@ def fp8_linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
     if x.device != w.device or not x.is_cuda:
         raise ValueError(f"fp8_linear: activations on {x.device}, weight on {w.device}: both on one GPU")
     if torch.is_grad_enabled() and x.requires_grad:
+        N.refuse_capture("fp8_linear of activations that want a gradient")
         return Fp8LinearFn.apply(x, w)
     return _linear(x, w)
 

@@ -90,10 +90,15 @@ class Q4Tensor:
 
     def scale_zero_by_group(self) -> torch.Tensor:
         """scale_zero() of [E, R, C] as int32 [E, C / 128, R]: neighbouring rows' words side by
-        side, as the few-token layer reads them (built once, on the tensor's device)."""
+        side, as the few-token layer reads them (built once, on the tensor's device, not in a
+        stream capture)."""
         if self._szg is None or self._szg.device != self.q.device:
+            N.refuse_capture("Q4Tensor.scale_zero_by_group: the first call")
             E, rows, cols = (int(d) for d in self.shape)
-            self._szg = self.scale_zero().view(E, rows, cols // 128).transpose(1, 2).contiguous()
+            words = torch.stack((self.s, self.z), -1).view(torch.int32)
+            szg = words.view(E, rows, cols // 128).transpose(1, 2).contiguous()
+            torch.cuda.current_stream(szg.device).synchronize()  # any stream may read it from here on
+            self._szg = szg
         return self._szg
 
     def transposed(self) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -781,6 +786,8 @@ def routed_experts(hs: torch.Tensor, weights: torch.Tensor, experts: ExpertWeigh
     gradient of both branches (HsGradLink)."""
     wg, wd = weight_params if weight_params is not None else (None, None)
     slots = None if slot_capacity is None and overflow is None else (slot_capacity, overflow)
+    if experts.is_fp8 and torch.is_grad_enabled() and (hs.requires_grad or weights.requires_grad):
+        N.refuse_capture("a pass over 8-bit experts that wants a gradient")
     return RoutedExpertsFn.apply(hs, weights, experts, capture, wg, wd, slots, link)
 
 
