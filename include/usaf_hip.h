@@ -591,7 +591,8 @@ int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, int64_t a_total,
 
 /*
  * usaf_hip_fp8_quantize_rows and usaf_hip_fp8_gemm of one weight [N, K] in one call:
- * x [M, K], row stride ld -> out [M, N].  ws: usaf_hip_fp8_linear_ws_bytes, 16-byte aligned.
+ * x [M, K], row stride ld -> out [M, N].  ws: usaf_hip_fp8_linear_ws_bytes, 16-byte aligned; 0
+ * bytes (ws may be NULL) for a few rows, which one launch serves, summed as with wide != 0.
  */
 int64_t usaf_hip_fp8_linear_ws_bytes(int64_t M, int64_t K);
 int usaf_hip_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* w,

@@ -107,6 +107,8 @@ def test_values_that_are_not_finite(F):
 
 SIZES = [(1, 1, 1), (1, 64, 128), (2, 5, 127), (7, 130, 129), (31, 257, 640), (33, 128, 256), (64, 96, 384), (65, 1411, 300),
          (129, 255, 1024), (300, 384, 512), (257, 640, 2027), (513, 300, 896)]
+# ... and of the product for a few rows: one to 32 rows, one to four rounds of column tiles, short and long contractions
+SIZES += [(8, 4100, 2000), (1, 70, 16001), (17, 33, 300), (32, 8200, 512), (5, 9001, 384), (1, 25000, 130), (16, 640, 1024)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=_ids)

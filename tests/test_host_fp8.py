@@ -81,11 +81,18 @@ def test_entry_points_check_their_arguments():
     assert gemm(p, p, 1 << 40, None, 1 << 40, p, p, None, 1, 8, 8, N.BF16, 0, p, None) == inval
     assert gemm(p, p, 1, None, 1, p, p, p, 256, 8, 8, N.BF16, 0, p, None) == N.USAF_ERR_UNSUPPORTED
     linear = lib.usaf_hip_fp8_linear
-    assert [lib.usaf_hip_fp8_linear_ws_bytes(m, k) for m, k in ((3, 130), (0, 5), (-1, 5))] == [3 * (256 + 4), 0, -1]
+    assert [lib.usaf_hip_fp8_linear_ws_bytes(m, k) for m, k in ((40, 130), (3, 130), (0, 5), (-1, 5))] == [40 * (256 + 4), 0, 0, -1]
     assert linear(None, N.BF16, 0, 8, 8, None, None, 8, None, None, 0, None) == ok
-    assert linear(p, N.BF16, 1, 8, 8, p, p, 8, p, p, 131, None) == inval
-    assert linear(p, N.BF16, 1, 8, 8, p, p, 8, p, None, 1 << 20, None) == inval
-    assert linear(p, N.BF16, 1, 8, 7, p, p, 8, p, p, 1 << 20, None) == inval
+    assert linear(p, N.BF16, 40, 8, 8, p, p, 8, p, p, 40 * 132 - 1, None) == inval
+    assert linear(p, N.BF16, 40, 8, 8, p, p, 8, p, None, 1 << 20, None) == inval
+    for m in (1, 40):
+        assert linear(p, N.BF16, m, 8, 7, p, p, 8, p, p, 1 << 20, None) == inval
+        assert linear(p, N.F32, m, 8, 8, p, p, 8, p, p, 1 << 20, None) == inval
+        assert linear(p, N.BF16, m, 8, 8, odd, p, 8, p, p, 1 << 20, None) == inval
+        assert linear(p, N.BF16, m, 8, 8, p, p, -8, p, p, 1 << 20, None) == inval
+        assert linear(None, N.BF16, m, 8, 8, p, p, 8, p, p, 1 << 20, None) == inval
+        assert linear(p, N.BF16, m, 8, 8, p, None, 8, p, p, 1 << 20, None) == inval
+        assert linear(p, N.BF16, m, 8, 8, p, p, 8, None, p, 1 << 20, None) == inval
     assert lib.usaf_hip_fp8_swiglu(p, 1, 100, N.BF16, p, p, p, p, None) == inval
     assert lib.usaf_hip_fp8_swiglu(p, 1, 128, N.BF16, None, p, p, p, None) == inval
     assert lib.usaf_hip_fp8_swiglu(None, 0, 128, N.BF16, None, None, None, None, None) == ok

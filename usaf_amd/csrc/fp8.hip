@@ -18,66 +18,6 @@ namespace {
 
 constexpr int FB = FP8_BLOCK;
 
-// E8M0 byte of a block's largest finite magnitude.
-__device__ __forceinline__ int e8m0_of(float amax) {
-  const uint32_t b = __float_as_uint(amax);
-  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7FFFFFu) > 0x600000u);  // 448 = 1.75 * 2^8
-  return (e < -120 ? -120 : e > 120 ? 120 : e) + 127;
-}
-__device__ __forceinline__ float inv_scale(int e8m0) { return __uint_as_float((uint32_t)(254 - e8m0) << 23); }
-
-__device__ __forceinline__ float finite_abs(float v) {
-  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
-  return b < 0x7F800000u ? __uint_as_float(b) : 0.f;
-}
-
-// Four scaled values -> four codes.
-__device__ __forceinline__ uint32_t to_codes(const float (&v)[4], float inv) {
-  uint32_t o = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
-  o = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, (int)o, true);
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if ((__float_as_uint(v[j]) & 0x7F800000u) == 0x7F800000u) o = (o & ~(0xFFu << (8 * j))) | (0x7Fu << (8 * j));
-  return o;
-}
-
-__device__ __forceinline__ float max16(float v) {  // over 16 neighbouring lanes
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
-  return v;
-}
-
-// 8 neighbouring values of a 16-bit row; `left` of them exist.
-template <int DT>
-__device__ __forceinline__ void load8(const uint16_t* p, bool vec, int left, float (&v)[8]) {
-  if (vec && left >= 8) {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x2 f = unpack2<DT>(w[j]);
-      v[2 * j] = f.x;
-      v[2 * j + 1] = f.y;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < left ? load_as_f32<DT>(p, j) : 0.f;
-  }
-}
-
-// Quantizes 16 lanes' 8 values each (one block of a row) and stores them: the codes
-// at q, the scale byte at s.
-__device__ __forceinline__ void store_block(const float (&v)[8], int lane16, uint8_t* q, uint8_t* s) {
-  float m = 0.f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(v[j]));
-  const int e = e8m0_of(max16(m));
-  const float inv = inv_scale(e);
-  const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
-  *reinterpret_cast<uint2*>(q) = uint2{to_codes(a, inv), to_codes(b, inv)};
-  if (lane16 == 0) *s = (uint8_t)e;
-}
-
 // Rows of 16-bit values -> codes [rows, kp] and scale bytes [rows, sp].  16 lanes a
 // block; columns past the row's end are zeros.  n_rows (device, may be null): rows
 // from there on are left as they are.
@@ -322,7 +262,8 @@ extern "C" int usaf_hip_fp8_quantize_rows(const void* x, int32_t dtype, int64_t 
     return set_error(USAF_ERR_INVALID, "fp8_quantize_rows: need 0 <= cols <= ld, cols <= 2^30");
   if (rows == 0 || cols == 0) return clear_error();
   if (!x || !q || !s) return set_error(USAF_ERR_INVALID, "fp8_quantize_rows: null pointer");
-  if ((uintptr_t)q % 16) return set_error(USAF_ERR_INVALID, "fp8_quantize_rows: codes must be 16-byte aligned");
+  if ((uintptr_t)q % 16 || (uintptr_t)x % 2)
+    return set_error(USAF_ERR_INVALID, "fp8_quantize_rows: codes must be 16-byte and values 2-byte aligned");
   const int64_t nkb = (cols + FP8_BLOCK - 1) / FP8_BLOCK;
   const bool vec = ((uintptr_t)x % 16) == 0 && ld % 8 == 0;
   unsigned blocks;

@@ -68,17 +68,6 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
   const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
   return reinterpret_cast<const uint8_t*>((uintptr_t)(((uint64_t)hi << 32) | (uint64_t)lo));
 }
-// 32 codes of a lane -> four bf16 fragment registers of their values, exact.
-__device__ __forceinline__ void values16(const u32x4 lo, const u32x4 hi, int e8m0, u32x4 (&o)[4]) {
-  const int b = e8m0 & 0xFF;
-  const float s = __uint_as_float(b == 0 ? 0x00400000u : (uint32_t)b << 23);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t w = j < 4 ? lo[j] : hi[j - 4];
-    o[j >> 1][2 * (j & 1)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
-    o[j >> 1][2 * (j & 1) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true));
-  }
-}
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -598,7 +587,7 @@ extern "C" int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, int64
 
 extern "C" int64_t usaf_hip_fp8_linear_ws_bytes(int64_t M, int64_t K) {
   if (M < 0 || K < 0 || K > 1 << 24 || M > 0x7FFFFFFF) return -1;
-  return M * ((K + FP8_BLOCK - 1) / FP8_BLOCK * FP8_BLOCK + usaf_hip_fp8_scale_stride(K));
+  return fp8_small_ok(M, K) ? 0 : M * ((K + FP8_BLOCK - 1) / FP8_BLOCK * FP8_BLOCK + usaf_hip_fp8_scale_stride(K));
 }
 
 extern "C" int usaf_hip_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* w,
@@ -606,6 +595,13 @@ extern "C" int usaf_hip_fp8_linear(const void* x, int32_t dtype, int64_t M, int6
   const int64_t need = usaf_hip_fp8_linear_ws_bytes(M, K);
   if (need < 0) return set_error(USAF_ERR_INVALID, "fp8_linear: bad size M=%lld K=%lld", (long long)M, (long long)K);
   if (M == 0 || N == 0) return clear_error();
+  if (N < 0 || N > 1 << 24 || ld < K || K == 0)
+    return set_error(USAF_ERR_INVALID, "fp8_linear: need 0 <= N <= 2^24 and ld >= K >= 1");
+  if (dtype != USAF_BF16 && dtype != USAF_F16) return set_error(USAF_ERR_INVALID, "fp8_linear: dtype must be fp16 or bf16");
+  if (!x || !w || !w_scale || !out) return set_error(USAF_ERR_INVALID, "fp8_linear: null pointer");
+  if ((uintptr_t)w % 16 || ((uintptr_t)out | (uintptr_t)x) % 2)
+    return set_error(USAF_ERR_INVALID, "fp8_linear: codes must be 16-byte, rows and output 2-byte aligned");
+  if (fp8_small_ok(M, K)) return fp8_small(x, dtype, M, K, ld, w, w_scale, N, out, as_stream(stream));
   if (!ws || ws_bytes < need)
     return set_error(USAF_ERR_INVALID, "fp8_linear: workspace of %lld bytes, need %lld", (long long)ws_bytes, (long long)need);
   uint8_t* const q = reinterpret_cast<uint8_t*>(ws);

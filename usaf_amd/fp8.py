@@ -185,17 +185,17 @@ def _linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
         rows = rows.contiguous()
     out = torch.empty(m, n, dtype=x.dtype, device=dev)
     if m:
-        need = m * (_blocks(k) * BLOCK + -(-_blocks(k) // 4) * 4)  # usaf_hip_fp8_linear_ws_bytes
+        need = N.load().usaf_hip_fp8_linear_ws_bytes(m, k)
         with on(dev):
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
             N.call("usaf_hip_fp8_linear", rows.data_ptr(), N.dtype_code(x.dtype), m, k, max(rows.stride(0), k),
-                   w.q.data_ptr(), w.s.data_ptr(), n, out.data_ptr(), ws.data_ptr(), need, N.stream_ptr(dev))
+                   w.q.data_ptr(), w.s.data_ptr(), n, out.data_ptr(), N.ptr(ws), need, N.stream_ptr(dev))
     return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
 
 
 def fp8_linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
     """F.linear with an 8-bit block-scaled weight: x [..., K] fp16 / bf16, w [N, K] ->
-    [..., N] in x's dtype, summed in fp32.  Differentiable in x (the weight is frozen);
+    [..., N] in x's dtype, summed in fp32 (in another order for a few rows than for many).  Differentiable in x (the weight is frozen);
     the first backward builds ``w.transposed()``.  A value of x that is not finite makes
     its output row NaN.  A stream capture takes the call without a gradient only, as the
     graph of a training step is switched off (graphs.py)."""
