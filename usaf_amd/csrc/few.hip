@@ -5,7 +5,7 @@
 //
 // Four launches, nothing read back to the host, no slot lists:
 //
-//   few_logits   a wave an expert of the router and up to four tokens
+//   few_logits   a block an expert of the router and up to four tokens
 //   few_route    a block a token: selection by rank, weights, a bit of the token in its experts' masks
 //   few_gate_up  a block takes (expert in use, 32 columns of a) tiles; its waves split the contraction
 //   few_down     a block has 64 columns of out; the waves of a column tile share its (expert,
@@ -62,12 +62,6 @@ __device__ __forceinline__ int frag_pos(int c) {
 
 // ---- routing ---------------------------------------------------------------------
 
-__device__ __forceinline__ double wave_sum_d(double v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
-  return v;
-}
-
 // A total order of doubles: larger is larger, a NaN below everything.
 __device__ __forceinline__ int64_t order_key(double v) {
   if (v != v) return INT64_MIN;
@@ -76,26 +70,14 @@ __device__ __forceinline__ int64_t order_key(double v) {
 }
 
 // logits[t, e], products of 8 in fp32 and their sums in 64 bits: which expert is the
-// k-th hangs on differences near fp32's own rounding.  Wave: one expert, TB tokens.
-// The router's weight (0.5 MB for 128 experts of 2,048) is read by as many CUs as
-// there are fours of experts: by one block for each token it took 13 us.
+// k-th hangs on differences near fp32's own rounding.  Block: one expert and TB tokens, a quarter
+// of a row for each wave, so that rows of 2,048 are one load deep (a wave a row: 4.3 us for
+// one token, 8.1 for 24, of which the loads' latency was most).
 template <int DT, int FMT, int TB>
 __global__ __launch_bounds__(256) void few_logits_kernel(const FewArgs g) {
+  __shared__ double s_part[4][TB];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n_eb = (g.E + 3) / 4, tb = blockIdx.x / n_eb, e = (blockIdx.x - tb * n_eb) * 4 + wave, t0 = tb * TB;
-  // what the later launches start from
-  const int id = blockIdx.x * 256 + tid, threads = gridDim.x * 256;
-  for (int i = id; i < F_MAX_E; i += threads) g.mask[i] = 0;
-  for (int i = id; i < g.H / 64; i += threads) g.done[i] = 0;
-  if constexpr (FMT == FMT_Q4) {
-    for (int i = id; i < g.T * (g.H / 8); i += threads) {
-      const uint4 v = *reinterpret_cast<const uint4*>(g.x + 8 * (int64_t)i);
-      const uint4 o = {__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
-                       __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u)};
-      *reinterpret_cast<uint4*>(g.xp + 8 * (int64_t)i) = o;
-    }
-  }
-  if (e >= g.E) return;
+  const int tb = blockIdx.x / g.E, e = blockIdx.x - tb * g.E, t0 = tb * TB;
   const uint16_t* const wr = g.router + (int64_t)e * g.H;
   const uint16_t* xr[TB];
 #pragma unroll
@@ -103,8 +85,8 @@ __global__ __launch_bounds__(256) void few_logits_kernel(const FewArgs g) {
   double acc[TB];
 #pragma unroll
   for (int i = 0; i < TB; ++i) acc[i] = 0;
-#pragma unroll 4
-  for (int h = 8 * lane; h < g.H; h += 512) {
+#pragma unroll 2
+  for (int h = 8 * tid; h < g.H; h += 2048) {
     const uint4 w = *reinterpret_cast<const uint4*>(wr + h);
     const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -121,11 +103,36 @@ __global__ __launch_bounds__(256) void few_logits_kernel(const FewArgs g) {
       acc[i] += (double)s;
     }
   }
-#pragma unroll
-  for (int i = 0; i < TB; ++i) {
-    const double l = wave_sum_d(acc[i]);
-    if (lane == 0 && t0 + i < g.T) g.logits[(int64_t)(t0 + i) * g.E + e] = l;
+  // what the later launches start from, while the loads are on their way
+  const int id = blockIdx.x * 256 + tid, threads = gridDim.x * 256;
+  for (int i = id; i < F_MAX_E; i += threads) g.mask[i] = 0;
+  for (int i = id; i < g.H / 64; i += threads) g.done[i] = 0;
+  if constexpr (FMT == FMT_Q4) {
+    for (int i = id; i < g.T * (g.H / 8); i += threads) {
+      const uint4 v = *reinterpret_cast<const uint4*>(g.x + 8 * (int64_t)i);
+      const uint4 o = {__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
+                       __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u)};
+      *reinterpret_cast<uint4*>(g.xp + 8 * (int64_t)i) = o;
+    }
   }
+  // a token's sum in the 64 / TB lanes that keep it: a quarter each of four tokens, half the shuffles at every step
+  int at = 0;
+  if constexpr (TB == 4) {
+    const bool up = lane & 32, odd = lane & 16;
+    const double a = (up ? acc[2] : acc[0]) + __shfl_xor(up ? acc[0] : acc[2], 32, 64);
+    const double b = (up ? acc[3] : acc[1]) + __shfl_xor(up ? acc[1] : acc[3], 32, 64);
+    acc[0] = (odd ? b : a) + __shfl_xor(odd ? a : b, 16, 64);
+    at = lane >> 4;
+  } else {
+    acc[0] += __shfl_xor(acc[0], 32, 64);
+    acc[0] += __shfl_xor(acc[0], 16, 64);
+  }
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) acc[0] += __shfl_xor(acc[0], d, 64);
+  if ((lane & 15) == 0 && (TB == 4 || lane == 0)) s_part[wave][at] = acc[0];
+  __syncthreads();
+  if (tid < TB && t0 + tid < g.T)
+    g.logits[(int64_t)(t0 + tid) * g.E + e] = (s_part[0][tid] + s_part[1][tid]) + (s_part[2][tid] + s_part[3][tid]);
 }
 
 __global__ __launch_bounds__(1024) void few_route_kernel(const FewArgs g) {
@@ -744,9 +751,8 @@ FewPlan few_plan(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I, bool eig
 
 template <int DT, int FMT>
 int launch_few_layer(const FewArgs& g, int64_t in_use, hipStream_t st) {
-  const int eb = (g.E + 3) / 4;
-  if (g.T == 1) few_logits_kernel<DT, FMT, 1><<<(unsigned)eb, 256, 0, st>>>(g);
-  else few_logits_kernel<DT, FMT, 4><<<(unsigned)(eb * ((g.T + 3) / 4)), 256, 0, st>>>(g);
+  if (g.T == 1) few_logits_kernel<DT, FMT, 1><<<(unsigned)g.E, 256, 0, st>>>(g);
+  else few_logits_kernel<DT, FMT, 4><<<(unsigned)(g.E * ((g.T + 3) / 4)), 256, 0, st>>>(g);
   if (int rc = check_launch("moe_few/logits")) return rc;
   few_route_kernel<<<(unsigned)g.T, 1024, 0, st>>>(g);
   if (int rc = check_launch("moe_few/route")) return rc;
