@@ -135,43 +135,62 @@ __global__ __launch_bounds__(256) void few_logits_kernel(const FewArgs g) {
     g.logits[(int64_t)(t0 + tid) * g.E + e] = (s_part[0][tid] + s_part[1][tid]) + (s_part[2][tid] + s_part[3][tid]);
 }
 
+// As order_key, and no two alike: the lowest 8 of a double's 52 bits give way to the expert's
+// number (logits are not known that well), the lower number first.
+__device__ __forceinline__ int64_t expert_key(double v, int e) { return (order_key(v) & ~(int64_t)255) | (255 - e); }
+
+__device__ __forceinline__ float rows16_max(float v) {  // of a wave's lanes, each row of 16 its own already
+  const float a = fmaxf(__shfl(v, 0, 64), __shfl(v, 16, 64)), b = fmaxf(__shfl(v, 32, 64), __shfl(v, 48, 64));
+  return fmaxf(a, b);
+}
+template <int N>
+__device__ __forceinline__ float add_rot(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float wave_add(float v) {  // the same bits in every lane
+  v = add_rot<1>(add_rot<2>(add_rot<4>(add_rot<8>(v))));
+  return (__shfl(v, 0, 64) + __shfl(v, 16, 64)) + (__shfl(v, 32, 64) + __shfl(v, 48, 64));
+}
+
+// Block: one token.  Every wave has the token's whole row, up to four experts a lane, and
+// ranks a sixteenth of the experts: how many come before one is a count of lanes.
 __global__ __launch_bounds__(1024) void few_route_kernel(const FewArgs g) {
-  __shared__ double s_l[F_MAX_E];
-  __shared__ int64_t s_key[F_MAX_E];
   __shared__ float s_p[F_MAX_K];
-  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-  if (tid < g.E) {
-    const double l = g.logits[(int64_t)t * g.E + tid];
-    s_l[tid] = l;
-    s_key[tid] = order_key(l);
-  }
-  __syncthreads();
-  // rank of expert tid / 4: how many come before it; its four threads look at a quarter each
-  const int e = tid >> 2;
-  int rank = 0;
-  if (e < g.E) {
-    const int64_t mine = s_key[e];
-    for (int o = tid & 3; o < g.E; o += 4) {
-      const int64_t other = s_key[o];
-      rank += other > mine || (other == mine && o < e);
-    }
-  }
-  rank += __shfl_xor(rank, 1, 64);
-  rank += __shfl_xor(rank, 2, 64);
-  // softmax: every wave has the whole row, in the same order
-  double m = -INFINITY;
-  for (int o = lane; o < g.E; o += 64) m = s_l[o] > m ? s_l[o] : m;
+  constexpr int N = F_MAX_E / 64, WAVES = 16;
+  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const double* const row = g.logits + (int64_t)t * g.E;
+  const int per = (g.E + WAVES - 1) / WAVES, e = wave * per + lane;  // the lane's own expert: lanes below `per`
+  const bool own = lane < per && e < g.E;
+  const double mine = own ? row[e] : 0;
+  double l[N];
+  int64_t key[N];
+  float m = -INFINITY;
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    const double o = __shfl_xor(m, d, 64);
-    m = o > m ? o : m;
+  for (int i = 0; i < N; ++i) {
+    const int o = 64 * i + lane;
+    l[i] = o < g.E ? row[o] : -INFINITY;
+    m = fmaxf(m, (float)l[i]);
   }
+#pragma unroll
+  for (int i = 0; i < N; ++i) key[i] = 64 * i + lane < g.E ? expert_key(l[i], 64 * i + lane) : INT64_MIN;
+  m = rows16_max(max16(m));
   float sum = 0.f;
-  for (int o = lane; o < g.E; o += 64) sum += expf((float)(s_l[o] - m));
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
-  const bool chosen = e < g.E && rank < g.k && (tid & 3) == 0;
-  const float p = chosen ? expf((float)(s_l[e] - m)) : 0.f;
+  for (int i = 0; i < N; ++i)
+    if (64 * i + lane < g.E) sum += expf((float)(l[i] - (double)m));
+  sum = wave_add(sum);
+  int rank = 0;
+  const int64_t my_key = own ? expert_key(mine, e) : 0;
+  for (int j = 0; j < per; ++j) {  // (past the last expert: a rank that nothing uses)
+    const int64_t k = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(my_key >> 32), j) << 32) |
+                                (uint32_t)__builtin_amdgcn_readlane((int)my_key, j));
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) before += __popcll(__ballot(key[i] > k));
+    rank = lane == j ? before : rank;
+  }
+  const bool chosen = own && rank < g.k;
+  const float p = chosen ? expf((float)(mine - (double)m)) : 0.f;
   if (chosen) s_p[rank] = p;
   __syncthreads();
   if (chosen) {
