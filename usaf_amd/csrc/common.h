@@ -25,7 +25,6 @@ int device_cu_count();
 // run by usaf_hip_init() and otherwise on first use.
 void prepare_gemm_kernels();
 void prepare_sparse_kernels();
-void prepare_fp8_kernels();
 // Resolves the current device's address of the no-alloc bucketing scratch
 // array (usaf_hip_bucket_by_expert_noalloc); returns a status code.
 int prepare_noalloc_scratch();

@@ -81,6 +81,9 @@ __device__ __forceinline__ void values16(const u32x4 lo, const u32x4 hi, int e8m
   }
 }
 
+// Raises the 8-bit product's dynamic-LDS limit, once per process (usaf_hip_init, or its first use).
+void prepare_fp8_kernels();
+
 // The product of up to 32 rows, quantized in the same launch (fp8_small.hip).
 bool fp8_small_ok(int64_t M, int64_t K);
 int fp8_small(const void* x, int dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* w, const uint8_t* w_scale, int64_t N,

@@ -1,5 +1,6 @@
 // Library-wide state: per-thread error text, ABI version, device queries.
 #include "common.h"
+#include "fp8.h"
 
 #include <stdio.h>
 #include <string.h>
