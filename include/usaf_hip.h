@@ -590,6 +590,16 @@ int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, int64_t a_total,
                       int32_t dtype, int32_t wide, void* out, void* stream);
 
 /*
+ * The gate and up product (usaf_hip_fp8_gemm with N = 2 I and wide) that ends in the gated activation's
+ * codes q and scale bytes s (usaf_hip_fp8_swiglu's, bit for bit) and leaves nothing else: for passes
+ * without a backward, at the sizes for which usaf_hip_fp8_gate_up_ok is 1 (UNSUPPORTED otherwise).
+ */
+int usaf_hip_fp8_gate_up_ok(int64_t M, int64_t E, int64_t I, int64_t K);
+int usaf_hip_fp8_gate_up(const uint8_t* a, const uint8_t* a_scale, int64_t a_total, const int32_t* a_rows, int64_t M,
+                         const uint8_t* w, const uint8_t* w_scale, const int32_t* offsets, int64_t E, int64_t I, int64_t K,
+                         int32_t dtype, uint8_t* q, uint8_t* s, void* stream);
+
+/*
  * usaf_hip_fp8_quantize_rows and usaf_hip_fp8_gemm of one weight [N, K] in one call:
  * x [M, K], row stride ld -> out [M, N].  ws: usaf_hip_fp8_linear_ws_bytes, 16-byte aligned; 0
  * bytes (ws may be NULL) for a few rows, which one launch serves, summed as with wide != 0.

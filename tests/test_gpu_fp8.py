@@ -258,9 +258,8 @@ def test_experts_step_by_step(F, T, E, k, H, I, only, dtype):
     _, gu, act, y = saved.saved_tensors
     b = saved.b
     assert act is None  # no weight gradient is wanted
-    act, again = torch.empty(b.n_slots, I, dtype=dtype, device="cuda"), [torch.empty_like(gu), torch.empty_like(y)]
-    F.experts_forward(hs.cuda(), ew, b, again[0], act, again[1])
-    assert torch.equal(again[0], gu) and torch.equal(again[1], y)
+    act, again = torch.empty(b.n_slots, I, dtype=dtype, device="cuda"), torch.empty_like(gu)
+    assert torch.equal(F.experts_forward(F.quantize_rows(hs.cuda()), ew, b, again, act, dtype), y) and torch.equal(again, gu)
     offs, tok = b.offsets.tolist(), b.token_idx.long().cpu()
     wgu, wd = ew.gate_up.dequantize().double().cpu(), ew.down.dequantize().double().cpu()
     h = O.half_step(dtype)
@@ -506,3 +505,41 @@ def test_a_layer_tuned_and_served(F):
     ref = whole.double()
     for got in (one, four):
         assert float((got.double() - ref).norm() / ref.norm()) < 0.2
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=_ids)
+@pytest.mark.parametrize("E,M,I,K", [(8, 1500, 2048, 256), (8, 500, 2176, 128), (40, 2000, 1024, 129), (200, 700, 384, 640)])
+def test_gate_up_ends_in_the_activations_codes(F, E, M, I, K, dtype):
+    """One launch or two: the same bits; slots behind the last one are left."""
+    from usaf_amd import _native as N
+    g = torch.Generator().manual_seed(M)
+    w = F.Fp8Tensor.quantize(_rand(E, 2 * I, K, seed=E, scale=0.1).cuda())
+    hs = _rand(M // 2, K, dtype=dtype, seed=K)
+    hs[3, 5], hs[7, 0] = float("inf"), float("nan")
+    x = F.quantize_rows(hs.cuda())
+    used = M - M // 9
+    ends = torch.randint(0, used + 1, (E - 1,), generator=g).sort().values.tolist()
+    offs = torch.tensor([0] + ends + [used], dtype=torch.int32, device="cuda")
+    tok = torch.randint(0, M // 2, (M,), generator=g).to(torch.int32).cuda()
+    gu = torch.empty(M, 2 * I, dtype=dtype, device="cuda")
+    F.product(x, w, gu, offs, tok, wide=True)
+    want, got = F.empty_rows(M, I, x.q.device), F.empty_rows(M, I, x.q.device)
+    for t in (want.q, want.s, got.q, got.s):
+        t.fill_(77)
+    N.call("usaf_hip_fp8_swiglu", gu.data_ptr(), M, I, N.dtype_code(dtype), offs[-1:].data_ptr(), None, want.q.data_ptr(),
+           want.s.data_ptr(), N.stream_ptr(x.q.device))
+    N.call("usaf_hip_fp8_gate_up", x.q.data_ptr(), x.s.data_ptr(), x.q.shape[0], tok.data_ptr(), M, w.q.data_ptr(),
+           w.s.data_ptr(), offs.data_ptr(), E, I, K, N.dtype_code(dtype), got.q.data_ptr(), got.s.data_ptr(),
+           N.stream_ptr(x.q.device))
+    assert torch.equal(got.q, want.q) and torch.equal(got.s, want.s)
+
+
+def test_experts_without_a_backward_keep_nothing(F):
+    """The same bits with and without a gradient in sight."""
+    from usaf_amd import moe as G
+    ew = _experts(F, 4, 256, 2048, seed=30)  # (gate and up in one launch)
+    hs, w = _rand(600, 256, seed=31).cuda(), _routing(600, 4, 2, torch.bfloat16, seed=32).cuda()
+    want = G.routed_experts(hs.clone().requires_grad_(True), w, ew).detach()
+    assert torch.equal(G.routed_experts(hs, w, ew), want)
+    with torch.no_grad():
+        assert torch.equal(G.routed_experts(hs.clone().requires_grad_(True), w, ew), want)

@@ -80,6 +80,17 @@ def test_entry_points_check_their_arguments():
     assert gemm(p, p, 1 << 33, p, 1, p, p, None, 1, 8, 8, N.BF16, 0, p, None) == N.USAF_ERR_UNSUPPORTED
     assert gemm(p, p, 1 << 40, None, 1 << 40, p, p, None, 1, 8, 8, N.BF16, 0, p, None) == inval
     assert gemm(p, p, 1, None, 1, p, p, p, 256, 8, 8, N.BF16, 0, p, None) == N.USAF_ERR_UNSUPPORTED
+    up, up_ok = lib.usaf_hip_fp8_gate_up, lib.usaf_hip_fp8_gate_up_ok
+    assert up(None, None, 0, None, 0, None, None, None, 1, 128, 8, N.BF16, None, None, None) == ok
+    assert up(p, p, 1, None, 1, p, p, p, 1, 100, 8, N.BF16, p, p, None) == inval
+    assert up(p, p, 1, None, 1, p, p, None, 1, 128, 8, N.BF16, p, p, None) == inval
+    assert up(p, p, 1, None, 1, p, p, p, 1, 128, 8, N.F32, p, p, None) == inval
+    assert up(p, p, 1, None, 1, p, p, p, 1, 128, 0, N.BF16, p, p, None) == inval
+    for bad in [dict(q=None), dict(q=odd), dict(s=None), dict(w=odd), dict(a=None)]:
+        v = {**dict(a=p, w=p, q=p, s=p), **bad}
+        assert up(v["a"], p, 1, None, 1, v["w"], p, p, 1, 128, 8, N.BF16, v["q"], v["s"], None) == inval, bad
+    assert [up_ok(*a) for a in [(4, 4, 128, 256), (0, 4, 128, 256), (16384, 64, 1024, 2048), (16384, 256, 1024, 2048)]] == [0, 0, 1, 0]
+    assert up(p, p, 4, None, 4, p, p, p, 4, 128, 256, N.BF16, p, p, None) == N.USAF_ERR_UNSUPPORTED
     linear = lib.usaf_hip_fp8_linear
     assert [lib.usaf_hip_fp8_linear_ws_bytes(m, k) for m, k in ((40, 130), (3, 130), (0, 5), (-1, 5))] == [40 * (256 + 4), 0, 0, -1]
     assert linear(None, N.BF16, 0, 8, 8, None, None, 8, None, None, 0, None) == ok

@@ -17,6 +17,13 @@
 // steps (a contraction of 768) would spend as long on its first lines as on its products.
 // 16-byte chunks of a row are XOR-swizzled by the row (by the DMA's source address), which
 // makes the fragment reads free of bank conflicts.
+//
+// ACT: W_e holds a gate's and an up projection's I rows each; a tile is 128 columns of both (each
+// wave 32 of one and the same 32 of the other), and what leaves it is only the next product's operand,
+// a block of 128 of every slot:  q, s = Q(dt(dt(silu(g)) u)),  with (g, u) = C.  A layer of 2,048
+// tokens on 64 experts of 1,024 takes 310 us so and 322 with C written and a kernel of its own behind it.  Where a
+// backward needs C as well the two are equal (846, 4,096 tokens on 128 experts of 768), or this
+// one is the slower (352 against 343, 256 tokens), so there they stay apart.
 #include "fp8.h"
 
 namespace usaf {
@@ -36,8 +43,12 @@ struct Fp8Args {
   const int32_t* offsets;  // [E + 1]; nullptr: one expert, M slots
   int E;
   int64_t M;
-  uint16_t* out;           // [M, N]
+  uint16_t* out;           // [M, N]; not ACT
   int n_nt;
+  // ACT: N = 2 I
+  uint8_t* q;              // [M, I] codes of the gated activation
+  uint8_t* qs;             // [M, q_sp] their scale bytes
+  int q_sp;
 };
 
 constexpr int G_WAVES = 8, G_THREADS = 64 * G_WAVES;
@@ -133,10 +144,11 @@ struct Tile {
   static_assert(KW > 1 ? G_WAVES * 4096 * NI <= STAGE : G_WAVES * 32 * OUT_ROW <= STAGE, "results go through a stage");
 };
 
-template <int MW, int NW, int MI, int NI, int DT, bool WIDE>
+template <int MW, int NW, int MI, int NI, int DT, bool WIDE, bool ACT = false>
 __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
   typedef Tile<MW, NW, MI, NI> T;
   constexpr int KW = T::KW;
+  static_assert(!ACT || (NI == 2 && NW == 4 && KW == 1), "a wave has 32 gate and 32 up columns of a block of 128");
   extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
   const uint32_t sm_lds = (uint32_t)(uintptr_t)(lds_void_ptr)sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -187,7 +199,7 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
   const int ws_shift = (int)((uintptr_t)g.ws & 3);
   // byte of the scale of columns 128 b + [0, 128) of the tile, k-block 0, from the word that ws sits in
   auto ws_at = [&](const Place& t, int b) {
-    int64_t at = (int64_t)t.nt * T::N / 128 + b;
+    int64_t at = ACT ? t.nt + b * (g.N / 256) : (int64_t)t.nt * T::N / 128 + b;
     return ((int64_t)t.e * nrb + (at < nrb ? at : nrb - 1)) * nkb + ws_shift;
   };
 
@@ -199,7 +211,7 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
   int64_t ws_off = 0;
   auto open = [&]() {
     const Place t = place(i_id);
-    const int64_t n0 = (int64_t)t.nt * T::N;
+    const int64_t n0 = (int64_t)t.nt * (ACT ? 128 : T::N);
     a_base = uniform(g.a_rows ? g.A : g.A + t.m_beg * g.Kp);
     as_base = uniform(g.a_rows ? g.as : g.as + t.m_beg * g.sp);
     w_base = uniform(g.W + ((int64_t)t.e * g.N + n0) * g.Kp);
@@ -215,7 +227,8 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
 #pragma unroll
     for (int i = 0; i < T::W_DMA; ++i) {
       const int r = 8 * (T::SHARE * i + part) + (lane >> 3);
-      const int64_t n = n0 + r < g.N ? r : g.N - 1 - n0;
+      // (ACT: rows 64 wn + 32 k + [0, 32) of the tile are columns 32 wn + [0, 32) of the gate, k = 0, or of up)
+      const int64_t n = ACT ? (r >> 5 & 1) * (g.N / 2) + (r >> 6) * 32 + (r & 31) : n0 + r < g.N ? r : g.N - 1 - n0;
       w_off[i] = (uint32_t)(n * g.Kp) + 16 * ((lane & 7) ^ g_swz(r));
     }
     // scale words: instruction s < A_WORDS those of 64 slots, the others (all the same) the
@@ -279,7 +292,7 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
     const int live = mine <= 0 ? 0 : mine >= 32 * MI ? MI : (mine + 31) >> 5;  // its blocks of 32 with any
     int64_t ws_byte[NI];
 #pragma unroll
-    for (int k = 0; k < NI; ++k) ws_byte[k] = ws_at(t, (32 * (NI * wn + k)) / 128);
+    for (int k = 0; k < NI; ++k) ws_byte[k] = ws_at(t, ACT ? k : (32 * (NI * wn + k)) / 128);
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -307,7 +320,7 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
       for (int i = 0; i < MI; ++i) s_a[i] = (int)(sc[32 * (MI * wm + i) + l32] >> (8 * (kb & 3)));
 #pragma unroll
       for (int k = 0; k < NI; ++k)
-        s_w[k] = (int)(sc[64 * T::A_WORDS + (32 * (NI * wn + k)) / 128] >> (8 * (int)((ws_byte[k] + kb) & 3)));
+        s_w[k] = (int)(sc[64 * T::A_WORDS + (ACT ? k : (32 * (NI * wn + k)) / 128)] >> (8 * (int)((ws_byte[k] + kb) & 3)));
       // A wave's DMAs go out PER at a time between its matrix instructions: eight waves sending all of
       // theirs first wait for the address unit (16 cycles each, 1,200 in all) before they multiply
       constexpr int SLOTS = MI > 1 ? MI : 2 * MI - 1, PER = (T::DMAS + SLOTS - 1) / SLOTS > 2 ? (T::DMAS + SLOTS - 1) / SLOTS : 2;
@@ -421,7 +434,7 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
           }
         }
       }
-    } else {
+    } else if constexpr (!ACT) {
       // 32 slots at a time through the wave's part, for whole lines to memory
       uint8_t* const so = free + wave * (32 * T::OUT_ROW);
       constexpr int CH = T::OUT_ROW / 16;  // 16-byte chunks of a row
@@ -452,6 +465,52 @@ __global__ __launch_bounds__(G_THREADS) void fp8_gemm_kernel(const Fp8Args g) {
           }
         }
       }
+    } else {
+      // the gated activation over the gate's accumulators; a slot's 128 columns are 16 in each of two lanes of
+      // each of the four waves that share the slots
+      float* const s_max = reinterpret_cast<float*>(free);  // [M, 4]
+      uint8_t* const s_q = free + T::M * 16;                // [M, 128], 16-byte chunks swizzled by the row
+      const int64_t I = g.N / 2;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        __builtin_amdgcn_sched_barrier(0);  // one block of 32 slots at a time: fewer registers
+        float top = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; v += 2) {
+          const f32x2 gate = unpack2<DT>(pack2<DT>(acc[i][0][v], acc[i][0][v + 1]));
+          const f32x2 up = unpack2<DT>(pack2<DT>(acc[i][1][v], acc[i][1][v + 1]));
+          const f32x2 sg = unpack2<DT>(pack2<DT>(silu_fast(gate.x), silu_fast(gate.y)));
+          const f32x2 a = unpack2<DT>(pack2<DT>(sg.x * up.x, sg.y * up.y));
+          acc[i][0][v] = a.x;
+          acc[i][0][v + 1] = a.y;
+          top = fmaxf(top, fmaxf(finite_abs(a.x), finite_abs(a.y)));
+        }
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (half == 0) s_max[4 * (32 * (MI * wm + i) + l32) + wn] = top;
+      }
+      lds_barrier();
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        const int r = 32 * (MI * wm + i) + l32;
+        const f32x4 m = *reinterpret_cast<const f32x4*>(s_max + 4 * r);
+        const int e = e8m0_of(fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w)));
+        const float inv = inv_scale(e);
+        if (wn == 0 && half == 0 && 32 * i + l32 < mine) g.qs[(mw + 32 * i + l32) * g.q_sp + t.nt] = (uint8_t)e;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float a[4] = {acc[i][0][4 * q], acc[i][0][4 * q + 1], acc[i][0][4 * q + 2], acc[i][0][4 * q + 3]};
+          *reinterpret_cast<uint32_t*>(s_q + r * 128 + 16 * ((2 * wn + (q >> 1)) ^ (r & 7)) + 8 * (q & 1) + 4 * half) =
+              to_codes(a, inv);
+        }
+      }
+      lds_barrier();
+      for (int c = tid; c < T::M * 8; c += G_THREADS) {
+        const int r = c >> 3;
+        if (r < t.valid)
+          *reinterpret_cast<u32x4*>(g.q + (t.m_beg + r) * I + (int64_t)t.nt * 128 + 16 * (c & 7)) =
+              *reinterpret_cast<const u32x4*>(s_q + r * 128 + 16 * ((c & 7) ^ (r & 7)));
+      }
     }
   }
   wait_vmcnt<0>();  // no DMA lands in LDS that is someone else's by then
@@ -462,17 +521,17 @@ bool raise_fp8_lds(const void* kernel, size_t bytes) {
   (void)hipGetLastError();
   return true;
 }
-template <int MW, int NW, int MI, int NI, int DT, bool WIDE>
+template <int MW, int NW, int MI, int NI, int DT, bool WIDE, bool ACT>
 void prepare_one() {
-  static const bool done = raise_fp8_lds(reinterpret_cast<const void*>(&fp8_gemm_kernel<MW, NW, MI, NI, DT, WIDE>),
+  static const bool done = raise_fp8_lds(reinterpret_cast<const void*>(&fp8_gemm_kernel<MW, NW, MI, NI, DT, WIDE, ACT>),
                                          Tile<MW, NW, MI, NI>::LDS);
   (void)done;
 }
 
-template <int MW, int NW, int MI, int NI, int DT, bool WIDE>
+template <int MW, int NW, int MI, int NI, int DT, bool WIDE, bool ACT = false>
 int launch_dt(const Fp8Args& g, unsigned blocks, hipStream_t st) {
-  prepare_one<MW, NW, MI, NI, DT, WIDE>();
-  fp8_gemm_kernel<MW, NW, MI, NI, DT, WIDE><<<blocks, G_THREADS, Tile<MW, NW, MI, NI>::LDS, st>>>(g);
+  prepare_one<MW, NW, MI, NI, DT, WIDE, ACT>();
+  fp8_gemm_kernel<MW, NW, MI, NI, DT, WIDE, ACT><<<blocks, G_THREADS, Tile<MW, NW, MI, NI>::LDS, st>>>(g);
   return check_launch("fp8_gemm");
 }
 
@@ -490,6 +549,11 @@ struct Shape {
     if (tiles >= (int64_t)1 << 31) return set_error(USAF_ERR_INVALID, "fp8_gemm: too many tiles");
     g.n_nt = (int)ceil_div(g.N, T::N);
     const unsigned blocks = (unsigned)(ceil_div(tiles < cus ? tiles : cus, G_XCDS) * G_XCDS);
+    if constexpr (NI == 2) {
+      if (g.q)  // gate and up
+        return dt == USAF_BF16 ? launch_dt<MW, NW, MI, NI, USAF_BF16, true, true>(g, blocks, st)
+                               : launch_dt<MW, NW, MI, NI, USAF_F16, true, true>(g, blocks, st);
+    }
     if (dt == USAF_BF16)
       return wide ? launch_dt<MW, NW, MI, NI, USAF_BF16, true>(g, blocks, st)
                   : launch_dt<MW, NW, MI, NI, USAF_BF16, false>(g, blocks, st);
@@ -497,10 +561,14 @@ struct Shape {
                 : launch_dt<MW, NW, MI, NI, USAF_F16, false>(g, blocks, st);
   }
   static void prepare() {
-    prepare_one<MW, NW, MI, NI, USAF_BF16, false>();
-    prepare_one<MW, NW, MI, NI, USAF_BF16, true>();
-    prepare_one<MW, NW, MI, NI, USAF_F16, false>();
-    prepare_one<MW, NW, MI, NI, USAF_F16, true>();
+    prepare_one<MW, NW, MI, NI, USAF_BF16, false, false>();
+    prepare_one<MW, NW, MI, NI, USAF_BF16, true, false>();
+    prepare_one<MW, NW, MI, NI, USAF_F16, false, false>();
+    prepare_one<MW, NW, MI, NI, USAF_F16, true, false>();
+    if constexpr (NI == 2) {
+      prepare_one<MW, NW, MI, NI, USAF_BF16, true, true>();
+      prepare_one<MW, NW, MI, NI, USAF_F16, true, true>();
+    }
   }
   // Cycles of a CU, roughly: a step is bound by its matrix instructions or by its lines
   static double cycles(const Fp8Args& g, bool wide) {
@@ -521,6 +589,25 @@ typedef Shape<1, 2, 2, 1> S64x64;
 typedef Shape<1, 4, 1, 1> S32x128;
 typedef Shape<1, 1, 1, 1> S32x32;
 
+typedef int (*Launch)(Fp8Args, int, bool, hipStream_t);
+Launch best_shape(const Fp8Args& g, bool wide) {
+  Launch best = S256x256::launch;
+  double least = S256x256::cycles(g, wide);
+  auto consider = [&](Launch f, double c) {
+    if (c < least) {
+      least = c;
+      best = f;
+    }
+  };
+  consider(S128x256::launch, S128x256::cycles(g, wide));
+  consider(S128x128::launch, S128x128::cycles(g, wide));
+  consider(S64x128::launch, S64x128::cycles(g, wide));
+  consider(S64x64::launch, S64x64::cycles(g, wide));
+  consider(S32x128::launch, S32x128::cycles(g, wide));
+  consider(S32x32::launch, S32x32::cycles(g, wide));
+  return best;
+}
+
 }  // namespace
 
 void prepare_fp8_kernels() {
@@ -537,22 +624,19 @@ void prepare_fp8_kernels() {
 
 using namespace usaf;
 
-extern "C" int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, int64_t a_total, const int32_t* a_rows, int64_t M,
-                                 const uint8_t* w, const uint8_t* w_scale, const int32_t* offsets, int64_t E, int64_t N,
-                                 int64_t K, int32_t dtype, int32_t wide, void* out, void* stream) {
-  if (M < 0 || N < 0 || K < 0 || E < 1 || N > 1 << 24 || K > 1 << 24 || M > 0x7FFFFFFF || a_total < 0)
-    return set_error(USAF_ERR_INVALID, "fp8_gemm: bad size M=%lld N=%lld K=%lld E=%lld", (long long)M, (long long)N,
-                     (long long)K, (long long)E);
-  if (dtype != USAF_BF16 && dtype != USAF_F16) return set_error(USAF_ERR_INVALID, "fp8_gemm: dtype must be fp16 or bf16");
-  if (M == 0 || N == 0) return clear_error();
-  if (K == 0) return set_error(USAF_ERR_INVALID, "fp8_gemm: need K >= 1");
-  if (!a || !a_scale || !w || !w_scale || !out) return set_error(USAF_ERR_INVALID, "fp8_gemm: null pointer");
-  if (!offsets && E != 1) return set_error(USAF_ERR_INVALID, "fp8_gemm: more than one expert needs offsets");
-  if (!a_rows && M > a_total) return set_error(USAF_ERR_INVALID, "fp8_gemm: more slots than rows");
-  if (E > Q_MAX_E) return set_error(USAF_ERR_UNSUPPORTED, "fp8_gemm: at most %d experts", Q_MAX_E);
-  if (((uintptr_t)a | (uintptr_t)w) % 16 || (uintptr_t)a_scale % 4 || (uintptr_t)out % 2)
-    return set_error(USAF_ERR_INVALID, "fp8_gemm: codes must be 16-byte, scales 4-byte and the output 2-byte aligned");
-  Fp8Args g{};
+// Checks of a product's operands, and its arguments.
+static int gemm_args(const char* what, const uint8_t* a, const uint8_t* a_scale, int64_t a_total, const int32_t* a_rows,
+                     int64_t M, const uint8_t* w, const uint8_t* w_scale, const int32_t* offsets, int64_t E, int64_t N,
+                     int64_t K, Fp8Args* args) {
+  if (K == 0) return set_error(USAF_ERR_INVALID, "%s: need K >= 1", what);
+  if (!a || !a_scale || !w || !w_scale) return set_error(USAF_ERR_INVALID, "%s: null pointer", what);
+  if (!offsets && E != 1) return set_error(USAF_ERR_INVALID, "%s: more than one expert needs offsets", what);
+  if (!a_rows && M > a_total) return set_error(USAF_ERR_INVALID, "%s: more slots than rows", what);
+  if (E > Q_MAX_E) return set_error(USAF_ERR_UNSUPPORTED, "%s: at most %d experts", what, Q_MAX_E);
+  if (((uintptr_t)a | (uintptr_t)w) % 16 || (uintptr_t)a_scale % 4)
+    return set_error(USAF_ERR_INVALID, "%s: codes must be 16-byte and scales 4-byte aligned", what);
+  Fp8Args& g = *args;
+  g = Fp8Args{};
   g.A = a;
   g.as = a_scale;
   g.Kp = (K + FP8_BLOCK - 1) / FP8_BLOCK * FP8_BLOCK;
@@ -564,29 +648,69 @@ extern "C" int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, int64
   g.offsets = offsets;
   g.E = (int)E;
   g.M = M;
-  g.out = reinterpret_cast<uint16_t*>(out);
   // 32-bit offsets: gathered rows, a tile of 256 rows of either operand, the weight's scales
   if ((a_rows && a_total * g.Kp >= (int64_t)1 << 32) || 256 * g.Kp >= (int64_t)1 << 32 ||
       E * ((N + 127) / 128) * (g.Kp / 128) >= (int64_t)1 << 31)
-    return set_error(USAF_ERR_UNSUPPORTED, "fp8_gemm: operands past 4 GiB of gathered rows or 2 GiB of scales");
-  hipStream_t st = as_stream(stream);
-  typedef int (*Launch)(Fp8Args, int, bool, hipStream_t);
-  const bool w16 = wide != 0;
-  Launch best = S256x256::launch;
-  double least = S256x256::cycles(g, w16);
-  auto consider = [&](Launch f, double c) {
-    if (c < least) {
-      least = c;
-      best = f;
-    }
-  };
-  consider(S128x256::launch, S128x256::cycles(g, w16));
-  consider(S128x128::launch, S128x128::cycles(g, w16));
-  consider(S64x128::launch, S64x128::cycles(g, w16));
-  consider(S64x64::launch, S64x64::cycles(g, w16));
-  consider(S32x128::launch, S32x128::cycles(g, w16));
-  consider(S32x32::launch, S32x32::cycles(g, w16));
-  return best(g, dtype, w16, st);
+    return set_error(USAF_ERR_UNSUPPORTED, "%s: operands past 4 GiB of gathered rows or 2 GiB of scales", what);
+  return USAF_OK;
+}
+
+static int gemm_sizes(const char* what, int64_t a_total, int64_t M, int64_t E, int64_t N, int64_t K, int32_t dtype) {
+  if (M < 0 || N < 0 || K < 0 || E < 1 || N > 1 << 24 || K > 1 << 24 || M > 0x7FFFFFFF || a_total < 0)
+    return set_error(USAF_ERR_INVALID, "%s: bad size M=%lld N=%lld K=%lld E=%lld", what, (long long)M, (long long)N,
+                     (long long)K, (long long)E);
+  if (dtype != USAF_BF16 && dtype != USAF_F16) return set_error(USAF_ERR_INVALID, "%s: dtype must be fp16 or bf16", what);
+  return USAF_OK;
+}
+
+extern "C" int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, int64_t a_total, const int32_t* a_rows, int64_t M,
+                                 const uint8_t* w, const uint8_t* w_scale, const int32_t* offsets, int64_t E, int64_t N,
+                                 int64_t K, int32_t dtype, int32_t wide, void* out, void* stream) {
+  if (int rc = gemm_sizes("fp8_gemm", a_total, M, E, N, K, dtype)) return rc;
+  if (M == 0 || N == 0) return clear_error();
+  Fp8Args g;
+  if (int rc = gemm_args("fp8_gemm", a, a_scale, a_total, a_rows, M, w, w_scale, offsets, E, N, K, &g)) return rc;
+  if (!out || (uintptr_t)out % 2) return set_error(USAF_ERR_INVALID, "fp8_gemm: null or misaligned output");
+  g.out = reinterpret_cast<uint16_t*>(out);
+  return best_shape(g, wide != 0)(g, dtype, wide != 0, as_stream(stream));
+}
+
+// Whether the gate-and-up product may end in the gated activation's codes: on the tiles of 256
+// columns, which the rule on sizes takes for all but the smallest calls, while an expert's gate rows
+// stay within the 32-bit offsets.
+static bool gate_up_ok(const Fp8Args& g) {
+  const Launch best = best_shape(g, true);
+  return (best == S256x256::launch || best == S128x256::launch) && (g.N / 2 + 128) * g.Kp < (int64_t)1 << 32;
+}
+
+extern "C" int usaf_hip_fp8_gate_up_ok(int64_t M, int64_t E, int64_t I, int64_t K) {
+  if (M < 1 || E < 1 || E > Q_MAX_E || I < 1 || K < 1 || I % FP8_BLOCK || I > 1 << 23 || K > 1 << 24 || M > 0x7FFFFFFF) return 0;
+  Fp8Args g{};
+  static const int32_t grouped = 0;
+  g.offsets = &grouped;  // not read
+  g.Kp = (K + FP8_BLOCK - 1) / FP8_BLOCK * FP8_BLOCK;
+  g.N = 2 * I;
+  g.E = (int)E;
+  g.M = M;
+  return gate_up_ok(g) ? 1 : 0;
+}
+
+extern "C" int usaf_hip_fp8_gate_up(const uint8_t* a, const uint8_t* a_scale, int64_t a_total, const int32_t* a_rows,
+                                    int64_t M, const uint8_t* w, const uint8_t* w_scale, const int32_t* offsets, int64_t E,
+                                    int64_t I, int64_t K, int32_t dtype, uint8_t* q, uint8_t* s, void* stream) {
+  if (I < 0 || I % FP8_BLOCK || I > 1 << 23)
+    return set_error(USAF_ERR_INVALID, "fp8_gate_up: I must be a multiple of %d, got %lld", FP8_BLOCK, (long long)I);
+  if (int rc = gemm_sizes("fp8_gate_up", a_total, M, E, 2 * I, K, dtype)) return rc;
+  if (M == 0 || I == 0) return clear_error();
+  Fp8Args g;
+  if (int rc = gemm_args("fp8_gate_up", a, a_scale, a_total, a_rows, M, w, w_scale, offsets, E, 2 * I, K, &g)) return rc;
+  if (!offsets || !q || !s || (uintptr_t)q % 16)
+    return set_error(USAF_ERR_INVALID, "fp8_gate_up: null pointer, or codes not 16-byte aligned");
+  if (!gate_up_ok(g)) return set_error(USAF_ERR_UNSUPPORTED, "fp8_gate_up: not at this size (usaf_hip_fp8_gate_up_ok)");
+  g.q = q;
+  g.qs = s;
+  g.q_sp = (int)usaf_hip_fp8_scale_stride(I);
+  return best_shape(g, true)(g, dtype, true, as_stream(stream));
 }
 
 extern "C" int64_t usaf_hip_fp8_linear_ws_bytes(int64_t M, int64_t K) {

@@ -225,15 +225,24 @@ def fp8_linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
 # two last products, whose results are only rounded, take the 8-bit one.
 
 
-def experts_forward(hs: torch.Tensor, ew, b, gu: torch.Tensor, act: Optional[torch.Tensor], y: torch.Tensor) -> None:
-    """gu, act (None: not stored) and y of the slots of bucketing b, for 8-bit experts ew. Each step's
-    output is rounded to the activations' dtype, as on the layer's other kernels."""
-    S, I = gu.shape[0], gu.shape[1] // 2
-    product(quantize_rows(hs), ew.gate_up, gu, b.offsets, b.token_idx, wide=True)
-    rows = empty_rows(S, I, hs.device)
-    N.call("usaf_hip_fp8_swiglu", gu.data_ptr(), S, I, N.dtype_code(gu.dtype), b.offsets[-1:].data_ptr(), N.ptr(act),
-           rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(hs.device))
-    product(rows, ew.down, y, b.offsets)
+def experts_forward(x: Rows, ew, b, gu: Optional[torch.Tensor], act: Optional[torch.Tensor], dtype: torch.dtype) -> torch.Tensor:
+    """y of the slots of bucketing b from the quantized hidden states, for 8-bit experts ew, with the steps before it in
+    gu and act (None: not kept). Each step's output is rounded to dtype, the activations', as on the
+    layer's other kernels."""
+    S, E, H, I, dev = b.n_slots, ew.E, ew.H, ew.I, x.q.device
+    with on(dev):
+        if gu is None and act is None and N.load().usaf_hip_fp8_gate_up_ok(S, E, I, H):
+            rows, w = empty_rows(S, I, dev), ew.gate_up
+            N.call("usaf_hip_fp8_gate_up", x.q.data_ptr(), x.s.data_ptr(), x.q.shape[0], b.token_idx.data_ptr(), S,
+                   w.q.data_ptr(), w.s.data_ptr(), b.offsets.data_ptr(), E, I, H, N.dtype_code(dtype), rows.q.data_ptr(),
+                   rows.s.data_ptr(), N.stream_ptr(dev))
+        else:
+            gu = torch.empty(S, 2 * I, dtype=dtype, device=dev) if gu is None else gu
+            product(x, ew.gate_up, gu, b.offsets, b.token_idx, wide=True)
+            rows = empty_rows(S, I, dev)
+            N.call("usaf_hip_fp8_swiglu", gu.data_ptr(), S, I, N.dtype_code(dtype), b.offsets[-1:].data_ptr(), N.ptr(act),
+                   rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(dev))
+    return product(rows, ew.down, torch.empty(S, H, dtype=dtype, device=dev), b.offsets)
 
 
 def experts_combine_bwd(dout: torch.Tensor, y: torch.Tensor, b, dcur: Optional[torch.Tensor],
@@ -241,9 +250,10 @@ def experts_combine_bwd(dout: torch.Tensor, y: torch.Tensor, b, dcur: Optional[t
     """The gradient of the down projection's outputs, quantized (and in dcur where given), and of the routing weights."""
     S, H = y.shape
     rows = empty_rows(S, H, y.device)
-    N.call("usaf_hip_fp8_combine_bwd", dout.data_ptr(), y.data_ptr(), b.token_idx.data_ptr(), b.slot_w.data_ptr(),
-           b.offsets.data_ptr(), S, b.offsets.numel() - 1, H, N.dtype_code(y.dtype), N.ptr(dcur), rows.q.data_ptr(),
-           rows.s.data_ptr(), dweights.data_ptr(), N.stream_ptr(y.device))
+    with on(y.device):
+        N.call("usaf_hip_fp8_combine_bwd", dout.data_ptr(), y.data_ptr(), b.token_idx.data_ptr(), b.slot_w.data_ptr(),
+               b.offsets.data_ptr(), S, b.offsets.numel() - 1, H, N.dtype_code(y.dtype), N.ptr(dcur), rows.q.data_ptr(),
+               rows.s.data_ptr(), dweights.data_ptr(), N.stream_ptr(y.device))
     return rows
 
 
@@ -252,6 +262,7 @@ def experts_bwd(dcur: Rows, gu: torch.Tensor, ew, b, dgu: Optional[torch.Tensor]
     S, I = gu.shape[0], gu.shape[1] // 2
     dact = product(dcur, ew.down.transposed(), torch.empty(S, I, dtype=gu.dtype, device=gu.device), b.offsets, wide=True)
     rows = empty_rows(S, 2 * I, gu.device)
-    N.call("usaf_hip_fp8_swiglu_bwd", gu.data_ptr(), dact.data_ptr(), S, I, N.dtype_code(gu.dtype), b.offsets[-1:].data_ptr(),
-           N.ptr(dgu), rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(gu.device))
+    with on(gu.device):
+        N.call("usaf_hip_fp8_swiglu_bwd", gu.data_ptr(), dact.data_ptr(), S, I, N.dtype_code(gu.dtype),
+               b.offsets[-1:].data_ptr(), N.ptr(dgu), rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(gu.device))
     product(rows, ew.gate_up.transposed(), dx_slots, b.offsets)

@@ -510,10 +510,12 @@ class RoutedExpertsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hs: torch.Tensor, weights: torch.Tensor, ew: ExpertWeights, capture,
                 w_gate_up: Optional[torch.Tensor] = None, w_down: Optional[torch.Tensor] = None,
-                slots: Optional[Tuple[int, torch.Tensor]] = None, link: Optional["HsGradLink"] = None):
+                slots: Optional[Tuple[int, torch.Tensor]] = None, link: Optional["HsGradLink"] = None,
+                backward: bool = True):
         # w_gate_up / w_down: the dense expert Parameters the kernels' weights were
         # taken from, passed only so that autograd delivers their gradients;
-        # slots: (capacity, overflow) for bucketing without a host read (bucket_by_expert)
+        # slots: (capacity, overflow) for bucketing without a host read (bucket_by_expert);
+        # backward: whether one may follow (8-bit experts keep nothing for it otherwise)
         dt = hs.dtype
         if dt not in (torch.float16, torch.bfloat16):
             raise TypeError(f"activations must be fp16 or bf16, got {dt}")
@@ -529,13 +531,15 @@ class RoutedExpertsFn(torch.autograd.Function):
             raise ValueError(f"activations on {dev}, 8-bit experts on {ew.gate_up.device}")
         st = N.stream_ptr(dev)
         code = N.dtype_code(dt)
+        # (before the bucketing, whose host read would leave the GPU idle for it)
+        x8 = fp8.quantize_rows(hs) if ew.is_fp8 and T > 0 else None
         b = bucket_by_expert(weights) if slots is None else bucket_by_expert(weights, *slots)
         S = b.n_slots
-        gu = torch.empty(S, 2 * I, dtype=dt, device=dev)
+        gu = torch.empty(S, 2 * I, dtype=dt, device=dev) if backward or not ew.is_fp8 else None
         # the gated activations of 8-bit experts are kept where a weight gradient will read them
-        keep = not ew.is_fp8 or capture is not None or ctx.needs_input_grad[5]
+        keep = not ew.is_fp8 or (backward and (capture is not None or ctx.needs_input_grad[5]))
         act = torch.empty(S, I, dtype=dt, device=dev) if keep else None
-        y = torch.empty(S, H, dtype=dt, device=dev)
+        y = None if ew.is_fp8 and S > 0 else torch.empty(S, H, dtype=dt, device=dev)
         act_blk = None
         if S > 0 and not ew.is_fp8 and _sampled_blocked(capture, b):
             # the down projection's sampled gradient reads act blocked slot-major:
@@ -545,7 +549,7 @@ class RoutedExpertsFn(torch.autograd.Function):
             n_blk = max(1, int(N.load().usaf_hip_blocked_elems(S, E, I)))
             act_blk = BlockedSlots(torch.empty(n_blk, dtype=dt, device=dev), I, b.offsets, b.blk_table)
         if S > 0 and ew.is_fp8:
-            fp8.experts_forward(hs, ew, b, gu, act, y)
+            y = fp8.experts_forward(x8, ew, b, gu, act, dt)
         elif S > 0:
             q, sz, w16 = ew._ptrs("gate_up", dt)
             timed_call("usaf_hip_moe_gate_up_fwd", hs.data_ptr(), T, H, b.token_idx.data_ptr(), b.offsets.data_ptr(),
@@ -583,7 +587,7 @@ class RoutedExpertsFn(torch.autograd.Function):
         if S == 0:
             d_wgu = torch.zeros(E, 2 * I, H, dtype=ctx.wdt[0], device=dev) if want_gu else None
             d_wdn = torch.zeros(E, H, I, dtype=ctx.wdt[1], device=dev) if want_dn else None
-            return torch.zeros_like(hs), dweights, None, None, d_wgu, d_wdn, None, None
+            return torch.zeros_like(hs), dweights, None, None, d_wgu, d_wdn, None, None, None
         if ew.is_fp8:
             return _fp8_experts_backward(ctx, dout, dweights)
         dcur = torch.empty(S, H, dtype=dt, device=dev)
@@ -641,7 +645,7 @@ class RoutedExpertsFn(torch.autograd.Function):
             # this one in the same kernel: one sum instead of autograd's extra add
             ctx.link.dx = dhs
             dhs = None
-        return dhs, dweights, None, None, d_wgu, d_wdn, None, None
+        return dhs, dweights, None, None, d_wgu, d_wdn, None, None, None
 
 
 def _fp8_experts_backward(ctx, dout: torch.Tensor, dweights: torch.Tensor):
@@ -664,7 +668,7 @@ def _fp8_experts_backward(ctx, dout: torch.Tensor, dweights: torch.Tensor):
     d_wgu = _dense_weight_grad(dgu, hs, b.token_idx, b, ctx.wdt[0]) if want_gu else None
     if ctx.link is not None:
         ctx.link.dx, dhs = dhs, None
-    return dhs, dweights, None, None, d_wgu, d_wdn, None, None
+    return dhs, dweights, None, None, d_wgu, d_wdn, None, None, None
 
 
 def _no_overlay(ew: ExpertWeights, which: str) -> None:
@@ -786,9 +790,10 @@ def routed_experts(hs: torch.Tensor, weights: torch.Tensor, experts: ExpertWeigh
     gradient of both branches (HsGradLink)."""
     wg, wd = weight_params if weight_params is not None else (None, None)
     slots = None if slot_capacity is None and overflow is None else (slot_capacity, overflow)
-    if experts.is_fp8 and torch.is_grad_enabled() and (hs.requires_grad or weights.requires_grad):
+    backward = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hs, weights, wg, wd))
+    if experts.is_fp8 and backward:
         N.refuse_capture("a pass over 8-bit experts that wants a gradient")
-    return RoutedExpertsFn.apply(hs, weights, experts, capture, wg, wd, slots, link)
+    return RoutedExpertsFn.apply(hs, weights, experts, capture, wg, wd, slots, link, backward)
 
 
 class RouteTopKFn(torch.autograd.Function):
