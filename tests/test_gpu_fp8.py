@@ -34,7 +34,8 @@ def _within(got, ref, bound):
 # ---- codec ---------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=_ids)
-@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 127), (5, 128), (2, 129), (17, 640), (4, 2027)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 127), (5, 128), (2, 129), (17, 640), (4, 2027), (9, 512), (5, 1536),
+                                       (33, 2048)])
 def test_quantize_rows_is_the_oracles(F, rows, cols, dtype):
     # magnitudes over the type's whole range, a row of zeros, a block border of every kind
     x = _rand(rows, cols, dtype=torch.float32, seed=rows + cols)
@@ -63,13 +64,14 @@ def test_scale_at_the_borders(F, amax):
     assert float(x.abs().max()) * 2.0 ** (127 - int(r.s[0, 0])) <= 448
 
 
-def test_rows_behind_the_given_count_are_left(F):
-    x = _rand(6, 256).cuda()
+@pytest.mark.parametrize("cols", [256, 512, 2048])
+def test_rows_behind_the_given_count_are_left(F, cols):
+    x = _rand(23, cols).cuda()
     n = torch.tensor([4], dtype=torch.int32, device="cuda")
-    rows = F.empty_rows(6, 256, x.device)
+    rows = F.empty_rows(23, cols, x.device)
     rows.q.fill_(17)
     from usaf_amd import _native as N
-    N.call("usaf_hip_fp8_quantize_rows", x.data_ptr(), N.BF16, 6, 256, 256, n.data_ptr(), rows.q.data_ptr(),
+    N.call("usaf_hip_fp8_quantize_rows", x.data_ptr(), N.BF16, 23, cols, cols, n.data_ptr(), rows.q.data_ptr(),
            rows.s.data_ptr(), N.stream_ptr(x.device))
     assert bool((rows.q[4:] == 17).all()) and torch.equal(rows.q[:4], F.quantize_rows(x[:4]).q)
 

@@ -38,18 +38,23 @@ __device__ __forceinline__ float max_rot(float v) {
 }
 __device__ __forceinline__ float max16(float v) { return max_rot<1>(max_rot<2>(max_rot<4>(max_rot<8>(v)))); }
 
+// Eight 16-bit values of a register quadruple.
+template <int DT>
+__device__ __forceinline__ void unpack8(const uint4 q, float (&v)[8]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const f32x2 f = unpack2<DT>(w[j]);
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
+  }
+}
+
 // 8 neighbouring values of a 16-bit row; `left` of them exist.
 template <int DT>
 __device__ __forceinline__ void load8(const uint16_t* p, bool vec, int left, float (&v)[8]) {
   if (vec && left >= 8) {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x2 f = unpack2<DT>(w[j]);
-      v[2 * j] = f.x;
-      v[2 * j + 1] = f.y;
-    }
+    unpack8<DT>(*reinterpret_cast<const uint4*>(p), v);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = j < left ? load_as_f32<DT>(p, j) : 0.f;

@@ -38,6 +38,48 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const uint16_t* __restric
   store_block(v, lane16, q + row * kp + c, s + row * sp + kb);
 }
 
+// The same for aligned rows of a multiple of 512 columns: a wave has four blocks of a row, whose
+// scale bytes are one word, R_AHEAD times, whose loads go out together.
+constexpr int R_AHEAD = 4;
+template <int DT>
+__global__ __launch_bounds__(256) void fp8_rows4_kernel(const uint16_t* __restrict__ x, int64_t rows, int64_t ld, int nkw,
+                                                        const int32_t* __restrict__ n_rows, uint8_t* __restrict__ q,
+                                                        uint8_t* __restrict__ s) {
+  const int lane = threadIdx.x & 63;
+  const int64_t end = n_rows && *n_rows < rows ? *n_rows : rows;
+  int64_t at = (int64_t)blockIdx.x * (4 * R_AHEAD) + (threadIdx.x >> 6), row[R_AHEAD];  // the wave's words
+  int kw[R_AHEAD];
+  row[0] = at / nkw;
+  kw[0] = (int)(at - row[0] * nkw);
+  uint4 v[R_AHEAD];
+#pragma unroll
+  for (int i = 0; i < R_AHEAD; ++i) {
+    if (i) {  // four words on
+      row[i] = row[i - 1];
+      kw[i] = kw[i - 1] + 4;
+      while (kw[i] >= nkw) {
+        kw[i] -= nkw;
+        ++row[i];
+      }
+    }
+    v[i] = *reinterpret_cast<const uint4*>(x + (row[i] < rows ? row[i] : rows - 1) * ld + kw[i] * 512 + 8 * lane);
+  }
+#pragma unroll
+  for (int i = 0; i < R_AHEAD; ++i) {
+    if (row[i] >= end) return;  // wave-uniform
+    float f[8], m = 0.f;
+    unpack8<DT>(v[i], f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(f[j]));
+    const int e = e8m0_of(max16(m));
+    const float inv = inv_scale(e), a[4] = {f[0], f[1], f[2], f[3]}, b[4] = {f[4], f[5], f[6], f[7]};
+    *reinterpret_cast<uint2*>(q + (row[i] * nkw + kw[i]) * 512 + 8 * lane) = uint2{to_codes(a, inv), to_codes(b, inv)};
+    const uint32_t word = (uint32_t)__builtin_amdgcn_readlane(e, 0) | (uint32_t)__builtin_amdgcn_readlane(e, 16) << 8 |
+                          (uint32_t)__builtin_amdgcn_readlane(e, 32) << 16 | (uint32_t)__builtin_amdgcn_readlane(e, 48) << 24;
+    if (lane == 0) *reinterpret_cast<uint32_t*>(s + (row[i] * nkw + kw[i]) * 4) = word;
+  }
+}
+
 // Weight [E, R, C] -> codes [E, R, kp], scale bytes [E, ceil(R / 128), kp / 128].
 // A block of threads takes one 128 x 128 block: 16 lanes a row, 16 rows at a time.
 template <int DT>
@@ -266,19 +308,24 @@ extern "C" int usaf_hip_fp8_quantize_rows(const void* x, int32_t dtype, int64_t 
     return set_error(USAF_ERR_INVALID, "fp8_quantize_rows: codes must be 16-byte and values 2-byte aligned");
   const int64_t nkb = (cols + FP8_BLOCK - 1) / FP8_BLOCK;
   const bool vec = ((uintptr_t)x % 16) == 0 && ld % 8 == 0;
-  unsigned blocks;
   if (rows > ((int64_t)1 << 40) / nkb) return set_error(USAF_ERR_INVALID, "fp8_quantize_rows: too many rows");
+  if (dtype != USAF_BF16 && dtype != USAF_F16)
+    return set_error(USAF_ERR_INVALID, "fp8_quantize_rows: dtype must be fp16 or bf16");
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(x);
+  const hipStream_t st = as_stream(stream);
+  unsigned blocks;
+  if (vec && cols % 512 == 0 && (uintptr_t)s % 4 == 0) {
+    if (int rc = blocks16((rows * nkb + R_AHEAD - 1) / R_AHEAD, "fp8_quantize_rows", &blocks)) return rc;
+    if (dtype == USAF_BF16) fp8_rows4_kernel<USAF_BF16><<<blocks, 256, 0, st>>>(p, rows, ld, (int)(nkb / 4), n_rows, q, s);
+    else fp8_rows4_kernel<USAF_F16><<<blocks, 256, 0, st>>>(p, rows, ld, (int)(nkb / 4), n_rows, q, s);
+    return check_launch("fp8_quantize_rows");
+  }
   if (int rc = blocks16(rows * nkb, "fp8_quantize_rows", &blocks)) return rc;
   const int sp = (int)usaf_hip_fp8_scale_stride(cols);
-  const uint16_t* p = reinterpret_cast<const uint16_t*>(x);
   if (dtype == USAF_BF16)
-    fp8_rows_kernel<USAF_BF16><<<blocks, 256, 0, as_stream(stream)>>>(p, rows, cols, ld, vec, (int)nkb, nkb * FP8_BLOCK,
-                                                                      sp, n_rows, q, s);
-  else if (dtype == USAF_F16)
-    fp8_rows_kernel<USAF_F16><<<blocks, 256, 0, as_stream(stream)>>>(p, rows, cols, ld, vec, (int)nkb, nkb * FP8_BLOCK,
-                                                                     sp, n_rows, q, s);
+    fp8_rows_kernel<USAF_BF16><<<blocks, 256, 0, st>>>(p, rows, cols, ld, vec, (int)nkb, nkb * FP8_BLOCK, sp, n_rows, q, s);
   else
-    return set_error(USAF_ERR_INVALID, "fp8_quantize_rows: dtype must be fp16 or bf16");
+    fp8_rows_kernel<USAF_F16><<<blocks, 256, 0, st>>>(p, rows, cols, ld, vec, (int)nkb, nkb * FP8_BLOCK, sp, n_rows, q, s);
   return check_launch("fp8_quantize_rows");
 }
 

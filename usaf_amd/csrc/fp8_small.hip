@@ -27,18 +27,6 @@ __device__ __forceinline__ f32x4 mfma16_bf16(const u32x4 a, const u32x4 b, f32x4
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Eight 16-bit values of a register quadruple.
-template <int DT>
-__device__ __forceinline__ void unpack8(const uint4 q, float (&v)[8]) {
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const f32x2 f = unpack2<DT>(w[j]);
-    v[2 * j] = f.x;
-    v[2 * j + 1] = f.y;
-  }
-}
-
 template <int DT, int MT>
 __global__ __launch_bounds__(S_THREADS) void fp8_small_kernel(const uint16_t* __restrict__ x, int M, int64_t K, int64_t ld,
                                                               bool vec, const uint8_t* __restrict__ w,
