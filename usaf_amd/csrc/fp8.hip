@@ -39,7 +39,8 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const uint16_t* __restric
 }
 
 // The same for aligned rows of a multiple of 512 columns: a wave has four blocks of a row, whose
-// scale bytes are one word, R_AHEAD times, whose loads go out together.
+// scale bytes are one word, R_AHEAD times, whose loads go out together.  Bytes bound it: 8,192 x 4,096, 101 MB,
+// 27 us, 3.7 TB/s (one block for each 16 lanes and a byte store for each scale: 29).
 constexpr int R_AHEAD = 4;
 template <int DT>
 __global__ __launch_bounds__(256) void fp8_rows4_kernel(const uint16_t* __restrict__ x, int64_t rows, int64_t ld, int nkw,
@@ -128,7 +129,8 @@ __global__ __launch_bounds__(256) void fp8_dequant_kernel(const uint8_t* __restr
 }
 
 // [R, kp] codes -> [C, rp] codes of the transpose, rows past R as zeros; with the
-// scale bytes transposed.  One 128 x 128 block per thread block, through LDS.
+// scale bytes transposed.  One 128 x 128 block per thread block, through LDS: 402 MB read and written
+// in 200 us, 4.0 TB/s, once for a weight.
 __global__ __launch_bounds__(256) void fp8_transpose_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ s,
                                                             int64_t R, int64_t C, int64_t kp, int64_t rp,
                                                             uint8_t* __restrict__ qt, uint8_t* __restrict__ st) {
@@ -153,7 +155,8 @@ __global__ __launch_bounds__(256) void fp8_transpose_kernel(const uint8_t* __res
 }
 
 // gu [S, 2I] -> act = dt(dt(silu(gate)) up) [S, I] (null: not stored), its codes and scale
-// bytes, for the slots in use (offsets[E]).  16 lanes a block of 128 columns.
+// bytes, for the slots in use (offsets[E]).  16 lanes a block of 128 columns.  Bytes bound it:
+// 32,768 slots of 768, 126 MB, 26 us, 4.8 TB/s.
 template <int DT>
 __global__ __launch_bounds__(256) void fp8_swiglu_kernel(const uint16_t* __restrict__ gu, int64_t S, int64_t I,
                                                          const int32_t* __restrict__ n_slots, uint16_t* __restrict__ act,
@@ -182,7 +185,8 @@ __global__ __launch_bounds__(256) void fp8_swiglu_kernel(const uint16_t* __restr
 }
 
 // gu, dact -> dgu [S, 2I] with the roundings of the layer's other grad-input kernels
-// (null: not stored), its codes and scale bytes.
+// (null: not stored), its codes and scale bytes.  Bytes bound it: 32,768 slots of 768, 202 MB, 42
+// us, 4.8 TB/s.
 template <int DT>
 __global__ __launch_bounds__(256) void fp8_swiglu_bwd_kernel(const uint16_t* __restrict__ gu,
                                                              const uint16_t* __restrict__ dact, int64_t S, int64_t I,
@@ -230,8 +234,8 @@ __global__ __launch_bounds__(256) void fp8_swiglu_bwd_kernel(const uint16_t* __r
 // Backward of the weighted sum, slot m (token t, expert e): dcur = dt(w dout[t]) as codes and
 // scale bytes (and, where a sampled or dense weight gradient reads it, in 16 bits), and
 // dweights[t, e] = dt(<dout[t], y[m]>).  One block a slot, 16 lanes a block of 128
-// columns.  With the 16-bit dcur written and read again this took 59 + 47 us where a pass over
-// 32,768 slots of 2,048 reads 268 MB and writes 67.
+// columns.  32,768 slots of 2,048: 134 MB of y and as much of dout from the caches in, 67 out, 54 us (with the
+// 16-bit dcur written and read again 59 + 47).
 template <int DT>
 __global__ __launch_bounds__(256) void fp8_combine_bwd_kernel(const uint16_t* __restrict__ dout,
                                                               const uint16_t* __restrict__ y,
