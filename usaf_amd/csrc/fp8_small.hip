@@ -7,7 +7,9 @@
 // are on their way before the block quantizes the rows into LDS, all of them again in every
 // block, which takes less than a launch of its own.  The weights stream through
 // registers, a tile's behind the last one's sums; both sides' codes become bf16 values, exactly,
-// for the 16-bit matrix instruction, whose sums keep fp32's precision.
+// for the 16-bit matrix instruction, whose sums keep fp32's precision.  The weights' way from
+// memory bounds it, and for small ones the launch: 8.4 MB 6.1 us, 59 MB 16.6 us (3.5 TB/s), 268 MB 57.5 us
+// (4.7 TB/s), one row each.
 #include "fp8.h"
 
 namespace usaf {
