@@ -142,6 +142,6 @@ def test_capture_refuses_what_is_kept_or_wants_a_gradient(monkeypatch):
     with pytest.raises(RuntimeError, match="captured"):
         q4.scale_zero_by_group()
     assert q4._szg is None
-    x = torch.zeros(3, 128, dtype=torch.bfloat16, requires_grad=True)
+    x = torch.zeros(3, 128, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="captured"):
         routed_experts(x, torch.zeros(3, 2, dtype=torch.bfloat16), ExpertWeights(_t(2, 256, 128), _t(2, 128, 128)))

@@ -211,7 +211,7 @@ def stream_ptr(device: torch.device) -> int:
 def refuse_capture(what: str) -> None:
     """Raise where the current stream is being captured into a graph."""
     if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{what} cannot be captured into a graph: make it before the capture, or without a gradient")
+        raise RuntimeError(f"{what}: not while a stream is captured into a graph")
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

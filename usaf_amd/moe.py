@@ -791,8 +791,8 @@ def routed_experts(hs: torch.Tensor, weights: torch.Tensor, experts: ExpertWeigh
     wg, wd = weight_params if weight_params is not None else (None, None)
     slots = None if slot_capacity is None and overflow is None else (slot_capacity, overflow)
     backward = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hs, weights, wg, wd))
-    if experts.is_fp8 and backward:
-        N.refuse_capture("a pass over 8-bit experts that wants a gradient")
+    if experts.is_fp8:
+        N.refuse_capture("the routed layer on 8-bit experts (few.few_token_block can)")
     return RoutedExpertsFn.apply(hs, weights, experts, capture, wg, wd, slots, link, backward)
 
 
