@@ -204,9 +204,10 @@ def test_linear_has_no_second_derivative(F):
     assert g.shape == x.shape
 
 
-def test_linear_in_a_graph(F):
+@pytest.mark.parametrize("rows", [3, 50])
+def test_linear_in_a_graph(F, rows):
     t = F.Fp8Tensor.quantize(_rand(200, 384, seed=2, scale=0.1).cuda())
-    x = _rand(50, 384, seed=1).cuda()
+    x = _rand(rows, 384, seed=1).cuda()
     with torch.no_grad():
         F.fp8_linear(x, t)
         graphs = []
@@ -216,7 +217,7 @@ def test_linear_in_a_graph(F):
                 out = F.fp8_linear(x, t)
             graphs.append((g, out))
         for i in range(4):
-            x.copy_(_rand(50, 384, seed=10 + i))
+            x.copy_(_rand(rows, 384, seed=10 + i))
             for g, out in graphs:
                 g.replay()
                 torch.cuda.synchronize()

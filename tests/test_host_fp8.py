@@ -6,6 +6,7 @@ import torch
 
 from usaf_amd import _native as N
 from usaf_amd import fp8
+from usaf_amd.few import few_token_block
 from usaf_amd.moe import ExpertWeights, Q4Tensor, routed_experts
 
 
@@ -145,3 +146,16 @@ def test_capture_refuses_what_is_kept_or_wants_a_gradient(monkeypatch):
     x = torch.zeros(3, 128, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="captured"):
         routed_experts(x, torch.zeros(3, 2, dtype=torch.bfloat16), ExpertWeights(_t(2, 256, 128), _t(2, 128, 128)))
+
+
+def test_no_launch_on_cpu_tensors():
+    """A CPU tensor's device has no stream: every entry point asks for one before it launches."""
+    with pytest.raises(ValueError, match="GPU"):
+        N.stream_ptr(torch.device("cpu"))
+    x = torch.zeros(2, 128, dtype=torch.bfloat16)
+    ew = ExpertWeights(_t(2, 256, 128), _t(2, 128, 128))
+    for call in (lambda: fp8.quantize_rows(x), lambda: routed_experts(x, torch.ones(2, 2, dtype=torch.bfloat16), ew),
+                 lambda: _t(64, 128).transposed(), lambda: _t(64, 128).dequantize(),
+                 lambda: few_token_block(x, torch.zeros(2, 128, dtype=torch.bfloat16), 1, True, ew)):
+        with pytest.raises((ValueError, RuntimeError, AssertionError)):
+            call()

@@ -204,6 +204,8 @@ def default_device() -> torch.device:
 
 def stream_ptr(device: torch.device) -> int:
     """Raw hipStream_t of torch's current stream on `device`."""
+    if device.type != "cuda":
+        raise ValueError(f"expected a tensor on a GPU, got one on {device}")
     # without a torch.cuda.Stream object, which takes 1.8 us to make (this call 0.1)
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 

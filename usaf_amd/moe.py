@@ -527,8 +527,8 @@ class RoutedExpertsFn(torch.autograd.Function):
             raise ValueError(f"shape mismatch: hs {tuple(hs.shape)}, weights {tuple(weights.shape)}, "
                              f"experts E={E} H={ew.H} I={I}")
         dev = hs.device
-        if ew.is_fp8 and ew.gate_up.device != dev:
-            raise ValueError(f"activations on {dev}, 8-bit experts on {ew.gate_up.device}")
+        if ew.is_fp8 and (ew.gate_up.device != dev or not hs.is_cuda):
+            raise ValueError(f"activations on {dev}, 8-bit experts on {ew.gate_up.device}: both on one GPU")
         st = N.stream_ptr(dev)
         code = N.dtype_code(dt)
         # (before the bucketing, whose host read would leave the GPU idle for it)
