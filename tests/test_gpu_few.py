@@ -277,6 +277,30 @@ def test_near_the_routed_layer(B):
     assert float(rel.max()) <= 10 * O.half_step(torch.bfloat16)
 
 
+@pytest.mark.parametrize("fmt", ["q4", "fp8"])
+def test_weights_past_32_bits(B, fmt):
+    """The last of the experts, past 4 GiB of codes: as the only expert of its own, in every bit."""
+    from usaf_amd.fp8 import Fp8Tensor
+    from usaf_amd.moe import ExpertWeights, Q4Tensor
+    E, H, I = (80 if fmt == "q4" else 40), 8192, 8192
+    small, _ = _random_experts(fmt, 1, H, I)
+    big = []
+    for t, shape in ((small.gate_up, (E, 2 * I, H)), (small.down, (E, H, I))):
+        parts = (t.q, t.s) if fmt == "fp8" else (t.q, t.s, t.z)
+        wide = []
+        for p in parts:
+            rows = p.shape[1:] if fmt == "fp8" else p.shape
+            a = torch.zeros(E * rows[0], *rows[1:], dtype=p.dtype, device="cuda")
+            a[-rows[0]:] = p.reshape(rows)
+            wide.append(a.view(E, *rows) if fmt == "fp8" else a)
+        big.append(Fp8Tensor(*wide, shape) if fmt == "fp8" else Q4Tensor(*wide, torch.Size(shape)))
+    x = _rand(2, H, seed=1).cuda()
+    router = torch.zeros(E, H, dtype=torch.bfloat16, device="cuda")
+    x[:, 0], router[-1, 0] = 30, 30  # both tokens to the last expert
+    got = B.few_token_block(x, router, 1, True, ExpertWeights(*big))
+    assert torch.equal(got, B.few_token_block(x, router[-1:], 1, True, small))
+
+
 def test_patched_block_uses_it(B):
     """A patched Qwen3-MoE block with _usaf_few_tokens set takes its few-token passes here, and no others."""
     from types import SimpleNamespace

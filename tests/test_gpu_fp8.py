@@ -383,6 +383,54 @@ def test_sampled_gradient_on_8_bit_experts(F):
         _within(store.compact[name], ref, ref.abs() * O.half_step(torch.bfloat16) + 2 * T * 2.0 ** -23 * mag)
 
 
+@pytest.mark.parametrize("which", [(True, True), (True, False), (False, True)])
+def test_dense_weight_gradients_beside_8_bit_experts(F, which):
+    """weight_params get dgu^T hs and dcur^T act of the 8-bit layer's own steps; a gradient that nobody wants is not made."""
+    from usaf_amd import moe as G
+    T, E, H, I, k = 60, 4, 256, 128, 2
+    ew = _experts(F, E, H, I)
+    wg, wd = (torch.zeros(*s, dtype=torch.float32, device="cuda").requires_grad_(r)
+              for s, r in (((E, 2 * I, H), which[0]), ((E, H, I), which[1])))
+    hs, w, dout = _rand(T, H, seed=9), _routing(T, E, k, torch.bfloat16, seed=3), _rand(T, H, seed=11)
+    out = G.routed_experts(hs.cuda(), w.cuda(), ew, weight_params=(wg, wd))  # no gradient but the weights'
+    b, gu = out.grad_fn.b, out.grad_fn.saved_tensors[1].clone()
+    out.backward(dout.cuda())
+    offs, tok = b.offsets.tolist(), b.token_idx.long().cpu()
+    slot_e = torch.repeat_interleave(torch.arange(E), torch.tensor(offs[1:]) - torch.tensor(offs[:-1]))
+    dcur = (w[tok, slot_e].double()[:, None] * dout[tok].double()).bfloat16()
+    dgu, act = torch.empty_like(gu), torch.empty(gu.shape[0], I, dtype=gu.dtype, device="cuda")
+    F.experts_bwd(F.quantize_rows(dcur.cuda()), gu, ew, b, dgu, torch.empty(gu.shape[0], H, dtype=gu.dtype, device="cuda"))
+    F.experts_forward(F.quantize_rows(hs.cuda()), ew, b, torch.empty_like(gu), act, gu.dtype)
+    for p, want, left, right in ((wg, which[0], dgu.double().cpu(), hs.double()[tok]), (wd, which[1], dcur.double(), act.double().cpu())):
+        if not want:
+            assert p.grad is None
+            continue
+        for e in range(E):
+            l, r = left[offs[e]:offs[e + 1]], right[offs[e]:offs[e + 1]]
+            # fp32 sums over at most T slots, stored in fp32
+            _within(p.grad[e], l.t() @ r, (2 * T + 1) * 2.0 ** -23 * (l.t().abs() @ r.abs()))
+
+
+def test_slots_without_a_host_read(F):
+    """slot_capacity: more slots than pairs, the ones behind them unused; the same output and gradients."""
+    from usaf_amd import moe as G
+    T, E, H, I, k = 60, 4, 256, 128, 2
+    ew = _experts(F, E, H, I)
+    hs, w, dout = _rand(T, H, seed=9).cuda(), _routing(T, E, k, torch.bfloat16, seed=3).cuda(), _rand(T, H, seed=11).cuda()
+    got = []
+    for extra in (None, 8):
+        x, ww = hs.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+        kw = {} if extra is None else {"slot_capacity": T * k + extra, "overflow": flag}
+        out = G.routed_experts(x, ww, ew, **kw)
+        out.backward(dout)
+        got.append((out.detach(), x.grad, ww.grad))
+        with torch.no_grad():
+            assert torch.equal(G.routed_experts(x, ww, ew, **kw), out)
+        assert int(flag) == 0
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_refusals_on_the_gpu(F):
     from usaf_amd.moe import ExpertWeights, routed_experts
     t = F.Fp8Tensor.quantize(_rand(64, 128).cuda())
@@ -433,6 +481,32 @@ def test_product_of_whole_numbers_on_every_tile(F, E, M, N, K, wide):
         lo, hi = offs[e], offs[e + 1]
         assert torch.equal(out[lo:hi].float(), picked[lo:hi] @ w[e].t())
     assert bool((out[offs[-1]:] == 333).all())
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_product_past_32_bits(F, wide):
+    """Weights past 4 GiB and an output past 2^32 bytes: the last expert's and the last rows' places."""
+    E, N, K = 40, 16384, 8192
+    w = torch.ones(128, K, device="cuda")
+    w[::3] = -1
+    q = torch.zeros(E, N, K, dtype=torch.uint8, device="cuda")
+    last = F.Fp8Tensor.quantize(w)
+    q[-1, -128:] = last.q
+    s = torch.full((E, N // 128, K // 128), 127, dtype=torch.uint8, device="cuda")
+    s[-1, -1] = last.s[0]
+    x = torch.randint(-1, 2, (5, K), generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    offs = torch.tensor([0] * E + [5], dtype=torch.int32, device="cuda")
+    out = torch.empty(5, N, dtype=torch.bfloat16, device="cuda")
+    F.product(F.quantize_rows(x), F.Fp8Tensor(q, s, (E, N, K)), out, offs, wide=wide)
+    assert torch.equal(out[:, -128:], (x.float() @ w.t()).bfloat16()) and not out[:, :-128].any()
+    del q, s, out
+    M, K = 140_000, 128
+    w = torch.randint(-1, 2, (N, K), generator=torch.Generator().manual_seed(2)).float().cuda()
+    x = torch.randint(-1, 2, (M, K), generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    out = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+    F.product(F.quantize_rows(x), F.Fp8Tensor.quantize(w), out, wide=wide)
+    for rows in (slice(0, 64), slice(M // 2, M // 2 + 64), slice(M - 64, M)):
+        assert torch.equal(out[rows].float(), x[rows].float() @ w.t())
 
 
 def test_what_is_kept_is_built_once_for_all_streams(F):
