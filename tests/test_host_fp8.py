@@ -148,6 +148,14 @@ def test_capture_refuses_what_is_kept_or_wants_a_gradient(monkeypatch):
         routed_experts(x, torch.zeros(3, 2, dtype=torch.bfloat16), ExpertWeights(_t(2, 256, 128), _t(2, 128, 128)))
 
 
+def test_overlays_on_8_bit_experts_are_refused():
+    """Trained values are held over 4-bit weights only: never left out in silence."""
+    ew = ExpertWeights(_t(2, 256, 128), _t(2, 128, 128))
+    ew.overlays["down"] = object()  # as a patched module's overlays are attached
+    with pytest.raises(NotImplementedError, match="overlay"):
+        routed_experts(torch.zeros(3, 128, dtype=torch.bfloat16), torch.zeros(3, 2, dtype=torch.bfloat16), ew)
+
+
 def test_no_launch_on_cpu_tensors():
     """A CPU tensor's device has no stream: every entry point asks for one before it launches."""
     with pytest.raises(ValueError, match="GPU"):

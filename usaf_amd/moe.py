@@ -792,6 +792,8 @@ def routed_experts(hs: torch.Tensor, weights: torch.Tensor, experts: ExpertWeigh
     slots = None if slot_capacity is None and overflow is None else (slot_capacity, overflow)
     backward = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hs, weights, wg, wd))
     if experts.is_fp8:
+        if experts.overlays:
+            raise NotImplementedError("trained values (overlays) apply to 4-bit experts, not to 8-bit ones")
         N.refuse_capture("the routed layer on 8-bit experts (few.few_token_block can)")
     return RoutedExpertsFn.apply(hs, weights, experts, capture, wg, wd, slots, link, backward)
 
