@@ -627,6 +627,27 @@ int usaf_hip_fp8_combine_bwd(const void* dout, const void* y, const int32_t* tok
                              uint8_t* q, uint8_t* s, void* dweights, void* stream);
 
 /*
+ * An 8-bit expert layer between the bucketing and the weighted sum (qwen3moe_dml.py:49-64), and its
+ * grad-input, each in one call of the entries above.  Forward: x, x_scale quantized hidden states
+ * [T, H]; gu [S, 2I] and act [S, I] are kept where not NULL (a backward reads gu; with both NULL the sizes must be
+ * ones of usaf_hip_fp8_gate_up_ok); y [S, H].  Backward: the transposed weights (usaf_hip_fp8_transpose); dcur [S, H] and
+ * dgu [S, 2I] kept where not NULL; dx_slots [S, H]; dweights [T, E], written at the routed pairs.  H and I multiples
+ * of 128; 16-byte aligned operands and workspace.
+ */
+int64_t usaf_hip_fp8_experts_fwd_ws_bytes(int64_t S, int64_t I);
+int usaf_hip_fp8_experts_fwd(const uint8_t* x, const uint8_t* x_scale, int64_t T, const int32_t* token_idx,
+                             const int32_t* offsets, int64_t S, int64_t E, int64_t H, int64_t I, int32_t dtype,
+                             const uint8_t* gate_up, const uint8_t* gate_up_scale, const uint8_t* down,
+                             const uint8_t* down_scale, void* gu, void* act, void* y, void* ws, int64_t ws_bytes,
+                             void* stream);
+int64_t usaf_hip_fp8_experts_bwd_ws_bytes(int64_t S, int64_t H, int64_t I);
+int usaf_hip_fp8_experts_bwd(const void* dout, const void* y, const void* gu, const int32_t* token_idx,
+                             const float* slot_w, const int32_t* offsets, int64_t S, int64_t E, int64_t H, int64_t I,
+                             int32_t dtype, const uint8_t* down_t, const uint8_t* down_t_scale, const uint8_t* gate_up_t,
+                             const uint8_t* gate_up_t_scale, void* dcur, void* dgu, void* dx_slots, void* dweights,
+                             void* ws, int64_t ws_bytes, void* stream);
+
+/*
  * A whole MoE layer for T <= 32 tokens (qwen3moe_dml.py:24-86 without the
  * intermediate 16-bit roundings of logits, gate, up and the experts' outputs):
  *   l = x router^T, the top_k largest l (ties: the lowest expert), w = softmax(l) of

@@ -3,9 +3,18 @@ import pytest
 import torch
 
 import fp8_oracle as O
+from usaf_amd import _native as N
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16]
+
+
+def _product(x, w, out, offsets=None, row_of=None, wide=False):
+    """out[m] = x[row_of[m] or m] @ w_e^T for the slots m of expert e, as the layer's calls make it."""
+    E, n, k = (1, *w.shape) if len(w.shape) == 2 else w.shape
+    N.call("usaf_hip_fp8_gemm", x.q.data_ptr(), x.s.data_ptr(), x.q.shape[0], N.ptr(row_of), out.shape[0], w.q.data_ptr(),
+           w.s.data_ptr(), N.ptr(offsets), E, n, k, N.dtype_code(out.dtype), 1 if wide else 0, out.data_ptr(),
+           N.stream_ptr(out.device))
 
 
 def _ids(d):
@@ -70,7 +79,6 @@ def test_rows_behind_the_given_count_are_left(F, cols):
     n = torch.tensor([4], dtype=torch.int32, device="cuda")
     rows = F.empty_rows(23, cols, x.device)
     rows.q.fill_(17)
-    from usaf_amd import _native as N
     N.call("usaf_hip_fp8_quantize_rows", x.data_ptr(), N.BF16, 23, cols, cols, n.data_ptr(), rows.q.data_ptr(),
            rows.s.data_ptr(), N.stream_ptr(x.device))
     assert bool((rows.q[4:] == 17).all()) and torch.equal(rows.q[:4], F.quantize_rows(x[:4]).q)
@@ -291,11 +299,17 @@ def test_experts_step_by_step(F, T, E, k, H, I, only, dtype):
     # the backward's own steps again, on its inputs
     dcur64 = pw * dout[tok].double()
     dcur = dcur64.to(dtype).cuda()
-    dgu, dx_slots, got_dcur = torch.empty_like(gu), torch.empty_like(y), torch.empty_like(y)
-    rows = F.experts_combine_bwd(dout.cuda(), y, b, got_dcur, torch.zeros(T, E, dtype=dtype, device="cuda"))
+    dgu, got_dcur, dweights = torch.empty_like(gu), torch.empty_like(y), torch.zeros(T, E, dtype=dtype, device="cuda")
+    dx_slots = F.experts_bwd(dout.cuda(), y, gu, ew, b, got_dcur, dgu, dweights)
     # (equal to the last bit but for the sign of zeros, which a code has too)
-    assert torch.equal(got_dcur, dcur) and torch.equal(rows.q, F.quantize_rows(got_dcur).q)
-    F.experts_bwd(rows, gu, ew, b, dgu, dx_slots)
+    assert torch.equal(got_dcur, dcur) and torch.equal(dweights, wv.grad)
+    rows = F.empty_rows(b.n_slots, H, y.device)
+    N.call("usaf_hip_fp8_combine_bwd", dout.cuda().data_ptr(), y.data_ptr(), b.token_idx.data_ptr(), b.slot_w.data_ptr(),
+           b.offsets.data_ptr(), b.n_slots, E, H, N.dtype_code(dtype), None, rows.q.data_ptr(), rows.s.data_ptr(),
+           dweights.data_ptr(), N.stream_ptr(y.device))
+    assert torch.equal(rows.q, F.quantize_rows(got_dcur).q) and torch.equal(dweights, wv.grad)
+    plain = F.experts_bwd(dout.cuda(), y, gu, ew, b, None, None, torch.zeros_like(dweights))
+    assert torch.equal(plain, dx_slots)
     qc = O.quantized_rows(dcur.cpu())[0]
     dgu64 = dgu.double().cpu()
     q_dgu = O.quantized_rows(dgu.cpu())[0]
@@ -366,15 +380,15 @@ def test_sampled_gradient_on_8_bit_experts(F):
     dout = _rand(T, H, seed=11)
     x = hs.cuda().requires_grad_(True)
     out = G.routed_experts(x, w.cuda(), ew, capture=(store, "L"))
-    _, gu, act, _ = out.grad_fn.saved_tensors
+    _, gu, act, y = out.grad_fn.saved_tensors
     b = out.grad_fn.b
-    gu, act = gu.clone(), act.double().cpu()
+    gu, act, y = gu.clone(), act.double().cpu(), y.clone()
     out.backward(dout.cuda())
     offs, tok = b.offsets.tolist(), b.token_idx.long().cpu()
     slot_e = torch.repeat_interleave(torch.arange(E), torch.tensor(offs[1:]) - torch.tensor(offs[:-1]))
     dcur = (w[tok, slot_e].double()[:, None] * dout[tok].double()).bfloat16()
     dgu = torch.empty_like(gu)
-    F.experts_bwd(F.quantize_rows(dcur.cuda()), gu, ew, b, dgu, torch.empty(gu.shape[0], H, dtype=gu.dtype, device="cuda"))
+    F.experts_bwd(dout.cuda(), y, gu, ew, b, None, dgu, torch.zeros(T, E, dtype=gu.dtype, device="cuda"))
     for name, left, right in (("L.gate_up_proj", dgu.double().cpu(), hs.double()[tok]), ("L.down_proj", dcur.double(), act)):
         ref = torch.stack([left[offs[e]:offs[e + 1]].t() @ right[offs[e]:offs[e + 1]] for e in range(E)]).reshape(-1)
         mag = torch.stack([left[offs[e]:offs[e + 1]].t().abs() @ right[offs[e]:offs[e + 1]].abs() for e in range(E)]).reshape(-1)
@@ -393,13 +407,13 @@ def test_dense_weight_gradients_beside_8_bit_experts(F, which):
               for s, r in (((E, 2 * I, H), which[0]), ((E, H, I), which[1])))
     hs, w, dout = _rand(T, H, seed=9), _routing(T, E, k, torch.bfloat16, seed=3), _rand(T, H, seed=11)
     out = G.routed_experts(hs.cuda(), w.cuda(), ew, weight_params=(wg, wd))  # no gradient but the weights'
-    b, gu = out.grad_fn.b, out.grad_fn.saved_tensors[1].clone()
+    b, gu, y = out.grad_fn.b, out.grad_fn.saved_tensors[1].clone(), out.grad_fn.saved_tensors[3].clone()
     out.backward(dout.cuda())
     offs, tok = b.offsets.tolist(), b.token_idx.long().cpu()
     slot_e = torch.repeat_interleave(torch.arange(E), torch.tensor(offs[1:]) - torch.tensor(offs[:-1]))
     dcur = (w[tok, slot_e].double()[:, None] * dout[tok].double()).bfloat16()
     dgu, act = torch.empty_like(gu), torch.empty(gu.shape[0], I, dtype=gu.dtype, device="cuda")
-    F.experts_bwd(F.quantize_rows(dcur.cuda()), gu, ew, b, dgu, torch.empty(gu.shape[0], H, dtype=gu.dtype, device="cuda"))
+    F.experts_bwd(dout.cuda(), y, gu, ew, b, None, dgu, torch.zeros(T, E, dtype=gu.dtype, device="cuda"))
     F.experts_forward(F.quantize_rows(hs.cuda()), ew, b, torch.empty_like(gu), act, gu.dtype)
     for p, want, left, right in ((wg, which[0], dgu.double().cpu(), hs.double()[tok]), (wd, which[1], dcur.double(), act.double().cpu())):
         if not want:
@@ -469,13 +483,13 @@ def test_product_of_whole_numbers_on_every_tile(F, E, M, N, K, wide):
     out = torch.full((M, N), 333.0, dtype=dtype, device="cuda")
     rows, t = F.quantize_rows(x), F.Fp8Tensor.quantize(w)
     if E is None:
-        F.product(rows, t, out, wide=wide)
+        _product(rows, t, out, wide=wide)
         assert torch.equal(out.float(), x.float() @ w.t())
         return
     ends = torch.randint(0, M - M // 8 + 1, (E,), generator=g).sort().values.tolist()
     offs = [0] + ends[:-1] + [M - M // 8]
     tok = torch.randint(0, n_rows, (M,), generator=g).to(torch.int32).cuda()
-    F.product(rows, t, out, torch.tensor(offs, dtype=torch.int32, device="cuda"), tok, wide=wide)
+    _product(rows, t, out, torch.tensor(offs, dtype=torch.int32, device="cuda"), tok, wide=wide)
     picked = x.float()[tok.long()]
     for e in range(E):
         lo, hi = offs[e], offs[e + 1]
@@ -497,14 +511,14 @@ def test_product_past_32_bits(F, wide):
     x = torch.randint(-1, 2, (5, K), generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
     offs = torch.tensor([0] * E + [5], dtype=torch.int32, device="cuda")
     out = torch.empty(5, N, dtype=torch.bfloat16, device="cuda")
-    F.product(F.quantize_rows(x), F.Fp8Tensor(q, s, (E, N, K)), out, offs, wide=wide)
+    _product(F.quantize_rows(x), F.Fp8Tensor(q, s, (E, N, K)), out, offs, wide=wide)
     assert torch.equal(out[:, -128:], (x.float() @ w.t()).bfloat16()) and not out[:, :-128].any()
     del q, s, out
     M, K = 140_000, 128
     w = torch.randint(-1, 2, (N, K), generator=torch.Generator().manual_seed(2)).float().cuda()
     x = torch.randint(-1, 2, (M, K), generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
     out = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
-    F.product(F.quantize_rows(x), F.Fp8Tensor.quantize(w), out, wide=wide)
+    _product(F.quantize_rows(x), F.Fp8Tensor.quantize(w), out, wide=wide)
     for rows in (slice(0, 64), slice(M // 2, M // 2 + 64), slice(M - 64, M)):
         assert torch.equal(out[rows].float(), x[rows].float() @ w.t())
 
@@ -588,7 +602,6 @@ def test_a_layer_tuned_and_served(F):
 @pytest.mark.parametrize("E,M,I,K", [(8, 1500, 2048, 256), (8, 500, 2176, 128), (40, 2000, 1024, 129), (200, 700, 384, 640)])
 def test_gate_up_ends_in_the_activations_codes(F, E, M, I, K, dtype):
     """One launch or two: the same bits; slots behind the last one are left."""
-    from usaf_amd import _native as N
     g = torch.Generator().manual_seed(M)
     w = F.Fp8Tensor.quantize(_rand(E, 2 * I, K, seed=E, scale=0.1).cuda())
     hs = _rand(M // 2, K, dtype=dtype, seed=K)
@@ -599,7 +612,7 @@ def test_gate_up_ends_in_the_activations_codes(F, E, M, I, K, dtype):
     offs = torch.tensor([0] + ends + [used], dtype=torch.int32, device="cuda")
     tok = torch.randint(0, M // 2, (M,), generator=g).to(torch.int32).cuda()
     gu = torch.empty(M, 2 * I, dtype=dtype, device="cuda")
-    F.product(x, w, gu, offs, tok, wide=True)
+    _product(x, w, gu, offs, tok, wide=True)
     want, got = F.empty_rows(M, I, x.q.device), F.empty_rows(M, I, x.q.device)
     for t in (want.q, want.s, got.q, got.s):
         t.fill_(77)

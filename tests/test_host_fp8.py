@@ -92,6 +92,22 @@ def test_entry_points_check_their_arguments():
         assert up(v["a"], p, 1, None, 1, v["w"], p, p, 1, 128, 8, N.BF16, v["q"], v["s"], None) == inval, bad
     assert [up_ok(*a) for a in [(4, 4, 128, 256), (0, 4, 128, 256), (16384, 64, 1024, 2048), (16384, 256, 1024, 2048)]] == [0, 0, 1, 0]
     assert up(p, p, 4, None, 4, p, p, p, 4, 128, 256, N.BF16, p, p, None) == N.USAF_ERR_UNSUPPORTED
+    fwd, bwd = lib.usaf_hip_fp8_experts_fwd, lib.usaf_hip_fp8_experts_bwd
+    fw, bw = lib.usaf_hip_fp8_experts_fwd_ws_bytes, lib.usaf_hip_fp8_experts_bwd_ws_bytes
+    assert [fw(3, 128), fw(0, 128), fw(-1, 128), bw(3, 256, 128), bw(-1, 8, 8)] == [3 * 132, 0, -1, 784 + 3 * 256, -1]
+    good = dict(x=p, xs=p, T=3, tok=p, offs=p, S=3, E=2, H=256, I=128, dt=N.BF16, gu=p, gus=p, dn=p, dns=p, keep=p, act=p, y=p,
+                ws=p, ws_bytes=3 * 132, stream=None)
+    assert fwd(*{**good, "S": 0, "ws": None, "ws_bytes": 0}.values()) == ok
+    for bad in [dict(H=100), dict(I=100), dict(tok=None), dict(offs=None), dict(y=None), dict(ws=None), dict(ws=odd),
+                dict(ws_bytes=3 * 132 - 1), dict(x=None), dict(keep=None), dict(dt=N.F32), dict(x=odd), dict(S=-1)]:
+        assert fwd(*{**good, **bad}.values()) == inval, bad
+    assert fwd(*{**good, "keep": None, "act": None}.values()) == N.USAF_ERR_UNSUPPORTED  # few slots keep gu
+    good = dict(dout=p, y=p, gu=p, tok=p, w=p, offs=p, S=3, E=2, H=256, I=128, dt=N.BF16, dn=p, dns=p, gut=p, guts=p, dcur=None,
+                dgu=None, dx=p, dw=p, ws=p, ws_bytes=784 + 768, stream=None)
+    assert bwd(*{**good, "S": 0, "ws": None, "ws_bytes": 0}.values()) == ok
+    for bad in [dict(H=100), dict(I=100), dict(gu=None), dict(dx=None), dict(ws=None), dict(ws=odd), dict(ws_bytes=784 + 767),
+                dict(dout=None), dict(dout=odd), dict(w=None), dict(dw=None), dict(dcur=odd), dict(dt=N.F32), dict(E=0)]:
+        assert bwd(*{**good, **bad}.values()) == inval, bad
     linear = lib.usaf_hip_fp8_linear
     assert [lib.usaf_hip_fp8_linear_ws_bytes(m, k) for m, k in ((40, 130), (3, 130), (0, 5), (-1, 5))] == [40 * (256 + 4), 0, 0, -1]
     assert linear(None, N.BF16, 0, 8, 8, None, None, 8, None, None, 0, None) == ok

@@ -52,6 +52,10 @@ _SIGNATURES: dict[str, list] = {
                           _c_p, _c_p],
     "usaf_hip_fp8_gate_up": [_c_p, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_p, _c_p,
                              _c_p],
+    "usaf_hip_fp8_experts_fwd": [_c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_p,
+                                 _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p],
+    "usaf_hip_fp8_experts_bwd": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_p, _c_p,
+                                 _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p],
     "usaf_hip_fp8_linear": [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p],
     "usaf_hip_fp8_swiglu": [_c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_p],
     "usaf_hip_fp8_combine_bwd": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_p, _c_p,
@@ -119,6 +123,8 @@ _VALUE_FUNCS: dict[str, tuple] = {
     "usaf_hip_topk_abs_ws_ints": (_c_i64, [_c_i64]),
     "usaf_hip_moe_few_ws_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
     "usaf_hip_fp8_gate_up_ok": (_c_i32, [_c_i64, _c_i64, _c_i64, _c_i64]),
+    "usaf_hip_fp8_experts_fwd_ws_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "usaf_hip_fp8_experts_bwd_ws_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64]),
     "usaf_hip_fp8_linear_ws_bytes": (_c_i64, [_c_i64, _c_i64]),
     "usaf_hip_fp8_scale_stride": (_c_i64, [_c_i64]),
     "usaf_hip_frag_slot_elems": (_c_i64, [_c_i64, _c_i64, _c_i64]),

@@ -753,3 +753,69 @@ extern "C" int usaf_hip_fp8_linear(const void* x, int32_t dtype, int64_t M, int6
   if (int rc = usaf_hip_fp8_quantize_rows(x, dtype, M, K, ld, nullptr, q, s, stream)) return rc;
   return usaf_hip_fp8_gemm(q, s, M, nullptr, M, w, w_scale, nullptr, 1, N, K, dtype, 0, out, stream);
 }
+
+// ---- an 8-bit expert layer between the bucketing and the weighted sums, in one call each way --------
+
+extern "C" int64_t usaf_hip_fp8_experts_fwd_ws_bytes(int64_t S, int64_t I) {
+  if (S < 0 || I < 0 || S > 0x7FFFFFFF || I > 1 << 23) return -1;
+  return S * (I + usaf_hip_fp8_scale_stride(I));
+}
+
+extern "C" int usaf_hip_fp8_experts_fwd(const uint8_t* x, const uint8_t* x_scale, int64_t T, const int32_t* token_idx,
+                                        const int32_t* offsets, int64_t S, int64_t E, int64_t H, int64_t I, int32_t dtype,
+                                        const uint8_t* gate_up, const uint8_t* gate_up_scale, const uint8_t* down,
+                                        const uint8_t* down_scale, void* gu, void* act, void* y, void* ws, int64_t ws_bytes,
+                                        void* stream) {
+  const int64_t need = usaf_hip_fp8_experts_fwd_ws_bytes(S, I);
+  if (need < 0 || H < 1 || H % FP8_BLOCK || I < 1 || I % FP8_BLOCK)
+    return set_error(USAF_ERR_INVALID, "fp8_experts_fwd: H and I must be positive multiples of %d", FP8_BLOCK);
+  if (S == 0) return clear_error();
+  if (!token_idx || !offsets || !y) return set_error(USAF_ERR_INVALID, "fp8_experts_fwd: null pointer");
+  if (!ws || (uintptr_t)ws % 16 || ws_bytes < need)
+    return set_error(USAF_ERR_INVALID, "fp8_experts_fwd: a workspace of %lld bytes, 16-byte aligned", (long long)need);
+  uint8_t *const q = reinterpret_cast<uint8_t*>(ws), *const s = q + S * I;
+  if (!gu && !act) {
+    if (int rc = usaf_hip_fp8_gate_up(x, x_scale, T, token_idx, S, gate_up, gate_up_scale, offsets, E, I, H, dtype, q, s, stream))
+      return rc;
+  } else {
+    if (int rc = usaf_hip_fp8_gemm(x, x_scale, T, token_idx, S, gate_up, gate_up_scale, offsets, E, 2 * I, H, dtype, 1, gu,
+                                   stream))
+      return rc;
+    if (int rc = usaf_hip_fp8_swiglu(gu, S, I, dtype, offsets + E, act, q, s, stream)) return rc;
+  }
+  return usaf_hip_fp8_gemm(q, s, S, nullptr, S, down, down_scale, offsets, E, H, I, dtype, 0, y, stream);
+}
+
+// The quantized gradients of y and of gu, one behind the other in the same place, then d(act).
+static int64_t bwd_rows_bytes(int64_t S, int64_t H, int64_t I) {
+  const int64_t a = S * (H + usaf_hip_fp8_scale_stride(H)), b = S * (2 * I + usaf_hip_fp8_scale_stride(2 * I));
+  return ((a > b ? a : b) + 15) / 16 * 16;
+}
+
+extern "C" int64_t usaf_hip_fp8_experts_bwd_ws_bytes(int64_t S, int64_t H, int64_t I) {
+  if (S < 0 || H < 0 || I < 0 || S > 0x7FFFFFFF || H > 1 << 24 || I > 1 << 23) return -1;
+  return bwd_rows_bytes(S, H, I) + 2 * S * I;
+}
+
+extern "C" int usaf_hip_fp8_experts_bwd(const void* dout, const void* y, const void* gu, const int32_t* token_idx,
+                                        const float* slot_w, const int32_t* offsets, int64_t S, int64_t E, int64_t H, int64_t I,
+                                        int32_t dtype, const uint8_t* down_t, const uint8_t* down_t_scale,
+                                        const uint8_t* gate_up_t, const uint8_t* gate_up_t_scale, void* dcur, void* dgu,
+                                        void* dx_slots, void* dweights, void* ws, int64_t ws_bytes, void* stream) {
+  const int64_t need = usaf_hip_fp8_experts_bwd_ws_bytes(S, H, I);
+  if (need < 0 || H < 1 || H % FP8_BLOCK || I < 1 || I % FP8_BLOCK)
+    return set_error(USAF_ERR_INVALID, "fp8_experts_bwd: H and I must be positive multiples of %d", FP8_BLOCK);
+  if (S == 0) return clear_error();
+  if (!gu || !dx_slots) return set_error(USAF_ERR_INVALID, "fp8_experts_bwd: null pointer");
+  if (!ws || (uintptr_t)ws % 16 || ws_bytes < need)
+    return set_error(USAF_ERR_INVALID, "fp8_experts_bwd: a workspace of %lld bytes, 16-byte aligned", (long long)need);
+  uint8_t* const q = reinterpret_cast<uint8_t*>(ws);
+  void* const dact = q + bwd_rows_bytes(S, H, I);
+  if (int rc = usaf_hip_fp8_combine_bwd(dout, y, token_idx, slot_w, offsets, S, E, H, dtype, dcur, q, q + S * H, dweights, stream))
+    return rc;
+  if (int rc = usaf_hip_fp8_gemm(q, q + S * H, S, nullptr, S, down_t, down_t_scale, offsets, E, I, H, dtype, 1, dact, stream))
+    return rc;
+  if (int rc = usaf_hip_fp8_swiglu_bwd(gu, dact, S, I, dtype, offsets + E, dgu, q, q + 2 * S * I, stream)) return rc;
+  return usaf_hip_fp8_gemm(q, q + 2 * S * I, S, nullptr, S, gate_up_t, gate_up_t_scale, offsets, E, H, 2 * I, dtype, 0, dx_slots,
+                           stream);
+}

@@ -147,20 +147,6 @@ def quantize_rows(x: torch.Tensor, n_rows: Optional[torch.Tensor] = None) -> Row
     return rows
 
 
-def product(x: Rows, w: Fp8Tensor, out: torch.Tensor, offsets: Optional[torch.Tensor] = None,
-            row_of: Optional[torch.Tensor] = None, wide: bool = False) -> torch.Tensor:
-    """out[m] = x[row_of[m] or m] @ w_e^T for the slots m of expert e (offsets; one expert without).
-    wide: sums to fp32's own precision, by the 16-bit matrix instruction (usaf_hip_fp8_gemm)."""
-    E, n, k = w._erc()
-    if x.cols != k or out.shape[1] != n:
-        raise ValueError(f"fp8 product: rows of {x.cols} and output {tuple(out.shape)} do not fit the weight {tuple(w.shape)}")
-    with on(out.device):
-        N.call("usaf_hip_fp8_gemm", x.q.data_ptr(), x.s.data_ptr(), x.q.shape[0], N.ptr(row_of), out.shape[0],
-               w.q.data_ptr(), w.s.data_ptr(), N.ptr(offsets), E, n, k, N.dtype_code(out.dtype), 1 if wide else 0,
-               out.data_ptr(), N.stream_ptr(out.device))
-    return out
-
-
 class Fp8LinearFn(torch.autograd.Function):
     """y = Q(x) W^T; dx = Q(dy) W."""
 
@@ -229,40 +215,31 @@ def experts_forward(x: Rows, ew, b, gu: Optional[torch.Tensor], act: Optional[to
     """y of the slots of bucketing b from the quantized hidden states, for 8-bit experts ew, with the steps before it in
     gu and act (None: not kept). Each step's output is rounded to dtype, the activations', as on the
     layer's other kernels."""
-    S, E, H, I, dev = b.n_slots, ew.E, ew.H, ew.I, x.q.device
+    S, E, H, I, dev, lib = b.n_slots, ew.E, ew.H, ew.I, x.q.device, N.load()
+    if gu is None and (act is not None or not lib.usaf_hip_fp8_gate_up_ok(S, E, I, H)):
+        gu = torch.empty(S, 2 * I, dtype=dtype, device=dev)
+    y = torch.empty(S, H, dtype=dtype, device=dev)
+    ws = torch.empty(lib.usaf_hip_fp8_experts_fwd_ws_bytes(S, I), dtype=torch.uint8, device=dev)
     with on(dev):
-        if gu is None and act is None and N.load().usaf_hip_fp8_gate_up_ok(S, E, I, H):
-            rows, w = empty_rows(S, I, dev), ew.gate_up
-            N.call("usaf_hip_fp8_gate_up", x.q.data_ptr(), x.s.data_ptr(), x.q.shape[0], b.token_idx.data_ptr(), S,
-                   w.q.data_ptr(), w.s.data_ptr(), b.offsets.data_ptr(), E, I, H, N.dtype_code(dtype), rows.q.data_ptr(),
-                   rows.s.data_ptr(), N.stream_ptr(dev))
-        else:
-            gu = torch.empty(S, 2 * I, dtype=dtype, device=dev) if gu is None else gu
-            product(x, ew.gate_up, gu, b.offsets, b.token_idx, wide=True)
-            rows = empty_rows(S, I, dev)
-            N.call("usaf_hip_fp8_swiglu", gu.data_ptr(), S, I, N.dtype_code(dtype), b.offsets[-1:].data_ptr(), N.ptr(act),
-                   rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(dev))
-    return product(rows, ew.down, torch.empty(S, H, dtype=dtype, device=dev), b.offsets)
+        N.call("usaf_hip_fp8_experts_fwd", x.q.data_ptr(), x.s.data_ptr(), x.q.shape[0], b.token_idx.data_ptr(),
+               b.offsets.data_ptr(), S, E, H, I, N.dtype_code(dtype), ew.gate_up.q.data_ptr(), ew.gate_up.s.data_ptr(),
+               ew.down.q.data_ptr(), ew.down.s.data_ptr(), N.ptr(gu), N.ptr(act), y.data_ptr(), ws.data_ptr(), ws.numel(),
+               N.stream_ptr(dev))
+    return y
 
 
-def experts_combine_bwd(dout: torch.Tensor, y: torch.Tensor, b, dcur: Optional[torch.Tensor],
-                        dweights: torch.Tensor) -> Rows:
-    """The gradient of the down projection's outputs, quantized (and in dcur where given), and of the routing weights."""
+def experts_bwd(dout: torch.Tensor, y: torch.Tensor, gu: torch.Tensor, ew, b, dcur: Optional[torch.Tensor],
+                dgu: Optional[torch.Tensor], dweights: torch.Tensor) -> torch.Tensor:
+    """The slots' gradient of the hidden states; that of the routing weights goes to dweights (zeros before), those of
+    the experts' outputs and of gu to dcur and dgu (None: not kept)."""
     S, H = y.shape
-    rows = empty_rows(S, H, y.device)
-    with on(y.device):
-        N.call("usaf_hip_fp8_combine_bwd", dout.data_ptr(), y.data_ptr(), b.token_idx.data_ptr(), b.slot_w.data_ptr(),
-               b.offsets.data_ptr(), S, b.offsets.numel() - 1, H, N.dtype_code(y.dtype), N.ptr(dcur), rows.q.data_ptr(),
-               rows.s.data_ptr(), dweights.data_ptr(), N.stream_ptr(y.device))
-    return rows
-
-
-def experts_bwd(dcur: Rows, gu: torch.Tensor, ew, b, dgu: Optional[torch.Tensor], dx_slots: torch.Tensor) -> None:
-    """dgu (None: not stored) and the slots' gradient of the hidden states."""
-    S, I = gu.shape[0], gu.shape[1] // 2
-    dact = product(dcur, ew.down.transposed(), torch.empty(S, I, dtype=gu.dtype, device=gu.device), b.offsets, wide=True)
-    rows = empty_rows(S, 2 * I, gu.device)
-    with on(gu.device):
-        N.call("usaf_hip_fp8_swiglu_bwd", gu.data_ptr(), dact.data_ptr(), S, I, N.dtype_code(gu.dtype),
-               b.offsets[-1:].data_ptr(), N.ptr(dgu), rows.q.data_ptr(), rows.s.data_ptr(), N.stream_ptr(gu.device))
-    product(rows, ew.gate_up.transposed(), dx_slots, b.offsets)
+    E, I, dev = ew.E, ew.I, y.device
+    down, gate_up = ew.down.transposed(), ew.gate_up.transposed()
+    dx_slots = torch.empty(S, H, dtype=y.dtype, device=dev)
+    ws = torch.empty(N.load().usaf_hip_fp8_experts_bwd_ws_bytes(S, H, I), dtype=torch.uint8, device=dev)
+    with on(dev):
+        N.call("usaf_hip_fp8_experts_bwd", dout.data_ptr(), y.data_ptr(), gu.data_ptr(), b.token_idx.data_ptr(),
+               b.slot_w.data_ptr(), b.offsets.data_ptr(), S, E, H, I, N.dtype_code(y.dtype), down.q.data_ptr(),
+               down.s.data_ptr(), gate_up.q.data_ptr(), gate_up.s.data_ptr(), N.ptr(dcur), N.ptr(dgu), dx_slots.data_ptr(),
+               dweights.data_ptr(), ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
+    return dx_slots

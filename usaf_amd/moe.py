@@ -658,9 +658,7 @@ def _fp8_experts_backward(ctx, dout: torch.Tensor, dweights: torch.Tensor):
     dcur = torch.empty(S, H, dtype=dt, device=dev) if capture is not None or want_dn else None
     dgu = torch.empty(S, 2 * I, dtype=dt, device=dev) if capture is not None or want_gu else None
     dout = dout if dout.data_ptr() % 16 == 0 else dout.clone()
-    dx_slots = torch.empty(S, H, dtype=dt, device=dev)
-    fp8.experts_bwd(fp8.experts_combine_bwd(dout, y, b, dcur, dweights), gu, ctx.ew, b, dgu, dx_slots)
-    dhs = combine(dx_slots, None, b.pair_slot, dt)
+    dhs = combine(fp8.experts_bwd(dout, y, gu, ctx.ew, b, dcur, dgu, dweights), None, b.pair_slot, dt)
     if capture is not None:
         _capture(capture, "down_proj", dcur, act, None, b, (E, H, I), dt)
         _capture(capture, "gate_up_proj", dgu, hs, b.token_idx, b, (E, 2 * I, H), dt)
