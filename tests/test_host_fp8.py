@@ -94,7 +94,7 @@ def test_entry_points_check_their_arguments():
     assert up(p, p, 4, None, 4, p, p, p, 4, 128, 256, N.BF16, p, p, None) == N.USAF_ERR_UNSUPPORTED
     fwd, bwd = lib.usaf_hip_fp8_experts_fwd, lib.usaf_hip_fp8_experts_bwd
     fw, bw = lib.usaf_hip_fp8_experts_fwd_ws_bytes, lib.usaf_hip_fp8_experts_bwd_ws_bytes
-    assert [fw(3, 128), fw(0, 128), fw(-1, 128), bw(3, 256, 128), bw(-1, 8, 8)] == [3 * 132, 0, -1, 784 + 3 * 256, -1]
+    assert [fw(3, 128), fw(0, 128), fw(-1, 128), bw(3, 256, 128), bw(-1, 8, 8)] == [3 * 132, 0, -1, 1024 + 3 * 256, -1]
     good = dict(x=p, xs=p, T=3, tok=p, offs=p, S=3, E=2, H=256, I=128, dt=N.BF16, gu=p, gus=p, dn=p, dns=p, keep=p, act=p, y=p,
                 ws=p, ws_bytes=3 * 132, stream=None)
     assert fwd(*{**good, "S": 0, "ws": None, "ws_bytes": 0}.values()) == ok
@@ -103,9 +103,9 @@ def test_entry_points_check_their_arguments():
         assert fwd(*{**good, **bad}.values()) == inval, bad
     assert fwd(*{**good, "keep": None, "act": None}.values()) == N.USAF_ERR_UNSUPPORTED  # few slots keep gu
     good = dict(dout=p, y=p, gu=p, tok=p, w=p, offs=p, S=3, E=2, H=256, I=128, dt=N.BF16, dn=p, dns=p, gut=p, guts=p, dcur=None,
-                dgu=None, dx=p, dw=p, ws=p, ws_bytes=784 + 768, stream=None)
+                dgu=None, dx=p, dw=p, ws=p, ws_bytes=1024 + 768, stream=None)
     assert bwd(*{**good, "S": 0, "ws": None, "ws_bytes": 0}.values()) == ok
-    for bad in [dict(H=100), dict(I=100), dict(gu=None), dict(dx=None), dict(ws=None), dict(ws=odd), dict(ws_bytes=784 + 767),
+    for bad in [dict(H=100), dict(I=100), dict(gu=None), dict(dx=None), dict(ws=None), dict(ws=odd), dict(ws_bytes=1024 + 767),
                 dict(dout=None), dict(dout=odd), dict(w=None), dict(dw=None), dict(dcur=odd), dict(dt=N.F32), dict(E=0)]:
         assert bwd(*{**good, **bad}.values()) == inval, bad
     linear = lib.usaf_hip_fp8_linear

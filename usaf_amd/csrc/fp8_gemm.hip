@@ -789,7 +789,7 @@ extern "C" int usaf_hip_fp8_experts_fwd(const uint8_t* x, const uint8_t* x_scale
 // The quantized gradients of y and of gu, one behind the other in the same place, then d(act).
 static int64_t bwd_rows_bytes(int64_t S, int64_t H, int64_t I) {
   const int64_t a = S * (H + usaf_hip_fp8_scale_stride(H)), b = S * (2 * I + usaf_hip_fp8_scale_stride(2 * I));
-  return ((a > b ? a : b) + 15) / 16 * 16;
+  return ((a > b ? a : b) + 255) / 256 * 256;  // d(act) starts a cache line
 }
 
 extern "C" int64_t usaf_hip_fp8_experts_bwd_ws_bytes(int64_t S, int64_t H, int64_t I) {
