@@ -3,10 +3,11 @@
 //   l = x Wr^T, the k largest l (ties: the lowest expert), w = softmax(l) there (renormalised or not)
 //   a_e = dt(silu(g) u),  (g, u) = Wgu_e x;   out = dt(sum_e w_e Wd_e a_e)
 //
-// Four launches, nothing read back to the host, no slot lists:
+// Four launches (three for one token), nothing read back to the host, no slot lists:
 //
 //   few_logits   a block an expert of the router and up to four tokens
-//   few_route    a block a token: selection by rank, weights, a bit of the token in its experts' masks
+//   few_route    a block a token: selection by rank, weights, a bit of the token in its experts' masks (one
+//                token: in few_gate_up)
 //   few_gate_up  a block takes (expert in use, 32 columns of a) tiles; its waves split the contraction
 //   few_down     a block has 64 columns of out; the waves of a column tile share its (expert,
 //                group of 128) pairs evenly and add them up by token; the tile's last block adds the parts in order
@@ -152,57 +153,70 @@ __device__ __forceinline__ float wave_add(float v) {  // the same bits in every 
   return (__shfl(v, 0, 64) + __shfl(v, 16, 64)) + (__shfl(v, 32, 64) + __shfl(v, 48, 64));
 }
 
-// Block: one token.  Every wave has the token's whole row, up to four experts a lane, and
-// ranks a sixteenth of the experts: how many come before one is a count of lanes.  3.8 us for one token
-// and 128 experts (each expert's threads counting through LDS: 4.7).
-__global__ __launch_bounds__(1024) void few_route_kernel(const FewArgs g) {
-  __shared__ float s_p[F_MAX_K];
-  constexpr int N = F_MAX_E / 64, WAVES = 16;
-  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const double* const row = g.logits + (int64_t)t * g.E;
-  const int per = (g.E + WAVES - 1) / WAVES, e = wave * per + lane;  // the lane's own expert: lanes below `per`
-  const bool own = lane < per && e < g.E;
-  const double mine = own ? row[e] : 0;
-  double l[N];
-  int64_t key[N];
-  float m = -INFINITY;
+// A token's row of logits, as every wave of a block has it, and the rank of the lane's own expert, one of
+// the wave's share: how many come before it is a count of lanes.
+template <int WAVES>
+struct Ranking {
+  static constexpr int N = F_MAX_E / 64;
+  double l[N], mine;  // the row, up to four experts a lane; the own expert's
+  int per, e, rank;   // experts of a wave; the own one
+  bool own;           // there is one
+  __device__ __forceinline__ Ranking(const double* row, int E, int lane, int wave) {
+    per = (E + WAVES - 1) / WAVES;
+    e = wave * per + lane;
+    own = lane < per && e < E;
+    mine = own ? row[e] : 0;
+    int64_t key[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int o = 64 * i + lane;
-    l[i] = o < g.E ? row[o] : -INFINITY;
-    m = fmaxf(m, (float)l[i]);
+    for (int i = 0; i < N; ++i) l[i] = 64 * i + lane < E ? row[64 * i + lane] : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) key[i] = 64 * i + lane < E ? expert_key(l[i], 64 * i + lane) : INT64_MIN;
+    const int64_t my_key = own ? expert_key(mine, e) : 0;
+    rank = 0;
+    for (int j = 0; j < per; ++j) {  // (past the last expert: a rank that nothing uses)
+      const int64_t k = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(my_key >> 32), j) << 32) |
+                                  (uint32_t)__builtin_amdgcn_readlane((int)my_key, j));
+      int before = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (64 * i < E) before += __popcll(__ballot(key[i] > k));
+      rank = lane == j ? before : rank;
+    }
   }
+  // The own expert's weight if it is one of the first k; s_p: room for k, read after a barrier of the block.
+  __device__ __forceinline__ float weight(int E, int k, bool norm, int lane, float* s_p) const {
+    float m = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) key[i] = 64 * i + lane < g.E ? expert_key(l[i], 64 * i + lane) : INT64_MIN;
-  m = rows16_max(max16(m));
-  float sum = 0.f;
+    for (int i = 0; i < N; ++i) m = fmaxf(m, (float)l[i]);
+    m = rows16_max(max16(m));
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (64 * i + lane < g.E) sum += expf((float)(l[i] - (double)m));
-  sum = wave_add(sum);
-  int rank = 0;
-  const int64_t my_key = own ? expert_key(mine, e) : 0;
-  for (int j = 0; j < per; ++j) {  // (past the last expert: a rank that nothing uses)
-    const int64_t k = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(my_key >> 32), j) << 32) |
-                                (uint32_t)__builtin_amdgcn_readlane((int)my_key, j));
-    int before = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) before += __popcll(__ballot(key[i] > k));
-    rank = lane == j ? before : rank;
-  }
-  const bool chosen = own && rank < g.k;
-  const float p = chosen ? expf((float)(mine - (double)m)) : 0.f;
-  if (chosen) s_p[rank] = p;
-  __syncthreads();
-  if (chosen) {
+    for (int i = 0; i < N; ++i)
+      if (64 * i + lane < E) sum += expf((float)(l[i] - (double)m));
+    sum = wave_add(sum);
+    const bool chosen = own && rank < k;
+    const float p = chosen ? expf((float)(mine - (double)m)) : 0.f;
+    if (chosen) s_p[rank] = p;
+    __syncthreads();
     float total = sum;
-    if (g.norm) {
+    if (norm) {
       total = 0.f;
-      for (int i = 0; i < g.k; ++i) total += s_p[i];
+      for (int i = 0; i < k; ++i) total += s_p[i];
       if (sum != sum) total = sum;  // a NaN anywhere in the row
     }
-    g.wt[e * FT + t] = p / total;
-    atomicOr(&g.mask[e], 1u << t);  // bits of different blocks: any order gives the same mask
+    __syncthreads();
+    return p / total;
+  }
+};
+
+// Block: one token.  3.8 us for one token and 128 experts (each expert's threads counting through LDS: 4.7).
+__global__ __launch_bounds__(1024) void few_route_kernel(const FewArgs g) {
+  __shared__ float s_p[F_MAX_K];
+  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Ranking<16> r(g.logits + (int64_t)t * g.E, g.E, lane, wave);
+  const float w = r.weight(g.E, g.k, g.norm, lane, s_p);
+  if (r.own && r.rank < g.k) {
+    g.wt[r.e * FT + t] = w;
+    atomicOr(&g.mask[r.e], 1u << t);  // bits of different blocks: any order gives the same mask
   }
 }
 
@@ -242,6 +256,9 @@ struct InUse {
   __device__ __forceinline__ void load(const uint32_t* m, int lane) {
 #pragma unroll
     for (int i = 0; i < N; ++i) mask[i] = m[64 * i + lane];
+    find();
+  }
+  __device__ __forceinline__ void find() {
     count = items = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -515,7 +532,7 @@ struct Tokens {
 // 265 MB: 51 us, 5.2 TB/s; one token, 13 MB: 8.5 us.
 constexpr int GU_NU = 4, GU_WAVES = 4, GU_THREADS = 64 * GU_WAVES;  // 32 gate rows and their 32 up rows
 
-template <int DT, int FMT>
+template <int DT, int FMT, bool ROUTES>
 __global__ __launch_bounds__(GU_THREADS, 3) void few_gate_up_kernel(const FewArgs g) {
   __shared__ f32x4 red[GU_WAVES][GU_NU][64];
   __shared__ __attribute__((aligned(16))) uint8_t s_codes[GU_WAVES][GU_NU * UNIT_LDS];
@@ -526,7 +543,31 @@ __global__ __launch_bounds__(GU_THREADS, 3) void few_gate_up_kernel(const FewArg
   const int n = some > 0 ? some : 1;  // a wave without a step of its own multiplies one and adds nothing
   const int first = STEP<FMT> * (s0 < ns ? s0 : ns - 1);
   InUse in;
-  in.load(g.mask, lane);
+  if constexpr (ROUTES) {
+    // every block ranks one token's experts for itself; the first keeps weights and masks for few_down
+    uint64_t* const s_chosen = reinterpret_cast<uint64_t*>(&red[0][0][0]);  // [waves]
+    float* const s_p = reinterpret_cast<float*>(s_chosen + GU_WAVES);
+    const Ranking<GU_WAVES> rk(g.logits, g.E, lane, wave);
+    const uint64_t chosen = __ballot(rk.own && rk.rank < g.k);
+    if (lane == 0) s_chosen[wave] = chosen;
+    if (blockIdx.x == 0) {
+      const float w = rk.weight(g.E, g.k, g.norm, lane, s_p);
+      if (rk.own && rk.rank < g.k) g.wt[rk.e * FT] = w;
+    }
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < InUse::N; ++i) {
+      const int e = 64 * i + lane, of = e / rk.per;
+      in.mask[i] = e < g.E ? (uint32_t)(s_chosen[of] >> (e - of * rk.per)) & 1 : 0;
+    }
+    lds_barrier();
+    if (blockIdx.x == 0 && wave == 0)
+#pragma unroll
+      for (int i = 0; i < InUse::N; ++i) g.mask[64 * i + lane] = in.mask[i];
+    in.find();
+  } else {
+    in.load(g.mask, lane);
+  }
   const int work = in.items * n_nt;
   int at = blockIdx.x, st = 0;  // the pair being loaded
   if (at >= work) return;       // block-uniform
@@ -782,10 +823,19 @@ int launch_few_layer(const FewArgs& g, int64_t in_use, hipStream_t st) {
   if (g.T == 1) few_logits_kernel<DT, FMT, 1><<<(unsigned)g.E, 256, 0, st>>>(g);
   else few_logits_kernel<DT, FMT, 4><<<(unsigned)(g.E * ((g.T + 3) / 4)), 256, 0, st>>>(g);
   if (int rc = check_launch("moe_few/logits")) return rc;
-  few_route_kernel<<<(unsigned)g.T, 1024, 0, st>>>(g);
-  if (int rc = check_launch("moe_few/route")) return rc;
+  // One token's experts are ranked by every block of few_gate_up, which saves a launch; more
+  // tokens' ranks, one behind the other there, take longer than few_route's blocks.  Measured (us, the whole
+  // layer, ranked there / by few_route): one token 23.0 / 23.5 (128 experts of 768, 4-bit), 21.2 / 22.5
+  // (64 of 1,024), 50.6 / 53.0 (8 of 14,336); two 31.7 / 29.0, 28.4 / 28.8, 77 / 79; four 45.2 / 35.8.
+  const bool routes = g.T == 1;
+  if (!routes) {
+    few_route_kernel<<<(unsigned)g.T, 1024, 0, st>>>(g);
+    if (int rc = check_launch("moe_few/route")) return rc;
+  }
   const int64_t most = 3 * (int64_t)device_cu_count(), work = (in_use + g.T * g.k / (FR + 1)) * (g.I / 32);
-  few_gate_up_kernel<DT, FMT><<<(unsigned)(work < most ? work : most), GU_THREADS, 0, st>>>(g);
+  const unsigned blocks = (unsigned)(work < most ? work : most);
+  if (routes) few_gate_up_kernel<DT, FMT, true><<<blocks, GU_THREADS, 0, st>>>(g);
+  else few_gate_up_kernel<DT, FMT, false><<<blocks, GU_THREADS, 0, st>>>(g);
   if (int rc = check_launch("moe_few/gate_up")) return rc;
   few_down_kernel<DT, FMT>
       <<<(unsigned)(g.H / DN_COLS * g.P), DN_THREADS,

@@ -2,7 +2,7 @@
 
 ``few_token_block`` is ``moe.moe_block`` for 1 to 32 tokens without gradients, on
 4-bit (``Q4Tensor``) or 8-bit (``Fp8Tensor``) experts: router, top-k, the experts in
-use and their weighted sum in four launches, with no host read and no state
+use and their weighted sum in three or four launches, with no host read and no state
 between calls.  It keeps more digits than the routed path between its steps
 (usaf/qwen3moe_dml.py:24-86 rounds each op's output to the activations' dtype):
 

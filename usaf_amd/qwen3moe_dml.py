@@ -22,7 +22,7 @@ reference (it detaches every per-expert slice).
 
 Decoding: with ``block._usaf_few_tokens = n`` (up to 32) a block's passes of at most
 n tokens that want no gradient run as ``few.few_token_block``, router and experts in
-four launches, where the experts are 4-bit or 8-bit and carry no trained values.
+three or four launches, where the experts are 4-bit or 8-bit and carry no trained values.
 Its numerics (``few.py``) differ from this path's in what is rounded to 16 bits, so it is off by default.
 """
 from __future__ import annotations
