@@ -659,7 +659,7 @@ int usaf_hip_fp8_experts_bwd(const void* dout, const void* y, const void* gu, co
  * and scale bytes as usaf_hip_fp8_quantize_weight writes them.
  * ws: usaf_hip_moe_few_ws_bytes bytes, 16-byte aligned, nothing in them matters before the
  * call; calls that may overlap need workspaces of their own.  E <= 256, top_k <= 16, H
- * and I multiples of 128, H <= 16384, I <= 65536.  Four launches, three for one token; no host read.
+ * and I multiples of 128, H <= 16384, I <= 65536.  Four launches, three for one or two tokens; no host read.
  */
 int64_t usaf_hip_moe_few_ws_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I);
 int usaf_hip_moe_few(const void* x, int64_t T, int64_t H, const void* router, int64_t E, int64_t top_k,

@@ -3,11 +3,11 @@
 //   l = x Wr^T, the k largest l (ties: the lowest expert), w = softmax(l) there (renormalised or not)
 //   a_e = dt(silu(g) u),  (g, u) = Wgu_e x;   out = dt(sum_e w_e Wd_e a_e)
 //
-// Four launches (three for one token), nothing read back to the host, no slot lists:
+// Four launches (three for one or two tokens), nothing read back to the host, no slot lists:
 //
 //   few_logits   a block an expert of the router and up to four tokens
-//   few_route    a block a token: selection by rank, weights, a bit of the token in its experts' masks (one
-//                token: in few_gate_up)
+//   few_route    a wave a token: the k largest, their weights, a bit of the token in their masks (one or two tokens: in
+//                few_gate_up)
 //   few_gate_up  a block takes (expert in use, 32 columns of a) tiles; its waves split the contraction
 //   few_down     a block has 64 columns of out; the waves of a column tile share its (expert,
 //                group of 128) pairs evenly and add them up by token; the tile's last block adds the parts in order
@@ -153,71 +153,98 @@ __device__ __forceinline__ float wave_add(float v) {  // the same bits in every 
   return (__shfl(v, 0, 64) + __shfl(v, 16, 64)) + (__shfl(v, 32, 64) + __shfl(v, 48, 64));
 }
 
-// A token's row of logits, as every wave of a block has it, and the rank of the lane's own expert, one of
-// the wave's share: how many come before it is a count of lanes.
-template <int WAVES>
-struct Ranking {
+template <int N>
+__device__ __forceinline__ int max_rot_i(int v) {
+  const int o = __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 0xf, 0xf, false);
+  return o > v ? o : v;
+}
+__device__ __forceinline__ int wave_max_i(int v) {  // uniform
+  v = max_rot_i<1>(max_rot_i<2>(max_rot_i<4>(max_rot_i<8>(v))));
+  const int a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16);
+  const int c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+  const int x = a > b ? a : b, y = c > d ? c : d;
+  return x > y ? x : y;
+}
+
+// The first k experts of a token, by one wave: up to four experts a lane, the largest key taken k
+// times, by its upper half first: 2 us for 8 of 128 (counting how many come before each expert: 3.7).
+struct Chosen {
   static constexpr int N = F_MAX_E / 64;
-  double l[N], mine;  // the row, up to four experts a lane; the own expert's
-  int per, e, rank;   // experts of a wave; the own one
-  bool own;           // there is one
-  __device__ __forceinline__ Ranking(const double* row, int E, int lane, int wave) {
-    per = (E + WAVES - 1) / WAVES;
-    e = wave * per + lane;
-    own = lane < per && e < E;
-    mine = own ? row[e] : 0;
-    int64_t key[N];
+  double l[N];
+  int rank[N];  // -1: not chosen
+  __device__ __forceinline__ Chosen(const double* row, int E, int k, int lane) {
+    int high[N], low[N];  // low: the unsigned order as a signed one
 #pragma unroll
     for (int i = 0; i < N; ++i) l[i] = 64 * i + lane < E ? row[64 * i + lane] : -INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; ++i) key[i] = 64 * i + lane < E ? expert_key(l[i], 64 * i + lane) : INT64_MIN;
-    const int64_t my_key = own ? expert_key(mine, e) : 0;
-    rank = 0;
-    for (int j = 0; j < per; ++j) {  // (past the last expert: a rank that nothing uses)
-      const int64_t k = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(my_key >> 32), j) << 32) |
-                                  (uint32_t)__builtin_amdgcn_readlane((int)my_key, j));
-      int before = 0;
+    for (int i = 0; i < N; ++i) {
+      const int64_t key = 64 * i + lane < E ? expert_key(l[i], 64 * i + lane) : INT64_MIN;
+      high[i] = (int)(key >> 32);
+      low[i] = (int)((uint32_t)key ^ 0x80000000u);
+      rank[i] = -1;
+    }
+    for (int n = 0; n < k; ++n) {
+      int m = high[0], at = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (64 * i < E) before += __popcll(__ballot(key[i] > k));
-      rank = lane == j ? before : rank;
+      for (int i = 1; i < N; ++i) m = high[i] > m ? high[i] : m;
+      m = wave_max_i(m);
+      bool first[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        first[i] = high[i] == m;
+        at += __popcll(__ballot(first[i]));
+      }
+      if (at > 1) {  // uniform
+        int q = INT32_MIN;
+#pragma unroll
+        for (int i = 0; i < N; ++i) q = first[i] && low[i] > q ? low[i] : q;
+        q = wave_max_i(q);
+#pragma unroll
+        for (int i = 0; i < N; ++i) first[i] = first[i] && low[i] == q;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {  // taken: below all others from here on
+        rank[i] = first[i] ? n : rank[i];
+        high[i] = first[i] ? INT32_MIN : high[i];
+        low[i] = first[i] ? INT32_MIN : low[i];
+      }
     }
   }
-  // The own expert's weight if it is one of the first k; s_p: room for k, read after a barrier of the block.
-  __device__ __forceinline__ float weight(int E, int k, bool norm, int lane, float* s_p) const {
-    float m = -INFINITY, sum = 0.f;
+  // Their weights to g.wt; s_p: room for k, the wave's own.
+  __device__ __forceinline__ void weights(const FewArgs& g, int t, int lane, float* s_p) const {
+    float m = -INFINITY, sum = 0.f, p[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) m = fmaxf(m, (float)l[i]);
     m = rows16_max(max16(m));
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (64 * i + lane < E) sum += expf((float)(l[i] - (double)m));
+    for (int i = 0; i < N; ++i) {
+      p[i] = 64 * i + lane < g.E ? expf((float)(l[i] - (double)m)) : 0.f;
+      sum += p[i];
+      if (rank[i] >= 0) s_p[rank[i]] = p[i];
+    }
     sum = wave_add(sum);
-    const bool chosen = own && rank < k;
-    const float p = chosen ? expf((float)(mine - (double)m)) : 0.f;
-    if (chosen) s_p[rank] = p;
-    __syncthreads();
+    __builtin_amdgcn_wave_barrier();  // one wave's LDS operations complete in order
     float total = sum;
-    if (norm) {
+    if (g.norm) {
       total = 0.f;
-      for (int i = 0; i < k; ++i) total += s_p[i];
+      for (int i = 0; i < g.k; ++i) total += s_p[i];
       if (sum != sum) total = sum;  // a NaN anywhere in the row
     }
-    __syncthreads();
-    return p / total;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (rank[i] >= 0) g.wt[(64 * i + lane) * FT + t] = p[i] / total;
   }
 };
 
-// Block: one token.  3.8 us for one token and 128 experts (each expert's threads counting through LDS: 4.7).
-__global__ __launch_bounds__(1024) void few_route_kernel(const FewArgs g) {
+// Block: one token, one wave: 4.8 us for 24 tokens and 128 experts, a launch, one trip to memory and the choice.
+__global__ __launch_bounds__(64) void few_route_kernel(const FewArgs g) {
   __shared__ float s_p[F_MAX_K];
-  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Ranking<16> r(g.logits + (int64_t)t * g.E, g.E, lane, wave);
-  const float w = r.weight(g.E, g.k, g.norm, lane, s_p);
-  if (r.own && r.rank < g.k) {
-    g.wt[r.e * FT + t] = w;
-    atomicOr(&g.mask[r.e], 1u << t);  // bits of different blocks: any order gives the same mask
-  }
+  const int t = blockIdx.x, lane = threadIdx.x;
+  const Chosen c(g.logits + (int64_t)t * g.E, g.E, g.k, lane);
+  c.weights(g, t, lane, s_p);
+#pragma unroll
+  for (int i = 0; i < Chosen::N; ++i)
+    if (c.rank[i] >= 0) atomicOr(&g.mask[64 * i + lane], 1u << t);  // bits of different blocks: any order gives the same mask
 }
 
 // ---- products --------------------------------------------------------------------
@@ -529,7 +556,7 @@ struct Tokens {
 // there.  32 gate and their 32 up rows are one item, so that the activation needs no second pass.  Measured
 // (weights with scales): 24 tokens, about 101 of 128 experts of 768 x 2,048, 4-bit, 169 MB: 38 us, 4.4 TB/s; 7
 // tokens, 8 of 14,336 x 4,096, 4-bit, 433 MB: 85 us, 5.1 TB/s; 32 tokens, 63 of 64 of 1,024 x 2,048, 8-bit,
-// 265 MB: 51 us, 5.2 TB/s; one token, 13 MB: 8.5 us.
+// 265 MB: 51 us, 5.2 TB/s; one token, 13 MB: 10.6 us with the choice of its experts.
 constexpr int GU_NU = 4, GU_WAVES = 4, GU_THREADS = 64 * GU_WAVES;  // 32 gate rows and their 32 up rows
 
 template <int DT, int FMT, bool ROUTES>
@@ -544,23 +571,15 @@ __global__ __launch_bounds__(GU_THREADS, 3) void few_gate_up_kernel(const FewArg
   const int first = STEP<FMT> * (s0 < ns ? s0 : ns - 1);
   InUse in;
   if constexpr (ROUTES) {
-    // every block ranks one token's experts for itself; the first keeps weights and masks for few_down
-    uint64_t* const s_chosen = reinterpret_cast<uint64_t*>(&red[0][0][0]);  // [waves]
-    float* const s_p = reinterpret_cast<float*>(s_chosen + GU_WAVES);
-    const Ranking<GU_WAVES> rk(g.logits, g.E, lane, wave);
-    const uint64_t chosen = __ballot(rk.own && rk.rank < g.k);
-    if (lane == 0) s_chosen[wave] = chosen;
-    if (blockIdx.x == 0) {
-      const float w = rk.weight(g.E, g.k, g.norm, lane, s_p);
-      if (rk.own && rk.rank < g.k) g.wt[rk.e * FT] = w;
-    }
-    lds_barrier();
+    // every wave chooses the experts for itself; the first keeps weights and masks for few_down
 #pragma unroll
-    for (int i = 0; i < InUse::N; ++i) {
-      const int e = 64 * i + lane, of = e / rk.per;
-      in.mask[i] = e < g.E ? (uint32_t)(s_chosen[of] >> (e - of * rk.per)) & 1 : 0;
+    for (int i = 0; i < InUse::N; ++i) in.mask[i] = 0;
+    for (int t = 0; t < g.T; ++t) {
+      const Chosen c(g.logits + (int64_t)t * g.E, g.E, g.k, lane);
+      if (blockIdx.x == 0 && wave == 0) c.weights(g, t, lane, reinterpret_cast<float*>(&red[0][0][0]));
+#pragma unroll
+      for (int i = 0; i < InUse::N; ++i) in.mask[i] |= c.rank[i] >= 0 ? 1u << t : 0u;
     }
-    lds_barrier();
     if (blockIdx.x == 0 && wave == 0)
 #pragma unroll
       for (int i = 0; i < InUse::N; ++i) g.mask[64 * i + lane] = in.mask[i];
@@ -823,13 +842,13 @@ int launch_few_layer(const FewArgs& g, int64_t in_use, hipStream_t st) {
   if (g.T == 1) few_logits_kernel<DT, FMT, 1><<<(unsigned)g.E, 256, 0, st>>>(g);
   else few_logits_kernel<DT, FMT, 4><<<(unsigned)(g.E * ((g.T + 3) / 4)), 256, 0, st>>>(g);
   if (int rc = check_launch("moe_few/logits")) return rc;
-  // One token's experts are ranked by every block of few_gate_up, which saves a launch; more
-  // tokens' ranks, one behind the other there, take longer than few_route's blocks.  Measured (us, the whole
-  // layer, ranked there / by few_route): one token 23.0 / 23.5 (128 experts of 768, 4-bit), 21.2 / 22.5
-  // (64 of 1,024), 50.6 / 53.0 (8 of 14,336); two 31.7 / 29.0, 28.4 / 28.8, 77 / 79; four 45.2 / 35.8.
-  const bool routes = g.T == 1;
+  // Every wave of few_gate_up chooses one or two tokens' experts itself, which saves a launch; more tokens, one
+  // behind the other there, take longer than few_route's blocks.  Measured (us, the whole layer, there / with
+  // few_route): one token 21.5 / 22.9 (128 experts of 768, 4-bit), 22.4 / 24.3 (8-bit), 21.2 / 23.1 (64 of 1,024), 50.9 /
+  // 52.9 (8 of 14,336); two 28.4 / 28.6, 31.9 / 32.0, 28.7 / 29.1; three 35.6 / 34.1, 41.2 / 39.1, 36.1 / 34.6.
+  const bool routes = g.T <= 2;
   if (!routes) {
-    few_route_kernel<<<(unsigned)g.T, 1024, 0, st>>>(g);
+    few_route_kernel<<<(unsigned)g.T, 64, 0, st>>>(g);
     if (int rc = check_launch("moe_few/route")) return rc;
   }
   const int64_t most = 3 * (int64_t)device_cu_count(), work = (in_use + g.T * g.k / (FR + 1)) * (g.I / 32);
