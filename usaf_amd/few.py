@@ -7,8 +7,8 @@ between calls.  It keeps more digits than the routed path between its steps
 (usaf/qwen3moe_dml.py:24-86 rounds each op's output to the activations' dtype):
 
 * the router's logits are not rounded to 16 bits.  Exactly ``top_k`` experts serve
-  each token, the lowest-numbered of equal ones, where the 16-bit rule takes all
-  experts that tie at the threshold;
+  each token, the lowest-numbered of equal ones (to 44 bits), where the 16-bit rule
+  takes all experts that tie at the threshold;
 * gate, up, each expert's output and the routing weights stay in fp32; only the
   gated activation, the operand of the second product, is rounded;
 * a 4-bit weight is code * scale + zero as a real number, without the codec's fp16
