@@ -468,7 +468,7 @@ def test_refusals_on_the_gpu(F):
 TILES = [(None, 1, 33, 128), (None, 70, 33, 640), (None, 1, 2000, 1300), (None, 33, 4100, 640), (None, 4100, 200, 300),
          (None, 1000, 4100, 128), (None, 2000, 4100, 300), (None, 513, 1030, 640), (1, 2000, 130, 640), (3, 33, 4100, 640),
          (8, 200, 4100, 300), (8, 500, 4100, 128), (8, 1500, 4100, 300), (40, 33, 1030, 300), (40, 2000, 2000, 129),
-         (255, 300, 130, 256)]
+         (255, 300, 130, 256), (None, 32, 9001, 1300), (8, 100, 2000, 1024)]
 
 
 @pytest.mark.parametrize("wide", [False, True])

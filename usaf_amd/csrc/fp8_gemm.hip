@@ -587,6 +587,8 @@ struct Shape {
   //   128 experts' 768 x 2,048 gate and up (wide), 256 slots each  273  267* 308  356   420   441   700
   //                                                16 slots each   108  82*  99   83    111   77    111
   //   and their down projections, 256 slots each                   98*  104  153  216   302   252   587
+  //   32 x 64 (between the last two) is taken for up to 32 rows of wide weights: 32 x 14,336 x 4,096 in 19.9, without it
+  //   23.9, 32 x 16,384 x 16,384 in 62.7 and 70.5, quantization included.
   static double cycles(const Fp8Args& g, bool wide) {
     const double steps = (double)ceil_div(g.Kp / 128, T::KW);
     const double mfma = 2.0 * MI * NI * 2 * (wide ? 128 : 64), lines = (double)T::KW * (T::M + T::N) * 128 / 24;
@@ -603,6 +605,7 @@ typedef Shape<2, 4, 2, 1> S128x128;
 typedef Shape<1, 4, 2, 1> S64x128;
 typedef Shape<1, 2, 2, 1> S64x64;
 typedef Shape<1, 4, 1, 1> S32x128;
+typedef Shape<1, 2, 1, 1> S32x64;
 typedef Shape<1, 1, 1, 1> S32x32;
 
 typedef int (*Launch)(Fp8Args, int, bool, hipStream_t);
@@ -620,6 +623,7 @@ Launch best_shape(const Fp8Args& g, bool wide) {
   consider(S64x128::launch, S64x128::cycles(g, wide));
   consider(S64x64::launch, S64x64::cycles(g, wide));
   consider(S32x128::launch, S32x128::cycles(g, wide));
+  consider(S32x64::launch, S32x64::cycles(g, wide));
   consider(S32x32::launch, S32x32::cycles(g, wide));
   return best;
 }
@@ -633,6 +637,7 @@ void prepare_fp8_kernels() {
   S64x128::prepare();
   S64x64::prepare();
   S32x128::prepare();
+  S32x64::prepare();
   S32x32::prepare();
 }
 
