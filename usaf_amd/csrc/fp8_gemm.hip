@@ -602,7 +602,7 @@ struct Shape {
 typedef Shape<2, 4, 4, 2> S256x256;
 typedef Shape<2, 4, 2, 2> S128x256;
 typedef Shape<2, 4, 2, 1> S128x128;
-typedef Shape<1, 4, 2, 1> S64x128;
+typedef Shape<2, 4, 1, 1> S64x128;
 typedef Shape<2, 2, 1, 1> S64x64;
 typedef Shape<1, 4, 1, 1> S32x128;
 typedef Shape<1, 2, 1, 1> S32x64;
