@@ -578,17 +578,15 @@ struct Shape {
   }
   // Cycles of a CU, roughly: a step is bound by its matrix instructions or by its lines (24 bytes a cycle), a
   // tile has its ends, and the last round of tiles counts whole.  The shape of the least is taken.  Measured (us;
-  // 256 x 256, 128 x 256, 128 x 128, 64 x 128, 64 x 64, 32 x 128, 32 x 32; * taken):
-  //   rows x columns x contraction   8,192 x 14,336 x 4,096   438*  525  893 1,039 1,254 1,212 2,435
-  //                                  4,096 x 4,096 x 2,048    35*   42   81   99   120   117   204
-  //                                  1,024 x 4,096 x 2,048    27    20*  21   29   32    31    55
-  //                                  333 x 1,411 x 2,027      35    23   23   14   9.6*  9.8   9.3
-  //                                  33 x 4,096 x 2,048       19    18   18   13   8.7   9.1   6.0*
-  //   128 experts' 768 x 2,048 gate and up (wide), 256 slots each  273  267* 308  356   420   441   700
-  //                                                16 slots each   108  82*  99   83    111   77    111
-  //   and their down projections, 256 slots each                   98*  104  153  216   302   252   587
-  //   32 x 64 (between the last two) is taken for up to 32 rows of wide weights: 32 x 14,336 x 4,096 in 19.9, without it
-  //   23.9, 32 x 16,384 x 16,384 in 62.7 and 70.5, quantization included.
+  // 256 x 256, 128 x 256, 128 x 128, 64 x 128, 64 x 64, 32 x 128, 32 x 64, 32 x 32; * taken):
+  //   rows x columns x contraction   8,192 x 14,336 x 4,096   438*  525  893  888  1,132 1,212 1,506 2,435
+  //                                  4,096 x 4,096 x 2,048    35*   42   81   78   108   117   147   204
+  //                                  1,024 x 4,096 x 2,048    27    20*  21   21   30    31    39    55
+  //                                  333 x 1,411 x 2,027      35    23   23   13   9.7   9.8   7.8*  9.3
+  //                                  33 x 4,096 x 2,048       19    18   18   11   8.7   9.1   7.0   6.0*
+  //   128 experts' 768 x 2,048 gate and up (wide), 256 slots each  273  267* 308  373  444  441  531  700
+  //                                                16 slots each   108  82*  99   81   99   77   93   111
+  //   and their down projections, 256 slots each                   98*  104  153  163  257  252  387  587
   static double cycles(const Fp8Args& g, bool wide) {
     const double steps = (double)ceil_div(g.Kp / 128, T::KW);
     const double mfma = 2.0 * MI * NI * 2 * (wide ? 128 : 64), lines = (double)T::KW * (T::M + T::N) * 128 / 24;
