@@ -216,11 +216,11 @@ def experts_forward(x: Rows, ew, b, gu: Optional[torch.Tensor], act: Optional[to
     gu and act (None: not kept). Each step's output is rounded to dtype, the activations', as on the
     layer's other kernels."""
     S, E, H, I, dev, lib = b.n_slots, ew.E, ew.H, ew.I, x.q.device, N.load()
-    if gu is None and (act is not None or not lib.usaf_hip_fp8_gate_up_ok(S, E, I, H)):
-        gu = torch.empty(S, 2 * I, dtype=dtype, device=dev)
-    y = torch.empty(S, H, dtype=dtype, device=dev)
-    ws = torch.empty(lib.usaf_hip_fp8_experts_fwd_ws_bytes(S, I), dtype=torch.uint8, device=dev)
     with on(dev):
+        if gu is None and (act is not None or not lib.usaf_hip_fp8_gate_up_ok(S, E, I, H)):
+            gu = torch.empty(S, 2 * I, dtype=dtype, device=dev)
+        y = torch.empty(S, H, dtype=dtype, device=dev)
+        ws = torch.empty(lib.usaf_hip_fp8_experts_fwd_ws_bytes(S, I), dtype=torch.uint8, device=dev)
         N.call("usaf_hip_fp8_experts_fwd", x.q.data_ptr(), x.s.data_ptr(), x.q.shape[0], b.token_idx.data_ptr(),
                b.offsets.data_ptr(), S, E, H, I, N.dtype_code(dtype), ew.gate_up.q.data_ptr(), ew.gate_up.s.data_ptr(),
                ew.down.q.data_ptr(), ew.down.s.data_ptr(), N.ptr(gu), N.ptr(act), y.data_ptr(), ws.data_ptr(), ws.numel(),
