@@ -425,6 +425,26 @@ def test_dense_weight_gradients_beside_8_bit_experts(F, which):
             _within(p.grad[e], l.t() @ r, (2 * T + 1) * 2.0 ** -23 * (l.t().abs() @ r.abs()))
 
 
+def test_backward_behind_saved_tensor_hooks(F):
+    """Tensors that come back from a hook in another layout, and a second backward through a kept graph: the same gradients."""
+    from usaf_amd import moe as G
+    ew = _experts(F, 4, 256, 128)
+    hs, w, dout = _rand(60, 256, seed=9).cuda(), _routing(60, 4, 2, torch.bfloat16, seed=3).cuda(), _rand(60, 256, seed=11).cuda()
+
+    def grads(twice=False):
+        x, ww = hs.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        out = G.routed_experts(x, ww, ew)
+        if twice:
+            torch.autograd.grad(out, (x, ww), dout, retain_graph=True)
+        return torch.autograd.grad(out, (x, ww), dout)
+
+    want = grads()
+    assert all(torch.equal(a, b) for a, b in zip(grads(twice=True), want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.t().contiguous() if t is not None and t.dim() == 2 else t,
+                                                  lambda t: t.t() if t is not None and t.dim() == 2 else t):
+        assert all(torch.equal(a, b) for a, b in zip(grads(), want))
+
+
 def test_slots_without_a_host_read(F):
     """slot_capacity: more slots than pairs, the ones behind them unused; the same output and gradients."""
     from usaf_amd import moe as G

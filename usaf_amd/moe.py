@@ -651,7 +651,8 @@ class RoutedExpertsFn(torch.autograd.Function):
 def _fp8_experts_backward(ctx, dout: torch.Tensor, dweights: torch.Tensor):
     """RoutedExpertsFn.backward on 8-bit experts.  The 16-bit gradients between the products
     are stored only where a weight gradient reads them."""
-    hs, gu, act, y = ctx.saved_tensors
+    # (contiguous: a saved-tensor hook may have changed their layout)
+    hs, gu, act, y = (t if t is None else t.contiguous() for t in ctx.saved_tensors)
     b, capture, dt, dev = ctx.b, ctx.capture, hs.dtype, hs.device
     E, H, I, S = ctx.ew.E, ctx.ew.H, ctx.ew.I, b.n_slots
     want_gu, want_dn = ctx.needs_input_grad[4], ctx.needs_input_grad[5]
