@@ -16,6 +16,8 @@ between calls.  It keeps more digits than the routed path between its steps
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _native as N
@@ -25,6 +27,12 @@ from .moe import ExpertWeights, Q4Tensor
 MAX_TOKENS = 32
 MAX_EXPERTS = 256
 MAX_TOP_K = 16
+
+
+@functools.lru_cache(maxsize=1024)
+def _ws_bytes(device: int, tokens: int, experts: int, top_k: int, hidden: int, inter: int) -> int:
+    """The workspace on a device (its CU count decides the split), which is the current one."""
+    return N.load().usaf_hip_moe_few_ws_bytes(tokens, experts, top_k, hidden, inter)
 
 
 def few_token_ok(tokens: int, top_k: int, experts: ExpertWeights) -> bool:
@@ -71,7 +79,7 @@ def few_token_block(hs: torch.Tensor, router_weight: torch.Tensor, top_k: int, n
         return out
     with on(dev):
         gu_s, dn_s = (gu.s, dn.s) if experts.is_fp8 else (gu.scale_zero_by_group(), dn.scale_zero_by_group())
-        ws = torch.empty(N.load().usaf_hip_moe_few_ws_bytes(tokens, E, top_k, H, I), dtype=torch.uint8, device=dev)
+        ws = torch.empty(_ws_bytes(dev.index, tokens, E, top_k, H, I), dtype=torch.uint8, device=dev)
         N.call("usaf_hip_moe_few", x.data_ptr(), tokens, H, router.data_ptr(), E, top_k, 1 if norm_topk_prob else 0,
                N.dtype_code(dt), I, 1 if experts.is_fp8 else 0, gu.q.data_ptr(), gu_s.data_ptr(), dn.q.data_ptr(),
                dn_s.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(), N.stream_ptr(dev))

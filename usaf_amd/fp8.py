@@ -19,6 +19,7 @@ The reference has no 8-bit format; its frozen weights are 4-bit
 from __future__ import annotations
 
 import contextlib
+import functools
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -33,9 +34,17 @@ def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on(device: torch.device):
     """The device made current for a call's launches (nothing to do where it is)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_ws_bytes(m: int, k: int) -> int:
+    return N.load().usaf_hip_fp8_linear_ws_bytes(m, k)
 
 
 class Fp8Tensor:
@@ -171,7 +180,7 @@ def _linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
         rows = rows.contiguous()
     out = torch.empty(m, n, dtype=x.dtype, device=dev)
     if m:
-        need = N.load().usaf_hip_fp8_linear_ws_bytes(m, k)
+        need = _linear_ws_bytes(m, k)
         with on(dev):
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
             N.call("usaf_hip_fp8_linear", rows.data_ptr(), N.dtype_code(x.dtype), m, k, max(rows.stride(0), k),
