@@ -370,3 +370,19 @@ def test_refusals(B):
     ew.set_overlay("down", torch.tensor([3], device="cuda"), torch.ones(1, device="cuda"), torch.bfloat16)
     with pytest.raises(NotImplementedError, match="overlays"):
         call(x, r, 2, True, ew)
+
+
+@pytest.mark.parametrize("fmt", ["q4", "fp8"])
+def test_under_a_trace_and_a_tangent(B, fmt):
+    """A trace replays the layer, not the memory it was written to; forward-mode derivatives are refused, as on the routed path."""
+    from torch.autograd import forward_ad
+    ew, _ = _random_experts(fmt, 8, 256, 128)
+    x, other, r = _rand(5, 256, seed=1).cuda(), _rand(5, 256, seed=2).cuda(), _rand(8, 256, seed=3, scale=0.1).cuda()
+    with torch.no_grad():
+        traced = torch.jit.trace(lambda v: B.few_token_block(v, r, 2, True, ew) * 2, (x,))
+        for v in (other, x):
+            assert torch.equal(traced(v), B.few_token_block(v, r, 2, True, ew) * 2)
+    with forward_ad.dual_level():
+        for args in ((forward_ad.make_dual(x, x), r), (x, forward_ad.make_dual(r, r))):
+            with pytest.raises((NotImplementedError, RuntimeError), match="forward"):
+                B.few_token_block(*args, 2, True, ew)

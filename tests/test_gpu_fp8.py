@@ -653,3 +653,19 @@ def test_experts_without_a_backward_keep_nothing(F):
     assert torch.equal(G.routed_experts(hs, w, ew), want)
     with torch.no_grad():
         assert torch.equal(G.routed_experts(hs.clone().requires_grad_(True), w, ew), want)
+
+
+@pytest.mark.parametrize("rows", [3, 50])
+def test_linear_under_a_trace_and_a_tangent(F, rows):
+    """A trace replays the product, not the memory it was written to; a forward-mode derivative is refused."""
+    from torch.autograd import forward_ad
+    t = F.Fp8Tensor.quantize(_rand(200, 384, seed=2, scale=0.1).cuda())
+    x, other = _rand(rows, 384, seed=1).cuda(), _rand(rows, 384, seed=2).cuda()
+    with torch.no_grad():
+        traced = torch.jit.trace(lambda v: F.fp8_linear(v, t) * 2, (x,))
+        for v in (other, x):
+            assert torch.equal(traced(v), F.fp8_linear(v, t) * 2)
+    with forward_ad.dual_level():
+        with pytest.raises((NotImplementedError, RuntimeError), match="forward"):
+            F.fp8_linear(forward_ad.make_dual(x, x), t)
+        assert torch.equal(F.fp8_linear(x, t), F.fp8_linear(x.clone(), t))

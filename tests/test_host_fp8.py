@@ -183,3 +183,56 @@ def test_no_launch_on_cpu_tensors():
                  lambda: few_token_block(x, torch.zeros(2, 128, dtype=torch.bfloat16), 1, True, ew)):
         with pytest.raises((ValueError, RuntimeError, AssertionError)):
             call()
+
+
+def test_followed_by_a_trace_or_a_tangent():
+    """What requires_grad does not show: forward-mode derivatives and traces."""
+    from torch.autograd import forward_ad
+    x, seen = torch.ones(3), []
+
+    def f(v):
+        seen.append(N.followed(v))
+        return v * 2
+
+    assert not N.followed(x) and not N.followed(x.clone().requires_grad_(True))
+    with torch.no_grad():
+        torch.jit.trace(f, (x,), check_trace=False)
+    assert seen == [True]
+    with forward_ad.dual_level():
+        assert not N.followed(x) and N.followed(x, forward_ad.make_dual(x, x))
+        for call in (fp8.quantize_rows, fp8.Fp8Tensor.quantize):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(forward_ad.make_dual(torch.ones(2, 128, dtype=torch.bfloat16), torch.ones(2, 128, dtype=torch.bfloat16)))
+    with pytest.raises(RuntimeError, match="trace"):
+        torch.jit.trace(lambda v: v + _t(2, 128).dequantize(), (x,), check_trace=False)
+
+
+class _OnGpu(torch.Tensor):
+    """A CPU tensor that says it is on the GPU."""
+    is_cuda = True
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        return super().__torch_function__(func, types, args, kwargs or {})
+
+
+@pytest.mark.parametrize("call", ["linear", "few"])
+def test_forward_mode_derivatives_are_refused(call, monkeypatch):
+    """Not left out of the output, with the launch replaced by an operation that torch does not see either."""
+    from torch.autograd import forward_ad
+    from usaf_amd import few
+    monkeypatch.setattr(fp8, "_linear", lambda x, w: torch.from_numpy(x.detach().as_subclass(torch.Tensor).float().numpy() * 3))
+    monkeypatch.setattr(few, "_layer", lambda x, *_: torch.from_numpy(x.detach().as_subclass(torch.Tensor).float().numpy() * 3))
+    x = torch.ones(2, 128, dtype=torch.bfloat16)
+    ew, w, router = ExpertWeights(_t(2, 256, 128), _t(2, 128, 128)), _t(64, 128), torch.ones(2, 128, dtype=torch.bfloat16)
+
+    def f(v, r=router):
+        v = v.as_subclass(_OnGpu)
+        return fp8.fp8_linear(v, w) if call == "linear" else few.few_token_block(v, r, 1, True, ew)
+
+    with torch.no_grad():
+        assert torch.equal(f(x).as_subclass(torch.Tensor), 3 * x.float())
+    with forward_ad.dual_level():
+        for args in [(forward_ad.make_dual(x, x),)] + ([(x, forward_ad.make_dual(router, router))] if call == "few" else []):
+            with pytest.raises((NotImplementedError, RuntimeError), match="forward"):
+                f(*args)

@@ -12,6 +12,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "libusaf_hip.so"
 
@@ -220,6 +221,20 @@ def refuse_capture(what: str) -> None:
     """Raise where the current stream is being captured into a graph."""
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{what}: not while a stream is captured into a graph")
+
+
+def followed(*tensors: torch.Tensor) -> bool:
+    """Whether more than a backward pass follows what is done to these tensors: a trace
+    (torch.jit.trace), or forward-mode derivatives, whose tensors need not require a gradient.
+    A call then goes through its autograd function: the trace records that, and not a launch,
+    and a derivative that the function lacks is refused."""
+    return torch.jit.is_tracing() or any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def refuse_followed(what: str, *tensors: torch.Tensor) -> None:
+    """Raise where a trace or a forward-mode derivative would lose what a call computes."""
+    if followed(*tensors):
+        raise RuntimeError(f"{what}: not in a trace, and it has no forward-mode derivative")
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

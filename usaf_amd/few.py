@@ -48,7 +48,8 @@ def few_token_block(hs: torch.Tensor, router_weight: torch.Tensor, top_k: int, n
                     experts: ExpertWeights) -> torch.Tensor:
     """hs [..., H] fp16 / bf16 with at most 32 tokens, router_weight [E, H] of the same
     dtype -> the layer's output, shaped as hs.  No gradients: call it under
-    ``torch.no_grad()`` or with tensors that need none.  Experts that carry trained values
+    ``torch.no_grad()`` or with tensors that need none, nor forward-mode derivatives
+    (torch.jit.trace records the call).  Experts that carry trained values
     (overlays), dense experts and more tokens go through ``moe.moe_block``."""
     dt, dev = hs.dtype, hs.device
     if dt not in (torch.float16, torch.bfloat16) or router_weight.dtype != dt:
@@ -72,6 +73,15 @@ def few_token_block(hs: torch.Tensor, router_weight: torch.Tensor, top_k: int, n
                          "all on one GPU")
     if torch.is_grad_enabled() and (hs.requires_grad or router_weight.requires_grad):
         raise RuntimeError("few_token_block has no backward: call it under torch.no_grad(), or moe.moe_block")
+    layer = FewTokensFn.apply if N.followed(hs, router_weight) else _layer
+    return layer(hs, router_weight, top_k, norm_topk_prob, experts)
+
+
+def _layer(hs: torch.Tensor, router_weight: torch.Tensor, top_k: int, norm_topk_prob: bool,
+           experts: ExpertWeights) -> torch.Tensor:
+    dt, dev = hs.dtype, hs.device
+    E, H, I, gu, dn = experts.E, experts.H, experts.I, experts.gate_up, experts.down
+    tokens = hs.numel() // H
     x = _aligned(hs)
     router = _aligned(router_weight)
     out = torch.empty(hs.shape, dtype=dt, device=dev)
@@ -84,6 +94,19 @@ def few_token_block(hs: torch.Tensor, router_weight: torch.Tensor, top_k: int, n
                N.dtype_code(dt), I, 1 if experts.is_fp8 else 0, gu.q.data_ptr(), gu_s.data_ptr(), dn.q.data_ptr(),
                dn_s.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
     return out
+
+
+class FewTokensFn(torch.autograd.Function):
+    """The layer as one operation, for a trace to record and forward-mode derivatives to be refused by."""
+
+    @staticmethod
+    def forward(ctx, hs: torch.Tensor, router_weight: torch.Tensor, top_k: int, norm_topk_prob: bool,
+                experts: ExpertWeights) -> torch.Tensor:
+        return _layer(hs, router_weight, top_k, norm_topk_prob, experts)
+
+    @staticmethod
+    def backward(ctx, dout: torch.Tensor):
+        raise RuntimeError("few_token_block has no backward")
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:

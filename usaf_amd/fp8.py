@@ -78,6 +78,7 @@ class Fp8Tensor:
         """From a float weight [R, C] or [E, R, C] (copied to the GPU first where it is on the CPU)."""
         if tensor.dim() not in (2, 3) or tensor.numel() == 0:
             raise ValueError(f"Fp8Tensor.quantize: need a non-empty [R, C] or [E, R, C] tensor, got {tuple(tensor.shape)}")
+        N.refuse_followed("Fp8Tensor.quantize", tensor)
         dev = torch.device(device) if device is not None else (tensor.device if tensor.is_cuda else N.default_device())
         if dev.index is None:
             dev = torch.device(dev.type, torch.cuda.current_device())
@@ -95,6 +96,7 @@ class Fp8Tensor:
 
     def dequantize(self, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values, exact in fp32 and bf16 and rounded in fp16, which lacks the smallest."""
+        N.refuse_followed("Fp8Tensor.dequantize")
         out = torch.empty(self.shape, dtype=out_dtype, device=self.device)
         with on(self.device):
             N.call("usaf_hip_fp8_dequantize", self.q.data_ptr(), self.s.data_ptr(), *self._erc(), out.data_ptr(),
@@ -147,6 +149,12 @@ def quantize_rows(x: torch.Tensor, n_rows: Optional[torch.Tensor] = None) -> Row
     optional int32 device value; rows from there on are left undefined."""
     if x.dim() != 2 or x.dtype not in _ACT:
         raise TypeError(f"quantize_rows: need fp16 or bf16 rows [M, K], got {x.dtype} {tuple(x.shape)}")
+    N.refuse_followed("quantize_rows", x)
+    return rows_of(x, n_rows)
+
+
+def rows_of(x: torch.Tensor, n_rows: Optional[torch.Tensor] = None) -> Rows:
+    """quantize_rows inside an autograd function, which a trace records as a whole."""
     if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
         x = x.contiguous()
     rows = empty_rows(x.shape[0], x.shape[1], x.device)
@@ -193,7 +201,8 @@ def fp8_linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
     [..., N] in x's dtype, summed in fp32 (in another order for a few rows than for many).  Differentiable in x (the weight is frozen);
     the first backward builds ``w.transposed()``.  A value of x that is not finite makes
     its output row NaN.  A stream capture takes the call without a gradient only, as the
-    graph of a training step is switched off (graphs.py)."""
+    graph of a training step is switched off (graphs.py).  There is no forward-mode derivative;
+    torch.jit.trace records the call."""
     if len(w.shape) != 2:
         raise ValueError(f"fp8_linear: need a weight [N, K], got {tuple(w.shape)}")
     if x.dtype not in _ACT:
@@ -205,7 +214,8 @@ def fp8_linear(x: torch.Tensor, w: Fp8Tensor) -> torch.Tensor:
     if torch.is_grad_enabled() and x.requires_grad:
         N.refuse_capture("fp8_linear of activations that want a gradient")
         return Fp8LinearFn.apply(x, w)
-    return _linear(x, w)
+    # (the function's own call takes 2 us of the host's time, beside 7 of a small product's launch)
+    return Fp8LinearFn.apply(x, w) if N.followed(x) else _linear(x, w)
 
 
 # ---------------------------------------------------------------------------

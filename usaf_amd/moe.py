@@ -95,8 +95,11 @@ class Q4Tensor:
         if self._szg is None or self._szg.device != self.q.device:
             N.refuse_capture("Q4Tensor.scale_zero_by_group: the first call")
             E, rows, cols = (int(d) for d in self.shape)
-            words = torch.stack((self.s, self.z), -1).view(torch.int32)
-            szg = words.view(E, rows, cols // 128).transpose(1, 2).contiguous()
+            words = torch.empty(E, rows, cols // 128, dtype=torch.int32, device=self.q.device)
+            with fp8.on(self.q.device):  # (not a view of another type, which a trace cannot hold)
+                N.call("usaf_hip_pack_scale_zero", self.s.data_ptr(), self.z.data_ptr(), self.s.numel(), words.data_ptr(),
+                       N.stream_ptr(self.q.device))
+            szg = words.transpose(1, 2).contiguous()
             torch.cuda.current_stream(szg.device).synchronize()  # any stream may read it from here on
             self._szg = szg
         return self._szg
@@ -532,7 +535,7 @@ class RoutedExpertsFn(torch.autograd.Function):
         st = N.stream_ptr(dev)
         code = N.dtype_code(dt)
         # (before the bucketing, whose host read would leave the GPU idle for it)
-        x8 = fp8.quantize_rows(hs) if ew.is_fp8 and T > 0 else None
+        x8 = fp8.rows_of(hs) if ew.is_fp8 and T > 0 else None
         b = bucket_by_expert(weights) if slots is None else bucket_by_expert(weights, *slots)
         S = b.n_slots
         gu = torch.empty(S, 2 * I, dtype=dt, device=dev) if backward or not ew.is_fp8 else None
