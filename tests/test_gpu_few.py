@@ -386,3 +386,57 @@ def test_under_a_trace_and_a_tangent(B, fmt):
         for args in ((forward_ad.make_dual(x, x), r), (x, forward_ad.make_dual(r, r))):
             with pytest.raises((NotImplementedError, RuntimeError), match="forward"):
                 B.few_token_block(*args, 2, True, ew)
+
+
+@pytest.mark.parametrize("cached", [False, True])
+def test_a_streamed_models_decoding_passes(B, cached):
+    """The switch on a model that the loader set up: the same bits as the layer called by itself; with trained values, and
+    without the switch, the routed path; 8-bit experts attached by hand in place of the streamed ones."""
+    from types import SimpleNamespace
+    from torch import nn
+    from usaf_amd import qwen3moe_dml as Q
+    from usaf_amd.fp8 import Fp8Tensor
+    from usaf_amd.moe import ExpertWeights
+    from usaf_amd.moe_loader import get_quantized_cache, setup_quantized_streaming
+    from usaf_amd.quantization import quantize_state_dict
+    E, H, I, k = 8, 256, 128, 2
+
+    class Experts(nn.Module):
+        forward = Q.dml_qwen3_experts_forward
+
+    class Block(nn.Module):
+        forward = Q.dml_qwen3_moe_block_forward
+
+    model, block = nn.Module(), Block()
+    model.mlp, block.experts = block, Experts()
+    block.gate = SimpleNamespace(weight=_rand(E, H, seed=5, scale=0.1).cuda(), top_k=k, norm_topk_prob=True)
+    model.scale = nn.Parameter(torch.ones(1, dtype=torch.bfloat16), requires_grad=False)
+    w = {"mlp.experts.gate_up_proj": _rand(E, 2 * I, H, dtype=torch.float16, seed=1, scale=0.05),
+         "mlp.experts.down_proj": _rand(E, H, I, dtype=torch.float16, seed=2, scale=0.05)}
+    kw = {"expert_cache_bytes": E * 3 * H * I * 2} if cached else {}
+    setup_quantized_streaming(model, quantize_state_dict(w, device="cuda"), torch.device("cuda", 0), verbose=False,
+                              expert_pattern="mlp.experts", **kw)
+    cache = get_quantized_cache(model)
+    q4 = cache.get_q4("mlp.experts")
+    x, longer = _rand(2, 3, H, seed=3).cuda(), _rand(3, 3, H, seed=4).cuda()
+    with torch.no_grad():
+        want = B.few_token_block(x, block.gate.weight, k, True, ExpertWeights(q4["gate_up_proj"], q4["down_proj"]))
+        routed, routed_longer = block(x), block(longer)
+        assert not torch.equal(routed, want)
+        block._usaf_few_tokens = 8
+        for _ in range(2):
+            assert torch.equal(block(x), want) and torch.equal(block(longer), routed_longer)
+        eight = {n.rsplit(".", 1)[1]: Fp8Tensor.quantize(t.cuda()) for n, t in w.items()}
+        block.experts._usaf_q4 = eight
+        ew = ExpertWeights(eight["gate_up_proj"], eight["down_proj"])
+        for _ in range(2):
+            assert torch.equal(block(x), B.few_token_block(x, block.gate.weight, k, True, ew))
+            assert not torch.equal(block(longer), routed_longer)
+        block.experts._usaf_q4 = None
+        assert torch.equal(block(x), want)
+        name, at = "mlp.experts.down_proj", torch.tensor([3, 500], device="cuda")
+        cache.overlays[name] = (at, torch.full((2,), 4.0, device="cuda"))
+        trained = block(x)
+        assert not torch.equal(trained, want)
+        del block._usaf_few_tokens
+        assert torch.equal(block(x), trained)

@@ -24,6 +24,7 @@ import torch.nn as nn
 from . import _native as N
 from .importance import TopKImportanceStore  # noqa: F401  (moe_loader.py:584-631, GPU selection)
 from .expert_cache import ExpertSlotCache
+from .fp8 import Fp8Tensor
 from .moe import ExpertWeights, OverlayTooDense, Q4Overlay, Q4Tensor, timed_call
 from .olmoe_streaming import _record_grad, apply_captured_expert_grads  # noqa: F401  (moe_loader.py:778-802)
 from .quantization import dequantize_4bit
@@ -665,7 +666,11 @@ def setup_quantized_streaming(model: nn.Module, quantized_dict: Dict[str, Any], 
     (QuantizedExpertCache.make_slot_cache, attached as ``module._usaf_slots``);
     the patched experts forward runs on the copies when it needs no gradients
     and the module has no trained values, and on the fused 4-bit GEMMs
-    otherwise."""
+    otherwise.  What the pre-hook attaches is also had from
+    ``module._usaf_q4_source(module)``, for a block whose pass does not call the experts
+    module (qwen3moe_dml: ``_usaf_few_tokens``).  8-bit tensors (fp8.Fp8Tensor) that the
+    user has put into ``module._usaf_q4`` stay there and serve every pass; a module
+    with trained values refuses them."""
     cache = QuantizedExpertCache(quantized_dict, device=device, max_cached=max_cached_experts,
                                  group_size=group_size)
     expert_names = [name for name, _ in model.named_modules() if fnmatch.fnmatch(name, expert_pattern)]
@@ -690,17 +695,33 @@ def setup_quantized_streaming(model: nn.Module, quantized_dict: Dict[str, Any], 
         if expert_cache_bytes:
             cache.make_slot_cache(int(expert_cache_bytes), act)
 
+    def eight_bit(module: nn.Module) -> bool:
+        return any(isinstance(t, Fp8Tensor) for t in (getattr(module, "_usaf_q4", None) or {}).values())
+
+    def weights(module: nn.Module, mod_name: str):
+        """The tensors and the overlay tables of a pass through an expert module."""
+        q4, overlays = cache.get_q4(mod_name), cache.get_q4_overlays(mod_name)
+        if not eight_bit(module):
+            return q4, overlays
+        if trained(mod_name):
+            raise NotImplementedError(f"{mod_name}: trained values apply to its 4-bit experts, not to the 8-bit ones attached to it")
+        return module._usaf_q4, overlays
+
+    def trained(mod_name: str) -> bool:
+        return any(n in cache.fused_overlays for n, _ in cache._expert_to_params.get(mod_name, []))
+
+    def source(mod_name: str):
+        return lambda module: weights(module, mod_name)
+
     def attach(mod_name: str):
         def pre_hook(module: nn.Module, _args) -> None:
             if fused:
-                module._usaf_q4 = cache.get_q4(mod_name)
-                module._usaf_q4_overlays = cache.get_q4_overlays(mod_name)
+                module._usaf_q4, module._usaf_q4_overlays = weights(module, mod_name)
                 # the copies hold the plain 4-bit values: modules with trained values
                 # (overlay tables or a dense fallback) stay on the fused path
                 sc = cache.slot_cache
-                trained = any(n in cache.fused_overlays for n, _ in cache._expert_to_params.get(mod_name, []))
-                module._usaf_slots = (sc, mod_name) if sc is not None and mod_name in sc.layers and not trained \
-                    else None
+                module._usaf_slots = (sc, mod_name) if sc is not None and mod_name in sc.layers \
+                    and not trained(mod_name) and not eight_bit(module) else None
             else:
                 for pname, param in cache.get_expert_weights(mod_name).items():
                     module._parameters[pname] = param
@@ -712,7 +733,8 @@ def setup_quantized_streaming(model: nn.Module, quantized_dict: Dict[str, Any], 
 
     def detach(module: nn.Module, _args, output):
         module._parameters.clear()
-        module._usaf_q4 = None
+        if not eight_bit(module):
+            module._usaf_q4 = None
         module._usaf_q4_overlays = None
         module._usaf_slots = None
         state["resident"] -= 1
@@ -723,6 +745,8 @@ def setup_quantized_streaming(model: nn.Module, quantized_dict: Dict[str, Any], 
         if name in experts:
             mod.register_forward_pre_hook(attach(name))
             mod.register_forward_hook(detach)
+            if fused:
+                mod._usaf_q4_source = source(name)
     model._quantized_cache = cache
     return model
 

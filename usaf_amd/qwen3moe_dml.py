@@ -22,7 +22,9 @@ reference (it detaches every per-expert slice).
 
 Decoding: with ``block._usaf_few_tokens = n`` (up to 32) a block's passes of at most
 n tokens that want no gradient run as ``few.few_token_block``, router and experts in
-three or four launches, where the experts are 4-bit or 8-bit and carry no trained values.
+three or four launches, where the experts are 4-bit or 8-bit (attached to the experts module, or streamed by
+``moe_loader.setup_quantized_streaming``) and carry no trained values.  Such a pass does not call the experts
+module: its hooks do not run, and copies of its weights (``expert_cache_bytes``) are not used.
 Its numerics (``few.py``) differ from this path's in what is rounded to 16 bits, so it is off by default.
 """
 from __future__ import annotations
@@ -33,17 +35,21 @@ from .few import few_token_block, few_token_ok
 from .moe import ExpertWeights, RouteTopKFn, routed_experts
 
 
+def _with_overlays(gate_up, down, overlays) -> ExpertWeights:
+    ew = ExpertWeights(gate_up, down)
+    # trained values over the 4-bit weights (QuantizedExpertCache.sync_resident)
+    for local, ov in (overlays or {}).items():
+        ew.overlays[local.replace("_proj", "")] = ov
+    return ew
+
+
 def _expert_weights(module) -> ExpertWeights:
     q4 = getattr(module, "_usaf_q4", None)
     if q4:
         gu, dn = q4.get("gate_up_proj"), q4.get("down_proj")
         if gu is None or dn is None:
             raise RuntimeError("module._usaf_q4 must hold gate_up_proj and down_proj")
-        ew = ExpertWeights(gu, dn)
-        # trained values over the 4-bit weights (QuantizedExpertCache.sync_resident)
-        for local, ov in (getattr(module, "_usaf_q4_overlays", None) or {}).items():
-            ew.overlays[local.replace("_proj", "")] = ov
-        return ew
+        return _with_overlays(gu, dn, getattr(module, "_usaf_q4_overlays", None))
     gu = getattr(module, "gate_up_proj", None)
     dn = getattr(module, "down_proj", None)
     if gu is None or dn is None:
@@ -87,9 +93,15 @@ def _few_weights(block, hs: torch.Tensor):
     if torch.is_grad_enabled() and (hs.requires_grad or router.weight.requires_grad
                                     or getattr(experts, "_grad_capture", None) is not None):
         return None
-    if not getattr(experts, "_usaf_q4", None) or router.weight.dtype != hs.dtype:
+    if router.weight.dtype != hs.dtype:
         return None
-    ew = _expert_weights(experts)
+    q4, overlays = getattr(experts, "_usaf_q4", None), getattr(experts, "_usaf_q4_overlays", None)
+    source = getattr(experts, "_usaf_q4_source", None)
+    if source is not None:  # a streamed module, whose hooks attach its weights in its own call only
+        q4, overlays = source(experts)
+    if not q4 or q4.get("gate_up_proj") is None or q4.get("down_proj") is None:
+        return None
+    ew = _with_overlays(q4["gate_up_proj"], q4["down_proj"], overlays)
     return ew if few_token_ok(hs.shape[0], int(router.top_k), ew) else None
 
 
