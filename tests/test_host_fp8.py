@@ -164,6 +164,23 @@ def test_capture_refuses_what_is_kept_or_wants_a_gradient(monkeypatch):
         routed_experts(x, torch.zeros(3, 2, dtype=torch.bfloat16), ExpertWeights(_t(2, 256, 128), _t(2, 128, 128)))
 
 
+def test_backward_is_not_captured(monkeypatch):
+    """Of a forward pass before the capture: as the forward pass with a gradient."""
+    from types import SimpleNamespace
+    from usaf_amd import moe
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    dy = torch.zeros(3, 128, dtype=torch.bfloat16)
+    w = _t(128, 128)
+    w._t = _t(128, 128)  # built before
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="captured"):
+            fp8.Fp8LinearFn.backward(SimpleNamespace(w=w, dtype=dy.dtype), dy)
+        ctx = SimpleNamespace(saved_tensors=(dy, None, None, dy), b=SimpleNamespace(n_slots=3), capture=None,
+                              ew=ExpertWeights(_t(2, 256, 128), _t(2, 128, 128)), needs_input_grad=(True,) * 9)
+        with pytest.raises(RuntimeError, match="captured"):
+            moe._fp8_experts_backward(ctx, dy, torch.zeros(3, 2, dtype=torch.bfloat16))
+
+
 def test_overlays_on_8_bit_experts_are_refused():
     """Trained values are held over 4-bit weights only: never left out in silence."""
     ew = ExpertWeights(_t(2, 256, 128), _t(2, 128, 128))

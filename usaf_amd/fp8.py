@@ -176,6 +176,7 @@ class Fp8LinearFn(torch.autograd.Function):
     def backward(ctx, dy: torch.Tensor):
         if torch.is_grad_enabled():
             raise RuntimeError("fp8_linear has no second derivative (create_graph=True)")
+        N.refuse_capture("fp8_linear's backward")
         return _linear(dy if dy.dtype == ctx.dtype else dy.to(ctx.dtype), ctx.w.transposed()), None
 
 

@@ -654,6 +654,7 @@ class RoutedExpertsFn(torch.autograd.Function):
 def _fp8_experts_backward(ctx, dout: torch.Tensor, dweights: torch.Tensor):
     """RoutedExpertsFn.backward on 8-bit experts.  The 16-bit gradients between the products
     are stored only where a weight gradient reads them."""
+    N.refuse_capture("the routed layer's backward on 8-bit experts")
     # (contiguous: a saved-tensor hook may have changed their layout)
     hs, gu, act, y = (t if t is None else t.contiguous() for t in ctx.saved_tensors)
     b, capture, dt, dev = ctx.b, ctx.capture, hs.dtype, hs.device
