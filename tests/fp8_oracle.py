@@ -74,3 +74,9 @@ def product_bound(a, w, ref, dtype):
     top = [torch.nn.functional.pad(v.abs(), pad).view(v.shape[0], -1, 64).amax(-1) for v in (a, w)]
     cut = 2.0 ** -7 * (top[0] @ top[1].t())
     return ref.abs() * half_step(dtype) + tiny(dtype) + ((a.shape[1] + 1) * 2.0 ** -23 * mags + cut) * (1 + half_step(dtype))
+
+
+def wide_bound(a, w, ref, dtype):
+    """As product_bound for the 16-bit instruction, which cuts nothing: the output's half step and the fp32 sum's steps."""
+    mags = a.abs() @ w.abs().t()
+    return ref.abs() * half_step(dtype) + tiny(dtype) + (a.shape[1] + 1) * 2.0 ** -23 * mags * (1 + half_step(dtype))
