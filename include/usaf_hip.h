@@ -581,9 +581,10 @@ int usaf_hip_fp8_transpose(const uint8_t* q, const uint8_t* s, int64_t E, int64_
  * a, a_scale: usaf_hip_fp8_quantize_rows' layout, a_total rows; row(m) = a_rows[m], or m for NULL.
  * w, w_scale: [E, N, K] in usaf_hip_fp8_quantize_weight's layout.  out [M, N] fp16 /
  * bf16.  Slots from offsets[E] on are left as they are.  E <= 255; gathered rows
- * (a_rows) below 4 GiB of codes.  The 8-bit matrix instruction aligns the products within
- * it to the largest, which costs 1.5e-5 of the result (rms); wide != 0 multiplies the same
- * values with the 16-bit one (1e-7, half its rate).
+ * (a_rows) below 4 GiB of codes.  The 8-bit matrix instruction aligns the 64 products within
+ * it to the largest and drops what lies below about 2^-13 of it: 1.5e-5 of the result (rms) on
+ * normal data, more where larger products cancel; wide != 0 multiplies the same values with the
+ * 16-bit one (1e-7, half its rate).
  */
 int usaf_hip_fp8_gemm(const uint8_t* a, const uint8_t* a_scale, int64_t a_total, const int32_t* a_rows, int64_t M,
                       const uint8_t* w, const uint8_t* w_scale, const int32_t* offsets, int64_t E, int64_t N, int64_t K,

@@ -11,6 +11,8 @@
 // blocks below 2^-112 lose their low codes, which no model's values reach.
 // A value that is not finite becomes the NaN code 0x7F and takes no part in max|x|:
 // its row of a product is NaN, as the row's 16-bit product would be (inf or NaN).
+// Values above 248 2^120 = 3.30e38, the last 3 % of bf16's range, round to 2^128, which no product can hold:
+// they count as infinite there.
 #include "fp8.h"
 
 namespace usaf {
