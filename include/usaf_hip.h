@@ -668,6 +668,41 @@ int usaf_hip_moe_few(const void* x, int64_t T, int64_t H, const void* router, in
                      const void* gate_up_scale, const uint8_t* down, const void* down_scale, void* out, void* ws,
                      int64_t ws_bytes, void* stream);
 
+/*
+ * Products with one 4-bit weight W [N, K], group size 128 along whole rows (K % 128 == 0): codes q as
+ * usaf_hip_quantize_q4 packs them, sz usaf_hip_pack_scale_zero's words; its values are
+ * usaf_hip_dequant_q4's of the activations' dtype (fp16 / bf16).
+ *   usaf_hip_q4_linear      out [M, N] = dtype(x W^T), x [M, K] with row stride ld
+ *   usaf_hip_q4_linear_bwd  dx [M, K] = dtype(dy W),   dy [M, N] with row stride ld
+ * fp32 sums.  ws: usaf_hip_q4_linear_ws_bytes (0 bytes: may be NULL), 16-byte aligned; rows 16-byte aligned (of dy: where N % 64
+ * == 0), codes 16-byte.  N, K <= 2^22.
+ */
+int64_t usaf_hip_q4_linear_ws_bytes(int64_t M, int64_t N, int64_t K, int32_t backward);
+int usaf_hip_q4_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* q,
+                       const uint32_t* sz, int64_t N, void* out, void* ws, int64_t ws_bytes, void* stream);
+int usaf_hip_q4_linear_bwd(const void* dy, int32_t dtype, int64_t M, int64_t N, int64_t ld, const uint8_t* q,
+                           const uint32_t* sz, int64_t K, void* dx, void* ws, int64_t ws_bytes, void* stream);
+
+/*
+ * Gate and up projection with the gated activation (qwen3moe_dml.py:58-61 for one expert, without its 16-bit
+ * roundings of gate, up and silu), W [2 I, K] = the gate's rows, then up's: 4-bit (q, sz as above) or 16-bit (w16).
+ *   usaf_hip_gated_fwd   (G, U) = x W^T, act [M, I] = dtype(silu(G) U).  kept (NULL: not wanted): what the backward reads.
+ *     kept_scales NULL: dtype(G), dtype(U) as [M, 2, round_up(I, 8)].  Else the 8-bit block format's codes (usaf_hip_fp8_*) of
+ *     the unrounded G and U, [M, 2, round_up(I, 128)], and scale bytes [M, 2, ceil(I / 128)].
+ *   usaf_hip_gated_bwd   dG = dtype(dact U s (1 + G (1 - s))), dU = dtype(dact G s), s = sigmoid(G), of the kept
+ *     values; dx [M, K] = dtype([dG, dU] W) and, 16-bit weights, dw [2 I, K] = dtype([dG, dU]^T x), each where not NULL.
+ *     dact [M, I] contiguous; x (row stride ldx) is read for dw only.
+ * ws: usaf_hip_gated_ws_bytes with what = 0 for the forward, else 1 for dx + 2 for dw; 16-byte aligned.  Weights, kept and (K
+ * % 64 == 0) rows of x 16-byte aligned.  2 I, K <= 2^22; K % 128 == 0 for 4-bit weights.
+ */
+int64_t usaf_hip_gated_ws_bytes(int64_t M, int64_t I, int64_t K, int32_t four_bit, int32_t what);
+int usaf_hip_gated_fwd(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* q,
+                       const uint32_t* sz, const void* w16, int64_t I, void* act, void* kept, uint8_t* kept_scales,
+                       void* ws, int64_t ws_bytes, void* stream);
+int usaf_hip_gated_bwd(const void* dact, int32_t dtype, int64_t M, int64_t I, int64_t K, const void* kept,
+                       const uint8_t* kept_scales, const uint8_t* q, const uint32_t* sz, const void* w16, const void* x,
+                       int64_t ldx, void* dx, void* dw, void* ws, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -64,6 +64,12 @@ _SIGNATURES: dict[str, list] = {
     "usaf_hip_fp8_swiglu_bwd": [_c_p, _c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_p],
     "usaf_hip_moe_few": [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i32, _c_i32, _c_i64, _c_i32, _c_p, _c_p, _c_p,
                          _c_p, _c_p, _c_p, _c_i64, _c_p],
+    "usaf_hip_q4_linear": [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p],
+    "usaf_hip_q4_linear_bwd": [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p],
+    "usaf_hip_gated_fwd": [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i64,
+                           _c_p],
+    "usaf_hip_gated_bwd": [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p,
+                           _c_p, _c_i64, _c_p],
     "usaf_hip_quantize_q4": [_c_p, _c_i32, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p],
     "usaf_hip_pack_scale_zero": [_c_p, _c_p, _c_i64, _c_p, _c_p],
     "usaf_hip_q4_transpose": [_c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p],
@@ -127,6 +133,8 @@ _VALUE_FUNCS: dict[str, tuple] = {
     "usaf_hip_fp8_experts_fwd_ws_bytes": (_c_i64, [_c_i64, _c_i64]),
     "usaf_hip_fp8_experts_bwd_ws_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64]),
     "usaf_hip_fp8_linear_ws_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "usaf_hip_q4_linear_ws_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i32]),
+    "usaf_hip_gated_ws_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i32, _c_i32]),
     "usaf_hip_fp8_scale_stride": (_c_i64, [_c_i64]),
     "usaf_hip_frag_slot_elems": (_c_i64, [_c_i64, _c_i64, _c_i64]),
 }

@@ -37,13 +37,13 @@
 // tokens on 64 experts of 1,024 takes 310 us so and 322 with C written and a kernel of its own behind it.  Where a
 // backward needs C as well the two are equal (846, 4,096 tokens on 128 experts of 768), or this
 // one is the slower (352 against 343, 256 tokens), so there they stay apart.
+#include "dma.h"
 #include "fp8.h"
 
 namespace usaf {
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(3))) void* lds_void_ptr;
 
 struct Fp8Args {
   const uint8_t* A;        // [.., Kp] codes
@@ -67,34 +67,11 @@ struct Fp8Args {
 constexpr int G_WAVES = 8, G_THREADS = 64 * G_WAVES;
 constexpr int G_XCDS = 8;  // accelerator dies, blocks dispatched round-robin over them
 
-__device__ __forceinline__ int g_swz(int r) { return (r >> 1) & 7; }
-
 __device__ __forceinline__ f32x16 mfma8(const u32x4 a0, const u32x4 a1, const u32x4 b0, const u32x4 b1, f32x16 c, int sa,
                                         int sb) {
   const i32x8 a = {(int)a0.x, (int)a0.y, (int)a0.z, (int)a0.w, (int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w};
   const i32x8 b = {(int)b0.x, (int)b0.y, (int)b0.z, (int)b0.w, (int)b1.x, (int)b1.y, (int)b1.z, (int)b1.w};
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
-}
-
-// LDS DMA: lane l's 16 (4) bytes at base + off land at lds + 16 l (4 l); base and lds are
-// wave-uniform.  Inline asm, since beside the compiler's own LDS DMA every LDS read would
-// wait for all of them.  M0 takes the LDS address; the wait states cover a base that comes
-// out of readfirstlane.  They count in vmcnt only, which the ring waits for itself.
-__device__ __forceinline__ void g_dma16(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0");
-}
-__device__ __forceinline__ void g_dma4(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0");
-}
-__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
-  const uint64_t v = (uint64_t)(uintptr_t)p;
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
-  return reinterpret_cast<const uint8_t*>((uintptr_t)(((uint64_t)hi << 32) | (uint64_t)lo));
-}
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 // The list of m-tiles (experts in order, each in tiles of SLOTS), held by a wave: lane l

@@ -1,0 +1,34 @@
+// Products with one 16-bit or 4-bit weight: what linear_kernel.h's two halves (linear_dense.hip, linear_q4.hip)
+// and their callers (linear.hip) share.
+#pragma once
+
+#include "moe_gemm.h"
+
+namespace usaf {
+
+// out[m, n] = dt( sum_k A[m, k] W[n, k] ), or with kept or gated set the gate and up product below.
+struct LinArgs {
+  const uint8_t* A;    // 16-bit rows, lda bytes apart (16-byte aligned, lda too)
+  int64_t lda;
+  int64_t M, K;        // K % 64 == 0 (4-bit: % 128)
+  const uint8_t* W;    // 16-bit rows or packed codes, ldw bytes apart (16-byte aligned, ldw too)
+  int64_t ldw;
+  const uint32_t* sz;  // 4-bit: scale | zero << 16 of every group of 128, [rows, K / 128]
+  int64_t N;           // columns of out; gated: W has 2 N rows, the gate's and then up's
+  uint16_t* out;       // [M, ldo], act where gated
+  int64_t ldo;
+  // gated: what a backward reads (linear.hip), or nullptr
+  void* kept;          // [M, 2, hs]: 16-bit values, hs = N in whole 8, or codes, hs = N in whole 128
+  uint8_t* kept_s;     // scale bytes [M, 2, hs / 128] of codes; nullptr: 16-bit values
+  int64_t hs;
+  int n_nt;            // set at the launch
+};
+
+int launch_linear_dense(const LinArgs& g, int dt, bool gated, hipStream_t st);
+int launch_linear_q4(const LinArgs& g, int dt, bool gated, hipStream_t st);
+void prepare_linear_dense();
+void prepare_linear_q4();
+// Raises the products' dynamic-LDS limits, once per process (usaf_hip_init, or their first use).
+void prepare_linear_kernels();
+
+}  // namespace usaf

@@ -1,0 +1,404 @@
+// Products with one 4-bit or 16-bit weight and the gated feed-forward projections: what runs around linear_kernel, and
+// the C-ABI.
+//
+//   q4_linear   out = dt(x W^T),  dx = dt(dy W),        W = dt(fp16(fp16(q s) + z)) (codec.hip)
+//   gated       (G, U) = x W^T,   act = dt(silu(G) U);  kept: dt(G), dt(U), or Q(G), Q(U) in blocks of 128 (fp8.hip)
+//               dG = dt(dact U s (1 + G (1 - s))), dU = dt(dact G s), s = sigmoid(G), of the kept values
+//               dx = dt([dG, dU] W),   dW = dt([dG, dU]^T x)
+//
+// Every product is linear_kernel's C = A W^T, so a grad-input reads a transposed 16-bit copy of the weight and a weight
+// gradient transposed copies of both operands, made in the workspace by the kernels here.
+#include "fp8.h"
+#include "linear.h"
+
+namespace usaf {
+namespace {
+
+constexpr int64_t LIN_MAX = (int64_t)1 << 22;  // columns: 256 rows of 16-bit values stay within 32-bit offsets
+
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// ---- copies of operands ----------------------------------------------------------
+
+// 4-bit rows [rows, K] -> 16-bit rows: 8 codes a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void q4_rows_kernel(const uint32_t* __restrict__ q, const uint32_t* __restrict__ sz,
+                                                      int64_t words, u32x4* __restrict__ out) {
+  const int64_t stride = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += stride) {
+    const uint32_t p = sz[i >> 4];  // 16 words a group
+    const f16 s = __builtin_bit_cast(f16, (uint16_t)p), z = __builtin_bit_cast(f16, (uint16_t)(p >> 16));
+    out[i] = dq8<DT>(q[i], f16x2{s, s}, f16x2{z, z});
+  }
+}
+
+// [S, C] (16-bit, row stride ld; or 4-bit codes, C = K) -> [C, ldo], zeros for s in [S, ldo); ldo % 64 == 0.  A block
+// has 64 x 64 values.
+template <int DT, bool Q4>
+__global__ __launch_bounds__(256) void transpose_kernel(const void* __restrict__ in, const uint32_t* __restrict__ sz, int64_t S,
+                                                        int64_t C, int64_t ld, bool vec, uint16_t* __restrict__ out,
+                                                        int64_t ldo) {
+  __shared__ __align__(16) uint32_t tile[TT_DWORDS];
+  const int64_t s0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
+  const int sp = threadIdx.x >> 3, cg = threadIdx.x & 7;
+  auto row = [&](int64_t s) -> uint4 {
+    const int64_t c = c0 + 8 * cg;
+    if (s >= S || c >= C) return uint4{0, 0, 0, 0};
+    if constexpr (Q4) {
+      const uint32_t w = reinterpret_cast<const uint32_t*>(in)[(s * C + c) >> 3], p = sz[s * (C >> 7) + (c >> 7)];
+      const f16 sc = __builtin_bit_cast(f16, (uint16_t)p), z = __builtin_bit_cast(f16, (uint16_t)(p >> 16));
+      const u32x4 v = dq8<DT>(w, f16x2{sc, sc}, f16x2{z, z});
+      return uint4{v.x, v.y, v.z, v.w};
+    } else {
+      const uint16_t* const p = reinterpret_cast<const uint16_t*>(in) + s * ld + c;
+      if (vec) return *reinterpret_cast<const uint4*>(p);  // C % 8 == 0
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = (c + 2 * j < C ? (uint32_t)p[2 * j] : 0u) | (c + 2 * j + 1 < C ? (uint32_t)p[2 * j + 1] << 16 : 0u);
+      return uint4{w[0], w[1], w[2], w[3]};
+    }
+  };
+  tt_write(tile, sp, cg, row(s0 + 2 * sp), row(s0 + 2 * sp + 1));
+  __syncthreads();
+#pragma unroll
+  for (int it = 0; it < 2; ++it) {
+    const int v = threadIdx.x + 256 * it, cl = v >> 3, sg = v & 7;
+    if (c0 + cl < C) *reinterpret_cast<uint4*>(out + (c0 + cl) * ldo + s0 + 8 * sg) = tt_read(tile, cl, sg);
+  }
+}
+
+// [rows, C] -> [rows, ldo] with zeros behind column C; ldo % 8 == 0.
+__global__ __launch_bounds__(256) void pad_kernel(const uint16_t* __restrict__ in, int64_t rows, int64_t C, int64_t ld,
+                                                  uint16_t* __restrict__ out, int64_t ldo) {
+  const int64_t chunks = ldo / 8, n = rows * chunks, stride = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+    const int64_t r = i / chunks, c = 8 * (i - r * chunks);
+    const uint16_t* const p = in + r * ld + c;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = (c + 2 * j < C ? (uint32_t)p[2 * j] : 0u) | (c + 2 * j + 1 < C ? (uint32_t)p[2 * j + 1] << 16 : 0u);
+    *reinterpret_cast<uint4*>(out + r * ldo + c) = uint4{w[0], w[1], w[2], w[3]};
+  }
+}
+
+// ---- the gated activation's backward ---------------------------------------------
+
+// dact [M, I], kept -> dgu [M, ldd] = [dG, dU, zeros]: 8 columns of both a thread.
+template <int DT, bool EIGHT>
+__global__ __launch_bounds__(256) void gated_bwd_kernel(const uint16_t* __restrict__ dact, const void* __restrict__ kept,
+                                                        const uint8_t* __restrict__ kept_s, int64_t M, int64_t I, int64_t hs,
+                                                        bool vec, uint16_t* __restrict__ dgu, int64_t ldd) {
+  const int64_t chunks = (I + 7) / 8, n = M * chunks, stride = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+    const int64_t m = i / chunks, c = 8 * (i - m * chunks), left = I - c;
+    float da[8], gate[8], up[8], dg[8], du[8];
+    load8<DT>(dact + m * I + c, vec, left > 8 ? 8 : (int)left, da);
+    if constexpr (EIGHT) {
+      const uint8_t* const p = reinterpret_cast<const uint8_t*>(kept) + 2 * m * hs + c;
+      const int64_t nb = hs / 128, at = 2 * m * nb + (c >> 7);
+      const float sg = __uint_as_float((uint32_t)kept_s[at] << 23), su = __uint_as_float((uint32_t)kept_s[at + nb] << 23);
+      const uint2 g8 = *reinterpret_cast<const uint2*>(p), u8 = *reinterpret_cast<const uint2*>(p + hs);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int wg = (int)(j < 2 ? g8.x : g8.y), wu = (int)(j < 2 ? u8.x : u8.y);
+        const f32x2 a = j & 1 ? __builtin_amdgcn_cvt_pk_f32_fp8(wg, true) : __builtin_amdgcn_cvt_pk_f32_fp8(wg, false);
+        const f32x2 b = j & 1 ? __builtin_amdgcn_cvt_pk_f32_fp8(wu, true) : __builtin_amdgcn_cvt_pk_f32_fp8(wu, false);
+        gate[2 * j] = a.x * sg;
+        gate[2 * j + 1] = a.y * sg;
+        up[2 * j] = b.x * su;
+        up[2 * j + 1] = b.y * su;
+      }
+    } else {
+      const uint16_t* const p = reinterpret_cast<const uint16_t*>(kept) + 2 * m * hs + c;
+      unpack8<DT>(*reinterpret_cast<const uint4*>(p), gate);
+      unpack8<DT>(*reinterpret_cast<const uint4*>(p + hs), up);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * gate[j]));
+      dg[j] = da[j] * up[j] * s * (1.0f + gate[j] * (1.0f - s));
+      du[j] = da[j] * gate[j] * s;
+    }
+    uint16_t* const to = dgu + m * ldd + c;
+    if (vec) {  // I % 8 == 0
+      *reinterpret_cast<uint4*>(to) = uint4{pack2<DT>(dg[0], dg[1]), pack2<DT>(dg[2], dg[3]), pack2<DT>(dg[4], dg[5]), pack2<DT>(dg[6], dg[7])};
+      *reinterpret_cast<uint4*>(to + I) = uint4{pack2<DT>(du[0], du[1]), pack2<DT>(du[2], du[3]), pack2<DT>(du[4], du[5]), pack2<DT>(du[6], du[7])};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < left) {
+          store_from_f32<DT>(to, j, dg[j]);
+          store_from_f32<DT>(to + I, j, du[j]);
+        }
+    }
+    if (left <= 8)
+      for (int64_t k = 2 * I; k < ldd; ++k) dgu[m * ldd + k] = 0;
+  }
+}
+
+unsigned blocks_of(int64_t items, int per) {
+  const int64_t b = (items + 256 * per - 1) / (256 * per);
+  return (unsigned)(b < 1 ? 1 : b > 65536 ? 65536 : b);
+}
+
+int q4_rows(const uint8_t* q, const uint32_t* sz, int64_t rows, int64_t K, int dt, void* out, hipStream_t st) {
+  const int64_t words = rows * K / 8;
+  if (dt == USAF_BF16)
+    q4_rows_kernel<USAF_BF16><<<blocks_of(words, 4), 256, 0, st>>>((const uint32_t*)q, sz, words, (u32x4*)out);
+  else
+    q4_rows_kernel<USAF_F16><<<blocks_of(words, 4), 256, 0, st>>>((const uint32_t*)q, sz, words, (u32x4*)out);
+  return check_launch("linear: weight rows");
+}
+
+// sz: in is 4-bit codes.
+int transpose(const void* in, const uint32_t* sz, int64_t S, int64_t C, int64_t ld, int dt, void* out, int64_t ldo,
+              hipStream_t st) {
+  const dim3 grid((unsigned)(ldo / 64), (unsigned)((C + 63) / 64));
+  const bool vec = C % 8 == 0 && ld % 8 == 0 && (uintptr_t)in % 16 == 0;
+  if (grid.y > 65535) return set_error(USAF_ERR_UNSUPPORTED, "linear: more than %d columns", 65535 * 64);
+  if (!sz) transpose_kernel<USAF_BF16, false><<<grid, 256, 0, st>>>(in, sz, S, C, ld, vec, (uint16_t*)out, ldo);
+  else if (dt == USAF_BF16) transpose_kernel<USAF_BF16, true><<<grid, 256, 0, st>>>(in, sz, S, C, ld, vec, (uint16_t*)out, ldo);
+  else transpose_kernel<USAF_F16, true><<<grid, 256, 0, st>>>(in, sz, S, C, ld, vec, (uint16_t*)out, ldo);
+  return check_launch("linear: transpose");
+}
+
+int pad(const void* in, int64_t rows, int64_t C, int64_t ld, void* out, int64_t ldo, hipStream_t st) {
+  pad_kernel<<<blocks_of(rows * (ldo / 8), 1), 256, 0, st>>>((const uint16_t*)in, rows, C, ld, (uint16_t*)out, ldo);
+  return check_launch("linear: pad");
+}
+
+// C = A W^T of 16-bit operands, contraction K % 64 == 0.
+LinArgs product(const void* a, int64_t lda, int64_t M, const void* w, int64_t ldw, int64_t N, int64_t K, void* out, int64_t ldo) {
+  LinArgs g{};
+  g.A = reinterpret_cast<const uint8_t*>(a);
+  g.lda = 2 * lda;
+  g.M = M;
+  g.K = K;
+  g.W = reinterpret_cast<const uint8_t*>(w);
+  g.ldw = 2 * ldw;
+  g.N = N;
+  g.out = reinterpret_cast<uint16_t*>(out);
+  g.ldo = ldo;
+  return g;
+}
+
+// Whether the 4-bit weight is multiplied as codes; else its 16-bit values are written once, to the workspace, and multiplied.
+bool as_codes(int64_t M) { return M <= 512; }
+
+// Pieces of a workspace, each a whole number of 256 bytes.
+struct Ws {
+  uint8_t* at;
+  int64_t used = 0;
+  explicit Ws(void* p) : at(reinterpret_cast<uint8_t*>(p)) {}
+  void* take(int64_t bytes) {
+    void* const p = at ? at + used : nullptr;
+    used += round_up(bytes, 256);
+    return p;
+  }
+};
+
+bool sizes_ok(int64_t M, int64_t N, int64_t K) {
+  return M >= 0 && M <= 0x7FFFFFFF && N >= 1 && N <= LIN_MAX && K >= 1 && K <= LIN_MAX;
+}
+bool half_type(int32_t dt) { return dt == USAF_BF16 || dt == USAF_F16; }
+
+struct Q4LinearWs {
+  void *w = nullptr, *dy = nullptr;
+  int64_t bytes, np;
+  Q4LinearWs(void* ws, int64_t M, int64_t N, int64_t K, bool backward) {
+    Ws at(ws);
+    np = round_up(N, 64);
+    if (backward) {
+      w = at.take(2 * K * np);
+      if (np != N) dy = at.take(2 * M * np);
+    } else if (!as_codes(M)) {
+      w = at.take(2 * N * K);
+    }
+    bytes = at.used;
+  }
+};
+
+struct GatedWs {
+  void *w = nullptr, *x = nullptr;                                  // forward: 16-bit or padded weight, padded x
+  void *dgu = nullptr, *wt = nullptr, *dgut = nullptr, *xt = nullptr;  // backward
+  int64_t bytes, kp, ldd, mp;
+  GatedWs(void* ws, int64_t M, int64_t I, int64_t K, bool four_bit, int what) {
+    Ws at(ws);
+    kp = round_up(K, 64);
+    ldd = round_up(2 * I, 64);
+    mp = round_up(M, 64);
+    if (what == 0) {
+      if (four_bit ? !as_codes(M) : kp != K) w = at.take(2 * 2 * I * kp);
+      if (kp != K) x = at.take(2 * M * kp);
+    } else {
+      dgu = at.take(2 * M * ldd);
+      if (what & 1) wt = at.take(2 * K * ldd);
+      if (what & 2) {
+        dgut = at.take(2 * 2 * I * mp);
+        xt = at.take(2 * K * mp);
+      }
+    }
+    bytes = at.used;
+  }
+};
+
+int check_ws(const char* what, const void* ws, int64_t have, int64_t need) {
+  if (need && (!ws || (uintptr_t)ws % 16 || have < need))
+    return set_error(USAF_ERR_INVALID, "%s: a workspace of %lld bytes, 16-byte aligned, got %lld", what, (long long)need,
+                     (long long)have);
+  return USAF_OK;
+}
+
+}  // namespace
+
+void prepare_linear_kernels() {
+  prepare_linear_dense();
+  prepare_linear_q4();
+}
+
+}  // namespace usaf
+
+using namespace usaf;
+
+extern "C" int64_t usaf_hip_q4_linear_ws_bytes(int64_t M, int64_t N, int64_t K, int32_t backward) {
+  return sizes_ok(M, N, K) ? Q4LinearWs(nullptr, M, N, K, backward != 0).bytes : -1;
+}
+
+static int q4_args(const char* what, const void* a, int32_t dtype, int64_t M, int64_t N, int64_t K, int64_t ld, int64_t cols,
+                   const uint8_t* q, const uint32_t* sz, const void* out) {
+  if (!sizes_ok(M, N, K) || K % 128)
+    return set_error(USAF_ERR_INVALID, "%s: need M >= 0, 1 <= N, K <= %lld and K %% 128 == 0, got M=%lld N=%lld K=%lld", what,
+                     (long long)LIN_MAX, (long long)M, (long long)N, (long long)K);
+  if (!half_type(dtype)) return set_error(USAF_ERR_INVALID, "%s: dtype must be fp16 or bf16", what);
+  if (M == 0) return USAF_OK;
+  if (!a || !q || !sz || !out) return set_error(USAF_ERR_INVALID, "%s: null pointer", what);
+  if (ld < cols || ld > LIN_MAX) return set_error(USAF_ERR_INVALID, "%s: rows of %lld values, %lld apart", what, (long long)cols, (long long)ld);
+  if ((uintptr_t)q % 16 || (uintptr_t)sz % 4 || ((uintptr_t)out | (uintptr_t)a) % 2)
+    return set_error(USAF_ERR_INVALID, "%s: codes must be 16-byte, scales 4-byte, rows and output 2-byte aligned", what);
+  return USAF_OK;
+}
+
+extern "C" int usaf_hip_q4_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* q,
+                                  const uint32_t* sz, int64_t N, void* out, void* ws, int64_t ws_bytes, void* stream) {
+  if (int rc = q4_args("q4_linear", x, dtype, M, N, K, ld, K, q, sz, out)) return rc;
+  if (M == 0) return clear_error();
+  if ((uintptr_t)x % 16 || ld % 8) return set_error(USAF_ERR_INVALID, "q4_linear: rows must be 16-byte aligned");
+  const Q4LinearWs w(ws, M, N, K, false);
+  if (int rc = check_ws("q4_linear", ws, ws_bytes, w.bytes)) return rc;
+  hipStream_t st = as_stream(stream);
+  if (as_codes(M)) {
+    LinArgs g = product(x, ld, M, q, 0, N, K, out, N);
+    g.ldw = K / 2;
+    g.sz = sz;
+    return launch_linear_q4(g, dtype, false, st);
+  }
+  if (int rc = q4_rows(q, sz, N, K, dtype, w.w, st)) return rc;
+  return launch_linear_dense(product(x, ld, M, w.w, K, N, K, out, N), dtype, false, st);
+}
+
+extern "C" int usaf_hip_q4_linear_bwd(const void* dy, int32_t dtype, int64_t M, int64_t N, int64_t ld, const uint8_t* q,
+                                      const uint32_t* sz, int64_t K, void* dx, void* ws, int64_t ws_bytes, void* stream) {
+  if (int rc = q4_args("q4_linear_bwd", dy, dtype, M, N, K, ld, N, q, sz, dx)) return rc;
+  if (M == 0) return clear_error();
+  const Q4LinearWs w(ws, M, N, K, true);
+  if (int rc = check_ws("q4_linear_bwd", ws, ws_bytes, w.bytes)) return rc;
+  if (!w.dy && ((uintptr_t)dy % 16 || ld % 8)) return set_error(USAF_ERR_INVALID, "q4_linear_bwd: rows must be 16-byte aligned");
+  hipStream_t st = as_stream(stream);
+  if (int rc = transpose(q, sz, N, K, K, dtype, w.w, w.np, st)) return rc;
+  if (w.dy)
+    if (int rc = pad(dy, M, N, ld, w.dy, w.np, st)) return rc;
+  return launch_linear_dense(product(w.dy ? w.dy : dy, w.dy ? w.np : ld, M, w.w, w.np, K, w.np, dx, K), dtype, false, st);
+}
+
+static int gated_args(const char* what, int32_t dtype, int64_t M, int64_t I, int64_t K, const uint8_t* q, const uint32_t* sz,
+                      const void* w16) {
+  if (!sizes_ok(M, 2 * I, K))
+    return set_error(USAF_ERR_INVALID, "%s: need M >= 0 and 1 <= 2 I, K <= %lld, got M=%lld I=%lld K=%lld", what, (long long)LIN_MAX,
+                     (long long)M, (long long)I, (long long)K);
+  if (!half_type(dtype)) return set_error(USAF_ERR_INVALID, "%s: dtype must be fp16 or bf16", what);
+  if (M == 0) return USAF_OK;
+  if ((q == nullptr) == (w16 == nullptr) || (q && !sz))
+    return set_error(USAF_ERR_INVALID, "%s: a 4-bit weight (codes and scales) or a 16-bit one", what);
+  if (((uintptr_t)q | (uintptr_t)w16) % 16 || (uintptr_t)sz % 4)
+    return set_error(USAF_ERR_INVALID, "%s: weights must be 16-byte, scales 4-byte aligned", what);
+  if (q && K % 128) return set_error(USAF_ERR_INVALID, "%s: a 4-bit weight's K must be a multiple of 128, got %lld", what, (long long)K);
+  if (q && (I + 256) * (K / 2) >= (int64_t)1 << 32)
+    return set_error(USAF_ERR_UNSUPPORTED, "%s: a gate of 4 GiB of codes", what);
+  return USAF_OK;
+}
+
+extern "C" int64_t usaf_hip_gated_ws_bytes(int64_t M, int64_t I, int64_t K, int32_t four_bit, int32_t what) {
+  return sizes_ok(M, 2 * I, K) && what >= 0 && what <= 3 ? GatedWs(nullptr, M, I, K, four_bit != 0, what).bytes : -1;
+}
+
+extern "C" int usaf_hip_gated_fwd(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* q,
+                                  const uint32_t* sz, const void* w16, int64_t I, void* act, void* kept, uint8_t* kept_scales,
+                                  void* ws, int64_t ws_bytes, void* stream) {
+  if (int rc = gated_args("gated_fwd", dtype, M, I, K, q, sz, w16)) return rc;
+  if (M == 0) return clear_error();
+  if (!x || !act || (kept_scales && !kept)) return set_error(USAF_ERR_INVALID, "gated_fwd: null pointer");
+  if (ld < K || ld > LIN_MAX) return set_error(USAF_ERR_INVALID, "gated_fwd: rows of %lld values, %lld apart", (long long)K, (long long)ld);
+  const GatedWs w(ws, M, I, K, q != nullptr, 0);
+  if ((uintptr_t)kept % 16 || (uintptr_t)act % 2 || (!w.x && ((uintptr_t)x % 16 || ld % 8)) || (uintptr_t)x % 2)
+    return set_error(USAF_ERR_INVALID, "gated_fwd: rows and what is kept must be 16-byte aligned");
+  if (int rc = check_ws("gated_fwd", ws, ws_bytes, w.bytes)) return rc;
+  hipStream_t st = as_stream(stream);
+  if (w.x)
+    if (int rc = pad(x, M, K, ld, w.x, w.kp, st)) return rc;
+  LinArgs g = product(w.x ? w.x : x, w.x ? w.kp : ld, M, w.w ? w.w : w16, w.kp, I, w.kp, act, I);
+  g.kept = kept;
+  g.kept_s = kept_scales;
+  g.hs = round_up(I, kept_scales ? 128 : 8);
+  if (q && !w.w) {
+    g.W = q;
+    g.ldw = K / 2;
+    g.sz = sz;
+    return launch_linear_q4(g, dtype, true, st);
+  }
+  if (q)
+    if (int rc = q4_rows(q, sz, 2 * I, K, dtype, w.w, st)) return rc;
+  if (!q && w.w)
+    if (int rc = pad(w16, 2 * I, K, K, w.w, w.kp, st)) return rc;
+  return launch_linear_dense(g, dtype, true, st);
+}
+
+extern "C" int usaf_hip_gated_bwd(const void* dact, int32_t dtype, int64_t M, int64_t I, int64_t K, const void* kept,
+                                  const uint8_t* kept_scales, const uint8_t* q, const uint32_t* sz, const void* w16,
+                                  const void* x, int64_t ldx, void* dx, void* dw, void* ws, int64_t ws_bytes, void* stream) {
+  if (int rc = gated_args("gated_bwd", dtype, M, I, K, q, sz, w16)) return rc;
+  if (M == 0) return clear_error();
+  if (!dact || !kept || (!dx && !dw) || (dw && !x)) return set_error(USAF_ERR_INVALID, "gated_bwd: null pointer");
+  if (dw && q) return set_error(USAF_ERR_INVALID, "gated_bwd: a 4-bit weight has no gradient");
+  if (dw && (ldx < K || M > LIN_MAX)) return set_error(USAF_ERR_INVALID, "gated_bwd: a weight gradient needs ldx >= K and M <= %lld", (long long)LIN_MAX);
+  if ((uintptr_t)kept % 16 || ((uintptr_t)dact | (uintptr_t)x | (uintptr_t)dx | (uintptr_t)dw) % 2)
+    return set_error(USAF_ERR_INVALID, "gated_bwd: what is kept must be 16-byte, rows 2-byte aligned");
+  const GatedWs w(ws, M, I, K, q != nullptr, (dx ? 1 : 0) | (dw ? 2 : 0));
+  if (int rc = check_ws("gated_bwd", ws, ws_bytes, w.bytes)) return rc;
+  hipStream_t st = as_stream(stream);
+  const int64_t hs = round_up(I, kept_scales ? 128 : 8), items = M * ((I + 7) / 8);
+  const bool vec = I % 8 == 0 && (uintptr_t)dact % 16 == 0;
+#define USAF_GATED_BWD(DT, EIGHT)                                                                                          \
+  gated_bwd_kernel<DT, EIGHT><<<blocks_of(items, 1), 256, 0, st>>>((const uint16_t*)dact, kept, kept_scales, M, I, hs, vec, \
+                                                                   (uint16_t*)w.dgu, w.ldd)
+  if (dtype == USAF_BF16) {
+    if (kept_scales) USAF_GATED_BWD(USAF_BF16, true);
+    else USAF_GATED_BWD(USAF_BF16, false);
+  } else {
+    if (kept_scales) USAF_GATED_BWD(USAF_F16, true);
+    else USAF_GATED_BWD(USAF_F16, false);
+  }
+#undef USAF_GATED_BWD
+  if (int rc = check_launch("gated_bwd")) return rc;
+  if (dx) {
+    if (int rc = transpose(q ? (const void*)q : w16, q ? sz : nullptr, 2 * I, K, K, dtype, w.wt, w.ldd, st)) return rc;
+    if (int rc = launch_linear_dense(product(w.dgu, w.ldd, M, w.wt, w.ldd, K, w.ldd, dx, K), dtype, false, st)) return rc;
+  }
+  if (dw) {
+    if (int rc = transpose(w.dgu, nullptr, M, 2 * I, w.ldd, dtype, w.dgut, w.mp, st)) return rc;
+    if (int rc = transpose(x, nullptr, M, K, ldx, dtype, w.xt, w.mp, st)) return rc;
+    return launch_linear_dense(product(w.dgut, w.mp, 2 * I, w.xt, w.mp, K, w.mp, dw, K), dtype, false, st);
+  }
+  return clear_error();
+}

@@ -1,6 +1,7 @@
 // Library-wide state: per-thread error text, ABI version, device queries.
 #include "common.h"
 #include "fp8.h"
+#include "linear.h"
 
 #include <stdio.h>
 #include <string.h>
@@ -55,6 +56,7 @@ extern "C" int usaf_hip_init(void) {
   usaf::prepare_gemm_kernels();
   usaf::prepare_sparse_kernels();
   usaf::prepare_fp8_kernels();
+  usaf::prepare_linear_kernels();
   if (int rc = usaf::prepare_noalloc_scratch()) return rc;
   return usaf::clear_error();
 }

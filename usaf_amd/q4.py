@@ -1,0 +1,121 @@
+"""The product with one 4-bit weight.
+
+``q4_linear`` is ``F.linear`` with a ``moe.Q4Tensor`` of shape [N, K], as
+``quantize_4bit`` makes it (group size 128 along whole rows), beside ``fp8.fp8_linear``:
+a projection or an output head that stays 4-bit in memory, for one token or a
+prompt, differentiable in the activations.  A weight's value is everywhere the
+codec's in the activations' dtype, ``w.dequantize(x.dtype)`` bit for bit
+(fp16(code * scale) + zero in fp16, usaf/quantization.py:88-132, then bf16 where
+the activations are), so decoding, prompts and gradients multiply the same numbers.
+"""
+from __future__ import annotations
+
+import functools
+
+import torch
+
+from . import _native as N
+from .fp8 import on
+from .moe import Q4Tensor
+
+ACT = (torch.float16, torch.bfloat16)
+MAX_COLS = 1 << 22
+
+
+@functools.lru_cache(maxsize=4096)
+def _ws_bytes(m: int, n: int, k: int, backward: int) -> int:
+    return N.load().usaf_hip_q4_linear_ws_bytes(m, n, k, backward)
+
+
+def check_weight(what: str, w: Q4Tensor) -> None:
+    """Raise unless w is a 4-bit matrix in the layout that the products read."""
+    if len(w.shape) != 2 or any(int(d) < 1 for d in w.shape):
+        raise ValueError(f"{what}: need a 4-bit weight [rows, K], got {tuple(w.shape)}")
+    rows, k = (int(d) for d in w.shape)
+    if w.group_size != 128 or k % 128:
+        raise NotImplementedError(f"{what}: needs group size 128 along whole rows (K a multiple of 128), got {tuple(w.shape)}, "
+                                  f"group size {w.group_size}; dequantize() takes any")
+    groups = rows * k // 128
+    if tuple(w.q.shape) != (groups, 64) or w.s.numel() != groups or w.z.numel() != groups:
+        raise ValueError(f"{what}: codes {tuple(w.q.shape)}, scales {tuple(w.s.shape)} and zeros {tuple(w.z.shape)} do not fit "
+                         f"{tuple(w.shape)}: need {(groups, 64)} and {groups} each")
+    if w.q.element_size() != 1 or w.s.dtype != torch.float16 or w.z.dtype != torch.float16:
+        raise TypeError(f"{what}: codes are bytes, scales and zeros fp16, got {w.q.dtype}, {w.s.dtype}, {w.z.dtype}")
+    if not (w.q.is_contiguous() and w.s.is_contiguous() and w.z.is_contiguous()) or w.q.data_ptr() % 16 \
+            or w.s.device != w.q.device or w.z.device != w.q.device:
+        raise ValueError(f"{what}: codes, scales and zeros must be contiguous, on one device, the codes 16-byte aligned")
+
+
+def words(what: str, w: Q4Tensor) -> torch.Tensor:
+    """w.scale_zero(), finished when first built, so that any stream may read it from then on."""
+    if w._sz is None or w._sz.device != w.device:
+        N.refuse_capture(f"{what}: the first call on a weight")
+        with on(w.device):
+            w.scale_zero()
+            torch.cuda.current_stream(w.device).synchronize()
+    return w._sz
+
+
+def rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """t as rows [M, cols] that start at multiples of 16 bytes, without a copy where they do."""
+    t = t if t.dim() == 2 else t.reshape(t.numel() // cols, cols)
+    if t.stride(1) != 1 or (t.shape[0] > 1 and not (cols <= t.stride(0) <= MAX_COLS and t.stride(0) % 8 == 0)):
+        t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
+
+
+class Q4LinearFn(torch.autograd.Function):
+    """y = x W^T; dx = dy W."""
+
+    @staticmethod
+    def forward(ctx, x: torch.Tensor, w: Q4Tensor):
+        ctx.w, ctx.dtype = w, x.dtype
+        return _linear(x, w)
+
+    @staticmethod
+    def backward(ctx, dy: torch.Tensor):
+        if torch.is_grad_enabled():
+            raise RuntimeError("q4_linear has no second derivative (create_graph=True)")
+        N.refuse_capture("q4_linear's backward")
+        return _linear(dy if dy.dtype == ctx.dtype else dy.to(ctx.dtype), ctx.w, backward=True), None
+
+
+def _linear(x: torch.Tensor, w: Q4Tensor, backward: bool = False) -> torch.Tensor:
+    n, k = (int(d) for d in w.shape)
+    dev, (cols, out_cols) = x.device, (n, k) if backward else (k, n)
+    rows = rows_of(x, cols)
+    m = rows.shape[0]
+    out = torch.empty(m, out_cols, dtype=x.dtype, device=dev)
+    if m:
+        need, sz = _ws_bytes(m, n, k, int(backward)), words("q4_linear", w)
+        with on(dev):
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+            name, size = ("usaf_hip_q4_linear_bwd", k) if backward else ("usaf_hip_q4_linear", n)
+            N.call(name, rows.data_ptr(), N.dtype_code(x.dtype), m, cols, _ld(rows), w.q.data_ptr(), sz.data_ptr(), size,
+                   out.data_ptr(), N.ptr(ws), max(need, 0), N.stream_ptr(dev))
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], out_cols)
+
+
+def q4_linear(x: torch.Tensor, w: Q4Tensor) -> torch.Tensor:
+    """F.linear with a 4-bit weight: x [..., K] fp16 / bf16, w [N, K] -> [..., N] in x's
+    dtype, summed in fp32 and rounded once.  Differentiable in x (the weight is
+    frozen).  The first call on a weight builds its scale words (1/17 of it), not in
+    a stream capture; a capture takes calls without a gradient only.  There is no
+    forward-mode derivative; torch.jit.trace records the call.  The weight is not
+    written to once used, and kept until the work that reads it has ended."""
+    check_weight("q4_linear", w)
+    if x.dtype not in ACT:
+        raise TypeError(f"q4_linear: activations must be fp16 or bf16, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"q4_linear: activations {tuple(x.shape)} do not fit the weight {tuple(w.shape)}")
+    if x.device != w.device or not x.is_cuda:
+        raise ValueError(f"q4_linear: activations on {x.device}, weight on {w.device}: both on one GPU")
+    if torch.is_grad_enabled() and x.requires_grad:
+        N.refuse_capture("q4_linear of activations that want a gradient")
+        return Q4LinearFn.apply(x, w)
+    # (the function's own call takes 2 us of the host's time)
+    return Q4LinearFn.apply(x, w) if N.followed(x) else _linear(x, w)
