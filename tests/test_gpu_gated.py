@@ -10,7 +10,8 @@ pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16]
 # tokens, intermediate, hidden: one row to many, columns that fill no 8, no 16, no 128
 Q4_SIZES = [(1, 1, 128), (1, 128, 256), (2, 5, 128), (9, 130, 384), (31, 257, 640), (33, 128, 256), (64, 96, 384), (65, 711, 256),
-            (130, 255, 512), (300, 384, 512), (511, 40, 256), (513, 300, 896), (1030, 264, 384)]
+            (130, 255, 512), (300, 384, 512), (511, 40, 256), (513, 300, 896), (1030, 264, 384),
+            (8, 33, 4096), (16, 300, 2048), (1, 40, 14336), (5, 1000, 1920), (1, 9000, 256)]
 DENSE_SIZES = [(1, 1, 1), (1, 128, 64), (2, 5, 127), (9, 130, 129), (31, 257, 640), (33, 128, 100), (65, 711, 200),
                (130, 255, 512), (300, 384, 512), (257, 70, 1000), (600, 520, 192)]
 
@@ -99,10 +100,8 @@ def test_4bit_weights(G, m, inter, k, dtype, checkpoint):
     act = _check(G, x, w, w64, checkpoint, dtype, _rand(m, inter, dtype=dtype, seed=2))
     with torch.no_grad():
         plain = G.gated_linear(x, w, checkpoint=checkpoint)
-    # (a pass that keeps 8-bit blocks takes tiles of whole blocks, whose sums may come in another order than without: both
-    # are within the sums' bound)
+    # (a pass without a gradient may take other tiles, whose sums come in another order: both are within the sums' bound)
     O.within(plain, *(lambda r, o: (r, O.rounded(r, o, dtype)))(*O.gated(x.detach().double().cpu(), w64)[2]), "without a gradient")
-    assert checkpoint is not None or torch.equal(plain, act)
 
 
 @pytest.mark.parametrize("checkpoint", [None, "fp8"])

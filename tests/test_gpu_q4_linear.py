@@ -11,7 +11,8 @@ DTYPES = [torch.bfloat16, torch.float16]
 # one row to many, every kind of tile's border; both sides of the sizes at which the weight is multiplied as codes
 SIZES = [(1, 1, 128), (1, 64, 256), (2, 5, 128), (3, 4096, 2048), (7, 130, 384), (16, 48, 4096), (17, 33, 512), (31, 257, 640),
          (32, 96, 1024), (33, 128, 256), (64, 96, 384), (65, 1411, 256), (100, 520, 2944), (129, 255, 1024), (300, 384, 512),
-         (257, 640, 1920), (511, 96, 256), (512, 130, 128), (513, 300, 896), (1030, 530, 384), (2049, 64, 128)]
+         (257, 640, 1920), (511, 96, 256), (512, 130, 128), (513, 300, 896), (1030, 530, 384), (2049, 64, 128),
+         (8, 33, 4096), (16, 300, 2048), (1, 40, 14336), (5, 1000, 1920), (1, 9000, 256), (100, 64, 14336), (700, 192, 8192)]
 
 
 def _ids(d):

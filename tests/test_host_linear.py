@@ -74,8 +74,8 @@ def test_entry_points_check_their_arguments():
     assert linear(m=0, x=None, q=None, sz=None, out=None, ws=None, size=0) == ok
     for bad in [dict(m=-1), dict(m=1 << 31), dict(cols=0), dict(cols=100), dict(cols=1 << 23), dict(other=0), dict(other=1 << 23),
                 dict(dtype=N.F32), dict(x=None), dict(q=None), dict(sz=None), dict(out=None), dict(ld=255), dict(ld=1 << 23),
-                dict(ld=257), dict(q=even), dict(sz=even), dict(x=even), dict(out=odd), dict(m=4096, ws=None),
-                dict(m=4096, size=100), dict(m=4096, ws=even)]:
+                dict(ld=257), dict(q=even), dict(sz=even), dict(x=even), dict(out=odd), dict(m=4096, other=4096, ws=None),
+                dict(m=4096, other=4096, size=100), dict(m=4096, other=4096, ws=even)]:
         assert linear(**bad) == inval, bad
     assert "q4_linear" in N.last_error()
     back = dict(name="usaf_hip_q4_linear_bwd", cols=64, ld=64, other=256)
@@ -91,7 +91,7 @@ def test_entry_points_check_their_arguments():
                 dict(w16=p), dict(sz=None), dict(q=even), dict(sz=even), dict(q=None, sz=None, w16=even), dict(x=None),
                 dict(act=None), dict(act=odd), dict(x=even), dict(ld=200), dict(ld=260), dict(scales=p), dict(kept=even),
                 dict(q=None, sz=None, w16=p, k=100, ld=100, ws=None), dict(q=None, sz=None, w16=p, k=100, ld=100, size=64),
-                dict(m=4096, ws=even)]:
+                dict(m=4096, inter=4096, ws=even)]:
         assert fwd(**bad) == inval, bad
     assert fwd(inter=1 << 20, k=1 << 14, ld=1 << 14) == unsup
 

@@ -22,10 +22,25 @@ struct LinArgs {
   uint8_t* kept_s;     // scale bytes [M, 2, hs / 128] of codes; nullptr: 16-bit values
   int64_t hs;
   int n_nt;            // set at the launch
+  // not gated: the contraction in parts, each part's fp32 sums [parts, M, ldp] to part instead of out
+  int parts = 1;
+  float* part = nullptr;
+  int64_t ldp = 0;     // N in whole 4
 };
 
-int launch_linear_dense(const LinArgs& g, int dt, bool gated, hipStream_t st);
-int launch_linear_q4(const LinArgs& g, int dt, bool gated, hipStream_t st);
+// The tile for a product of these sizes, how many parts its contraction is taken in, and about how many cycles of a CU it
+// takes.
+struct LinPlan {
+  int (*launch)(const LinArgs&, int dt, bool gated, hipStream_t) = nullptr;
+  int parts = 1;
+  double cycles = 0;
+};
+LinPlan plan_linear_dense(const LinArgs& g, int dt, bool gated);
+LinPlan plan_linear_q4(const LinArgs& g, int dt, bool gated);
+// A few rows of a 4-bit weight's product, out [M, N] (ldo = N), nothing kept: whether it takes them, and its launch (q4_small.hip).
+bool q4_small_ok(int64_t M, int64_t K);
+int q4_small(const LinArgs& g, int dt, bool gated, hipStream_t st);
+void prepare_q4_small();
 void prepare_linear_dense();
 void prepare_linear_q4();
 // Raises the products' dynamic-LDS limits, once per process (usaf_hip_init, or their first use).

@@ -138,6 +138,28 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(const uint16_t* __restri
   }
 }
 
+// out[m, n] = dt( sum over parts of part[p, m, n] ): 4 columns a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int parts, int64_t M, int64_t N, int64_t ldp,
+                                                   bool vec, uint16_t* __restrict__ out, int64_t ldo) {
+  const int64_t chunks = ldp / 4, n = M * chunks, stride = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+    const int64_t m = i / chunks, c = 4 * (i - m * chunks);
+    f32x4 v = *reinterpret_cast<const f32x4*>(part + m * ldp + c);
+#pragma unroll 4
+    for (int p = 1; p < parts; ++p) v += *reinterpret_cast<const f32x4*>(part + (p * M + m) * ldp + c);
+    uint16_t* const to = out + m * ldo + c;
+    const uint2 w = {pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w)};
+    if (vec) {  // N % 4 == 0
+      *reinterpret_cast<uint2*>(to) = w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < N) to[j] = (uint16_t)((j < 2 ? w.x : w.y) >> (16 * (j & 1)));
+    }
+  }
+}
+
 unsigned blocks_of(int64_t items, int per) {
   const int64_t b = (items + 256 * per - 1) / (256 * per);
   return (unsigned)(b < 1 ? 1 : b > 65536 ? 65536 : b);
@@ -184,8 +206,13 @@ LinArgs product(const void* a, int64_t lda, int64_t M, const void* w, int64_t ld
   return g;
 }
 
-// Whether the 4-bit weight is multiplied as codes; else its 16-bit values are written once, to the workspace, and multiplied.
-bool as_codes(int64_t M) { return M <= 512; }
+// Whether a 4-bit weight of `rows` rows is multiplied as codes; else its 16-bit values are written once, to the workspace, and
+// multiplied: 2.5 bytes a weight at about 4 TB/s, and a launch.
+bool as_codes(int64_t M, int64_t rows, int64_t K, bool gated) {
+  const LinArgs g = product(nullptr, K, M, nullptr, K, gated ? rows / 2 : rows, K, nullptr, 0);
+  return plan_linear_q4(g, USAF_BF16, gated).cycles <=
+         plan_linear_dense(g, USAF_BF16, gated).cycles + (double)rows * (double)K * 2.5 / 2000 + 6000;
+}
 
 // Pieces of a workspace, each a whole number of 256 bytes.
 struct Ws {
@@ -199,6 +226,35 @@ struct Ws {
   }
 };
 
+// A product's place for the sums of its parts.  q4: of codes.
+struct Parts {
+  LinPlan plan;
+  void* at;
+  int64_t ldp;
+  Parts() = default;
+  Parts(Ws& ws, int64_t M, int64_t N, int64_t K, bool q4) {
+    const LinArgs g = product(nullptr, K, M, nullptr, K, N, K, nullptr, N);
+    plan = q4 ? plan_linear_q4(g, USAF_BF16, false) : plan_linear_dense(g, USAF_BF16, false);
+    ldp = round_up(N, 4);
+    at = plan.parts > 1 ? ws.take(4 * plan.parts * M * ldp) : nullptr;
+  }
+};
+
+int run(LinArgs g, const Parts& p, int dt, hipStream_t st) {
+  g.parts = p.plan.parts;
+  g.part = reinterpret_cast<float*>(p.at);
+  g.ldp = p.ldp;
+  if (int rc = p.plan.launch(g, dt, false, st)) return rc;
+  if (g.parts == 1) return clear_error();
+  const int64_t items = g.M * (g.ldp / 4);
+  const bool vec = g.N % 4 == 0 && g.ldo % 4 == 0 && (uintptr_t)g.out % 8 == 0;
+  if (dt == USAF_BF16)
+    join_kernel<USAF_BF16><<<blocks_of(items, 1), 256, 0, st>>>(g.part, g.parts, g.M, g.N, g.ldp, vec, g.out, g.ldo);
+  else
+    join_kernel<USAF_F16><<<blocks_of(items, 1), 256, 0, st>>>(g.part, g.parts, g.M, g.N, g.ldp, vec, g.out, g.ldo);
+  return check_launch("linear: sums of the parts");
+}
+
 bool sizes_ok(int64_t M, int64_t N, int64_t K) {
   return M >= 0 && M <= 0x7FFFFFFF && N >= 1 && N <= LIN_MAX && K >= 1 && K <= LIN_MAX;
 }
@@ -206,15 +262,20 @@ bool half_type(int32_t dt) { return dt == USAF_BF16 || dt == USAF_F16; }
 
 struct Q4LinearWs {
   void *w = nullptr, *dy = nullptr;
+  Parts parts;
+  bool codes;
   int64_t bytes, np;
   Q4LinearWs(void* ws, int64_t M, int64_t N, int64_t K, bool backward) {
     Ws at(ws);
     np = round_up(N, 64);
+    codes = !backward && as_codes(M, N, K, false);
     if (backward) {
       w = at.take(2 * K * np);
       if (np != N) dy = at.take(2 * M * np);
-    } else if (!as_codes(M)) {
-      w = at.take(2 * N * K);
+      parts = Parts(at, M, K, np, false);
+    } else if (!q4_small_ok(M, K)) {
+      if (!codes) w = at.take(2 * N * K);
+      parts = Parts(at, M, N, K, codes);
     }
     bytes = at.used;
   }
@@ -223,6 +284,8 @@ struct Q4LinearWs {
 struct GatedWs {
   void *w = nullptr, *x = nullptr;                                  // forward: 16-bit or padded weight, padded x
   void *dgu = nullptr, *wt = nullptr, *dgut = nullptr, *xt = nullptr;  // backward
+  Parts dx_parts, dw_parts;
+  bool codes = false;
   int64_t bytes, kp, ldd, mp;
   GatedWs(void* ws, int64_t M, int64_t I, int64_t K, bool four_bit, int what) {
     Ws at(ws);
@@ -230,14 +293,19 @@ struct GatedWs {
     ldd = round_up(2 * I, 64);
     mp = round_up(M, 64);
     if (what == 0) {
-      if (four_bit ? !as_codes(M) : kp != K) w = at.take(2 * 2 * I * kp);
+      codes = four_bit && (q4_small_ok(M, K) || as_codes(M, 2 * I, K, true));
+      if (four_bit ? !codes : kp != K) w = at.take(2 * 2 * I * kp);
       if (kp != K) x = at.take(2 * M * kp);
     } else {
       dgu = at.take(2 * M * ldd);
-      if (what & 1) wt = at.take(2 * K * ldd);
+      if (what & 1) {
+        wt = at.take(2 * K * ldd);
+        dx_parts = Parts(at, M, K, ldd, false);
+      }
       if (what & 2) {
         dgut = at.take(2 * 2 * I * mp);
         xt = at.take(2 * K * mp);
+        dw_parts = Parts(at, 2 * I, K, mp, false);
       }
     }
     bytes = at.used;
@@ -256,6 +324,7 @@ int check_ws(const char* what, const void* ws, int64_t have, int64_t need) {
 void prepare_linear_kernels() {
   prepare_linear_dense();
   prepare_linear_q4();
+  prepare_q4_small();
 }
 
 }  // namespace usaf
@@ -288,14 +357,15 @@ extern "C" int usaf_hip_q4_linear(const void* x, int32_t dtype, int64_t M, int64
   const Q4LinearWs w(ws, M, N, K, false);
   if (int rc = check_ws("q4_linear", ws, ws_bytes, w.bytes)) return rc;
   hipStream_t st = as_stream(stream);
-  if (as_codes(M)) {
+  if (w.codes || q4_small_ok(M, K)) {
     LinArgs g = product(x, ld, M, q, 0, N, K, out, N);
     g.ldw = K / 2;
     g.sz = sz;
-    return launch_linear_q4(g, dtype, false, st);
+    if (q4_small_ok(M, K)) return q4_small(g, dtype, false, st);
+    return run(g, w.parts, dtype, st);
   }
   if (int rc = q4_rows(q, sz, N, K, dtype, w.w, st)) return rc;
-  return launch_linear_dense(product(x, ld, M, w.w, K, N, K, out, N), dtype, false, st);
+  return run(product(x, ld, M, w.w, K, N, K, out, N), w.parts, dtype, st);
 }
 
 extern "C" int usaf_hip_q4_linear_bwd(const void* dy, int32_t dtype, int64_t M, int64_t N, int64_t ld, const uint8_t* q,
@@ -309,7 +379,7 @@ extern "C" int usaf_hip_q4_linear_bwd(const void* dy, int32_t dtype, int64_t M, 
   if (int rc = transpose(q, sz, N, K, K, dtype, w.w, w.np, st)) return rc;
   if (w.dy)
     if (int rc = pad(dy, M, N, ld, w.dy, w.np, st)) return rc;
-  return launch_linear_dense(product(w.dy ? w.dy : dy, w.dy ? w.np : ld, M, w.w, w.np, K, w.np, dx, K), dtype, false, st);
+  return run(product(w.dy ? w.dy : dy, w.dy ? w.np : ld, M, w.w, w.np, K, w.np, dx, K), w.parts, dtype, st);
 }
 
 static int gated_args(const char* what, int32_t dtype, int64_t M, int64_t I, int64_t K, const uint8_t* q, const uint32_t* sz,
@@ -355,13 +425,14 @@ extern "C" int usaf_hip_gated_fwd(const void* x, int32_t dtype, int64_t M, int64
     g.W = q;
     g.ldw = K / 2;
     g.sz = sz;
-    return launch_linear_q4(g, dtype, true, st);
+    if (!kept && q4_small_ok(M, K)) return q4_small(g, dtype, true, st);
+    return plan_linear_q4(g, dtype, true).launch(g, dtype, true, st);
   }
   if (q)
     if (int rc = q4_rows(q, sz, 2 * I, K, dtype, w.w, st)) return rc;
   if (!q && w.w)
     if (int rc = pad(w16, 2 * I, K, K, w.w, w.kp, st)) return rc;
-  return launch_linear_dense(g, dtype, true, st);
+  return plan_linear_dense(g, dtype, true).launch(g, dtype, true, st);
 }
 
 extern "C" int usaf_hip_gated_bwd(const void* dact, int32_t dtype, int64_t M, int64_t I, int64_t K, const void* kept,
@@ -393,12 +464,12 @@ extern "C" int usaf_hip_gated_bwd(const void* dact, int32_t dtype, int64_t M, in
   if (int rc = check_launch("gated_bwd")) return rc;
   if (dx) {
     if (int rc = transpose(q ? (const void*)q : w16, q ? sz : nullptr, 2 * I, K, K, dtype, w.wt, w.ldd, st)) return rc;
-    if (int rc = launch_linear_dense(product(w.dgu, w.ldd, M, w.wt, w.ldd, K, w.ldd, dx, K), dtype, false, st)) return rc;
+    if (int rc = run(product(w.dgu, w.ldd, M, w.wt, w.ldd, K, w.ldd, dx, K), w.dx_parts, dtype, st)) return rc;
   }
   if (dw) {
     if (int rc = transpose(w.dgu, nullptr, M, 2 * I, w.ldd, dtype, w.dgut, w.mp, st)) return rc;
     if (int rc = transpose(x, nullptr, M, K, ldx, dtype, w.xt, w.mp, st)) return rc;
-    return launch_linear_dense(product(w.dgut, w.mp, 2 * I, w.xt, w.mp, K, w.mp, dw, K), dtype, false, st);
+    return run(product(w.dgut, w.mp, 2 * I, w.xt, w.mp, K, w.mp, dw, K), w.dw_parts, dtype, st);
   }
   return clear_error();
 }

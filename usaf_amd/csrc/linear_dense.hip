@@ -3,7 +3,7 @@
 
 namespace usaf {
 namespace {
-typedef LinShape<2, 4, 4, 2, false> D256x256;
+typedef LinShape<2, 4, 4, 2, false, true> D256x256;
 typedef LinShape<2, 4, 2, 2, false> D128x256;
 typedef LinShape<2, 4, 2, 1, false> D128x128;
 typedef LinShape<2, 4, 1, 1, false> D64x128;
@@ -12,16 +12,16 @@ typedef LinShape<1, 8, 1, 1, false> D32x256;
 typedef LinShape<1, 2, 1, 1, false> D32x64;
 }  // namespace
 
-int launch_linear_dense(const LinArgs& g, int dt, bool gated, hipStream_t st) {
-  LinChoice best;
-  best.consider<D256x256>(g, dt, gated);
-  best.consider<D128x256>(g, dt, gated);
-  best.consider<D128x128>(g, dt, gated);
-  best.consider<D64x128>(g, dt, gated);
-  best.consider<D64x64>(g, dt, gated);
-  best.consider<D32x256>(g, dt, gated);
-  best.consider<D32x64>(g, dt, gated);
-  return best.launch(g, dt, gated, st);
+LinPlan plan_linear_dense(const LinArgs& g, int dt, bool gated) {
+  LinPlan best;
+  consider<D256x256>(best, g, dt, gated);
+  consider<D128x256>(best, g, dt, gated);
+  consider<D128x128>(best, g, dt, gated);
+  consider<D64x128>(best, g, dt, gated);
+  consider<D64x64>(best, g, dt, gated);
+  consider<D32x256>(best, g, dt, gated);
+  consider<D32x64>(best, g, dt, gated);
+  return best;
 }
 
 void prepare_linear_dense() {

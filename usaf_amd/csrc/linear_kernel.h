@@ -7,11 +7,13 @@
 // accumulator holds 4 consecutive columns of one slot.  Gated tiles take 16 rows of the gate and the same 16 of up into
 // each 32 x 32 block: values v and v + 8 of a lane are then a column's gate and up.
 //
-// A block of eight waves has tiles of 32 MW MI slots x 32 NW NI weight rows; KW of its waves split the
+// A block of eight or four waves has tiles of 32 MW MI slots x 32 NW NI weight rows; KW of its waves split the
 // contraction's blocks of 64.  Blocks stay (one a CU) and walk a die's run of the tile list.  Both operands come by LDS
-// DMA into a ring of NS stages; at a step's one barrier its stage has landed and the stage before it has been read, so
-// the DMAs of the step NS - 1 ahead go there, straight across tile ends.  16-byte chunks are XOR-swizzled by the
-// row (by the DMA's source address), which spreads the fragment reads over the banks.
+// DMA, 128-byte lines, into a ring of NS stages, straight across tile ends.  16-byte chunks are XOR-swizzled by the row
+// (by the DMA's source address), which spreads the fragment reads over the banks.  A step has four slices, 16 of the
+// contraction for each half of the lanes; a slice's fragments are read while the one before it is multiplied, the first
+// of the next step's behind the step's one barrier, in front of its last slice: there the next stage has landed and this
+// one has been read, so its next lines are sent for.
 //
 // 4-bit weights (MW = 1: a weight row's codes belong to one wave) are dequantized as they come out of LDS, into the
 // matrix instruction's operand registers: dt(fp16(fp16(q s) + z)), the codec's value bit for bit.
@@ -21,43 +23,45 @@
 #include "fp8.h"
 #include "linear.h"
 
+#include <type_traits>
+
 namespace usaf {
 namespace {
 
-constexpr int L_WAVES = 8, L_THREADS = 64 * L_WAVES;
 constexpr int L_XCDS = 8;  // accelerator dies, blocks dispatched round-robin over them
 
 enum { LIN_STORE = 0, LIN_GATED = 1, LIN_CK8 = 2 };
 
-template <int MW, int NW, int MI, int NI, bool Q4, int EPI>
+template <int WAVES, int MW, int NW, int MI, int NI, bool Q4, int EPI>
 struct LinTile {
-  static constexpr int KW = L_WAVES / (MW * NW), NB = NW * NI;
+  static constexpr int KW = WAVES / (MW * NW), NB = NW * NI;
   static constexpr int M = 32 * MW * MI, N = 32 * NB;
   static constexpr int COLS = EPI == LIN_STORE ? N : N / 2;          // columns of out
   static constexpr int W_ROW = Q4 ? 32 : 128;                        // bytes of a weight row's 64 values
   static constexpr int A_BYTES = M * 128, W_BYTES = N * W_ROW;
   static constexpr int S_WORDS = Q4 ? (N + 63) / 64 : 0;             // instructions of 64 scale words
   static constexpr int SLAB = A_BYTES + W_BYTES + 256 * S_WORDS, STAGE = KW * SLAB;
-  // the results' way out: partial sums of KW waves, then 32 MW slots' rows of out and of what is kept
-  static constexpr int RED = KW > 1 ? L_WAVES * NI * 16 * 64 * 4 : 0;
+  // the results' way out: partial sums of KW waves, then 32 EW slots' rows of out and of what is kept
+  static constexpr int RED = KW > 1 ? WAVES * NI * 16 * 64 * 4 : 0;
   static constexpr int OUT_ROW = 2 * COLS, KEPT_ROW = EPI == LIN_GATED ? 2 * N : EPI == LIN_CK8 ? N : 0;
-  static constexpr int MAXIMA = EPI == LIN_CK8 ? 32 * MW * 2 * NW * 4 : 0;
-  static constexpr int ENDS = RED + 32 * MW * (OUT_ROW + KEPT_ROW) + MAXIMA;
-  static constexpr bool IN_STAGE = ENDS <= STAGE;                    // ENDS goes through the stage read last, or has its own place
-  static constexpr int FIT = (160 * 1024 - (IN_STAGE ? 0 : ENDS)) / STAGE, NS = FIT > 4 ? 4 : FIT;
-  static constexpr int LDS = NS * STAGE + (IN_STAGE ? 0 : ENDS);
+  static constexpr int SLOT_ENDS = OUT_ROW + KEPT_ROW;
+  static constexpr int EW = KW > 1 || 32 * MW * SLOT_ENDS <= 32 * 1024 ? MW : 1, ER = 32 * EW;
+  static constexpr int ENDS = RED + ER * SLOT_ENDS;
+    static constexpr int FIT = (160 * 1024 - ENDS) / STAGE, NS = FIT > 4 ? 4 : FIT;
+  static constexpr int LDS = NS * STAGE + ENDS;
   // DMA instructions of a wave and step: the rows of its own k-block, shared by the MW NW waves that have it
   static constexpr int SHARE = MW * NW;
   static constexpr int W_RPI = 1024 / W_ROW;                         // weight rows of an instruction
   static constexpr int A_DMA = (M / 8 + SHARE - 1) / SHARE, W_DMA = (N / W_RPI + SHARE - 1) / SHARE;
   static constexpr int S_DMA = Q4 ? (S_WORDS + SHARE - 1) / SHARE : 0, DMAS = A_DMA + W_DMA + S_DMA;
-  static_assert(NS >= 2 && MW * NW * KW == L_WAVES && (!Q4 || MW == 1), "tile");
-  static_assert(EPI != LIN_CK8 || (N == 256 && KW == 1), "a tile has whole blocks of 128 columns");
+  static_assert(NS >= 2 && MW * NW * KW == WAVES && (!Q4 || MW == 1), "tile");
+  static_assert(EPI != LIN_CK8 || (N == 256 && KW == 1 && EW == MW), "a tile has whole blocks of 128 columns");
 };
 
-template <int MW, int NW, int MI, int NI, int DT, bool Q4, int EPI>
-__global__ __launch_bounds__(L_THREADS) void linear_kernel(const LinArgs g) {
-  typedef LinTile<MW, NW, MI, NI, Q4, EPI> T;
+template <int WAVES, int MW, int NW, int MI, int NI, int DT, bool Q4, int EPI>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const LinArgs g) {
+  typedef LinTile<WAVES, MW, NW, MI, NI, Q4, EPI> T;
+  constexpr int THREADS = 64 * WAVES;
   constexpr int KW = T::KW, NB = T::NB;
   constexpr bool GATED = EPI != LIN_STORE;
   extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
@@ -69,17 +73,22 @@ __global__ __launch_bounds__(L_THREADS) void linear_kernel(const LinArgs g) {
   // ---- the block's tiles: its die's run of the list, every blocks-of-a-die-th; what a die's blocks share at a
   //      time, eight slot tiles of one weight tile, sits in its L2
   const int m_tiles = (int)((g.M + T::M - 1) / T::M);
-  const int tiles = m_tiles * g.n_nt, per = (tiles + L_XCDS - 1) / L_XCDS, stride = (int)gridDim.x / L_XCDS;
-  const int xcd = (int)blockIdx.x % L_XCDS, run = xcd * per;
-  const int end = run + per < tiles ? run + per : tiles, id0 = run + (int)blockIdx.x / L_XCDS;
+  const int tiles = m_tiles * g.n_nt, units = tiles * g.parts;  // a part of the contraction after the other
+  const int per = (units + L_XCDS - 1) / L_XCDS, stride = (int)gridDim.x / L_XCDS, xcd = (int)blockIdx.x % L_XCDS;
+  const int run = xcd * per, end = run + per < units ? run + per : units, id0 = run + (int)blockIdx.x / L_XCDS;
   if (id0 >= end) return;  // block-uniform
   struct Place {
-    int valid, nt;
+    int valid, nt, part, s_beg, s_end;
     int64_t m_beg;
   };
-  auto place = [&](int id) {
+  const int nkb = (int)(g.K / 64), all_steps = (nkb + KW - 1) / KW, groups = (int)(g.K / 128);
+  auto place = [&](int unit) {
     constexpr int GROUP = 8;
     Place t;
+    t.part = g.parts > 1 ? unit / tiles : 0;
+    t.s_beg = all_steps * t.part / g.parts;
+    t.s_end = all_steps * (t.part + 1) / g.parts;
+    const int id = unit - t.part * tiles;
     const int band = id / (GROUP * g.n_nt), rest = id - band * GROUP * g.n_nt;
     const int tall = m_tiles - band * GROUP < GROUP ? m_tiles - band * GROUP : GROUP;
     t.nt = rest / tall;
@@ -87,18 +96,19 @@ __global__ __launch_bounds__(L_THREADS) void linear_kernel(const LinArgs g) {
     t.valid = g.M - t.m_beg < T::M ? (int)(g.M - t.m_beg) : T::M;
     return t;
   };
-  const int nkb = (int)(g.K / 64), steps = (nkb + KW - 1) / KW, groups = (int)(g.K / 128);
   const int64_t up_rows = GATED ? g.N : 0;
 
   // ---- the DMA stream: uniform bases, 32-bit lane offsets.  Instruction i of wave `part` fills rows
   //      (SHARE i + part) of 8 (4-bit: 32) of the k-block; lane l of 128-byte rows chunk l % 8 of row l / 8.  A tile row r is
   //      column r of out's tile, gated: 16 (r / 32) + r % 16, of the gate for r / 16 even
-  int i_id = id0, i_step = 0, i_stage = 0;
+  int i_id = id0, i_step = 0, i_end = 0, i_stage = 0;
   const uint8_t *a_base, *w_base, *s_base = nullptr;
   uint32_t a_off[T::A_DMA], w_off[T::W_DMA], s_off[T::S_DMA > 0 ? T::S_DMA : 1];
   auto open = [&]() {
     const Place t = place(i_id);
     const int64_t n0 = (int64_t)t.nt * T::COLS;
+    i_step = t.s_beg;
+    i_end = t.s_end;
     auto column = [&](int r) {  // from n0, of a column that exists
       const int c = GATED ? 16 * (r >> 5) + (r & 15) : r;
       return n0 + c < g.N ? (int64_t)c : g.N - 1 - n0;
@@ -141,121 +151,150 @@ __global__ __launch_bounds__(L_THREADS) void linear_kernel(const LinArgs g) {
     i_a = a_base + (int64_t)i_k * 128;
     i_w = w_base + (int64_t)i_k * T::W_ROW;
   };
+  // (readfirstlane of what is uniform already is a move at most; without it the compiler may hold it in vector registers)
+  auto to_lds = [](uint32_t at) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)at); };
+  auto from = [](const uint8_t* p) { return Q4 ? uniform(p) : p; };
   auto piece = [&](int p) {
     if (p < T::W_DMA) {
       const int at = T::SHARE * p + part;  // wave-uniform
       const uint8_t* base = i_w;
       if (!Q4 && GATED && (at & 2)) base += up_rows * g.ldw;
-      g_dma16(base, w_off[p < T::W_DMA ? p : 0], i_to + T::A_BYTES + at * 1024 % T::W_BYTES);
+      g_dma16(from(base), w_off[p < T::W_DMA ? p : 0], to_lds(i_to + T::A_BYTES + at * 1024 % T::W_BYTES));
     } else if (p < T::W_DMA + T::A_DMA) {
       const int i = p - T::W_DMA;
-      g_dma16(i_a, a_off[i < T::A_DMA ? i : 0], i_to + (T::SHARE * i + part) * 1024 % T::A_BYTES);
+      g_dma16(from(i_a), a_off[i < T::A_DMA ? i : 0], to_lds(i_to + (T::SHARE * i + part) * 1024 % T::A_BYTES));
     } else if (p < T::DMAS) {
       const int i = p - T::W_DMA - T::A_DMA, s = (T::SHARE * i + part) % (T::S_WORDS > 0 ? T::S_WORDS : 1);
-      g_dma4(s_base + (i_k >> 1) * 4, s_off[i < T::S_DMA ? i : 0], i_to + T::A_BYTES + T::W_BYTES + 256 * s);
+      g_dma4(from(s_base + (i_k >> 1) * 4), s_off[i < T::S_DMA ? i : 0], to_lds(i_to + T::A_BYTES + T::W_BYTES + 256 * s));
     }
   };
   auto advance = [&]() {
     i_stage = i_stage + 1 == T::NS ? 0 : i_stage + 1;
-    if (++i_step == steps) {
+    if (++i_step == i_end) {
       if (i_id + stride < end) {
         i_id += stride;
-        i_step = 0;
         open();
       } else {
-        i_step = steps - 1;  // past the block's last step: that one again, which nobody reads
+        i_step = i_end - 1;  // past the block's last step: that one again, which nobody reads
       }
     }
   };
 
+  // ---- fragments.  Half h of a 32 x 32 x 16 product's 64 lanes has k = 32 h + 8 j + [0, 8) of a step's product j, on
+  //      both sides.  A slice is product j's of all the wave's blocks; the next slice's come while one is multiplied
+  u32x4 wf[2][NI], af[2][MI], codes[Q4 ? NI : 1];
+  uint32_t scale[Q4 ? NI : 1];
+  auto load_one = [&](int stage, int j, int n, u32x4(&w)[NI], u32x4(&a)[MI]) {
+    const uint8_t* const sa = sm + stage * T::STAGE + kw * T::SLAB;
+    const uint8_t* const sw = sa + T::A_BYTES;
+    auto word = [&](const uint8_t* rows, int r, int c) {
+      return *reinterpret_cast<const u32x4*>(rows + r * 128 + 16 * (c ^ g_swz(r)));
+    };
+    if (n < NI) {
+      const int k = n, r = 32 * (NI * wn + k) + l32;
+      if constexpr (Q4) {
+        if (j == 0) {
+          codes[k] = *reinterpret_cast<const u32x4*>(sw + r * 32 + 16 * (half ^ (r >> 3 & 1)));
+          scale[k] = reinterpret_cast<const uint32_t*>(sw + T::W_BYTES)[r];
+        }
+        const f16 s = __builtin_bit_cast(f16, (uint16_t)scale[k]), z = __builtin_bit_cast(f16, (uint16_t)(scale[k] >> 16));
+        w[k] = dq8<DT>(codes[k][j], f16x2{s, s}, f16x2{z, z});
+      } else {
+        w[k] = word(sw, r, 4 * half + j);
+      }
+    } else if (n < NI + MI) {
+      a[n - NI] = word(sa, 32 * (MI * wm + n - NI) + l32, 4 * half + j);
+    }
+  };
+  auto load_slice = [&](int stage, int j, u32x4(&w)[NI], u32x4(&a)[MI]) {
+#pragma unroll
+    for (int n = 0; n < NI + MI; ++n) load_one(stage, j, n, w, a);
+  };
+
   f32x16 acc[MI][NI];
   int stage = 0;
+  // A step's DMAs go out behind its barrier.  Of eight waves, a SIMD's two send at different times (one in front of the last
+  // slice, one in front of the next step's first), so that one has products while the other waits for the address unit:
+  // all at once cost 4 % of a large product.  Four waves send between the products of the same two slices.
+  const bool early = wave < WAVES / 2;
+  constexpr int HALF = (T::DMAS + 1) / 2;
+  auto send = [&](int first, int last) {
+#pragma unroll
+    for (int p = 0; p < T::DMAS; ++p)
+      if (p >= first && p < last) piece(p);
+  };
+  auto next_stage = [&]() {
+    wait_vmcnt<(T::NS - 2) * T::DMAS>();  // the wave's DMAs of the next stage (and what is older) have landed
+    lds_barrier();                        // and everyone's; this stage has been read
+    stage = stage + 1 == T::NS ? 0 : stage + 1;
+  };
   open();
   for (int s = 0; s < T::NS - 1; ++s) {
     begin();
-#pragma unroll
-    for (int p = 0; p < T::DMAS; ++p) piece(p);
+    send(0, T::DMAS);
     advance();
   }
+  stage = T::NS - 1;
+  next_stage();
+  load_slice(0, 0, wf[0], af[0]);
+  begin();
+  if (WAVES == 4) send(0, HALF);
+  else if (early) send(0, T::DMAS);
   for (int id = id0; id < end; id += stride) {
     const Place t = place(id);
     const int mine = t.valid - 32 * MI * wm;  // slots of the wave's part
-    const int live = mine <= 0 ? 0 : mine >= 32 * MI ? MI : (mine + 31) >> 5;  // its blocks of 32 with any
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int k = 0; k < NI; ++k) acc[i][k] = f32x16{};
-    for (int step = 0; step < steps; ++step) {
-      wait_vmcnt<(T::NS - 2) * T::DMAS>();  // the wave's DMAs of this step (and what is older)
-      lds_barrier();                        // and everyone's; the stage before this one has been read
-      begin();
-      const uint8_t* const sa = sm + stage * T::STAGE + kw * T::SLAB;
-      const uint8_t* const sw = sa + T::A_BYTES;
-      stage = stage + 1 == T::NS ? 0 : stage + 1;
-      if (KW > 1 && step * KW + kw >= nkb) {  // wave-uniform
+    for (int step = t.s_beg; step < t.s_end; ++step) {
+      const bool mine_too = KW == 1 || step * KW + kw < nkb;  // wave-uniform
 #pragma unroll
-        for (int p = 0; p < T::DMAS; ++p) piece(p);
-        advance();
-        continue;
-      }
-      auto word = [&](const uint8_t* rows, int r, int c) {
-        return *reinterpret_cast<const u32x4*>(rows + r * 128 + 16 * (c ^ g_swz(r)));
-      };
-      // half h of a 32 x 32 x 16 product's 64 lanes has k = 32 h + 8 j + [0, 8) of product j, on both sides
-      u32x4 wf[NI][4], af[4];
-      auto load_a = [&](int i, u32x4(&x)[4]) {
+      for (int j = 0; j < 4; ++j) {
+        u32x4(&w)[NI] = wf[j & 1];
+        u32x4(&x)[MI] = af[j & 1];
+        if (j == 3) next_stage();
+        if constexpr (WAVES == 8) {
+          load_slice(stage, (j + 1) & 3, wf[(j + 1) & 1], af[(j + 1) & 1]);
+          if (j == 3) begin();
+          if (early ? j == 3 : j == 0) send(0, T::DMAS);
+          __builtin_amdgcn_sched_barrier(0);
+          if (mine_too) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = word(sa, 32 * (MI * wm + i) + l32, 4 * half + j);
-      };
+            for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int k = 0; k < NI; ++k) {
-        const int r = 32 * (NI * wn + k) + l32;
-        if constexpr (Q4) {
-          const u32x4 c = *reinterpret_cast<const u32x4*>(sw + r * 32 + 16 * (half ^ (r >> 3 & 1)));
-          const uint32_t p = reinterpret_cast<const uint32_t*>(sw + T::W_BYTES)[r];
-          const f16 s = __builtin_bit_cast(f16, (uint16_t)p), z = __builtin_bit_cast(f16, (uint16_t)(p >> 16));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) wf[k][j] = dq8<DT>(c[j], f16x2{s, s}, f16x2{z, z});
+              for (int k = 0; k < NI; ++k) acc[i][k] = mfma32<DT>(w[k], x[i], acc[i][k]);
+          }
         } else {
+          // one wave a SIMD: reads and DMAs in turn between the products
+          static_assert(KW == 1 && 2 * (MI + NI) <= MI * NI && 2 * HALF <= MI * NI, "they fit between");
+          if (j == 3) begin();
 #pragma unroll
-          for (int j = 0; j < 4; ++j) wf[k][j] = word(sw, r, 4 * half + j);
+          for (int n = 0; n < MI * NI; ++n) {
+            if (n % 2 == 0) load_one(stage, (j + 1) & 3, n / 2, wf[(j + 1) & 1], af[(j + 1) & 1]);
+            else if (j == 3 && n / 2 < HALF) send(n / 2, n / 2 + 1);
+            else if (j == 0 && HALF + n / 2 < T::DMAS) send(HALF + n / 2, HALF + n / 2 + 1);
+            acc[n / NI][n % NI] = mfma32<DT>(w[n % NI], x[n / NI], acc[n / NI][n % NI]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
-      }
-      load_a(0, af);
-      // A wave's DMAs go out between its matrix instructions, PER at a time
-      constexpr int PER = MI > 1 ? (T::DMAS + MI - 2) / (MI - 1) : T::DMAS;
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        u32x4 bf[4];
-        if (i + 1 < MI) load_a(i + 1, bf);  // the next fragments, while these are multiplied
-#pragma unroll
-        for (int p = 0; p < PER; ++p) {
-          const int at = (MI > 1 ? i - 1 : 0) * PER + p;  // none before the first matrix instructions
-          if (at >= 0) piece(at);
-        }
-        if (i < live) {  // wave-uniform
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int k = 0; k < NI; ++k) acc[i][k] = mfma32<DT>(wf[k][j], af[j], acc[i][k]);
-        }
-        if (i + 1 < MI) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) af[j] = bf[j];
-        }
+        if (j == 0) advance();
         __builtin_amdgcn_sched_barrier(0);
       }
-      advance();
     }
 
-    // ---- results, 32 MW slots at a time through LDS, for whole lines to memory.  Through the stage that was read
-    //      last: nothing is sent there before the next step's barrier.  Wave kw finishes values VH kw + [0, VH) of a
-    //      block's lower 16 rows and the same of its upper 16
+    // ---- results, the same 32 of EW of the wave rows' slots at a time through LDS, for whole lines to memory.  Wave kw
+    //      finishes values VH kw + [0, VH) of a block's lower 16 rows and the same of its upper 16
+    // (the lane's place is taken anew, or what hangs on it is computed ahead of the tiles and held in
+    // registers that the steps lack)
+    int tid_now = threadIdx.x;
+    asm volatile("" : "+v"(tid_now));
+    const int e_l32 = tid_now & 31, e_half = tid_now >> 5 & 1, e_lane = tid_now & 63;
     constexpr int VH = KW > 1 ? 8 / KW : 8, RL = VH < 4 ? VH : 4;
-    uint8_t* const ends = sm + (T::IN_STAGE ? (stage == 0 ? T::NS - 1 : stage - 1) * T::STAGE : T::NS * T::STAGE);
+    uint8_t* const ends = sm + T::NS * T::STAGE;
     float* const red = reinterpret_cast<float*>(ends);
     uint8_t* const s_out = ends + T::RED;
-    uint8_t* const s_kept = s_out + 32 * MW * T::OUT_ROW;
+    uint8_t* const s_kept = s_out + T::ER * T::OUT_ROW;
     const int64_t n0 = (int64_t)t.nt * T::COLS;
     // RL values to column c of row r of `row` bytes
     auto put = [&](uint8_t* rows, int row, int r, int c, const float* v) {
@@ -265,27 +304,29 @@ __global__ __launch_bounds__(L_THREADS) void linear_kernel(const LinArgs g) {
       else *reinterpret_cast<uint16_t*>(to) = (uint16_t)pack2<DT>(v[0], v[0]);
     };
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      if (32 * i >= t.valid) break;  // block-uniform: no slots in any wave's i-th 32
-      lds_barrier();  // the step's reads, or the last 32 slots', are done
+    for (int ih = 0; ih < MI * (MW / T::EW); ++ih) {
+      const int i = ih / (MW / T::EW), h = ih % (MW / T::EW);
+      if (32 * (MI * T::EW * h + i) >= t.valid) continue;  // block-uniform: no slots
+      lds_barrier();  // the last slots' reads are done
+      if (T::EW == MW || wm == h) {  // wave-uniform
       float lo[NI][VH], hi[NI][VH];
       if constexpr (KW > 1) {
 #pragma unroll
         for (int k = 0; k < NI; ++k)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) red[((k * 16 + v) * L_WAVES + wave) * 64 + lane] = acc[i][k][v];
+          for (int v = 0; v < 16; ++v) red[((k * 16 + v) * WAVES + wave) * 64 + e_lane] = acc[i][k][v];
         lds_barrier();
 #pragma unroll
         for (int k = 0; k < NI; ++k)
 #pragma unroll
           for (int v = 0; v < VH; ++v) {
-            const int at = ((k * 16 + VH * kw + v) * L_WAVES + part) * 64 + lane;
+            const int at = ((k * 16 + VH * kw + v) * WAVES + part) * 64 + e_lane;
             lo[k][v] = red[at];
-            hi[k][v] = red[at + 8 * L_WAVES * 64];
+            hi[k][v] = red[at + 8 * WAVES * 64];
 #pragma unroll
             for (int w = 1; w < KW; ++w) {
               lo[k][v] += red[at + w * T::SHARE * 64];
-              hi[k][v] += red[at + (8 * L_WAVES + w * T::SHARE) * 64];
+              hi[k][v] += red[at + (8 * WAVES + w * T::SHARE) * 64];
             }
           }
       } else {
@@ -297,41 +338,65 @@ __global__ __launch_bounds__(L_THREADS) void linear_kernel(const LinArgs g) {
             hi[k][v] = acc[i][k][v + 8];
           }
       }
-      const int row = 32 * wm + l32;
+      if constexpr (EPI == LIN_STORE) {
+        if (g.parts > 1) {  // fp32 sums of a part of the contraction, RL columns at a time
+          if (32 * i + e_l32 < mine) {
+            float* const to = g.part + (t.part * g.M + t.m_beg + 32 * (MI * wm + i) + e_l32) * g.ldp;
+#pragma unroll
+            for (int k = 0; k < NI; ++k)
+#pragma unroll
+              for (int r0 = 0; r0 < VH; r0 += RL)
+#pragma unroll
+                for (int up = 0; up < 2; ++up) {
+                  const int v = VH * (KW > 1 ? kw : 0) + r0;
+                  const int64_t n = n0 + 32 * (NI * wn + k) + 16 * up + 8 * (v >> 2) + 4 * e_half + (v & 3);
+                  const float* const f = up ? &hi[k][r0] : &lo[k][r0];
+                  if (n < g.ldp) {
+                    if constexpr (RL == 4) *reinterpret_cast<f32x4*>(to + n) = f32x4{f[0], f[1], f[2], f[3]};
+                    else if constexpr (RL == 2) *reinterpret_cast<f32x2*>(to + n) = f32x2{f[0], f[1]};
+                    else to[n] = f[0];
+                  }
+                }
+          }
+          continue;
+        }
+      }
+      const int row = 32 * (wm % T::EW) + e_l32;
       if constexpr (EPI == LIN_CK8) {
         // a block's largest magnitude: the lane's columns, the other half's, the other waves'
-        float* const s_max = reinterpret_cast<float*>(s_kept + 32 * MW * T::KEPT_ROW);  // [2, NW, 32 MW]
+        float* const s_max = reinterpret_cast<float*>(s_out);  // [2, NW, ER]
         float tg = 0.f, tu = 0.f;
 #pragma unroll
         for (int k = 0; k < NI; ++k)
 #pragma unroll
           for (int v = 0; v < 8; ++v) {
-            const bool real = n0 + 16 * (NI * wn + k) + 8 * (v >> 2) + 4 * half + (v & 3) < g.N;
+            const bool real = n0 + 16 * (NI * wn + k) + 8 * (v >> 2) + 4 * e_half + (v & 3) < g.N;
             if (!real) lo[k][v] = hi[k][v] = 0.f;
             tg = fmaxf(tg, finite_abs(lo[k][v]));
             tu = fmaxf(tu, finite_abs(hi[k][v]));
           }
         tg = fmaxf(tg, __shfl_xor(tg, 32, 64));
         tu = fmaxf(tu, __shfl_xor(tu, 32, 64));
-        s_max[(half * NW + wn) * (32 * MW) + row] = half ? tu : tg;
+        s_max[(e_half * NW + wn) * T::ER + row] = e_half ? tu : tg;
         lds_barrier();
         tg = tu = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-          tg = fmaxf(tg, s_max[w * (32 * MW) + row]);
-          tu = fmaxf(tu, s_max[(NW + w) * (32 * MW) + row]);
+          tg = fmaxf(tg, s_max[w * T::ER + row]);
+          tu = fmaxf(tu, s_max[(NW + w) * T::ER + row]);
         }
+        lds_barrier();  // out goes to the same place
         const int eg = e8m0_of(tg), eu = e8m0_of(tu);
         const float ig = inv_scale(eg), iu = inv_scale(eu);
-        if (wn == 0 && 32 * i + l32 < mine) {
-          const int64_t m = t.m_beg + 32 * (MI * wm + i) + l32, nb = g.hs / 128;
-          g.kept_s[(2 * m + half) * nb + t.nt] = (uint8_t)(half ? eu : eg);
+        if (wn == 0 && 32 * i + e_l32 < mine) {
+          const int64_t m = t.m_beg + 32 * (MI * wm + i) + e_l32, nb = g.hs / 128;
+          g.kept_s[(2 * m + e_half) * nb + t.nt] = (uint8_t)(e_half ? eu : eg);
         }
 #pragma unroll
         for (int k = 0; k < NI; ++k)
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const int c = 16 * (NI * wn + k) + 8 * q + 4 * half;  // of the 128 columns
+            const int c = 16 * (NI * wn + k) + 8 * q + 4 * e_half;  // of the 128 columns
             const float a[4] = {lo[k][4 * q], lo[k][4 * q + 1], lo[k][4 * q + 2], lo[k][4 * q + 3]};
             const float b[4] = {hi[k][4 * q], hi[k][4 * q + 1], hi[k][4 * q + 2], hi[k][4 * q + 3]};
             uint8_t* const to = s_kept + row * T::KEPT_ROW;
@@ -339,11 +404,12 @@ __global__ __launch_bounds__(L_THREADS) void linear_kernel(const LinArgs g) {
             *reinterpret_cast<uint32_t*>(to + 128 + 16 * ((c >> 4) ^ (row & 7)) + (c & 15)) = to_codes(b, iu);
           }
       }
+      if (GATED || g.parts == 1)
 #pragma unroll
       for (int k = 0; k < NI; ++k)
 #pragma unroll
         for (int r0 = 0; r0 < VH; r0 += RL) {
-          const int v = VH * (KW > 1 ? kw : 0) + r0, c16 = 8 * (v >> 2) + 4 * half + (v & 3), b = NI * wn + k;
+          const int v = VH * (KW > 1 ? kw : 0) + r0, c16 = 8 * (v >> 2) + 4 * e_half + (v & 3), b = NI * wn + k;
           if constexpr (!GATED) {
             put(s_out, T::OUT_ROW, row, 32 * b + c16, &lo[k][r0]);
             put(s_out, T::OUT_ROW, row, 32 * b + 16 + c16, &hi[k][r0]);
@@ -360,11 +426,13 @@ __global__ __launch_bounds__(L_THREADS) void linear_kernel(const LinArgs g) {
             }
           }
         }
+      }
+      if (!GATED && g.parts > 1) continue;  // block-uniform
       lds_barrier();
       constexpr int CH = T::OUT_ROW / 16;  // chunks of a row
       const bool vec = g.ldo % 8 == 0 && ((uintptr_t)g.out & 15) == 0;
-      for (int at = tid; at < 32 * MW * CH; at += L_THREADS) {
-        const int r = at / CH, c = at % CH, slot = 32 * (MI * (r >> 5) + i) + (r & 31);
+      for (int at = tid_now; at < T::ER * CH; at += THREADS) {
+        const int r = at / CH, c = at % CH, slot = 32 * (MI * (T::EW * h + (r >> 5)) + i) + (r & 31);
         const int64_t n = n0 + 8 * c;
         if (slot < t.valid && n < g.N) {
           const u32x4 v = *reinterpret_cast<const u32x4*>(s_out + r * T::OUT_ROW + 16 * (c ^ (r & (CH - 1))));
@@ -380,8 +448,8 @@ __global__ __launch_bounds__(L_THREADS) void linear_kernel(const LinArgs g) {
       }
       if constexpr (EPI == LIN_GATED) {
         if (g.kept) {
-          for (int at = tid; at < 64 * MW * CH; at += L_THREADS) {  // rows 2 r (gate) and 2 r + 1 (up)
-            const int rr = at / CH, c = at % CH, r = rr >> 1, slot = 32 * (MI * (r >> 5) + i) + (r & 31);
+          for (int at = tid_now; at < 2 * T::ER * CH; at += THREADS) {  // rows 2 r (gate) and 2 r + 1 (up)
+            const int rr = at / CH, c = at % CH, r = rr >> 1, slot = 32 * (MI * (T::EW * h + (r >> 5)) + i) + (r & 31);
             const int64_t n = n0 + 8 * c;
             if (slot < t.valid && n < g.N)
               *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(g.kept) + (2 * (t.m_beg + slot) + (rr & 1)) * g.hs + n) =
@@ -389,8 +457,8 @@ __global__ __launch_bounds__(L_THREADS) void linear_kernel(const LinArgs g) {
           }
         }
       } else if constexpr (EPI == LIN_CK8) {
-        for (int at = tid; at < 32 * MW * 16; at += L_THREADS) {
-          const int r = at >> 4, c = at & 15, slot = 32 * (MI * (r >> 5) + i) + (r & 31);
+        for (int at = tid_now; at < T::ER * 16; at += THREADS) {
+          const int r = at >> 4, c = at & 15, slot = 32 * (MI * (T::EW * h + (r >> 5)) + i) + (r & 31);
           if (slot < t.valid)
             *reinterpret_cast<u32x4*>(reinterpret_cast<uint8_t*>(g.kept) + (2 * (t.m_beg + slot) + (c >> 3)) * g.hs + n0 +
                                       16 * (c & 7)) =
@@ -408,80 +476,79 @@ inline bool raise_linear_lds(const void* kernel, size_t bytes) {
   return true;
 }
 
-// One shape of tile: launch, one-time set-up, and what a call would take with it.
-template <int MW, int NW, int MI, int NI, bool Q4>
-struct LinShape {
-  template <int EPI>
-  using T = LinTile<MW, NW, MI, NI, Q4, EPI>;
-  static constexpr bool CK8 = T<LIN_STORE>::N == 256 && T<LIN_STORE>::KW == 1;  // may keep 8-bit blocks
-
-  template <int DT, int EPI>
+// One kernel: launch and one-time set-up.
+template <int WAVES, int MW, int NW, int MI, int NI, bool Q4, int EPI>
+struct LinLaunch {
+  typedef LinTile<WAVES, MW, NW, MI, NI, Q4, EPI> T;
+  template <int DT>
   static void prepare_one() {
     static const bool done =
-        raise_linear_lds(reinterpret_cast<const void*>(&linear_kernel<MW, NW, MI, NI, DT, Q4, EPI>), T<EPI>::LDS);
+        raise_linear_lds(reinterpret_cast<const void*>(&linear_kernel<WAVES, MW, NW, MI, NI, DT, Q4, EPI>), T::LDS);
     (void)done;
   }
   static void prepare() {
-    prepare_one<USAF_BF16, LIN_STORE>();
-    prepare_one<USAF_F16, LIN_STORE>();
-    prepare_one<USAF_BF16, LIN_GATED>();
-    prepare_one<USAF_F16, LIN_GATED>();
-    if constexpr (CK8) {
-      prepare_one<USAF_BF16, LIN_CK8>();
-      prepare_one<USAF_F16, LIN_CK8>();
-    }
+    prepare_one<USAF_BF16>();
+    prepare_one<USAF_F16>();
   }
-  template <int EPI>
-  static int launch_epi(LinArgs g, int dt, hipStream_t st) {
-    typedef T<EPI> Tile;
-    const int64_t n_nt = (g.N + Tile::COLS - 1) / Tile::COLS, tiles = (g.M + Tile::M - 1) / Tile::M * n_nt;
+  static int launch(LinArgs g, int dt, hipStream_t st) {
+    const int64_t n_nt = (g.N + T::COLS - 1) / T::COLS, units = (g.M + T::M - 1) / T::M * n_nt * g.parts;
     const int64_t cus = device_cu_count();
-    if (tiles >= (int64_t)1 << 30) return set_error(USAF_ERR_UNSUPPORTED, "linear: too many tiles");
+    if (units >= (int64_t)1 << 30) return set_error(USAF_ERR_UNSUPPORTED, "linear: too many tiles");
     g.n_nt = (int)n_nt;
-    const unsigned blocks = (unsigned)(((tiles < cus ? tiles : cus) + L_XCDS - 1) / L_XCDS * L_XCDS);
-    if (dt == USAF_BF16) {
-      prepare_one<USAF_BF16, EPI>();
-      linear_kernel<MW, NW, MI, NI, USAF_BF16, Q4, EPI><<<blocks, L_THREADS, Tile::LDS, st>>>(g);
-    } else {
-      prepare_one<USAF_F16, EPI>();
-      linear_kernel<MW, NW, MI, NI, USAF_F16, Q4, EPI><<<blocks, L_THREADS, Tile::LDS, st>>>(g);
-    }
+    const unsigned blocks = (unsigned)(((units < cus ? units : cus) + L_XCDS - 1) / L_XCDS * L_XCDS);
+    prepare();
+    if (dt == USAF_BF16) linear_kernel<WAVES, MW, NW, MI, NI, USAF_BF16, Q4, EPI><<<blocks, 64 * WAVES, T::LDS, st>>>(g);
+    else linear_kernel<WAVES, MW, NW, MI, NI, USAF_F16, Q4, EPI><<<blocks, 64 * WAVES, T::LDS, st>>>(g);
     return check_launch("linear");
-  }
-  static int launch(const LinArgs& g, int dt, bool gated, hipStream_t st) {
-    if (!gated) return launch_epi<LIN_STORE>(g, dt, st);
-    if constexpr (CK8) {
-      if (g.kept && g.kept_s) return launch_epi<LIN_CK8>(g, dt, st);
-    }
-    return launch_epi<LIN_GATED>(g, dt, st);
-  }
-  // Cycles of a CU, roughly: a step is bound by its matrix instructions, by its lines (24 bytes a cycle) or, 4-bit,
-  // by the dequantization; a tile has its ends, and the last round of tiles counts whole.
-  static double cycles(const LinArgs& g, int dt, bool gated) {
-    typedef T<LIN_STORE> Tile;
-    const double steps = (double)((g.K / 64 + Tile::KW - 1) / Tile::KW);
-    const double mfma = 2.0 * MI * NI * 4 * 32, lines = (double)Tile::STAGE / 24;
-    const double codes = Q4 ? 2.0 * NI * 16 * (dt == USAF_BF16 ? 8 : 5) * 4 : 0;
-    const double step = (mfma + codes > lines ? mfma + codes : lines) + 250, tile = steps * step + 1500;
-    const double m = (double)((g.M + Tile::M - 1) / Tile::M), cols = gated ? Tile::N / 2 : Tile::N;
-    const double rounds = m * (double)(int64_t)((g.N + cols - 1) / cols) / device_cu_count();
-    return tile * (rounds < 1 ? 1 : (double)(int64_t)(rounds + 0.999));
   }
 };
 
-struct LinChoice {
-  int (*launch)(const LinArgs&, int, bool, hipStream_t) = nullptr;
-  double least = 0;
-  template <class S>
-  void consider(const LinArgs& g, int dt, bool gated) {
-    if (gated && g.kept && g.kept_s && !S::CK8) return;
-    const double c = S::cycles(g, dt, gated);
-    if (launch == nullptr || c < least) {
-      least = c;
-      launch = S::launch;
-    }
+// One shape of tile for all that leaves it.  FOUR: the plain product on four waves (those of MW NW MI NI, 2 x 2 of them)
+// instead of eight.
+template <int MW, int NW, int MI, int NI, bool Q4, bool FOUR = false>
+struct LinShape {
+  typedef LinTile<8, MW, NW, MI, NI, Q4, LIN_STORE> T;
+  typedef LinLaunch<FOUR ? 4 : 8, FOUR ? 2 : MW, FOUR ? 2 : NW, FOUR ? T::M / 64 : MI, FOUR ? T::N / 64 : NI, Q4, LIN_STORE> Store;
+  typedef LinLaunch<8, MW, NW, MI, NI, Q4, LIN_GATED> Gated;
+  static constexpr bool CK8 = T::N == 256 && T::KW == 1;  // may keep 8-bit blocks
+
+  static void prepare() {
+    Store::prepare();
+    Gated::prepare();
+    if constexpr (CK8) LinLaunch<8, MW, NW, MI, NI, Q4, LIN_CK8>::prepare();
   }
+  static int launch(const LinArgs& g, int dt, bool gated, hipStream_t st) {
+    if (!gated) return Store::launch(g, dt, st);
+    if constexpr (CK8) {
+      if (g.kept && g.kept_s) return LinLaunch<8, MW, NW, MI, NI, Q4, LIN_CK8>::launch(g, dt, st);
+    }
+    return Gated::launch(g, dt, st);
+  }
+  // Cycles of a CU, roughly: a step is bound by its matrix instructions, by its lines (24 bytes a cycle) or, 4-bit,
+  // by the dequantization; a tile has its ends, and the last round of tiles counts whole.
+  static double cycles(const LinArgs& g, int dt, bool gated, int parts) {
+    const double steps = (double)((g.K / 64 + T::KW - 1) / T::KW) / parts;
+    const double mfma = 2.0 * MI * NI * 4 * 32, lines = (double)T::STAGE / 24;
+    const double codes = Q4 ? 2.0 * NI * 16 * (dt == USAF_BF16 ? 8 : 5) * 4 : 0;
+    const double step = (mfma + codes > lines ? mfma + codes : lines) + 250, tile = steps * step + 1500;
+    const double m = (double)((g.M + T::M - 1) / T::M), cols = gated ? T::N / 2 : T::N;
+    const double rounds = m * (double)(int64_t)((g.N + cols - 1) / cols) * parts / device_cu_count();
+    // fp32 sums of the parts: written and read at about 4 TB/s, and a launch
+    const double join = parts > 1 ? (double)parts * (double)g.M * (double)g.N * 8 / 2000 + 6000 : 0;
+    return tile * (rounds < 1 ? 1 : (double)(int64_t)(rounds + 0.999)) + join;
+  }
+  static constexpr int KW = T::KW;
 };
+
+template <class S>
+void consider(LinPlan& best, const LinArgs& g, int dt, bool gated) {
+  if (gated && g.kept && g.kept_s && !S::CK8) return;
+  for (int parts = 1; parts <= (gated ? 1 : 16); parts *= 2) {
+    if (parts > 1 && g.K / 64 < 4 * parts * S::KW) break;
+    const double c = S::cycles(g, dt, gated, parts);
+    if (best.launch == nullptr || c < best.cycles) best = {S::launch, parts, c};
+  }
+}
 
 }  // namespace
 }  // namespace usaf

@@ -12,16 +12,16 @@ typedef LinShape<1, 2, 1, 1, true> Q32x64;
 typedef LinShape<1, 1, 1, 1, true> Q32x32;
 }  // namespace
 
-int launch_linear_q4(const LinArgs& g, int dt, bool gated, hipStream_t st) {
-  LinChoice best;
-  best.consider<Q128x256>(g, dt, gated);
-  best.consider<Q128x128>(g, dt, gated);
-  best.consider<Q64x128>(g, dt, gated);
-  best.consider<Q64x64>(g, dt, gated);
-  best.consider<Q32x256>(g, dt, gated);
-  best.consider<Q32x64>(g, dt, gated);
-  best.consider<Q32x32>(g, dt, gated);
-  return best.launch(g, dt, gated, st);
+LinPlan plan_linear_q4(const LinArgs& g, int dt, bool gated) {
+  LinPlan best;
+  consider<Q128x256>(best, g, dt, gated);
+  consider<Q128x128>(best, g, dt, gated);
+  consider<Q64x128>(best, g, dt, gated);
+  consider<Q64x64>(best, g, dt, gated);
+  consider<Q32x256>(best, g, dt, gated);
+  consider<Q32x64>(best, g, dt, gated);
+  consider<Q32x32>(best, g, dt, gated);
+  return best;
 }
 
 void prepare_linear_q4() {

@@ -29,7 +29,8 @@ CHECKPOINTS = (None, "fp8")
 
 
 @functools.lru_cache(maxsize=4096)
-def _ws_bytes(m: int, inter: int, k: int, four_bit: int, what: int) -> int:
+def _ws_bytes(device: int, m: int, inter: int, k: int, four_bit: int, what: int) -> int:
+    """The workspace on a device (its CU count decides the split), which is the current one."""
     return N.load().usaf_hip_gated_ws_bytes(m, inter, k, four_bit, what)
 
 
@@ -58,8 +59,9 @@ def _forward(x: torch.Tensor, w, checkpoint: Optional[str], keep: bool):
         kept = torch.empty(m, 2, blocks * 128, dtype=torch.uint8, device=dev)
         scales = torch.empty(m, 2, blocks, dtype=torch.uint8, device=dev)
     if m:
-        need, ptrs = _ws_bytes(m, inter, k, int(isinstance(w, Q4Tensor)), 0), _weight_ptrs(w)
+        ptrs = _weight_ptrs(w)
         with on(dev):
+            need = _ws_bytes(dev.index, m, inter, k, int(isinstance(w, Q4Tensor)), 0)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
             N.call("usaf_hip_gated_fwd", x.data_ptr(), N.dtype_code(x.dtype), m, k, _ld(x), *ptrs, inter, act.data_ptr(),
                    N.ptr(kept), N.ptr(scales), N.ptr(ws), max(need, 0), N.stream_ptr(dev))
@@ -103,8 +105,8 @@ class GatedLinearFn(torch.autograd.Function):
             ptrs = (None, None, weight.data_ptr())
         if want_w:
             x = rows_of(x, k)
-        need = _ws_bytes(m, rows // 2, k, int(ctx.q4 is not None), int(want_x) + 2 * int(want_w))
         with on(dev):
+            need = _ws_bytes(dev.index, m, rows // 2, k, int(ctx.q4 is not None), int(want_x) + 2 * int(want_w))
             ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dev)
             N.call("usaf_hip_gated_bwd", dact.data_ptr(), N.dtype_code(ctx.dtype), m, rows // 2, k, kept.data_ptr(),
                    N.ptr(scales), *ptrs, x.data_ptr() if want_w else None, _ld(x) if want_w else k, N.ptr(dx), N.ptr(dw),

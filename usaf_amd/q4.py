@@ -23,7 +23,8 @@ MAX_COLS = 1 << 22
 
 
 @functools.lru_cache(maxsize=4096)
-def _ws_bytes(m: int, n: int, k: int, backward: int) -> int:
+def _ws_bytes(device: int, m: int, n: int, k: int, backward: int) -> int:
+    """The workspace on a device (its CU count decides the split), which is the current one."""
     return N.load().usaf_hip_q4_linear_ws_bytes(m, n, k, backward)
 
 
@@ -91,8 +92,9 @@ def _linear(x: torch.Tensor, w: Q4Tensor, backward: bool = False) -> torch.Tenso
     m = rows.shape[0]
     out = torch.empty(m, out_cols, dtype=x.dtype, device=dev)
     if m:
-        need, sz = _ws_bytes(m, n, k, int(backward)), words("q4_linear", w)
+        sz = words("q4_linear", w)
         with on(dev):
+            need = _ws_bytes(dev.index, m, n, k, int(backward))
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
             name, size = ("usaf_hip_q4_linear_bwd", k) if backward else ("usaf_hip_q4_linear", n)
             N.call(name, rows.data_ptr(), N.dtype_code(x.dtype), m, cols, _ld(rows), w.q.data_ptr(), sz.data_ptr(), size,
