@@ -28,15 +28,14 @@ struct LinArgs {
   int64_t ldp = 0;     // N in whole 4
 };
 
-// The tile for a product of these sizes, how many parts its contraction is taken in, and about how many cycles of a CU it
-// takes.
+// The tile for a product of these sizes, how many parts its contraction is taken in, and about how long it takes.
 struct LinPlan {
   int (*launch)(const LinArgs&, int dt, bool gated, hipStream_t) = nullptr;
   int parts = 1;
-  double cycles = 0;
+  double us = 0;
 };
-LinPlan plan_linear_dense(const LinArgs& g, int dt, bool gated);
-LinPlan plan_linear_q4(const LinArgs& g, int dt, bool gated);
+LinPlan plan_linear_dense(const LinArgs& g, bool gated);
+LinPlan plan_linear_q4(const LinArgs& g, bool gated);
 // A few rows of a 4-bit weight's product, out [M, N] (ldo = N), nothing kept: whether it takes them, and its launch (q4_small.hip).
 bool q4_small_ok(int64_t M, int64_t K);
 int q4_small(const LinArgs& g, int dt, bool gated, hipStream_t st);

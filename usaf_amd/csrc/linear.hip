@@ -210,8 +210,7 @@ LinArgs product(const void* a, int64_t lda, int64_t M, const void* w, int64_t ld
 // multiplied: 2.5 bytes a weight at about 4 TB/s, and a launch.
 bool as_codes(int64_t M, int64_t rows, int64_t K, bool gated) {
   const LinArgs g = product(nullptr, K, M, nullptr, K, gated ? rows / 2 : rows, K, nullptr, 0);
-  return plan_linear_q4(g, USAF_BF16, gated).cycles <=
-         plan_linear_dense(g, USAF_BF16, gated).cycles + (double)rows * (double)K * 2.5 / 2000 + 6000;
+  return plan_linear_q4(g, gated).us <= plan_linear_dense(g, gated).us + (double)rows * (double)K * 2.5 / 4e6 + 3;
 }
 
 // Pieces of a workspace, each a whole number of 256 bytes.
@@ -234,7 +233,7 @@ struct Parts {
   Parts() = default;
   Parts(Ws& ws, int64_t M, int64_t N, int64_t K, bool q4) {
     const LinArgs g = product(nullptr, K, M, nullptr, K, N, K, nullptr, N);
-    plan = q4 ? plan_linear_q4(g, USAF_BF16, false) : plan_linear_dense(g, USAF_BF16, false);
+    plan = q4 ? plan_linear_q4(g, false) : plan_linear_dense(g, false);
     ldp = round_up(N, 4);
     at = plan.parts > 1 ? ws.take(4 * plan.parts * M * ldp) : nullptr;
   }
@@ -426,13 +425,13 @@ extern "C" int usaf_hip_gated_fwd(const void* x, int32_t dtype, int64_t M, int64
     g.ldw = K / 2;
     g.sz = sz;
     if (!kept && q4_small_ok(M, K)) return q4_small(g, dtype, true, st);
-    return plan_linear_q4(g, dtype, true).launch(g, dtype, true, st);
+    return plan_linear_q4(g, true).launch(g, dtype, true, st);
   }
   if (q)
     if (int rc = q4_rows(q, sz, 2 * I, K, dtype, w.w, st)) return rc;
   if (!q && w.w)
     if (int rc = pad(w16, 2 * I, K, K, w.w, w.kp, st)) return rc;
-  return plan_linear_dense(g, dtype, true).launch(g, dtype, true, st);
+  return plan_linear_dense(g, true).launch(g, dtype, true, st);
 }
 
 extern "C" int usaf_hip_gated_bwd(const void* dact, int32_t dtype, int64_t M, int64_t I, int64_t K, const void* kept,

@@ -3,24 +3,24 @@
 
 namespace usaf {
 namespace {
-typedef LinShape<2, 4, 4, 2, false, true> D256x256;
-typedef LinShape<2, 4, 2, 2, false> D128x256;
-typedef LinShape<2, 4, 2, 1, false> D128x128;
-typedef LinShape<2, 4, 1, 1, false> D64x128;
-typedef LinShape<2, 2, 1, 1, false> D64x64;
-typedef LinShape<1, 8, 1, 1, false> D32x256;
-typedef LinShape<1, 2, 1, 1, false> D32x64;
+typedef LinShape<2, 4, 4, 2, false, 163, 700, true> D256x256;
+typedef LinShape<2, 4, 2, 2, false, 95, 450> D128x256;
+typedef LinShape<2, 4, 2, 1, false, 50, 350> D128x128;
+typedef LinShape<2, 4, 1, 1, false, 33, 250> D64x128;
+typedef LinShape<2, 2, 1, 1, false, 40, 250> D64x64;
+typedef LinShape<1, 8, 1, 1, false, 41, 250> D32x256;
+typedef LinShape<1, 2, 1, 1, false, 75, 200> D32x64;
 }  // namespace
 
-LinPlan plan_linear_dense(const LinArgs& g, int dt, bool gated) {
+LinPlan plan_linear_dense(const LinArgs& g, bool gated) {
   LinPlan best;
-  consider<D256x256>(best, g, dt, gated);
-  consider<D128x256>(best, g, dt, gated);
-  consider<D128x128>(best, g, dt, gated);
-  consider<D64x128>(best, g, dt, gated);
-  consider<D64x64>(best, g, dt, gated);
-  consider<D32x256>(best, g, dt, gated);
-  consider<D32x64>(best, g, dt, gated);
+  consider<D256x256>(best, g, gated);
+  consider<D128x256>(best, g, gated);
+  consider<D128x128>(best, g, gated);
+  consider<D64x128>(best, g, gated);
+  consider<D64x64>(best, g, gated);
+  consider<D32x256>(best, g, gated);
+  consider<D32x64>(best, g, gated);
   return best;
 }
 

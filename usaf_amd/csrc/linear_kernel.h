@@ -63,7 +63,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
   typedef LinTile<WAVES, MW, NW, MI, NI, Q4, EPI> T;
   constexpr int THREADS = 64 * WAVES;
   constexpr int KW = T::KW, NB = T::NB;
-  constexpr bool GATED = EPI != LIN_STORE;
+  constexpr bool GATED = EPI != LIN_STORE, PARTS = !GATED && WAVES == 8;  // PARTS: takes a contraction in parts
   extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
   const uint32_t sm_lds = (uint32_t)(uintptr_t)(lds_void_ptr)sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
             hi[k][v] = acc[i][k][v + 8];
           }
       }
-      if constexpr (EPI == LIN_STORE) {
+      if constexpr (PARTS) {
         if (g.parts > 1) {  // fp32 sums of a part of the contraction, RL columns at a time
           if (32 * i + e_l32 < mine) {
             float* const to = g.part + (t.part * g.M + t.m_beg + 32 * (MI * wm + i) + e_l32) * g.ldp;
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
             *reinterpret_cast<uint32_t*>(to + 128 + 16 * ((c >> 4) ^ (row & 7)) + (c & 15)) = to_codes(b, iu);
           }
       }
-      if (GATED || g.parts == 1)
+      if (!PARTS || g.parts == 1)
 #pragma unroll
       for (int k = 0; k < NI; ++k)
 #pragma unroll
@@ -427,7 +427,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
           }
         }
       }
-      if (!GATED && g.parts > 1) continue;  // block-uniform
+      if (PARTS && g.parts > 1) continue;  // block-uniform
       lds_barrier();
       constexpr int CH = T::OUT_ROW / 16;  // chunks of a row
       const bool vec = g.ldo % 8 == 0 && ((uintptr_t)g.out & 15) == 0;
@@ -503,50 +503,47 @@ struct LinLaunch {
   }
 };
 
-// One shape of tile for all that leaves it.  FOUR: the plain product on four waves (those of MW NW MI NI, 2 x 2 of them)
-// instead of eight.
-template <int MW, int NW, int MI, int NI, bool Q4, bool FOUR = false>
+// One shape of tile for all that leaves it.  FOUR: the plain product of the whole contraction on four waves (2 x 2 of them)
+// instead of eight.  STEP: what a step of KW blocks of 64 takes, END: what a tile takes beside its steps, in 10 ns.
+template <int MW, int NW, int MI, int NI, bool Q4, int STEP, int END, bool FOUR = false>
 struct LinShape {
   typedef LinTile<8, MW, NW, MI, NI, Q4, LIN_STORE> T;
-  typedef LinLaunch<FOUR ? 4 : 8, FOUR ? 2 : MW, FOUR ? 2 : NW, FOUR ? T::M / 64 : MI, FOUR ? T::N / 64 : NI, Q4, LIN_STORE> Store;
+  typedef LinLaunch<8, MW, NW, MI, NI, Q4, LIN_STORE> Store;
+  typedef LinLaunch<FOUR ? 4 : 8, FOUR ? 2 : MW, FOUR ? 2 : NW, FOUR ? T::M / 64 : MI, FOUR ? T::N / 64 : NI, Q4, LIN_STORE> Whole;
   typedef LinLaunch<8, MW, NW, MI, NI, Q4, LIN_GATED> Gated;
   static constexpr bool CK8 = T::N == 256 && T::KW == 1;  // may keep 8-bit blocks
+  static constexpr int KW = T::KW;
 
   static void prepare() {
     Store::prepare();
+    Whole::prepare();
     Gated::prepare();
     if constexpr (CK8) LinLaunch<8, MW, NW, MI, NI, Q4, LIN_CK8>::prepare();
   }
   static int launch(const LinArgs& g, int dt, bool gated, hipStream_t st) {
-    if (!gated) return Store::launch(g, dt, st);
+    if (!gated) return g.parts > 1 ? Store::launch(g, dt, st) : Whole::launch(g, dt, st);
     if constexpr (CK8) {
       if (g.kept && g.kept_s) return LinLaunch<8, MW, NW, MI, NI, Q4, LIN_CK8>::launch(g, dt, st);
     }
     return Gated::launch(g, dt, st);
   }
-  // Cycles of a CU, roughly: a step is bound by its matrix instructions, by its lines (24 bytes a cycle) or, 4-bit,
-  // by the dequantization; a tile has its ends, and the last round of tiles counts whole.
-  static double cycles(const LinArgs& g, int dt, bool gated, int parts) {
-    const double steps = (double)((g.K / 64 + T::KW - 1) / T::KW) / parts;
-    const double mfma = 2.0 * MI * NI * 4 * 32, lines = (double)T::STAGE / 24;
-    const double codes = Q4 ? 2.0 * NI * 16 * (dt == USAF_BF16 ? 8 : 5) * 4 : 0;
-    const double step = (mfma + codes > lines ? mfma + codes : lines) + 250, tile = steps * step + 1500;
-    const double m = (double)((g.M + T::M - 1) / T::M), cols = gated ? T::N / 2 : T::N;
-    const double rounds = m * (double)(int64_t)((g.N + cols - 1) / cols) * parts / device_cu_count();
-    // fp32 sums of the parts: written and read at about 4 TB/s, and a launch
-    const double join = parts > 1 ? (double)parts * (double)g.M * (double)g.N * 8 / 2000 + 6000 : 0;
-    return tile * (rounds < 1 ? 1 : (double)(int64_t)(rounds + 0.999)) + join;
+  // Microseconds of a call: rounds of tiles over the CUs, the last one whole, and a launch.  The parts' fp32 sums are
+  // written and read at about 4 TB/s, in one more launch.
+  static double us(const LinArgs& g, bool gated, int parts) {
+    const int64_t steps = (g.K / 64 + T::KW - 1) / T::KW, cols = gated ? T::N / 2 : T::N;
+    const int64_t tiles = (g.M + T::M - 1) / T::M * ((g.N + cols - 1) / cols) * parts, cus = device_cu_count();
+    const double tile = 0.01 * ((double)((steps + parts - 1) / parts) * STEP + END);
+    return 3 + tile * (double)((tiles + cus - 1) / cus) + (parts > 1 ? 3 + (double)parts * (double)g.M * (double)g.N * 8 / 4e6 : 0);
   }
-  static constexpr int KW = T::KW;
 };
 
 template <class S>
-void consider(LinPlan& best, const LinArgs& g, int dt, bool gated) {
+void consider(LinPlan& best, const LinArgs& g, bool gated) {
   if (gated && g.kept && g.kept_s && !S::CK8) return;
   for (int parts = 1; parts <= (gated ? 1 : 16); parts *= 2) {
     if (parts > 1 && g.K / 64 < 4 * parts * S::KW) break;
-    const double c = S::cycles(g, dt, gated, parts);
-    if (best.launch == nullptr || c < best.cycles) best = {S::launch, parts, c};
+    const double us = S::us(g, gated, parts);
+    if (best.launch == nullptr || us < best.us) best = {S::launch, parts, us};
   }
 }
 

@@ -3,24 +3,24 @@
 
 namespace usaf {
 namespace {
-typedef LinShape<1, 8, 4, 1, true> Q128x256;
-typedef LinShape<1, 4, 4, 1, true> Q128x128;
-typedef LinShape<1, 4, 2, 1, true> Q64x128;
-typedef LinShape<1, 2, 2, 1, true> Q64x64;
-typedef LinShape<1, 8, 1, 1, true> Q32x256;
-typedef LinShape<1, 2, 1, 1, true> Q32x64;
-typedef LinShape<1, 1, 1, 1, true> Q32x32;
+typedef LinShape<1, 8, 4, 1, true, 132, 660> Q128x256;
+typedef LinShape<1, 4, 4, 1, true, 139, 470> Q128x128;
+typedef LinShape<1, 4, 2, 1, true, 103, 310> Q64x128;
+typedef LinShape<1, 2, 2, 1, true, 104, 260> Q64x64;
+typedef LinShape<1, 8, 1, 1, true, 88, 200> Q32x256;
+typedef LinShape<1, 2, 1, 1, true, 88, 160> Q32x64;
+typedef LinShape<1, 1, 1, 1, true, 89, 140> Q32x32;
 }  // namespace
 
-LinPlan plan_linear_q4(const LinArgs& g, int dt, bool gated) {
+LinPlan plan_linear_q4(const LinArgs& g, bool gated) {
   LinPlan best;
-  consider<Q128x256>(best, g, dt, gated);
-  consider<Q128x128>(best, g, dt, gated);
-  consider<Q64x128>(best, g, dt, gated);
-  consider<Q64x64>(best, g, dt, gated);
-  consider<Q32x256>(best, g, dt, gated);
-  consider<Q32x64>(best, g, dt, gated);
-  consider<Q32x32>(best, g, dt, gated);
+  consider<Q128x256>(best, g, gated);
+  consider<Q128x128>(best, g, gated);
+  consider<Q64x128>(best, g, gated);
+  consider<Q64x64>(best, g, gated);
+  consider<Q32x256>(best, g, gated);
+  consider<Q32x64>(best, g, gated);
+  consider<Q32x32>(best, g, gated);
   return best;
 }
 
