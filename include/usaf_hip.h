@@ -670,7 +670,7 @@ int usaf_hip_moe_few(const void* x, int64_t T, int64_t H, const void* router, in
 
 /*
  * Products with one 4-bit weight W [N, K], group size 128 along whole rows (K % 128 == 0): codes q as
- * usaf_hip_quantize_q4 packs them, sz usaf_hip_pack_scale_zero's words; its values are
+ * usaf_hip_quantize_q4 packs them, sz usaf_hip_pack_scale_zero's words by group, [K / 128, N]; its values are
  * usaf_hip_dequant_q4's of the activations' dtype (fp16 / bf16).
  *   usaf_hip_q4_linear      out [M, N] = dtype(x W^T), x [M, K] with row stride ld
  *   usaf_hip_q4_linear_bwd  dx [M, K] = dtype(dy W),   dy [M, N] with row stride ld
@@ -692,7 +692,8 @@ int usaf_hip_q4_linear_bwd(const void* dy, int32_t dtype, int64_t M, int64_t N, 
  *   usaf_hip_gated_bwd   dG = dtype(dact U s (1 + G (1 - s))), dU = dtype(dact G s), s = sigmoid(G), of the kept
  *     values; dx [M, K] = dtype([dG, dU] W) and, 16-bit weights, dw [2 I, K] = dtype([dG, dU]^T x), each where not NULL.
  *     dact [M, I] contiguous; x (row stride ldx) is read for dw only.
- * ws: usaf_hip_gated_ws_bytes with what = 0 for the forward, else 1 for dx + 2 for dw; 16-byte aligned.  Weights, kept and (K
+ * ws: usaf_hip_gated_ws_bytes with what = 0 for the forward, 4 for one with kept_scales, else 1 for dx + 2 for dw;
+ * 16-byte aligned.  Weights, kept and (K
  * % 64 == 0) rows of x 16-byte aligned.  2 I, K <= 2^22; K % 128 == 0 for 4-bit weights.
  */
 int64_t usaf_hip_gated_ws_bytes(int64_t M, int64_t I, int64_t K, int32_t four_bit, int32_t what);

@@ -223,8 +223,7 @@ def test_second_derivatives_tangents_and_traces(L):
 
 def test_workspaces_that_are_too_small(L):
     w, _ = _weight(256, 256)
-    x, sz = _x(600, 256, torch.float16).cuda(), None
-    sz = w.scale_zero()
+    x, sz = _x(600, 256, torch.float16).cuda(), L.words("", w)
     out = torch.empty(600, 256, dtype=torch.float16, device="cuda")
     need = N.load().usaf_hip_q4_linear_ws_bytes(600, 256, 256, 1)
     ws = torch.empty(need, dtype=torch.uint8, device="cuda")

@@ -111,7 +111,7 @@ def test_workspace_sizes():
     sizes, gated = lib.usaf_hip_q4_linear_ws_bytes, lib.usaf_hip_gated_ws_bytes
     for bad in [(-1, 64, 128, 0), (1, 0, 128, 0), (1, 64, 0, 0), (1, 1 << 23, 128, 0), (1 << 31, 64, 128, 0)]:
         assert sizes(*bad) == -1
-    for bad in [(-1, 64, 128, 0, 0), (1, 0, 128, 0, 0), (1, 64, 128, 0, 4), (1, 64, 128, 0, -1), (1, 1 << 22, 128, 0, 0)]:
+    for bad in [(-1, 64, 128, 0, 0), (1, 0, 128, 0, 0), (1, 64, 128, 0, 5), (1, 64, 128, 0, -1), (1, 1 << 22, 128, 0, 0)]:
         assert gated(*bad) == -1
     assert sizes(1, 4096, 4096, 0) == 0 and gated(1, 4096, 4096, 1, 0) == 0
     for m in (0, 1, 700):  # more is wanted, more is needed

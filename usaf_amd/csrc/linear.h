@@ -13,7 +13,7 @@ struct LinArgs {
   int64_t M, K;        // K % 64 == 0 (4-bit: % 128)
   const uint8_t* W;    // 16-bit rows or packed codes, ldw bytes apart (16-byte aligned, ldw too)
   int64_t ldw;
-  const uint32_t* sz;  // 4-bit: scale | zero << 16 of every group of 128, [rows, K / 128]
+  const uint32_t* sz;  // 4-bit: scale | zero << 16 of every group of 128, [K / 128, rows]
   int64_t N;           // columns of out; gated: W has 2 N rows, the gate's and then up's
   uint16_t* out;       // [M, ldo], act where gated
   int64_t ldo;

@@ -23,10 +23,11 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // 4-bit rows [rows, K] -> 16-bit rows: 8 codes a thread.
 template <int DT>
 __global__ __launch_bounds__(256) void q4_rows_kernel(const uint32_t* __restrict__ q, const uint32_t* __restrict__ sz,
-                                                      int64_t words, u32x4* __restrict__ out) {
+                                                      int64_t rows, int row_words, u32x4* __restrict__ out) {
   const int64_t stride = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += stride) {
-    const uint32_t p = sz[i >> 4];  // 16 words a group
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * row_words; i += stride) {
+    const int64_t n = i / row_words;
+    const uint32_t p = sz[((i - n * row_words) >> 4) * rows + n];  // 16 words a group
     const f16 s = __builtin_bit_cast(f16, (uint16_t)p), z = __builtin_bit_cast(f16, (uint16_t)(p >> 16));
     out[i] = dq8<DT>(q[i], f16x2{s, s}, f16x2{z, z});
   }
@@ -45,7 +46,7 @@ __global__ __launch_bounds__(256) void transpose_kernel(const void* __restrict__
     const int64_t c = c0 + 8 * cg;
     if (s >= S || c >= C) return uint4{0, 0, 0, 0};
     if constexpr (Q4) {
-      const uint32_t w = reinterpret_cast<const uint32_t*>(in)[(s * C + c) >> 3], p = sz[s * (C >> 7) + (c >> 7)];
+      const uint32_t w = reinterpret_cast<const uint32_t*>(in)[(s * C + c) >> 3], p = sz[(c >> 7) * S + s];
       const f16 sc = __builtin_bit_cast(f16, (uint16_t)p), z = __builtin_bit_cast(f16, (uint16_t)(p >> 16));
       const u32x4 v = dq8<DT>(w, f16x2{sc, sc}, f16x2{z, z});
       return uint4{v.x, v.y, v.z, v.w};
@@ -168,9 +169,9 @@ unsigned blocks_of(int64_t items, int per) {
 int q4_rows(const uint8_t* q, const uint32_t* sz, int64_t rows, int64_t K, int dt, void* out, hipStream_t st) {
   const int64_t words = rows * K / 8;
   if (dt == USAF_BF16)
-    q4_rows_kernel<USAF_BF16><<<blocks_of(words, 4), 256, 0, st>>>((const uint32_t*)q, sz, words, (u32x4*)out);
+    q4_rows_kernel<USAF_BF16><<<blocks_of(words, 4), 256, 0, st>>>((const uint32_t*)q, sz, rows, (int)(K / 8), (u32x4*)out);
   else
-    q4_rows_kernel<USAF_F16><<<blocks_of(words, 4), 256, 0, st>>>((const uint32_t*)q, sz, words, (u32x4*)out);
+    q4_rows_kernel<USAF_F16><<<blocks_of(words, 4), 256, 0, st>>>((const uint32_t*)q, sz, rows, (int)(K / 8), (u32x4*)out);
   return check_launch("linear: weight rows");
 }
 
@@ -208,8 +209,10 @@ LinArgs product(const void* a, int64_t lda, int64_t M, const void* w, int64_t ld
 
 // Whether a 4-bit weight of `rows` rows is multiplied as codes; else its 16-bit values are written once, to the workspace, and
 // multiplied: 2.5 bytes a weight at about 4 TB/s, and a launch.
-bool as_codes(int64_t M, int64_t rows, int64_t K, bool gated) {
-  const LinArgs g = product(nullptr, K, M, nullptr, K, gated ? rows / 2 : rows, K, nullptr, 0);
+bool as_codes(int64_t M, int64_t rows, int64_t K, bool gated, bool eight_bit = false) {
+  LinArgs g = product(nullptr, K, M, nullptr, K, gated ? rows / 2 : rows, K, nullptr, 0);
+  static uint8_t kept;  // (not read: that there is one decides which tiles may be taken)
+  if (eight_bit) g.kept = g.kept_s = &kept;
   return plan_linear_q4(g, gated).us <= plan_linear_dense(g, gated).us + (double)rows * (double)K * 2.5 / 4e6 + 3;
 }
 
@@ -286,13 +289,14 @@ struct GatedWs {
   Parts dx_parts, dw_parts;
   bool codes = false;
   int64_t bytes, kp, ldd, mp;
+  // what: 0 forward, 4 forward that keeps 8-bit blocks, else 1 for dx + 2 for dw
   GatedWs(void* ws, int64_t M, int64_t I, int64_t K, bool four_bit, int what) {
     Ws at(ws);
     kp = round_up(K, 64);
     ldd = round_up(2 * I, 64);
     mp = round_up(M, 64);
-    if (what == 0) {
-      codes = four_bit && (q4_small_ok(M, K) || as_codes(M, 2 * I, K, true));
+    if ((what & 3) == 0) {
+      codes = four_bit && (q4_small_ok(M, K) || as_codes(M, 2 * I, K, true, what == 4));
       if (four_bit ? !codes : kp != K) w = at.take(2 * 2 * I * kp);
       if (kp != K) x = at.take(2 * M * kp);
     } else {
@@ -399,7 +403,7 @@ static int gated_args(const char* what, int32_t dtype, int64_t M, int64_t I, int
 }
 
 extern "C" int64_t usaf_hip_gated_ws_bytes(int64_t M, int64_t I, int64_t K, int32_t four_bit, int32_t what) {
-  return sizes_ok(M, 2 * I, K) && what >= 0 && what <= 3 ? GatedWs(nullptr, M, I, K, four_bit != 0, what).bytes : -1;
+  return sizes_ok(M, 2 * I, K) && what >= 0 && what <= 4 ? GatedWs(nullptr, M, I, K, four_bit != 0, what).bytes : -1;
 }
 
 extern "C" int usaf_hip_gated_fwd(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* q,
@@ -409,7 +413,7 @@ extern "C" int usaf_hip_gated_fwd(const void* x, int32_t dtype, int64_t M, int64
   if (M == 0) return clear_error();
   if (!x || !act || (kept_scales && !kept)) return set_error(USAF_ERR_INVALID, "gated_fwd: null pointer");
   if (ld < K || ld > LIN_MAX) return set_error(USAF_ERR_INVALID, "gated_fwd: rows of %lld values, %lld apart", (long long)K, (long long)ld);
-  const GatedWs w(ws, M, I, K, q != nullptr, 0);
+  const GatedWs w(ws, M, I, K, q != nullptr, kept_scales ? 4 : 0);
   if ((uintptr_t)kept % 16 || (uintptr_t)act % 2 || (!w.x && ((uintptr_t)x % 16 || ld % 8)) || (uintptr_t)x % 2)
     return set_error(USAF_ERR_INVALID, "gated_fwd: rows and what is kept must be 16-byte aligned");
   if (int rc = check_ws("gated_fwd", ws, ws_bytes, w.bytes)) return rc;

@@ -81,7 +81,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
     int valid, nt, part, s_beg, s_end;
     int64_t m_beg;
   };
-  const int nkb = (int)(g.K / 64), all_steps = (nkb + KW - 1) / KW, groups = (int)(g.K / 128);
+  const int nkb = (int)(g.K / 64), all_steps = (nkb + KW - 1) / KW;
+  const int64_t s_row = 4 * (GATED ? 2 * g.N : g.N);  // bytes of a group's words
   auto place = [&](int unit) {
     constexpr int GROUP = 8;
     Place t;
@@ -132,11 +133,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
       }
     }
     if constexpr (Q4) {
-      s_base = uniform(reinterpret_cast<const uint8_t*>(g.sz + n0 * groups));
+      s_base = uniform(reinterpret_cast<const uint8_t*>(g.sz + n0));
 #pragma unroll
       for (int i = 0; i < T::S_DMA; ++i) {
         const int r = (64 * (T::SHARE * i + part) + lane) % T::N;
-        s_off[i] = (uint32_t)((column(r) + (GATED && (r & 16) ? up_rows : 0)) * groups * 4);
+        s_off[i] = (uint32_t)((column(r) + (GATED && (r & 16) ? up_rows : 0)) * 4);
       }
     }
   };
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
       g_dma16(from(i_a), a_off[i < T::A_DMA ? i : 0], to_lds(i_to + (T::SHARE * i + part) * 1024 % T::A_BYTES));
     } else if (p < T::DMAS) {
       const int i = p - T::W_DMA - T::A_DMA, s = (T::SHARE * i + part) % (T::S_WORDS > 0 ? T::S_WORDS : 1);
-      g_dma4(from(s_base + (i_k >> 1) * 4), s_off[i < T::S_DMA ? i : 0], to_lds(i_to + T::A_BYTES + T::W_BYTES + 256 * s));
+      g_dma4(from(s_base + (i_k >> 1) * s_row), s_off[i < T::S_DMA ? i : 0], to_lds(i_to + T::A_BYTES + T::W_BYTES + 256 * s));
     }
   };
   auto advance = [&]() {
@@ -184,6 +185,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
   //      both sides.  A slice is product j's of all the wave's blocks; the next slice's come while one is multiplied
   u32x4 wf[2][NI], af[2][MI], codes[Q4 ? NI : 1];
   uint32_t scale[Q4 ? NI : 1];
+  // fragment n of a slice's NI of the weights (4-bit: a step's codes, in front of its first slice) and MI of the slots
   auto load_one = [&](int stage, int j, int n, u32x4(&w)[NI], u32x4(&a)[MI]) {
     const uint8_t* const sa = sm + stage * T::STAGE + kw * T::SLAB;
     const uint8_t* const sw = sa + T::A_BYTES;
@@ -192,15 +194,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
     };
     if (n < NI) {
       const int k = n, r = 32 * (NI * wn + k) + l32;
-      if constexpr (Q4) {
-        if (j == 0) {
-          codes[k] = *reinterpret_cast<const u32x4*>(sw + r * 32 + 16 * (half ^ (r >> 3 & 1)));
-          scale[k] = reinterpret_cast<const uint32_t*>(sw + T::W_BYTES)[r];
-        }
-        const f16 s = __builtin_bit_cast(f16, (uint16_t)scale[k]), z = __builtin_bit_cast(f16, (uint16_t)(scale[k] >> 16));
-        w[k] = dq8<DT>(codes[k][j], f16x2{s, s}, f16x2{z, z});
-      } else {
+      if constexpr (!Q4) {
         w[k] = word(sw, r, 4 * half + j);
+      } else if (j == 0) {
+        codes[k] = *reinterpret_cast<const u32x4*>(sw + r * 32 + 16 * (half ^ (r >> 3 & 1)));
+        scale[k] = reinterpret_cast<const uint32_t*>(sw + T::W_BYTES)[r];
       }
     } else if (n < NI + MI) {
       a[n - NI] = word(sa, 32 * (MI * wm + n - NI) + l32, 4 * half + j);
@@ -209,6 +207,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
   auto load_slice = [&](int stage, int j, u32x4(&w)[NI], u32x4(&a)[MI]) {
 #pragma unroll
     for (int n = 0; n < NI + MI; ++n) load_one(stage, j, n, w, a);
+  };
+  // 4-bit: pair n of a slice's 4 NI
+  auto dequant = [&](int j, int n, u32x4(&w)[NI]) {
+    if constexpr (Q4) {
+      const int k = n >> 2;
+      const f16 s = __builtin_bit_cast(f16, (uint16_t)scale[k]), z = __builtin_bit_cast(f16, (uint16_t)(scale[k] >> 16));
+      w[k][n & 3] = dq_pair<DT>(codes[k][j], n & 3, f16x2{s, s}, f16x2{z, z});
+    }
   };
 
   f32x16 acc[MI][NI];
@@ -237,6 +243,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
   stage = T::NS - 1;
   next_stage();
   load_slice(0, 0, wf[0], af[0]);
+#pragma unroll
+  for (int n = 0; n < 4 * NI; ++n) dequant(0, n, wf[0]);
   begin();
   if (WAVES == 4) send(0, HALF);
   else if (early) send(0, T::DMAS);
@@ -259,12 +267,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
           if (j == 3) begin();
           if (early ? j == 3 : j == 0) send(0, T::DMAS);
           __builtin_amdgcn_sched_barrier(0);
-          if (mine_too) {
+          // 4-bit: the next slice's weights are dequantized between this one's products, 4 / MI pairs behind each
+          auto products = [&](auto with) {
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
+            for (int i = 0; i < MI; ++i) {
 #pragma unroll
-              for (int k = 0; k < NI; ++k) acc[i][k] = mfma32<DT>(w[k], x[i], acc[i][k]);
-          }
+              for (int k = 0; k < NI; ++k)
+                if constexpr (decltype(with)::value) acc[i][k] = mfma32<DT>(w[k], x[i], acc[i][k]);
+              if constexpr (Q4) {
+                if (MI > 1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int n = 4 * NI * i / MI; n < 4 * NI * (i + 1) / MI; ++n) dequant((j + 1) & 3, n, wf[(j + 1) & 1]);
+                if (MI > 1) __builtin_amdgcn_sched_barrier(0);
+              }
+            }
+          };
+          if (mine_too) products(std::true_type());
+          else products(std::false_type());
         } else {
           // one wave a SIMD: reads and DMAs in turn between the products
           static_assert(KW == 1 && 2 * (MI + NI) <= MI * NI && 2 * HALF <= MI * NI, "they fit between");

@@ -3,13 +3,13 @@
 
 namespace usaf {
 namespace {
-typedef LinShape<1, 8, 4, 1, true, 132, 660> Q128x256;
-typedef LinShape<1, 4, 4, 1, true, 139, 470> Q128x128;
-typedef LinShape<1, 4, 2, 1, true, 103, 310> Q64x128;
-typedef LinShape<1, 2, 2, 1, true, 104, 260> Q64x64;
-typedef LinShape<1, 8, 1, 1, true, 88, 200> Q32x256;
-typedef LinShape<1, 2, 1, 1, true, 88, 160> Q32x64;
-typedef LinShape<1, 1, 1, 1, true, 89, 140> Q32x32;
+typedef LinShape<1, 8, 4, 1, true, 120, 800> Q128x256;
+typedef LinShape<1, 4, 4, 1, true, 123, 500> Q128x128;
+typedef LinShape<1, 4, 2, 1, true, 93, 370> Q64x128;
+typedef LinShape<1, 2, 2, 1, true, 97, 260> Q64x64;
+typedef LinShape<1, 8, 1, 1, true, 80, 250> Q32x256;
+typedef LinShape<1, 2, 1, 1, true, 81, 150> Q32x64;
+typedef LinShape<1, 1, 1, 1, true, 79, 130> Q32x32;
 }  // namespace
 
 LinPlan plan_linear_q4(const LinArgs& g, bool gated) {

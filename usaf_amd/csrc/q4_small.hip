@@ -85,7 +85,8 @@ __global__ __launch_bounds__(QS_THREADS) void q4_small_kernel(const uint16_t* __
 
   // ---- the wave's loads: uniform places of the tile's first row, 32-bit lane offsets (rows past the last: that one again).
   //      Lane l of code instruction u has chunk l % 8 of row 8 u + l / 8; lanes of the scales' a row's two words
-  const int row_q = K / 2, row_s = 4 * groups;
+  const int row_q = K / 2;
+  const int64_t row_s = 4 * (GATED ? 2 * N : N);  // bytes of a group's words
   const uint8_t *l_q, *l_s;
   uint32_t o_q[2], o_s;
   int l_tile = blockIdx.x, l_i = 0, l_slot = 0;
@@ -93,16 +94,15 @@ __global__ __launch_bounds__(QS_THREADS) void q4_small_kernel(const uint16_t* __
     const int64_t n0 = (int64_t)(l_tile < tiles ? l_tile : tiles - 1) * QS_COLS;
     const int left = N - 1 - n0 < QS_COLS ? (int)(N - 1 - n0) : QS_COLS;
     l_q = q + (n0 + half * N) * row_q;
-    l_s = reinterpret_cast<const uint8_t*>(sz) + (n0 + half * N) * row_s;
-    const uint32_t most_q = (uint32_t)(left * row_q), most_s = (uint32_t)(left * row_s);
+    l_s = reinterpret_cast<const uint8_t*>(sz + n0 + half * N);
+    const uint32_t most_q = (uint32_t)(left * row_q);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int row = 8 * u + (lane >> 3);
       const uint32_t o = (uint32_t)(row * row_q);
       o_q[u] = (o < most_q ? o : most_q) + 16 * ((lane & 7) ^ g_swz(row));
     }
-    const uint32_t o = (uint32_t)(r * row_s);
-    o_s = (o < most_s ? o : most_s) + 4 * (quad & 1);
+    o_s = 4 * (uint32_t)(r < left ? r : left);
   };
   auto load = [&] {
     const int step = kw + WAVES * l_i, s = step < steps ? step : steps - 1;
@@ -110,10 +110,10 @@ __global__ __launch_bounds__(QS_THREADS) void q4_small_kernel(const uint16_t* __
     // an odd last group has half a line: its upper chunks are the lower ones again, the second scale is the first
     const bool odd = 2 * s + 1 == groups;
     const uint8_t* const at_q = uniform(l_q + s * 128);
-    const uint8_t* const at_s = uniform(l_s + s * 8);
+    const uint8_t* const at_s = uniform(l_s + 2 * s * row_s);
 #pragma unroll
     for (int u = 0; u < 2; ++u) g_dma16(at_q, odd ? o_q[u] - 16 * (((lane & 7) ^ g_swz(8 * u + (lane >> 3))) & 4) : o_q[u], to + 1024 * u);
-    g_dma4(at_s, odd ? o_s - 4 * (quad & 1) : o_s, to + 2048);
+    g_dma4(at_s, o_s + (!odd && (quad & 1) ? (uint32_t)row_s : 0), to + 2048);
     l_slot = l_slot + 1 == QS_DEPTH ? 0 : l_slot + 1;
     if (++l_i == per) {
       l_i = 0;

@@ -61,7 +61,7 @@ def _forward(x: torch.Tensor, w, checkpoint: Optional[str], keep: bool):
     if m:
         ptrs = _weight_ptrs(w)
         with on(dev):
-            need = _ws_bytes(dev.index, m, inter, k, int(isinstance(w, Q4Tensor)), 0)
+            need = _ws_bytes(dev.index, m, inter, k, int(isinstance(w, Q4Tensor)), 0 if scales is None else 4)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
             N.call("usaf_hip_gated_fwd", x.data_ptr(), N.dtype_code(x.dtype), m, k, _ld(x), *ptrs, inter, act.data_ptr(),
                    N.ptr(kept), N.ptr(scales), N.ptr(ws), max(need, 0), N.stream_ptr(dev))

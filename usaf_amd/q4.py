@@ -53,13 +53,19 @@ def check_weight(what: str, w: Q4Tensor) -> None:
 
 
 def words(what: str, w: Q4Tensor) -> torch.Tensor:
-    """w.scale_zero(), finished when first built, so that any stream may read it from then on."""
-    if w._sz is None or w._sz.device != w.device:
+    """The scale/zero words by group, int32 [K / 128, rows] (Q4Tensor.scale_zero_by_group's of one matrix): built once and
+    kept with the weight, finished when built, so that any stream may read them from then on."""
+    if w._szg is None or w._szg.device != w.device:
         N.refuse_capture(f"{what}: the first call on a weight")
+        rows, k = (int(d) for d in w.shape)
         with on(w.device):
-            w.scale_zero()
+            by_row = torch.empty(rows, k // 128, dtype=torch.int32, device=w.device)
+            N.call("usaf_hip_pack_scale_zero", w.s.data_ptr(), w.z.data_ptr(), by_row.numel(), by_row.data_ptr(),
+                   N.stream_ptr(w.device))
+            by_group = by_row.t().contiguous()
             torch.cuda.current_stream(w.device).synchronize()
-    return w._sz
+        w._szg = by_group
+    return w._szg
 
 
 def rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
