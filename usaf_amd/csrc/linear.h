@@ -37,7 +37,7 @@ struct LinPlan {
 LinPlan plan_linear_dense(const LinArgs& g, bool gated);
 LinPlan plan_linear_q4(const LinArgs& g, bool gated);
 // A few rows of a 4-bit weight's product, out [M, N] (ldo = N), nothing kept: whether it takes them, and its launch (q4_small.hip).
-bool q4_small_ok(int64_t M, int64_t K);
+bool q4_small_ok(int64_t M, int64_t N, int64_t K);
 int q4_small(const LinArgs& g, int dt, bool gated, hipStream_t st);
 void prepare_q4_small();
 void prepare_linear_dense();

@@ -24,12 +24,22 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 template <int DT>
 __global__ __launch_bounds__(256) void q4_rows_kernel(const uint32_t* __restrict__ q, const uint32_t* __restrict__ sz,
                                                       int64_t rows, int row_words, u32x4* __restrict__ out) {
-  const int64_t stride = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * row_words; i += stride) {
-    const int64_t n = i / row_words;
-    const uint32_t p = sz[((i - n * row_words) >> 4) * rows + n];  // 16 words a group
+  const int64_t stride = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  // (a division for each word would take as long as the word)
+  const int64_t down = stride / row_words;
+  const int right = (int)(stride - down * row_words);
+  int64_t n = first / row_words;
+  int c = (int)(first - n * row_words);
+  for (int64_t i = first; n < rows; i += stride) {
+    const uint32_t p = sz[(c >> 4) * rows + n];  // 16 words a group
     const f16 s = __builtin_bit_cast(f16, (uint16_t)p), z = __builtin_bit_cast(f16, (uint16_t)(p >> 16));
     out[i] = dq8<DT>(q[i], f16x2{s, s}, f16x2{z, z});
+    n += down;
+    c += right;
+    if (c >= row_words) {
+      c -= row_words;
+      ++n;
+    }
   }
 }
 
@@ -275,7 +285,7 @@ struct Q4LinearWs {
       w = at.take(2 * K * np);
       if (np != N) dy = at.take(2 * M * np);
       parts = Parts(at, M, K, np, false);
-    } else if (!q4_small_ok(M, K)) {
+    } else if (!q4_small_ok(M, N, K)) {
       if (!codes) w = at.take(2 * N * K);
       parts = Parts(at, M, N, K, codes);
     }
@@ -296,7 +306,7 @@ struct GatedWs {
     ldd = round_up(2 * I, 64);
     mp = round_up(M, 64);
     if ((what & 3) == 0) {
-      codes = four_bit && (q4_small_ok(M, K) || as_codes(M, 2 * I, K, true, what == 4));
+      codes = four_bit && (q4_small_ok(M, I, K) || as_codes(M, 2 * I, K, true, what == 4));
       if (four_bit ? !codes : kp != K) w = at.take(2 * 2 * I * kp);
       if (kp != K) x = at.take(2 * M * kp);
     } else {
@@ -360,11 +370,11 @@ extern "C" int usaf_hip_q4_linear(const void* x, int32_t dtype, int64_t M, int64
   const Q4LinearWs w(ws, M, N, K, false);
   if (int rc = check_ws("q4_linear", ws, ws_bytes, w.bytes)) return rc;
   hipStream_t st = as_stream(stream);
-  if (w.codes || q4_small_ok(M, K)) {
+  if (w.codes || q4_small_ok(M, N, K)) {
     LinArgs g = product(x, ld, M, q, 0, N, K, out, N);
     g.ldw = K / 2;
     g.sz = sz;
-    if (q4_small_ok(M, K)) return q4_small(g, dtype, false, st);
+    if (q4_small_ok(M, N, K)) return q4_small(g, dtype, false, st);
     return run(g, w.parts, dtype, st);
   }
   if (int rc = q4_rows(q, sz, N, K, dtype, w.w, st)) return rc;
@@ -428,7 +438,7 @@ extern "C" int usaf_hip_gated_fwd(const void* x, int32_t dtype, int64_t M, int64
     g.W = q;
     g.ldw = K / 2;
     g.sz = sz;
-    if (!kept && q4_small_ok(M, K)) return q4_small(g, dtype, true, st);
+    if (!kept && q4_small_ok(M, I, K)) return q4_small(g, dtype, true, st);
     return plan_linear_q4(g, true).launch(g, dtype, true, st);
   }
   if (q)

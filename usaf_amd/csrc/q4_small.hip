@@ -22,7 +22,11 @@ constexpr int QS_WAVES = 8, QS_THREADS = 64 * QS_WAVES;
 constexpr int QS_COLS = 16, QS_ROWS = 16;
 constexpr int QS_STEP = 2048 + 256;               // bytes of a wave's step: 16 weight rows' lines of codes, their scales twice
 constexpr int QS_DEPTH = 2;                       // steps of a wave in its ring
-constexpr int64_t QS_VALUES = 1 << 15;            // values of x that a block keeps
+// Values of x that a block keeps at most, and for how many a CU has room for a second block.  Measured (us, here / linear_kernel's
+// best tile, bf16, one behind the other in a graph): 1, 8, 16 rows of 2,048 to 4,096 outputs 4.3 / 7.4, 5.0 / 7.5, 5.8 / 7.5; 4, 12 of
+// 4,096 to 4,096 6.2 / 9.6, 7.5 / 9.6; 3 of 14,336 to 4,096 13.0 / 18.3; with many columns and one block a CU 8 of 4,096 to
+// 14,336 17.7 / 17.7, 12 19.2 / 17.4, 16 of 2,048 to 14,336 12.7 / 10.9.
+constexpr int64_t QS_VALUES = 3 << 14, QS_TWO = 1 << 14, QS_MANY = 8192;
 
 template <int DT>
 __device__ __forceinline__ f32x4 mfma16(const u32x4 a, const u32x4 b, f32x4 c) {
@@ -230,7 +234,9 @@ void launch(const LinArgs& g, hipStream_t st) {
 
 }  // namespace
 
-bool q4_small_ok(int64_t M, int64_t K) { return M >= 1 && M <= QS_ROWS && M * K <= QS_VALUES; }
+bool q4_small_ok(int64_t M, int64_t N, int64_t K) {
+  return M >= 1 && M <= QS_ROWS && M * K <= (N <= QS_MANY ? QS_VALUES : QS_TWO);
+}
 
 int q4_small(const LinArgs& g, int dt, bool gated, hipStream_t st) {
   if (dt == USAF_BF16) {
