@@ -44,108 +44,165 @@ __global__ __launch_bounds__(256) void q4_rows_kernel(const uint32_t* __restrict
 }
 
 // [S, C] (16-bit, row stride ld; or 4-bit codes, C = K) -> [C, ldo], zeros for s in [S, ldo); ldo % 64 == 0.  A block
-// has 64 x 64 values.
+// has 64 x 64 values; blocks from `first` on are the second matrix's (16-bit): one launch for both.
+struct Transpose {
+  const void* in;
+  int64_t S, C, ld;
+  uint16_t* out;
+  int64_t ldo;
+  int wide;  // blocks along S
+  bool vec;
+};
 template <int DT, bool Q4>
-__global__ __launch_bounds__(256) void transpose_kernel(const void* __restrict__ in, const uint32_t* __restrict__ sz, int64_t S,
-                                                        int64_t C, int64_t ld, bool vec, uint16_t* __restrict__ out,
-                                                        int64_t ldo) {
+__global__ __launch_bounds__(256) void transpose_kernel(const Transpose a, const uint32_t* __restrict__ sz, int64_t first,
+                                                        const Transpose b) {
   __shared__ __align__(16) uint32_t tile[TT_DWORDS];
-  const int64_t s0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
+  const bool second = blockIdx.x >= first;  // block-uniform
+  const Transpose& t = second ? b : a;
+  const int64_t at = blockIdx.x - (second ? first : 0), tall = at / t.wide;
+  const int64_t s0 = (at - tall * t.wide) * 64, c0 = tall * 64;
   const int sp = threadIdx.x >> 3, cg = threadIdx.x & 7;
   auto row = [&](int64_t s) -> uint4 {
     const int64_t c = c0 + 8 * cg;
-    if (s >= S || c >= C) return uint4{0, 0, 0, 0};
+    if (s >= t.S || c >= t.C) return uint4{0, 0, 0, 0};
     if constexpr (Q4) {
-      const uint32_t w = reinterpret_cast<const uint32_t*>(in)[(s * C + c) >> 3], p = sz[(c >> 7) * S + s];
-      const f16 sc = __builtin_bit_cast(f16, (uint16_t)p), z = __builtin_bit_cast(f16, (uint16_t)(p >> 16));
-      const u32x4 v = dq8<DT>(w, f16x2{sc, sc}, f16x2{z, z});
-      return uint4{v.x, v.y, v.z, v.w};
-    } else {
-      const uint16_t* const p = reinterpret_cast<const uint16_t*>(in) + s * ld + c;
-      if (vec) return *reinterpret_cast<const uint4*>(p);  // C % 8 == 0
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = (c + 2 * j < C ? (uint32_t)p[2 * j] : 0u) | (c + 2 * j + 1 < C ? (uint32_t)p[2 * j + 1] << 16 : 0u);
-      return uint4{w[0], w[1], w[2], w[3]};
+      if (!second) {
+        const uint32_t w = reinterpret_cast<const uint32_t*>(t.in)[(s * t.C + c) >> 3], p = sz[(c >> 7) * t.S + s];
+        const f16 sc = __builtin_bit_cast(f16, (uint16_t)p), z = __builtin_bit_cast(f16, (uint16_t)(p >> 16));
+        const u32x4 v = dq8<DT>(w, f16x2{sc, sc}, f16x2{z, z});
+        return uint4{v.x, v.y, v.z, v.w};
+      }
     }
+    const uint16_t* const p = reinterpret_cast<const uint16_t*>(t.in) + s * t.ld + c;
+    if (t.vec) return *reinterpret_cast<const uint4*>(p);  // C % 8 == 0
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = (c + 2 * j < t.C ? (uint32_t)p[2 * j] : 0u) | (c + 2 * j + 1 < t.C ? (uint32_t)p[2 * j + 1] << 16 : 0u);
+    return uint4{w[0], w[1], w[2], w[3]};
   };
   tt_write(tile, sp, cg, row(s0 + 2 * sp), row(s0 + 2 * sp + 1));
   __syncthreads();
 #pragma unroll
   for (int it = 0; it < 2; ++it) {
     const int v = threadIdx.x + 256 * it, cl = v >> 3, sg = v & 7;
-    if (c0 + cl < C) *reinterpret_cast<uint4*>(out + (c0 + cl) * ldo + s0 + 8 * sg) = tt_read(tile, cl, sg);
+    if (c0 + cl < t.C) *reinterpret_cast<uint4*>(t.out + (c0 + cl) * t.ldo + s0 + 8 * sg) = tt_read(tile, cl, sg);
   }
 }
 
-// [rows, C] -> [rows, ldo] with zeros behind column C; ldo % 8 == 0.
-__global__ __launch_bounds__(256) void pad_kernel(const uint16_t* __restrict__ in, int64_t rows, int64_t C, int64_t ld,
-                                                  uint16_t* __restrict__ out, int64_t ldo) {
-  const int64_t chunks = ldo / 8, n = rows * chunks, stride = (int64_t)gridDim.x * 256;
+// [rows, C] -> [rows, ldo] with zeros behind column C; ldo % 8 == 0.  Two matrices of as many columns, one behind the other.
+__global__ __launch_bounds__(256) void pad_kernel(const uint16_t* __restrict__ a, int64_t rows_a, int64_t ld_a,
+                                                  uint16_t* __restrict__ out_a, const uint16_t* __restrict__ b, int64_t rows_b,
+                                                  int64_t ld_b, uint16_t* __restrict__ out_b, int64_t C, int64_t ldo) {
+  const int64_t chunks = ldo / 8, n = (rows_a + rows_b) * chunks, stride = (int64_t)gridDim.x * 256;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
-    const int64_t r = i / chunks, c = 8 * (i - r * chunks);
-    const uint16_t* const p = in + r * ld + c;
+    const int64_t row = i / chunks, c = 8 * (i - row * chunks);
+    const bool second = row >= rows_a;
+    const int64_t r = second ? row - rows_a : row;
+    const uint16_t* const p = (second ? b + r * ld_b : a + r * ld_a) + c;
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       w[j] = (c + 2 * j < C ? (uint32_t)p[2 * j] : 0u) | (c + 2 * j + 1 < C ? (uint32_t)p[2 * j + 1] << 16 : 0u);
-    *reinterpret_cast<uint4*>(out + r * ldo + c) = uint4{w[0], w[1], w[2], w[3]};
+    *reinterpret_cast<uint4*>((second ? out_b : out_a) + r * ldo + c) = uint4{w[0], w[1], w[2], w[3]};
   }
 }
 
 // ---- the gated activation's backward ---------------------------------------------
 
-// dact [M, I], kept -> dgu [M, ldd] = [dG, dU, zeros]: 8 columns of both a thread.
+struct GatedBwd {
+  const uint16_t* dact;   // [M, I]
+  const void* kept;
+  const uint8_t* kept_s;
+  int64_t M, I, hs;
+  bool vec;               // I % 8 == 0 and dact 16-byte aligned
+  uint16_t* dgu;          // [M, ldd] = [dG, dU, zeros]
+  int64_t ldd;
+};
+
+// 8 columns from c on of row m: dG and dU, to dgu too.
 template <int DT, bool EIGHT>
-__global__ __launch_bounds__(256) void gated_bwd_kernel(const uint16_t* __restrict__ dact, const void* __restrict__ kept,
-                                                        const uint8_t* __restrict__ kept_s, int64_t M, int64_t I, int64_t hs,
-                                                        bool vec, uint16_t* __restrict__ dgu, int64_t ldd) {
-  const int64_t chunks = (I + 7) / 8, n = M * chunks, stride = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
-    const int64_t m = i / chunks, c = 8 * (i - m * chunks), left = I - c;
-    float da[8], gate[8], up[8], dg[8], du[8];
-    load8<DT>(dact + m * I + c, vec, left > 8 ? 8 : (int)left, da);
-    if constexpr (EIGHT) {
-      const uint8_t* const p = reinterpret_cast<const uint8_t*>(kept) + 2 * m * hs + c;
-      const int64_t nb = hs / 128, at = 2 * m * nb + (c >> 7);
-      const float sg = __uint_as_float((uint32_t)kept_s[at] << 23), su = __uint_as_float((uint32_t)kept_s[at + nb] << 23);
-      const uint2 g8 = *reinterpret_cast<const uint2*>(p), u8 = *reinterpret_cast<const uint2*>(p + hs);
+__device__ __forceinline__ void gated_bwd8(const GatedBwd& g, int64_t m, int64_t c, uint4& dg4, uint4& du4) {
+  const int64_t left = g.I - c;
+  float da[8], gate[8], up[8], dg[8], du[8];
+  load8<DT>(g.dact + m * g.I + c, g.vec, left > 8 ? 8 : (int)left, da);
+  if constexpr (EIGHT) {
+    const uint8_t* const p = reinterpret_cast<const uint8_t*>(g.kept) + 2 * m * g.hs + c;
+    const int64_t nb = g.hs / 128, at = 2 * m * nb + (c >> 7);
+    const float sg = __uint_as_float((uint32_t)g.kept_s[at] << 23), su = __uint_as_float((uint32_t)g.kept_s[at + nb] << 23);
+    const uint2 g8 = *reinterpret_cast<const uint2*>(p), u8 = *reinterpret_cast<const uint2*>(p + g.hs);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int wg = (int)(j < 2 ? g8.x : g8.y), wu = (int)(j < 2 ? u8.x : u8.y);
-        const f32x2 a = j & 1 ? __builtin_amdgcn_cvt_pk_f32_fp8(wg, true) : __builtin_amdgcn_cvt_pk_f32_fp8(wg, false);
-        const f32x2 b = j & 1 ? __builtin_amdgcn_cvt_pk_f32_fp8(wu, true) : __builtin_amdgcn_cvt_pk_f32_fp8(wu, false);
-        gate[2 * j] = a.x * sg;
-        gate[2 * j + 1] = a.y * sg;
-        up[2 * j] = b.x * su;
-        up[2 * j + 1] = b.y * su;
+    for (int j = 0; j < 4; ++j) {
+      const int wg = (int)(j < 2 ? g8.x : g8.y), wu = (int)(j < 2 ? u8.x : u8.y);
+      const f32x2 a = j & 1 ? __builtin_amdgcn_cvt_pk_f32_fp8(wg, true) : __builtin_amdgcn_cvt_pk_f32_fp8(wg, false);
+      const f32x2 b = j & 1 ? __builtin_amdgcn_cvt_pk_f32_fp8(wu, true) : __builtin_amdgcn_cvt_pk_f32_fp8(wu, false);
+      gate[2 * j] = a.x * sg;
+      gate[2 * j + 1] = a.y * sg;
+      up[2 * j] = b.x * su;
+      up[2 * j + 1] = b.y * su;
+    }
+  } else {
+    const uint16_t* const p = reinterpret_cast<const uint16_t*>(g.kept) + 2 * m * g.hs + c;
+    unpack8<DT>(*reinterpret_cast<const uint4*>(p), gate);
+    unpack8<DT>(*reinterpret_cast<const uint4*>(p + g.hs), up);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * gate[j]));
+    dg[j] = da[j] * up[j] * s * (1.0f + gate[j] * (1.0f - s));
+    du[j] = da[j] * gate[j] * s;
+  }
+  dg4 = uint4{pack2<DT>(dg[0], dg[1]), pack2<DT>(dg[2], dg[3]), pack2<DT>(dg[4], dg[5]), pack2<DT>(dg[6], dg[7])};
+  du4 = uint4{pack2<DT>(du[0], du[1]), pack2<DT>(du[2], du[3]), pack2<DT>(du[4], du[5]), pack2<DT>(du[6], du[7])};
+  uint16_t* const to = g.dgu + m * g.ldd + c;
+  if (g.vec) {
+    *reinterpret_cast<uint4*>(to) = dg4;
+    *reinterpret_cast<uint4*>(to + g.I) = du4;
+  } else {
+    const uint32_t wg[4] = {dg4.x, dg4.y, dg4.z, dg4.w}, wu[4] = {du4.x, du4.y, du4.z, du4.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < left) {
+        to[j] = (uint16_t)(wg[j >> 1] >> (16 * (j & 1)));
+        to[g.I + j] = (uint16_t)(wu[j >> 1] >> (16 * (j & 1)));
       }
-    } else {
-      const uint16_t* const p = reinterpret_cast<const uint16_t*>(kept) + 2 * m * hs + c;
-      unpack8<DT>(*reinterpret_cast<const uint4*>(p), gate);
-      unpack8<DT>(*reinterpret_cast<const uint4*>(p + hs), up);
-    }
+  }
+  if (left <= 8)
+    for (int64_t k = 2 * g.I; k < g.ldd; ++k) g.dgu[m * g.ldd + k] = 0;
+}
+
+template <int DT, bool EIGHT>
+__global__ __launch_bounds__(256) void gated_bwd_kernel(const GatedBwd g) {
+  const int64_t chunks = (g.I + 7) / 8, n = g.M * chunks, stride = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+    const int64_t m = i / chunks;
+    uint4 dg, du;
+    gated_bwd8<DT, EIGHT>(g, m, 8 * (i - m * chunks), dg, du);
+  }
+}
+
+// The same with dgu's transpose [2 I, mp] beside it (zeros for m in [M, mp), mp % 64 == 0), which the weight gradient
+// reads: 64 tokens x 64 columns a block.
+template <int DT, bool EIGHT>
+__global__ __launch_bounds__(256) void gated_bwd_t_kernel(const GatedBwd g, uint16_t* __restrict__ dgut, int64_t mp, int wide) {
+  __shared__ __align__(16) uint32_t tiles[2][TT_DWORDS];
+  const int64_t tall = blockIdx.x / wide, m0 = (blockIdx.x - tall * wide) * 64, c0 = tall * 64;
+  const int sp = threadIdx.x >> 3, cg = threadIdx.x & 7;
+  uint4 dg[2], du[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * gate[j]));
-      dg[j] = da[j] * up[j] * s * (1.0f + gate[j] * (1.0f - s));
-      du[j] = da[j] * gate[j] * s;
-    }
-    uint16_t* const to = dgu + m * ldd + c;
-    if (vec) {  // I % 8 == 0
-      *reinterpret_cast<uint4*>(to) = uint4{pack2<DT>(dg[0], dg[1]), pack2<DT>(dg[2], dg[3]), pack2<DT>(dg[4], dg[5]), pack2<DT>(dg[6], dg[7])};
-      *reinterpret_cast<uint4*>(to + I) = uint4{pack2<DT>(du[0], du[1]), pack2<DT>(du[2], du[3]), pack2<DT>(du[4], du[5]), pack2<DT>(du[6], du[7])};
-    } else {
+  for (int u = 0; u < 2; ++u) {
+    const int64_t m = m0 + 2 * sp + u, c = c0 + 8 * cg;
+    dg[u] = du[u] = uint4{0, 0, 0, 0};
+    if (m < g.M && c < g.I) gated_bwd8<DT, EIGHT>(g, m, c, dg[u], du[u]);
+  }
+  tt_write(tiles[0], sp, cg, dg[0], dg[1]);
+  tt_write(tiles[1], sp, cg, du[0], du[1]);
+  __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < left) {
-          store_from_f32<DT>(to, j, dg[j]);
-          store_from_f32<DT>(to + I, j, du[j]);
-        }
-    }
-    if (left <= 8)
-      for (int64_t k = 2 * I; k < ldd; ++k) dgu[m * ldd + k] = 0;
+  for (int it = 0; it < 4; ++it) {
+    const int v = threadIdx.x + 256 * (it & 1), cl = v >> 3, sg = v & 7;
+    if (c0 + cl < g.I)
+      *reinterpret_cast<uint4*>(dgut + ((it >> 1) * g.I + c0 + cl) * mp + m0 + 8 * sg) = tt_read(tiles[it >> 1], cl, sg);
   }
 }
 
@@ -185,21 +242,39 @@ int q4_rows(const uint8_t* q, const uint32_t* sz, int64_t rows, int64_t K, int d
   return check_launch("linear: weight rows");
 }
 
-// sz: in is 4-bit codes.
-int transpose(const void* in, const uint32_t* sz, int64_t S, int64_t C, int64_t ld, int dt, void* out, int64_t ldo,
-              hipStream_t st) {
-  const dim3 grid((unsigned)(ldo / 64), (unsigned)((C + 63) / 64));
-  const bool vec = C % 8 == 0 && ld % 8 == 0 && (uintptr_t)in % 16 == 0;
-  if (grid.y > 65535) return set_error(USAF_ERR_UNSUPPORTED, "linear: more than %d columns", 65535 * 64);
-  if (!sz) transpose_kernel<USAF_BF16, false><<<grid, 256, 0, st>>>(in, sz, S, C, ld, vec, (uint16_t*)out, ldo);
-  else if (dt == USAF_BF16) transpose_kernel<USAF_BF16, true><<<grid, 256, 0, st>>>(in, sz, S, C, ld, vec, (uint16_t*)out, ldo);
-  else transpose_kernel<USAF_F16, true><<<grid, 256, 0, st>>>(in, sz, S, C, ld, vec, (uint16_t*)out, ldo);
+Transpose transpose_of(const void* in, int64_t S, int64_t C, int64_t ld, void* out, int64_t ldo) {
+  return {in, S, C, ld, reinterpret_cast<uint16_t*>(out), ldo, (int)(ldo / 64), C % 8 == 0 && ld % 8 == 0 && (uintptr_t)in % 16 == 0};
+}
+int64_t blocks_of(const Transpose& t) { return t.in ? t.wide * ((t.C + 63) / 64) : 0; }
+
+// a and b, each where its `in` is not null; sz: a is 4-bit codes.
+int transpose(const Transpose& a, const uint32_t* sz, const Transpose& b, int dt, hipStream_t st) {
+  const int64_t first = blocks_of(a), all = first + blocks_of(b);
+  if (all == 0) return USAF_OK;
+  if (all > 0x7FFFFFFF) return set_error(USAF_ERR_UNSUPPORTED, "linear: too large a transpose");
+  if (!sz) transpose_kernel<USAF_BF16, false><<<(unsigned)all, 256, 0, st>>>(a, sz, first, b);
+  else if (dt == USAF_BF16) transpose_kernel<USAF_BF16, true><<<(unsigned)all, 256, 0, st>>>(a, sz, first, b);
+  else transpose_kernel<USAF_F16, true><<<(unsigned)all, 256, 0, st>>>(a, sz, first, b);
   return check_launch("linear: transpose");
 }
 
-int pad(const void* in, int64_t rows, int64_t C, int64_t ld, void* out, int64_t ldo, hipStream_t st) {
-  pad_kernel<<<blocks_of(rows * (ldo / 8), 1), 256, 0, st>>>((const uint16_t*)in, rows, C, ld, (uint16_t*)out, ldo);
+int pad(const void* a, int64_t rows_a, int64_t ld_a, void* out_a, const void* b, int64_t rows_b, int64_t ld_b, void* out_b,
+        int64_t C, int64_t ldo, hipStream_t st) {
+  pad_kernel<<<blocks_of((rows_a + rows_b) * (ldo / 8), 1), 256, 0, st>>>(
+      (const uint16_t*)a, rows_a, ld_a, (uint16_t*)out_a, (const uint16_t*)b, rows_b, ld_b, (uint16_t*)out_b, C, ldo);
   return check_launch("linear: pad");
+}
+
+template <int DT, bool EIGHT>
+int gated_bwd(const GatedBwd& g, void* dgut, int64_t mp, hipStream_t st) {
+  if (dgut) {
+    const int64_t wide = mp / 64, blocks = wide * ((g.I + 63) / 64);
+    if (blocks > 0x7FFFFFFF) return set_error(USAF_ERR_UNSUPPORTED, "gated_bwd: too large");
+    gated_bwd_t_kernel<DT, EIGHT><<<(unsigned)blocks, 256, 0, st>>>(g, reinterpret_cast<uint16_t*>(dgut), mp, (int)wide);
+  } else {
+    gated_bwd_kernel<DT, EIGHT><<<blocks_of(g.M * ((g.I + 7) / 8), 1), 256, 0, st>>>(g);
+  }
+  return check_launch("gated_bwd");
 }
 
 // C = A W^T of 16-bit operands, contraction K % 64 == 0.
@@ -389,9 +464,9 @@ extern "C" int usaf_hip_q4_linear_bwd(const void* dy, int32_t dtype, int64_t M, 
   if (int rc = check_ws("q4_linear_bwd", ws, ws_bytes, w.bytes)) return rc;
   if (!w.dy && ((uintptr_t)dy % 16 || ld % 8)) return set_error(USAF_ERR_INVALID, "q4_linear_bwd: rows must be 16-byte aligned");
   hipStream_t st = as_stream(stream);
-  if (int rc = transpose(q, sz, N, K, K, dtype, w.w, w.np, st)) return rc;
+  if (int rc = transpose(transpose_of(q, N, K, K, w.w, w.np), sz, Transpose{}, dtype, st)) return rc;
   if (w.dy)
-    if (int rc = pad(dy, M, N, ld, w.dy, w.np, st)) return rc;
+    if (int rc = pad(dy, M, ld, w.dy, nullptr, 0, 0, nullptr, N, w.np, st)) return rc;
   return run(product(w.dy ? w.dy : dy, w.dy ? w.np : ld, M, w.w, w.np, K, w.np, dx, K), w.parts, dtype, st);
 }
 
@@ -428,8 +503,8 @@ extern "C" int usaf_hip_gated_fwd(const void* x, int32_t dtype, int64_t M, int64
     return set_error(USAF_ERR_INVALID, "gated_fwd: rows and what is kept must be 16-byte aligned");
   if (int rc = check_ws("gated_fwd", ws, ws_bytes, w.bytes)) return rc;
   hipStream_t st = as_stream(stream);
-  if (w.x)
-    if (int rc = pad(x, M, K, ld, w.x, w.kp, st)) return rc;
+  if (w.x)  // (then the weight is a 16-bit one, padded as well)
+    if (int rc = pad(x, M, ld, w.x, w16, 2 * I, K, w.w, K, w.kp, st)) return rc;
   LinArgs g = product(w.x ? w.x : x, w.x ? w.kp : ld, M, w.w ? w.w : w16, w.kp, I, w.kp, act, I);
   g.kept = kept;
   g.kept_s = kept_scales;
@@ -443,8 +518,6 @@ extern "C" int usaf_hip_gated_fwd(const void* x, int32_t dtype, int64_t M, int64
   }
   if (q)
     if (int rc = q4_rows(q, sz, 2 * I, K, dtype, w.w, st)) return rc;
-  if (!q && w.w)
-    if (int rc = pad(w16, 2 * I, K, K, w.w, w.kp, st)) return rc;
   return plan_linear_dense(g, true).launch(g, dtype, true, st);
 }
 
@@ -461,28 +534,17 @@ extern "C" int usaf_hip_gated_bwd(const void* dact, int32_t dtype, int64_t M, in
   const GatedWs w(ws, M, I, K, q != nullptr, (dx ? 1 : 0) | (dw ? 2 : 0));
   if (int rc = check_ws("gated_bwd", ws, ws_bytes, w.bytes)) return rc;
   hipStream_t st = as_stream(stream);
-  const int64_t hs = round_up(I, kept_scales ? 128 : 8), items = M * ((I + 7) / 8);
-  const bool vec = I % 8 == 0 && (uintptr_t)dact % 16 == 0;
-#define USAF_GATED_BWD(DT, EIGHT)                                                                                          \
-  gated_bwd_kernel<DT, EIGHT><<<blocks_of(items, 1), 256, 0, st>>>((const uint16_t*)dact, kept, kept_scales, M, I, hs, vec, \
-                                                                   (uint16_t*)w.dgu, w.ldd)
-  if (dtype == USAF_BF16) {
-    if (kept_scales) USAF_GATED_BWD(USAF_BF16, true);
-    else USAF_GATED_BWD(USAF_BF16, false);
-  } else {
-    if (kept_scales) USAF_GATED_BWD(USAF_F16, true);
-    else USAF_GATED_BWD(USAF_F16, false);
-  }
-#undef USAF_GATED_BWD
-  if (int rc = check_launch("gated_bwd")) return rc;
-  if (dx) {
-    if (int rc = transpose(q ? (const void*)q : w16, q ? sz : nullptr, 2 * I, K, K, dtype, w.wt, w.ldd, st)) return rc;
-    if (int rc = run(product(w.dgu, w.ldd, M, w.wt, w.ldd, K, w.ldd, dx, K), w.dx_parts, dtype, st)) return rc;
-  }
-  if (dw) {
-    if (int rc = transpose(w.dgu, nullptr, M, 2 * I, w.ldd, dtype, w.dgut, w.mp, st)) return rc;
-    if (int rc = transpose(x, nullptr, M, K, ldx, dtype, w.xt, w.mp, st)) return rc;
-    return run(product(w.dgut, w.mp, 2 * I, w.xt, w.mp, K, w.mp, dw, K), w.dw_parts, dtype, st);
-  }
+  GatedBwd g{reinterpret_cast<const uint16_t*>(dact), kept, kept_scales, M, I, round_up(I, kept_scales ? 128 : 8),
+             I % 8 == 0 && (uintptr_t)dact % 16 == 0, reinterpret_cast<uint16_t*>(w.dgu), w.ldd};
+  const int rc = dtype == USAF_BF16
+                     ? (kept_scales ? gated_bwd<USAF_BF16, true>(g, w.dgut, w.mp, st) : gated_bwd<USAF_BF16, false>(g, w.dgut, w.mp, st))
+                     : (kept_scales ? gated_bwd<USAF_F16, true>(g, w.dgut, w.mp, st) : gated_bwd<USAF_F16, false>(g, w.dgut, w.mp, st));
+  if (rc) return rc;
+  const Transpose wt = dx ? transpose_of(q ? (const void*)q : w16, 2 * I, K, K, w.wt, w.ldd) : Transpose{};
+  const Transpose xt = dw ? transpose_of(x, M, K, ldx, w.xt, w.mp) : Transpose{};
+  if (int rc2 = transpose(wt, q ? sz : nullptr, xt, dtype, st)) return rc2;
+  if (dx)
+    if (int rc2 = run(product(w.dgu, w.ldd, M, w.wt, w.ldd, K, w.ldd, dx, K), w.dx_parts, dtype, st)) return rc2;
+  if (dw) return run(product(w.dgut, w.mp, 2 * I, w.xt, w.mp, K, w.mp, dw, K), w.dw_parts, dtype, st);
   return clear_error();
 }
