@@ -4,7 +4,7 @@
 namespace usaf {
 namespace {
 typedef LinShape<2, 4, 4, 2, false, 163, 700, true> D256x256;
-typedef LinShape<2, 4, 2, 2, false, 95, 450> D128x256;
+typedef LinShape<2, 4, 2, 2, false, 90, 450> D128x256;
 typedef LinShape<2, 4, 2, 1, false, 56, 350> D128x128;
 typedef LinShape<2, 4, 1, 1, false, 33, 250> D64x128;
 typedef LinShape<2, 2, 1, 1, false, 40, 250> D64x64;

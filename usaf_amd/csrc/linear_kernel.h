@@ -45,9 +45,11 @@ struct LinTile {
   static constexpr int RED = KW > 1 ? WAVES * NI * 16 * 64 * 4 : 0;
   static constexpr int OUT_ROW = 2 * COLS, KEPT_ROW = EPI == LIN_GATED ? 2 * N : EPI == LIN_CK8 ? N : 0;
   static constexpr int SLOT_ENDS = OUT_ROW + KEPT_ROW;
-  static constexpr int EW = KW > 1 || 32 * MW * SLOT_ENDS <= 32 * 1024 ? MW : 1, ER = 32 * EW;
+  // (of one wave row's slots where that leaves room for one more stage)
+  static constexpr int stages(int ew) { return (160 * 1024 - RED - 32 * ew * SLOT_ENDS) / STAGE; }
+  static constexpr int EW = KW > 1 || EPI == LIN_CK8 || stages(MW) == stages(1) || stages(MW) >= 4 ? MW : 1, ER = 32 * EW;
   static constexpr int ENDS = RED + ER * SLOT_ENDS;
-    static constexpr int FIT = (160 * 1024 - ENDS) / STAGE, NS = FIT > 4 ? 4 : FIT;
+  static constexpr int NS = stages(EW) > 4 ? 4 : stages(EW);
   static constexpr int LDS = NS * STAGE + ENDS;
   // DMA instructions of a wave and step: the rows of its own k-block, shared by the MW NW waves that have it
   static constexpr int SHARE = MW * NW;
