@@ -28,12 +28,19 @@ def _ws_bytes(device: int, m: int, n: int, k: int, backward: int) -> int:
     return N.load().usaf_hip_q4_linear_ws_bytes(m, n, k, backward)
 
 
+def _versions(w: Q4Tensor):
+    """Counts of the writes to the scales and zeros (tensors made in inference mode have none)."""
+    return tuple(None if t.is_inference() else t._version for t in (w.s, w.z))
+
+
 def check_weight(what: str, w: Q4Tensor) -> None:
     """Raise unless w is a 4-bit matrix in the layout that the products read (looked at once for each set of tensors: 5 us)."""
-    parts = (w.q, w.s, w.z, w.shape, w.group_size)
+    parts = (w.q, w.s, w.z, w.shape, w.group_size, *_versions(w))
     seen = w.__dict__.get("_seen")
-    if seen is not None and all(a is b for a, b in zip(seen, parts)):
-        return
+    if seen is not None:
+        if all(a is b or a == b for a, b in zip(seen[3:], parts[3:])) and all(a is b for a, b in zip(seen[:3], parts[:3])):
+            return
+        w._szg = None  # not what its words were built from
     if len(w.shape) != 2 or any(int(d) < 1 for d in w.shape):
         raise ValueError(f"{what}: need a 4-bit weight [rows, K], got {tuple(w.shape)}")
     rows, k = (int(d) for d in w.shape)
@@ -118,8 +125,9 @@ def q4_linear(x: torch.Tensor, w: Q4Tensor) -> torch.Tensor:
     dtype, summed in fp32 and rounded once.  Differentiable in x (the weight is
     frozen).  The first call on a weight builds its scale words (1/17 of it), not in
     a stream capture; a capture takes calls without a gradient only.  There is no
-    forward-mode derivative; torch.jit.trace records the call.  The weight is not
-    written to once used, and kept until the work that reads it has ended."""
+    forward-mode derivative; torch.jit.trace records the call.  Scales or zeros that torch
+    has written to since are laid out again; a weight is kept, and not written to, until the
+    work that reads it, a graph's replays too, has ended."""
     check_weight("q4_linear", w)
     if x.dtype not in ACT:
         raise TypeError(f"q4_linear: activations must be fp16 or bf16, got {x.dtype}")
