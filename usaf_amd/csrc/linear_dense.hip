@@ -1,4 +1,5 @@
-// linear_kernel on 16-bit weights: its tiles, and the rule that chooses one.
+// linear_kernel on 16-bit weights: its tiles, and the rule that chooses one: the shortest by a step's and a tile's end's times,
+// measured tile by tile (10 ns, bf16; the smallest tiles' steps are of two and four blocks of the contraction).
 #include "linear_kernel.h"
 
 namespace usaf {

