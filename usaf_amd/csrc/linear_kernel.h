@@ -19,7 +19,7 @@
 // matrix instruction's operand registers: dt(fp16(fp16(q s) + z)), the codec's value bit for bit.
 //
 // What bounds it (bf16).  Large tiles: the matrix instructions and the clock that they leave; 1.27 us of a 256 x 256 x 64 step's
-// 1.6 are theirs alone.  8,192 x 14,336 x 4,096 takes 720 to 790 us (1.2 to 1.34 PFLOP/s; the library's 606).  Smaller tiles:
+// 1.6 are theirs alone.  8,192 x 14,336 x 4,096 takes 720 to 770 us (1.25 to 1.34 PFLOP/s; the library's 606).  Smaller tiles:
 // the trip of their lines, so stages count: 2,048 x 2,048 of 16,384 took 182 us with two stages of 128 x 256 tiles and
 // takes 145 with three.  4-bit weights: the dequantization's vector instructions, 1.20 us a step of 128 x 256 x 64 against 0.90.
 #pragma once
@@ -463,8 +463,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
         if (slot < t.valid && n < g.N) {
           const u32x4 v = *reinterpret_cast<const u32x4*>(s_out + r * T::OUT_ROW + 16 * (c ^ (r & (CH - 1))));
           uint16_t* const to = g.out + (t.m_beg + slot) * g.ldo + n;
-          if (vec && n + 8 <= g.N) {
-            *reinterpret_cast<u32x4*>(to) = v;
+          if (vec && n + 8 <= g.N) {  // (past the operands in the caches: 8,192 x 14,336 x 4,096 790 -> 768 us)
+            __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(to));
           } else {
 #pragma unroll
             for (int x = 0; x < 8; ++x)
@@ -478,17 +478,19 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
             const int rr = at / CH, c = at % CH, r = rr >> 1, slot = 32 * (MI * (T::EW * h + (r >> 5)) + i) + (r & 31);
             const int64_t n = n0 + 8 * c;
             if (slot < t.valid && n < g.N)
-              *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(g.kept) + (2 * (t.m_beg + slot) + (rr & 1)) * g.hs + n) =
-                  *reinterpret_cast<const u32x4*>(s_kept + rr * (T::KEPT_ROW / 2) + 16 * (c ^ (rr & (CH - 1))));
+              __builtin_nontemporal_store(
+                  *reinterpret_cast<const u32x4*>(s_kept + rr * (T::KEPT_ROW / 2) + 16 * (c ^ (rr & (CH - 1)))),
+                  reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(g.kept) + (2 * (t.m_beg + slot) + (rr & 1)) * g.hs + n));
           }
         }
       } else if constexpr (EPI == LIN_CK8) {
         for (int at = tid_now; at < T::ER * 16; at += THREADS) {
           const int r = at >> 4, c = at & 15, slot = 32 * (MI * (T::EW * h + (r >> 5)) + i) + (r & 31);
           if (slot < t.valid)
-            *reinterpret_cast<u32x4*>(reinterpret_cast<uint8_t*>(g.kept) + (2 * (t.m_beg + slot) + (c >> 3)) * g.hs + n0 +
-                                      16 * (c & 7)) =
-                *reinterpret_cast<const u32x4*>(s_kept + r * T::KEPT_ROW + 128 * (c >> 3) + 16 * ((c & 7) ^ (r & 7)));
+            __builtin_nontemporal_store(
+                *reinterpret_cast<const u32x4*>(s_kept + r * T::KEPT_ROW + 128 * (c >> 3) + 16 * ((c & 7) ^ (r & 7))),
+                reinterpret_cast<u32x4*>(reinterpret_cast<uint8_t*>(g.kept) + (2 * (t.m_beg + slot) + (c >> 3)) * g.hs + n0 +
+                                         16 * (c & 7)));
         }
       }
     }
