@@ -1,4 +1,4 @@
-// Products with one 16-bit or 4-bit weight: what linear_kernel.h's two halves (linear_dense.hip, linear_q4.hip)
+// Products with one 16-bit or 4-bit weight: what linear_kernel.h's parts (linear_dense.hip, linear_q4.hip, linear_turned.hip)
 // and their callers (linear.hip) share.
 #pragma once
 
@@ -36,12 +36,15 @@ struct LinPlan {
 };
 LinPlan plan_linear_dense(const LinArgs& g, bool gated);
 LinPlan plan_linear_q4(const LinArgs& g, bool gated);
+// C = A W of W [K, N] (both: C = A^T W of A [K, M] too), lda and ldw the distances of these rows; K % 64 == 0, N (M) % 8 == 0.
+LinPlan plan_linear_turned(const LinArgs& g, bool both);
 // A few rows of a 4-bit weight's product, out [M, N] (ldo = N), nothing kept: whether it takes them, and its launch (q4_small.hip).
 bool q4_small_ok(int64_t M, int64_t N, int64_t K);
 int q4_small(const LinArgs& g, int dt, bool gated, hipStream_t st);
 void prepare_q4_small();
 void prepare_linear_dense();
 void prepare_linear_q4();
+void prepare_linear_turned();
 // Raises the products' dynamic-LDS limits, once per process (usaf_hip_init, or their first use).
 void prepare_linear_kernels();
 

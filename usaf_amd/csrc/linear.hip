@@ -6,8 +6,9 @@
 //               dG = dt(dact U s (1 + G (1 - s))), dU = dt(dact G s), s = sigmoid(G), of the kept values
 //               dx = dt([dG, dU] W),   dW = dt([dG, dU]^T x)
 //
-// Every product is linear_kernel's C = A W^T, so a grad-input reads a transposed 16-bit copy of the weight and a weight
-// gradient transposed copies of both operands, made in the workspace by the kernels here.
+// The products are linear_kernel's C = A W^T.  A grad-input's weight and both of a weight gradient's operands have the
+// contraction's index first: 16-bit ones of whole blocks of 64 are read turned (linear_turned.hip), others from transposed copies
+// that the kernels here make in the workspace.
 #include "fp8.h"
 #include "linear.h"
 
@@ -323,12 +324,13 @@ struct Parts {
   void* at;
   int64_t ldp;
   Parts() = default;
-  Parts(Ws& ws, int64_t M, int64_t N, int64_t K, bool q4) {
-    const LinArgs g = product(nullptr, K, M, nullptr, K, N, K, nullptr, N);
-    plan = q4 ? plan_linear_q4(g, false) : plan_linear_dense(g, false);
+  Parts(Ws& ws, int64_t M, int64_t N, int64_t K, bool q4)
+      : Parts(ws, M, N, q4 ? plan_linear_q4(sizes(M, N, K), false) : plan_linear_dense(sizes(M, N, K), false)) {}
+  Parts(Ws& ws, int64_t M, int64_t N, const LinPlan& of) : plan(of) {
     ldp = round_up(N, 4);
     at = plan.parts > 1 ? ws.take(4 * plan.parts * M * ldp) : nullptr;
   }
+  static LinArgs sizes(int64_t M, int64_t N, int64_t K) { return product(nullptr, K, M, nullptr, K, N, K, nullptr, N); }
 };
 
 int run(LinArgs g, const Parts& p, int dt, hipStream_t st) {
@@ -376,7 +378,7 @@ struct GatedWs {
   void *w = nullptr, *x = nullptr;                                  // forward: 16-bit or padded weight, padded x
   void *dgu = nullptr, *wt = nullptr, *dgut = nullptr, *xt = nullptr;  // backward
   Parts dx_parts, dw_parts;
-  bool codes = false;
+  bool codes = false, dx_turned = false, dw_turned = false;
   int64_t bytes, kp, ldd, mp;
   // what: 0 forward, 4 forward that keeps 8-bit blocks, else 1 for dx + 2 for dw
   GatedWs(void* ws, int64_t M, int64_t I, int64_t K, bool four_bit, int what) {
@@ -389,15 +391,26 @@ struct GatedWs {
       if (four_bit ? !codes : kp != K) w = at.take(2 * 2 * I * kp);
       if (kp != K) x = at.take(2 * M * kp);
     } else {
+      // Operands are read turned where the rows are whole blocks of 64 and chunks of 8 and that is shorter than the product of
+      // copies and the copies, 4 bytes a value at about 4 TB/s (dgu's is written with it) and for dx a launch
       dgu = at.take(2 * M * ldd);
       if (what & 1) {
-        wt = at.take(2 * K * ldd);
-        dx_parts = Parts(at, M, K, ldd, false);
+        const LinArgs g = Parts::sizes(M, K, ldd);
+        const LinPlan turned = plan_linear_turned(g, false);
+        dx_turned = !four_bit && ldd == 2 * I && K % 8 == 0 && turned.us <= plan_linear_dense(g, false).us + (double)K * (double)ldd * 4 / 4e6 + 3;
+        if (!dx_turned) wt = at.take(2 * K * ldd);
+        dx_parts = dx_turned ? Parts(at, M, K, turned) : Parts(at, M, K, ldd, false);
       }
       if (what & 2) {
-        dgut = at.take(2 * 2 * I * mp);
-        xt = at.take(2 * K * mp);
-        dw_parts = Parts(at, 2 * I, K, mp, false);
+        const LinArgs g = Parts::sizes(2 * I, K, mp);
+        const LinPlan turned = plan_linear_turned(g, true);
+        dw_turned = mp == M && I % 4 == 0 && K % 8 == 0 &&
+                    turned.us <= plan_linear_dense(g, false).us + (double)M * (double)(2 * K + 2 * I) * 2 / 4e6;
+        if (!dw_turned) {
+          dgut = at.take(2 * 2 * I * mp);
+          xt = at.take(2 * K * mp);
+        }
+        dw_parts = dw_turned ? Parts(at, 2 * I, K, turned) : Parts(at, 2 * I, K, mp, false);
       }
     }
     bytes = at.used;
@@ -416,6 +429,7 @@ int check_ws(const char* what, const void* ws, int64_t have, int64_t need) {
 void prepare_linear_kernels() {
   prepare_linear_dense();
   prepare_linear_q4();
+  prepare_linear_turned();
   prepare_q4_small();
 }
 
@@ -536,6 +550,7 @@ extern "C" int usaf_hip_gated_bwd(const void* dact, int32_t dtype, int64_t M, in
   if ((uintptr_t)kept % 16 || ((uintptr_t)dact | (uintptr_t)x | (uintptr_t)dx | (uintptr_t)dw) % 2)
     return set_error(USAF_ERR_INVALID, "gated_bwd: what is kept must be 16-byte, rows 2-byte aligned");
   const GatedWs w(ws, M, I, K, q != nullptr, (dx ? 1 : 0) | (dw ? 2 : 0));
+  if (w.dw_turned && ((uintptr_t)x % 16 || ldx % 8)) return set_error(USAF_ERR_INVALID, "gated_bwd: rows of x must be 16-byte aligned");
   if (int rc = check_ws("gated_bwd", ws, ws_bytes, w.bytes)) return rc;
   hipStream_t st = as_stream(stream);
   GatedBwd g{reinterpret_cast<const uint16_t*>(dact), kept, kept_scales, M, I, round_up(I, kept_scales ? 128 : 8),
@@ -544,11 +559,14 @@ extern "C" int usaf_hip_gated_bwd(const void* dact, int32_t dtype, int64_t M, in
                      ? (kept_scales ? gated_bwd<USAF_BF16, true>(g, w.dgut, w.mp, st) : gated_bwd<USAF_BF16, false>(g, w.dgut, w.mp, st))
                      : (kept_scales ? gated_bwd<USAF_F16, true>(g, w.dgut, w.mp, st) : gated_bwd<USAF_F16, false>(g, w.dgut, w.mp, st));
   if (rc) return rc;
-  const Transpose wt = dx ? transpose_of(q ? (const void*)q : w16, 2 * I, K, K, w.wt, w.ldd) : Transpose{};
-  const Transpose xt = dw ? transpose_of(x, M, K, ldx, w.xt, w.mp) : Transpose{};
+  const Transpose wt = w.wt ? transpose_of(q ? (const void*)q : w16, 2 * I, K, K, w.wt, w.ldd) : Transpose{};
+  const Transpose xt = w.xt ? transpose_of(x, M, K, ldx, w.xt, w.mp) : Transpose{};
   if (int rc2 = transpose(wt, q ? sz : nullptr, xt, dtype, st)) return rc2;
   if (dx)
-    if (int rc2 = run(product(w.dgu, w.ldd, M, w.wt, w.ldd, K, w.ldd, dx, K), w.dx_parts, dtype, st)) return rc2;
-  if (dw) return run(product(w.dgut, w.mp, 2 * I, w.xt, w.mp, K, w.mp, dw, K), w.dw_parts, dtype, st);
+    if (int rc2 = run(w.dx_turned ? product(w.dgu, w.ldd, M, w16, K, K, w.ldd, dx, K)
+                                  : product(w.dgu, w.ldd, M, w.wt, w.ldd, K, w.ldd, dx, K), w.dx_parts, dtype, st)) return rc2;
+  if (dw)
+    return run(w.dw_turned ? product(w.dgu, w.ldd, 2 * I, x, ldx, K, w.mp, dw, K)
+                           : product(w.dgut, w.mp, 2 * I, w.xt, w.mp, K, w.mp, dw, K), w.dw_parts, dtype, st);
   return clear_error();
 }

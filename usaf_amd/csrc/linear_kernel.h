@@ -65,11 +65,23 @@ struct LinTile {
   static_assert(EPI != LIN_CK8 || (N == 256 && KW == 1 && EW == MW), "a tile has whole blocks of 128 columns");
 };
 
-template <int WAVES, int MW, int NW, int MI, int NI, int DT, bool Q4, int EPI>
+// Four columns' values of 16 of four rows: each 16 lanes' 16 addresses are of 8 bytes, lane 4 r + c's of row r, and lane i
+// gets column i of the four rows.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint2 read_turned(const uint8_t* p) {
+  typedef __attribute__((address_space(3))) s16x4* Ptr;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)p));
+}
+
+template <int WAVES, int MW, int NW, int MI, int NI, int DT, bool Q4, int EPI, int TR>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const LinArgs g) {
   typedef LinTile<WAVES, MW, NW, MI, NI, Q4, EPI> T;
   constexpr int THREADS = 64 * WAVES;
   constexpr int KW = T::KW, NB = T::NB;
+  constexpr bool TW = TR >= 1, TA = TR == 2;  // stored with the contraction's index first
+  constexpr int W_CH = T::N / 8, A_CH = T::M / 8;  // chunks of such a row
+  static_assert(!TW || (!Q4 && EPI == LIN_STORE && KW == 1 && W_CH % 16 == 0 && W_CH <= 32), "tile");
+  static_assert(!TA || (A_CH % 16 == 0 && A_CH <= 32), "tile");
   constexpr bool GATED = EPI != LIN_STORE, PARTS = !GATED && WAVES == 8;  // PARTS: takes a contraction in parts
   extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
   const uint32_t sm_lds = (uint32_t)(uintptr_t)(lds_void_ptr)sm;
@@ -121,16 +133,25 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
       const int c = GATED ? 16 * (r >> 5) + (r & 15) : r;
       return n0 + c < g.N ? (int64_t)c : g.N - 1 - n0;
     };
-    a_base = uniform(g.A + t.m_beg * g.lda);
-    w_base = uniform(g.W + n0 * g.ldw);
+    a_base = uniform(g.A + t.m_beg * (TA ? 2 : g.lda));
+    w_base = uniform(g.W + n0 * (TW ? 2 : g.ldw));
+    // chunk p of row r holds the row's chunk p ^ 4 (r % 4); columns past the last: its chunk again
+    auto chunk = [&](int at, int ch, int have, int64_t ld) {
+      const int r = 64 / ch * at + lane / ch, c = (lane % ch) ^ (4 * (r & 3));
+      return (uint32_t)(r * ld) + 16 * (c < have ? c : have - 1);
+    };
 #pragma unroll
     for (int i = 0; i < T::A_DMA; ++i) {
       const int r = (8 * (T::SHARE * i + part) + (lane >> 3)) % T::M;  // (of few rows, some twice)
-      a_off[i] = (uint32_t)((r < t.valid ? r : t.valid - 1) * g.lda) + 16 * ((lane & 7) ^ g_swz(r));
+      if constexpr (TA) a_off[i] = chunk((T::SHARE * i + part) % A_CH, A_CH, t.valid / 8, g.lda);
+      else a_off[i] = (uint32_t)((r < t.valid ? r : t.valid - 1) * g.lda) + 16 * ((lane & 7) ^ g_swz(r));
     }
 #pragma unroll
     for (int i = 0; i < T::W_DMA; ++i) {
-      if constexpr (Q4) {
+      if constexpr (TW) {
+        const int64_t left = g.N - n0;
+        w_off[i] = chunk((T::SHARE * i + part) % W_CH, W_CH, left < T::N ? (int)left / 8 : W_CH, g.ldw);
+      } else if constexpr (Q4) {
         const int r = (32 * (T::SHARE * i + part) + (lane >> 1)) % T::N;
         const int64_t n = column(r) + (GATED && (r & 16) ? up_rows : 0);
         w_off[i] = (uint32_t)(n * g.ldw) + 16 * ((lane & 1) ^ (r >> 3 & 1));
@@ -156,8 +177,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
     const int kb = i_step * KW + kw;
     i_k = kb < nkb ? kb : nkb - 1;
     i_to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(sm_lds + i_stage * T::STAGE + kw * T::SLAB));
-    i_a = a_base + (int64_t)i_k * 128;
-    i_w = w_base + (int64_t)i_k * T::W_ROW;
+    i_a = a_base + (int64_t)i_k * (TA ? 64 * g.lda : 128);
+    i_w = w_base + (int64_t)i_k * (TW ? 64 * g.ldw : T::W_ROW);
   };
   // (readfirstlane of what is uniform already is a move at most; without it the compiler may hold it in vector registers)
   auto to_lds = [](uint32_t at) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)at); };
@@ -199,16 +220,26 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_kernel(const Lin
     auto word = [&](const uint8_t* rows, int r, int c) {
       return *reinterpret_cast<const u32x4*>(rows + r * 128 + 16 * (c ^ g_swz(r)));
     };
+    // block b's values of rows 32 half + 8 j + [0, 8) of the contraction
+    auto turned = [&](const uint8_t* rows, int ch, int b) {
+      const int r = lane >> 2 & 3, c = 4 * b + 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
+      const uint8_t* const at = rows + (32 * half + 8 * j + r) * 16 * ch + 16 * (c ^ 4 * r) + 8 * (lane & 1);
+      const uint2 lo = read_turned(at), hi = read_turned(at + 64 * ch);
+      return u32x4{lo.x, lo.y, hi.x, hi.y};
+    };
     if (n < NI) {
       const int k = n, r = 32 * (NI * wn + k) + l32;
-      if constexpr (!Q4) {
+      if constexpr (TW) {
+        w[k] = turned(sw, W_CH, NI * wn + k);
+      } else if constexpr (!Q4) {
         w[k] = word(sw, r, 4 * half + j);
       } else if (j == 0) {
         codes[k] = *reinterpret_cast<const u32x4*>(sw + r * 32 + 16 * (half ^ (r >> 3 & 1)));
         scale[k] = reinterpret_cast<const uint32_t*>(sw + T::W_BYTES)[r];
       }
     } else if (n < NI + MI) {
-      a[n - NI] = word(sa, 32 * (MI * wm + n - NI) + l32, 4 * half + j);
+      if constexpr (TA) a[n - NI] = turned(sa, A_CH, MI * wm + n - NI);
+      else a[n - NI] = word(sa, 32 * (MI * wm + n - NI) + l32, 4 * half + j);
     }
   };
   auto load_slice = [&](int stage, int j, u32x4(&w)[NI], u32x4(&a)[MI]) {
@@ -505,13 +536,13 @@ inline bool raise_linear_lds(const void* kernel, size_t bytes) {
 }
 
 // One kernel: launch and one-time set-up.
-template <int WAVES, int MW, int NW, int MI, int NI, bool Q4, int EPI>
+template <int WAVES, int MW, int NW, int MI, int NI, bool Q4, int EPI, int TR = 0>
 struct LinLaunch {
   typedef LinTile<WAVES, MW, NW, MI, NI, Q4, EPI> T;
   template <int DT>
   static void prepare_one() {
     static const bool done =
-        raise_linear_lds(reinterpret_cast<const void*>(&linear_kernel<WAVES, MW, NW, MI, NI, DT, Q4, EPI>), T::LDS);
+        raise_linear_lds(reinterpret_cast<const void*>(&linear_kernel<WAVES, MW, NW, MI, NI, DT, Q4, EPI, TR>), T::LDS);
     (void)done;
   }
   static void prepare() {
@@ -525,11 +556,23 @@ struct LinLaunch {
     g.n_nt = (int)n_nt;
     const unsigned blocks = (unsigned)(((units < cus ? units : cus) + L_XCDS - 1) / L_XCDS * L_XCDS);
     prepare();
-    if (dt == USAF_BF16) linear_kernel<WAVES, MW, NW, MI, NI, USAF_BF16, Q4, EPI><<<blocks, 64 * WAVES, T::LDS, st>>>(g);
-    else linear_kernel<WAVES, MW, NW, MI, NI, USAF_F16, Q4, EPI><<<blocks, 64 * WAVES, T::LDS, st>>>(g);
+    if (dt == USAF_BF16) linear_kernel<WAVES, MW, NW, MI, NI, USAF_BF16, Q4, EPI, TR><<<blocks, 64 * WAVES, T::LDS, st>>>(g);
+    else linear_kernel<WAVES, MW, NW, MI, NI, USAF_F16, Q4, EPI, TR><<<blocks, 64 * WAVES, T::LDS, st>>>(g);
     return check_launch("linear");
   }
 };
+
+// Microseconds of a call: rounds of tiles over the CUs, the last one whole, and a launch.  The parts' fp32 sums are
+// written and read at about 4 TB/s, in one more launch.  Measured (us, with parts where the rule takes them / without, 4-bit bf16):
+// 32 and 100 rows of 14,336 to 4,096 20.8 / 28.0 and 30.3 / 50.1, 32 and 300 of 8,192 to 1,024 11.4 / 16.9 and 22.8 / 29.9,
+// 1,000 of 16,384 to 2,048 88.6 / 103.4; 2,048 of them 161.5 / 162.7.
+template <class T, int STEP, int END>
+double lin_us(const LinArgs& g, bool gated, int parts) {
+  const int64_t steps = (g.K / 64 + T::KW - 1) / T::KW, cols = gated ? T::N / 2 : T::N;
+  const int64_t tiles = (g.M + T::M - 1) / T::M * ((g.N + cols - 1) / cols) * parts, cus = device_cu_count();
+  const double tile = 0.01 * ((double)((steps + parts - 1) / parts) * STEP + END);
+  return 3 + tile * (double)((tiles + cus - 1) / cus) + (parts > 1 ? 3 + (double)parts * (double)g.M * (double)g.N * 8 / 4e6 : 0);
+}
 
 // One shape of tile for all that leaves it.  FOUR: the plain product of the whole contraction on four waves (2 x 2 of them)
 // instead of eight.  STEP: what a step of KW blocks of 64 takes, END: what a tile takes beside its steps, in 10 ns.
@@ -555,16 +598,26 @@ struct LinShape {
     }
     return Gated::launch(g, dt, st);
   }
-  // Microseconds of a call: rounds of tiles over the CUs, the last one whole, and a launch.  The parts' fp32 sums are
-  // written and read at about 4 TB/s, in one more launch.  Measured (us, with parts where the rule takes them / without, 4-bit bf16):
-  // 32 and 100 rows of 14,336 to 4,096 20.8 / 28.0 and 30.3 / 50.1, 32 and 300 of 8,192 to 1,024 11.4 / 16.9 and 22.8 / 29.9,
-  // 1,000 of 16,384 to 2,048 88.6 / 103.4; 2,048 of them 161.5 / 162.7.
-  static double us(const LinArgs& g, bool gated, int parts) {
-    const int64_t steps = (g.K / 64 + T::KW - 1) / T::KW, cols = gated ? T::N / 2 : T::N;
-    const int64_t tiles = (g.M + T::M - 1) / T::M * ((g.N + cols - 1) / cols) * parts, cus = device_cu_count();
-    const double tile = 0.01 * ((double)((steps + parts - 1) / parts) * STEP + END);
-    return 3 + tile * (double)((tiles + cus - 1) / cus) + (parts > 1 ? 3 + (double)parts * (double)g.M * (double)g.N * 8 / 4e6 : 0);
+  static double us(const LinArgs& g, bool gated, int parts) { return lin_us<T, STEP, END>(g, gated, parts); }
+};
+
+// The same for products whose weights (TR = 1) or both operands (2) are stored with the contraction's index first: C = A W,
+// C = A^T W.  Their lines of 512 or 256 bytes are a tile's columns of a row; the fragments are read turned out of LDS.
+template <int MW, int NW, int MI, int NI, int TR, int STEP, int END, bool FOUR = false>
+struct LinTurned {
+  typedef LinTile<8, MW, NW, MI, NI, false, LIN_STORE> T;
+  typedef LinLaunch<8, MW, NW, MI, NI, false, LIN_STORE, TR> Store;
+  typedef LinLaunch<FOUR ? 4 : 8, FOUR ? 2 : MW, FOUR ? 2 : NW, FOUR ? T::M / 64 : MI, FOUR ? T::N / 64 : NI, false, LIN_STORE, TR> Whole;
+  static constexpr bool CK8 = false;
+  static constexpr int KW = T::KW;
+  static void prepare() {
+    Store::prepare();
+    Whole::prepare();
   }
+  static int launch(const LinArgs& g, int dt, bool, hipStream_t st) {
+    return g.parts > 1 ? Store::launch(g, dt, st) : Whole::launch(g, dt, st);
+  }
+  static double us(const LinArgs& g, bool, int parts) { return lin_us<T, STEP, END>(g, false, parts); }
 };
 
 template <class S>
