@@ -392,12 +392,16 @@ struct GatedWs {
       if (kp != K) x = at.take(2 * M * kp);
     } else {
       // Operands are read turned where the rows are whole blocks of 64 and chunks of 8 and that is shorter than the product of
-      // copies and the copies, 4 bytes a value at about 4 TB/s (dgu's is written with it) and for dx a launch
+      // copies and the copies, 4 bytes a value at about 4 TB/s (dgu's is written with it) and a launch.  Measured (us, dx and dW,
+      // turned / copies, tokens x I x K, bf16): 2,048 x 8,192 x 2,048 280 / 324, 512 x 2,816 x 2,048 50 / 59, 64 x 8,192 x 2,048 46 / 66,
+      // 4,096 x 14,336 x 4,096 1,572 / 1,732; dW alone, few tiles of a long contraction, 65,536 x 64 x 64 45 / 35; 8,192 x 256 x 256
+      // 24.7 / 22.8, on the wrong side
       dgu = at.take(2 * M * ldd);
       if (what & 1) {
         const LinArgs g = Parts::sizes(M, K, ldd);
         const LinPlan turned = plan_linear_turned(g, false);
-        dx_turned = !four_bit && ldd == 2 * I && K % 8 == 0 && turned.us <= plan_linear_dense(g, false).us + (double)K * (double)ldd * 4 / 4e6 + 3;
+        dx_turned = !four_bit && ldd == 2 * I && K % 8 == 0 &&
+                    turned.us <= plan_linear_dense(g, false).us + (double)K * (double)ldd * 4 / 4e6 + 3;
         if (!dx_turned) wt = at.take(2 * K * ldd);
         dx_parts = dx_turned ? Parts(at, M, K, turned) : Parts(at, M, K, ldd, false);
       }
@@ -405,7 +409,8 @@ struct GatedWs {
         const LinArgs g = Parts::sizes(2 * I, K, mp);
         const LinPlan turned = plan_linear_turned(g, true);
         dw_turned = mp == M && I % 4 == 0 && K % 8 == 0 &&
-                    turned.us <= plan_linear_dense(g, false).us + (double)M * (double)(2 * K + 2 * I) * 2 / 4e6;
+                    turned.us <= plan_linear_dense(g, false).us + (double)M * (double)(2 * K + 2 * I) * 2 / 4e6 +
+                                     ((what & 1) && !dx_turned ? 0 : 3);
         if (!dw_turned) {
           dgut = at.take(2 * 2 * I * mp);
           xt = at.take(2 * K * mp);
