@@ -21,7 +21,7 @@
 // What bounds it (bf16).  Large tiles: the matrix instructions and the clock that they leave; 1.27 us of a 256 x 256 x 64 step's
 // 1.6 are theirs alone.  8,192 x 14,336 x 4,096 takes 720 to 770 us (1.25 to 1.34 PFLOP/s; the library's 606).  Smaller tiles:
 // the trip of their lines, so stages count: 2,048 x 2,048 of 16,384 took 182 us with two stages of 128 x 256 tiles and
-// takes 145 with three.  4-bit weights: the dequantization's vector instructions, 1.20 us a step of 128 x 256 x 64 against 0.90.
+// takes 136 to 150 with three.  4-bit weights: the dequantization's vector instructions, 1.20 us a step of 128 x 256 x 64 against 0.90.
 #pragma once
 
 #include "dma.h"
@@ -602,7 +602,8 @@ struct LinShape {
 };
 
 // The same for products whose weights (TR = 1) or both operands (2) are stored with the contraction's index first: C = A W,
-// C = A^T W.  Their lines of 512 or 256 bytes are a tile's columns of a row; the fragments are read turned out of LDS.
+// C = A^T W.  Their lines of 512 or 256 bytes are a tile's columns of a row; the fragments are read turned out of LDS, at the
+// steps' times of the others (2,048 x 2,048 of 16,384 136 to 157 us, 16,384 x 2,048 of 2,048 128 to 140, with the copies' product alike).
 template <int MW, int NW, int MI, int NI, int TR, int STEP, int END, bool FOUR = false>
 struct LinTurned {
   typedef LinTile<8, MW, NW, MI, NI, false, LIN_STORE> T;
