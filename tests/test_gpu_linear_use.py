@@ -47,6 +47,21 @@ def test_a_weight_that_changes(m):
     assert not torch.equal(before, after)
 
 
+def test_copies_of_a_weight():
+    import copy
+    import dataclasses
+    n, k = 160, 384
+    w, (q, s, z) = _weight(n, k)
+    x = _x(40, k)
+    _check(q4_linear(x, w), x, (q, s, z), n, k, "as made")
+    other = dataclasses.replace(w, s=(s * 2).cuda())
+    _check(q4_linear(x, other), x, (q, s * 2, z), n, k, "replaced")
+    same = copy.copy(w)
+    same.z = (z * 4).cuda()
+    _check(q4_linear(x, same), x, (q, s, z * 4), n, k, "copied")
+    _check(q4_linear(x, w), x, (q, s, z), n, k, "the first one")
+
+
 def test_weights_and_rows_made_in_inference_mode():
     n, k = 64, 256
     with torch.inference_mode():

@@ -37,10 +37,9 @@ def check_weight(what: str, w: Q4Tensor) -> None:
     """Raise unless w is a 4-bit matrix in the layout that the products read (looked at once for each set of tensors: 5 us)."""
     parts = (w.q, w.s, w.z, w.shape, w.group_size, *_versions(w))
     seen = w.__dict__.get("_seen")
-    if seen is not None:
-        if all(a is b or a == b for a, b in zip(seen[3:], parts[3:])) and all(a is b for a, b in zip(seen[:3], parts[:3])):
-            return
-        w._szg = None  # not what its words were built from
+    if seen is not None and all(a is b or a == b for a, b in zip(seen[3:], parts[3:])) \
+            and all(a is b for a, b in zip(seen[:3], parts[:3])):
+        return
     if len(w.shape) != 2 or any(int(d) < 1 for d in w.shape):
         raise ValueError(f"{what}: need a 4-bit weight [rows, K], got {tuple(w.shape)}")
     rows, k = (int(d) for d in w.shape)
@@ -56,23 +55,25 @@ def check_weight(what: str, w: Q4Tensor) -> None:
     if not (w.q.is_contiguous() and w.s.is_contiguous() and w.z.is_contiguous()) or w.q.data_ptr() % 16 \
             or w.s.device != w.q.device or w.z.device != w.q.device:
         raise ValueError(f"{what}: codes, scales and zeros must be contiguous, on one device, the codes 16-byte aligned")
+    w._szg = None  # (a copy of a tensor with other parts may have brought its words along)
     w.__dict__["_seen"] = parts
 
 
 def words(what: str, w: Q4Tensor) -> torch.Tensor:
     """The scale/zero words by group, int32 [K / 128, rows] (Q4Tensor.scale_zero_by_group's of one matrix): built once and
     kept with the weight, finished when built, so that any stream may read them from then on."""
-    if w._szg is None or w._szg.device != w.device:
+    szg = w._szg
+    if szg is None or szg.device != w.device:
         N.refuse_capture(f"{what}: the first call on a weight")
         rows, k = (int(d) for d in w.shape)
         with on(w.device):
             by_row = torch.empty(rows, k // 128, dtype=torch.int32, device=w.device)
             N.call("usaf_hip_pack_scale_zero", w.s.data_ptr(), w.z.data_ptr(), by_row.numel(), by_row.data_ptr(),
                    N.stream_ptr(w.device))
-            by_group = by_row.t().contiguous()
+            szg = by_row.t().contiguous()
             torch.cuda.current_stream(w.device).synchronize()
-        w._szg = by_group
-    return w._szg
+        w._szg = szg
+    return szg
 
 
 def rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
