@@ -695,6 +695,7 @@ int usaf_hip_q4_linear_bwd(const void* dy, int32_t dtype, int64_t M, int64_t N, 
  * ws: usaf_hip_gated_ws_bytes with what = 0 for the forward, 4 for one with kept_scales, else 1 for dx + 2 for dw;
  * 16-byte aligned.  Weights, kept and (K
  * % 64 == 0) rows of x 16-byte aligned.  2 I, K <= 2^22; K % 128 == 0 for 4-bit weights.
+ * Of a weight gradient with M % 64 == 0, K % 8 == 0 and I % 4 == 0, x's rows must be 16-byte aligned.
  */
 int64_t usaf_hip_gated_ws_bytes(int64_t M, int64_t I, int64_t K, int32_t four_bit, int32_t what);
 int usaf_hip_gated_fwd(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* q,
