@@ -675,7 +675,7 @@ int usaf_hip_moe_few(const void* x, int64_t T, int64_t H, const void* router, in
  *   usaf_hip_q4_linear      out [M, N] = dtype(x W^T), x [M, K] with row stride ld
  *   usaf_hip_q4_linear_bwd  dx [M, K] = dtype(dy W),   dy [M, N] with row stride ld
  * fp32 sums.  ws: usaf_hip_q4_linear_ws_bytes (0 bytes: may be NULL), 16-byte aligned; rows 16-byte aligned (of dy: where N % 64
- * == 0), codes 16-byte.  N, K <= 2^22.
+ * == 0), codes 16-byte.  N, K, ld <= 2^22.
  */
 int64_t usaf_hip_q4_linear_ws_bytes(int64_t M, int64_t N, int64_t K, int32_t backward);
 int usaf_hip_q4_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* q,
@@ -692,10 +692,10 @@ int usaf_hip_q4_linear_bwd(const void* dy, int32_t dtype, int64_t M, int64_t N, 
  *   usaf_hip_gated_bwd   dG = dtype(dact U s (1 + G (1 - s))), dU = dtype(dact G s), s = sigmoid(G), of the kept
  *     values; dx [M, K] = dtype([dG, dU] W) and, 16-bit weights, dw [2 I, K] = dtype([dG, dU]^T x), each where not NULL.
  *     dact [M, I] contiguous; x (row stride ldx) is read for dw only.
- * ws: usaf_hip_gated_ws_bytes with what = 0 for the forward, 4 for one with kept_scales, else 1 for dx + 2 for dw;
- * 16-byte aligned.  Weights, kept and (K
- * % 64 == 0) rows of x 16-byte aligned.  2 I, K <= 2^22; K % 128 == 0 for 4-bit weights.
- * Of a weight gradient with M % 64 == 0, K % 8 == 0 and I % 4 == 0, x's rows must be 16-byte aligned.
+ * ws: usaf_hip_gated_ws_bytes with what = 0 for the forward, 4 for one with kept_scales, else 1 for dx + 2 for dw; 16-byte
+ * aligned.  Weights, kept and (K % 64 == 0) rows of x 16-byte aligned.  2 I, K <= 2^22; K % 128 == 0 for 4-bit weights.  Rows of
+ * x at most 2^22 values apart and, of a weight gradient, at most 2^22 of them; where M % 64 == 0, K % 8 == 0 and I % 4 == 0
+ * they must be 16-byte aligned there.
  */
 int64_t usaf_hip_gated_ws_bytes(int64_t M, int64_t I, int64_t K, int32_t four_bit, int32_t what);
 int usaf_hip_gated_fwd(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* q,

@@ -551,7 +551,10 @@ extern "C" int usaf_hip_gated_bwd(const void* dact, int32_t dtype, int64_t M, in
   if (M == 0) return clear_error();
   if (!dact || !kept || (!dx && !dw) || (dw && !x)) return set_error(USAF_ERR_INVALID, "gated_bwd: null pointer");
   if (dw && q) return set_error(USAF_ERR_INVALID, "gated_bwd: a 4-bit weight has no gradient");
-  if (dw && (ldx < K || M > LIN_MAX)) return set_error(USAF_ERR_INVALID, "gated_bwd: a weight gradient needs ldx >= K and M <= %lld", (long long)LIN_MAX);
+  // (x read turned has 32-bit offsets within 64 rows)
+  if (dw && (ldx < K || ldx > LIN_MAX || M > LIN_MAX))
+    return set_error(USAF_ERR_INVALID, "gated_bwd: a weight gradient needs K <= ldx <= %lld and M <= %lld, got ldx=%lld M=%lld",
+                     (long long)LIN_MAX, (long long)LIN_MAX, (long long)ldx, (long long)M);
   if ((uintptr_t)kept % 16 || ((uintptr_t)dact | (uintptr_t)x | (uintptr_t)dx | (uintptr_t)dw) % 2)
     return set_error(USAF_ERR_INVALID, "gated_bwd: what is kept must be 16-byte, rows 2-byte aligned");
   const GatedWs w(ws, M, I, K, q != nullptr, (dx ? 1 : 0) | (dw ? 2 : 0));
