@@ -691,7 +691,8 @@ int usaf_hip_q4_linear_bwd(const void* dy, int32_t dtype, int64_t M, int64_t N, 
  *     the unrounded G and U, [M, 2, round_up(I, 128)], and scale bytes [M, 2, ceil(I / 128)].
  *   usaf_hip_gated_bwd   dG = dtype(dact U s (1 + G (1 - s))), dU = dtype(dact G s), s = sigmoid(G), of the kept
  *     values; dx [M, K] = dtype([dG, dU] W) and, 16-bit weights, dw [2 I, K] = dtype([dG, dU]^T x), each where not NULL.
- *     dact [M, I] contiguous; x (row stride ldx) is read for dw only.
+ *     dact [M, I] contiguous; x (row stride ldx) is read for dw only.  M == 0 writes nothing: dw, a sum over no rows,
+ *     is left as it was, for the caller to clear.
  * ws: usaf_hip_gated_ws_bytes with what = 0 for the forward, 4 for one with kept_scales, else 1 for dx + 2 for dw; 16-byte
  * aligned.  Weights, kept and (K % 64 == 0) rows of x 16-byte aligned.  2 I, K <= 2^22; K % 128 == 0 for 4-bit weights.  Rows of
  * x at most 2^22 values apart and, of a weight gradient, at most 2^22 of them; where M % 64 == 0, K % 8 == 0 and I % 4 == 0

@@ -30,3 +30,12 @@ def test_rows_at_the_limit_and_rows_that_nobody_reads(m, inter, k):
     assert "workspace" in N.last_error()
     assert _bwd(lib, m, inter, k, 1 << 40, dx=p, dw=None, size=0) == N.USAF_ERR_INVALID
     assert "workspace" in N.last_error()
+
+
+def test_a_weight_gradient_of_no_rows_is_the_callers_to_clear():
+    """Documented: the entry point writes nothing then, in memory of the host's here (gated_linear gives zeros)."""
+    lib = N.load()
+    dw = (ctypes.c_uint16 * 4096)(*([7] * 4096))
+    at = ctypes.cast(dw, ctypes.c_void_p)
+    assert _bwd(lib, 0, 32, 64, 64, dw=at, size=0) == N.USAF_OK
+    assert list(dw) == [7] * 4096
