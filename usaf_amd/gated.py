@@ -34,11 +34,9 @@ def _ws_bytes(device: int, m: int, inter: int, k: int, four_bit: int, what: int)
     return N.load().usaf_hip_gated_ws_bytes(m, inter, k, four_bit, what)
 
 
-def _weight_ptrs(w: Union[Q4Tensor, torch.Tensor]):
-    """(codes, scale words, 16-bit) pointers."""
-    if isinstance(w, Q4Tensor):
-        return w.q.data_ptr(), words("gated_linear", w).data_ptr(), None
-    return None, None, w.data_ptr()
+def _weight_parts(w: Union[Q4Tensor, torch.Tensor]):
+    """(codes, scale words, 16-bit) tensors, which a call holds until its launch."""
+    return (w.q, words("gated_linear", w), None) if isinstance(w, Q4Tensor) else (None, None, w)
 
 
 def _dense(w: torch.Tensor) -> torch.Tensor:
@@ -59,12 +57,12 @@ def _forward(x: torch.Tensor, w, checkpoint: Optional[str], keep: bool):
         kept = torch.empty(m, 2, blocks * 128, dtype=torch.uint8, device=dev)
         scales = torch.empty(m, 2, blocks, dtype=torch.uint8, device=dev)
     if m:
-        ptrs = _weight_ptrs(w)
+        parts = _weight_parts(w)
         with on(dev):
             need = _ws_bytes(dev.index, m, inter, k, int(isinstance(w, Q4Tensor)), 0 if scales is None else 4)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-            N.call("usaf_hip_gated_fwd", x.data_ptr(), N.dtype_code(x.dtype), m, k, _ld(x), *ptrs, inter, act.data_ptr(),
-                   N.ptr(kept), N.ptr(scales), N.ptr(ws), max(need, 0), N.stream_ptr(dev))
+            N.call("usaf_hip_gated_fwd", x.data_ptr(), N.dtype_code(x.dtype), m, k, _ld(x), *map(N.ptr, parts), inter,
+                   act.data_ptr(), N.ptr(kept), N.ptr(scales), N.ptr(ws), max(need, 0), N.stream_ptr(dev))
     return act, kept, scales
 
 
@@ -99,18 +97,17 @@ class GatedLinearFn(torch.autograd.Function):
         # (a saved-tensor hook may have changed what was kept: its layout, its place)
         kept, scales = _dense(kept), None if scales is None else scales.contiguous()
         if ctx.q4 is not None:
-            ptrs = _weight_ptrs(ctx.q4)
+            parts = _weight_parts(ctx.q4)
         else:  # only dx reads the weight; without it any 16-bit pointer says that there is no 4-bit one
-            weight = kept if weight is None else _dense(weight)
-            ptrs = (None, None, weight.data_ptr())
+            parts = _weight_parts(kept if weight is None else _dense(weight))
         if want_w:
             x = rows_of(x, k)
         with on(dev):
             need = _ws_bytes(dev.index, m, rows // 2, k, int(ctx.q4 is not None), int(want_x) + 2 * int(want_w))
             ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dev)
             N.call("usaf_hip_gated_bwd", dact.data_ptr(), N.dtype_code(ctx.dtype), m, rows // 2, k, kept.data_ptr(),
-                   N.ptr(scales), *ptrs, x.data_ptr() if want_w else None, _ld(x) if want_w else k, N.ptr(dx), N.ptr(dw),
-                   ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
+                   N.ptr(scales), *map(N.ptr, parts), x.data_ptr() if want_w else None, _ld(x) if want_w else k, N.ptr(dx),
+                   N.ptr(dw), ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
         return dx, dw, None, None
 
 
