@@ -61,18 +61,22 @@ def check_weight(what: str, w: Q4Tensor) -> None:
 
 def words(what: str, w: Q4Tensor) -> torch.Tensor:
     """The scale/zero words by group, int32 [K / 128, rows] (Q4Tensor.scale_zero_by_group's of one matrix): built once and
-    kept with the weight, finished when built, so that any stream may read them from then on."""
-    szg = w._szg
+    kept with the weight, finished when built, so that any stream may read them from then on.  Of scales or zeros made in
+    inference mode, whose writes nobody counts, they are the call's own instead, built on its stream, in a capture too."""
+    kept = not (w.s.is_inference() or w.z.is_inference())
+    szg = w._szg if kept else None
     if szg is None or szg.device != w.device:
-        N.refuse_capture(f"{what}: the first call on a weight")
+        if kept:
+            N.refuse_capture(f"{what}: the first call on a weight")
         rows, k = (int(d) for d in w.shape)
         with on(w.device):
             by_row = torch.empty(rows, k // 128, dtype=torch.int32, device=w.device)
             N.call("usaf_hip_pack_scale_zero", w.s.data_ptr(), w.z.data_ptr(), by_row.numel(), by_row.data_ptr(),
                    N.stream_ptr(w.device))
             szg = by_row.t().contiguous()
-            torch.cuda.current_stream(w.device).synchronize()
-        w._szg = szg
+            if kept:
+                torch.cuda.current_stream(w.device).synchronize()
+                w._szg = szg
     return szg
 
 
@@ -127,8 +131,10 @@ def q4_linear(x: torch.Tensor, w: Q4Tensor) -> torch.Tensor:
     frozen).  The first call on a weight builds its scale words (1/17 of it), not in
     a stream capture; a capture takes calls without a gradient only.  There is no
     forward-mode derivative; torch.jit.trace records the call.  Scales or zeros that torch
-    has written to since are laid out again; a weight is kept, and not written to, until the
-    work that reads it, a graph's replays too, has ended."""
+    has written to since are laid out again, but for writes through ``.data`` or by other
+    kernels, which torch does not count; those made in inference mode, where it counts
+    none, are laid out by every call (two more launches).  A weight is kept, and not written
+    to, until the work that reads it, a graph's replays too, has ended."""
     check_weight("q4_linear", w)
     if x.dtype not in ACT:
         raise TypeError(f"q4_linear: activations must be fp16 or bf16, got {x.dtype}")
