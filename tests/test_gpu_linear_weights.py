@@ -62,3 +62,64 @@ def test_a_graph_over_a_weight_made_in_inference_mode(m):
             w.s.mul_(2)
             s = s * 2
             assert torch.equal(q4_linear(x, w), q4_linear(x.clone(), w))
+
+
+CALLS = {"linear": q4_linear, "gated": gated_linear, "checkpoint": lambda x, w: gated_linear(x, w, "fp8")}
+
+
+def _leaf(m):
+    return U._x(m, K).requires_grad_()
+
+
+@pytest.mark.parametrize("m", [1, 40, 600])
+@pytest.mark.parametrize("call", list(CALLS))
+@pytest.mark.parametrize("part", ["q", "s", "z"])
+def test_a_weight_written_to_before_its_backward(call, part, m):
+    """As torch does for a tensor that a backward needs."""
+    w, _ = U._weight(N_, K)
+    y = CALLS[call](_leaf(m), w)
+    t = getattr(w, part)
+    t.copy_(t.flip(0))
+    with pytest.raises(RuntimeError, match="written to"):
+        y.float().sum().backward()
+    with torch.no_grad():
+        CALLS[call](U._x(m, K), w)  # (lays the scale words out anew)
+    with pytest.raises(RuntimeError, match="written to"):
+        CALLS[call](_leaf(m), w)
+        y.float().sum().backward()
+
+
+@pytest.mark.parametrize("made", ["as usual", "in inference mode"])
+@pytest.mark.parametrize("m", [1, 40, 600])
+@pytest.mark.parametrize("call", list(CALLS))
+def test_a_weight_given_other_tensors_before_its_backward(call, m, made):
+    """The gradient is that of the weight that the forward read, also where another forward has read the new one."""
+    with torch.inference_mode(made != "as usual"):
+        w, _ = U._weight(N_, K, seed=1)
+        other, _ = U._weight(N_, K, seed=2)
+    x = _leaf(m)
+    dy = torch.ones_like(CALLS[call](x, w))
+    want = torch.autograd.grad(CALLS[call](x, w), x, dy)[0]
+    for between in (False, True):
+        y = CALLS[call](x, w)
+        old = w.q, w.s, w.z
+        w.q, w.s, w.z = other.q, other.s, other.z
+        z = CALLS[call](x, w) if between else None
+        assert torch.equal(torch.autograd.grad(y, x, dy, retain_graph=True)[0], want)
+        assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
+        if between:
+            new = torch.autograd.grad(CALLS[call](x, other), x, dy)[0]
+            assert torch.equal(torch.autograd.grad(z, x, dy)[0], new) and not torch.equal(new, want)
+        w.q, w.s, w.z = old
+
+
+def test_calls_of_no_rows_need_no_words():
+    """Also in a capture, on a weight that has not been used."""
+    w, _ = U._weight(N_, K)
+    x = torch.empty(0, K, dtype=torch.bfloat16, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph), torch.no_grad():
+        assert q4_linear(x, w).shape == (0, N_) and gated_linear(x, w).shape == (0, N_ // 2)
+    x = x.clone().requires_grad_()
+    (q4_linear(x, w).sum() + gated_linear(x, w).sum()).backward()
+    assert x.grad.shape == (0, K) and w._szg is None

@@ -23,7 +23,7 @@ import torch
 from . import _native as N
 from .fp8 import on
 from .moe import Q4Tensor
-from .q4 import ACT, _ld, check_weight, rows_of, words
+from .q4 import ACT, Reading, _ld, check_weight, rows_of, words
 
 CHECKPOINTS = (None, "fp8")
 
@@ -34,18 +34,14 @@ def _ws_bytes(device: int, m: int, inter: int, k: int, four_bit: int, what: int)
     return N.load().usaf_hip_gated_ws_bytes(m, inter, k, four_bit, what)
 
 
-def _weight_parts(w: Union[Q4Tensor, torch.Tensor]):
-    """(codes, scale words, 16-bit) tensors, which a call holds until its launch."""
-    return (w.q, words("gated_linear", w), None) if isinstance(w, Q4Tensor) else (None, None, w)
-
-
 def _dense(w: torch.Tensor) -> torch.Tensor:
     w = w.contiguous()
     return w if w.data_ptr() % 16 == 0 else w.clone()
 
 
-def _forward(x: torch.Tensor, w, checkpoint: Optional[str], keep: bool):
-    """act [M, I], and what the backward reads (None where nothing is kept): values and scales."""
+def _forward(x: torch.Tensor, w, checkpoint: Optional[str], keep: bool, read: Optional[Reading] = None):
+    """act [M, I], and what the backward reads (None where nothing is kept): values and scales.  read: a 4-bit w's Reading, if
+    there is one."""
     rows, k = (int(d) for d in w.shape)
     inter, m, dev = rows // 2, x.shape[0], x.device
     act = torch.empty(m, inter, dtype=x.dtype, device=dev)
@@ -57,7 +53,10 @@ def _forward(x: torch.Tensor, w, checkpoint: Optional[str], keep: bool):
         kept = torch.empty(m, 2, blocks * 128, dtype=torch.uint8, device=dev)
         scales = torch.empty(m, 2, blocks, dtype=torch.uint8, device=dev)
     if m:
-        parts = _weight_parts(w)
+        if isinstance(w, Q4Tensor):  # (codes, scale words, 16-bit weight), held until the launch
+            parts = (w.q, words("gated_linear", w), None) if read is None else (read.q, read.sz, None)
+        else:
+            parts = (None, None, w)
         with on(dev):
             need = _ws_bytes(dev.index, m, inter, k, int(isinstance(w, Q4Tensor)), 0 if scales is None else 4)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
@@ -74,9 +73,11 @@ class GatedLinearFn(torch.autograd.Function):
         keep = any(ctx.needs_input_grad[:2])
         rows = rows_of(x, x.shape[1])
         w = q4 if weight is None else _dense(weight)
-        act, kept, scales = _forward(rows, w, checkpoint, keep)
-        ctx.q4, ctx.dtype, ctx.shape = q4, x.dtype, tuple(w.shape)
+        read = None if q4 is None else Reading.of("gated_linear", q4, x)
+        act, kept, scales = _forward(rows, w, checkpoint, keep, read)
+        ctx.dtype, ctx.shape = x.dtype, tuple(w.shape)
         if keep:
+            ctx.read = read
             ctx.save_for_backward(kept, scales, x if ctx.needs_input_grad[1] else None,
                                   weight if ctx.needs_input_grad[0] else None)
         return act
@@ -86,6 +87,8 @@ class GatedLinearFn(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise RuntimeError("gated_linear has no second derivative (create_graph=True)")
         N.refuse_capture("gated_linear's backward")
+        if ctx.read is not None:
+            ctx.read.refuse_written("gated_linear's backward")
         want_x, want_w = ctx.needs_input_grad[:2]
         kept, scales, x, weight = ctx.saved_tensors
         (rows, k), (m, dev) = ctx.shape, (dact.shape[0], dact.device)
@@ -96,14 +99,14 @@ class GatedLinearFn(torch.autograd.Function):
         dact = dact.to(ctx.dtype).contiguous()
         # (a saved-tensor hook may have changed what was kept: its layout, its place)
         kept, scales = _dense(kept), None if scales is None else scales.contiguous()
-        if ctx.q4 is not None:
-            parts = _weight_parts(ctx.q4)
+        if ctx.read is not None:
+            parts = (ctx.read.q, ctx.read.sz, None)
         else:  # only dx reads the weight; without it any 16-bit pointer says that there is no 4-bit one
-            parts = _weight_parts(kept if weight is None else _dense(weight))
+            parts = (None, None, kept if weight is None else _dense(weight))
         if want_w:
             x = rows_of(x, k)
         with on(dev):
-            need = _ws_bytes(dev.index, m, rows // 2, k, int(ctx.q4 is not None), int(want_x) + 2 * int(want_w))
+            need = _ws_bytes(dev.index, m, rows // 2, k, int(ctx.read is not None), int(want_x) + 2 * int(want_w))
             ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dev)
             N.call("usaf_hip_gated_bwd", dact.data_ptr(), N.dtype_code(ctx.dtype), m, rows // 2, k, kept.data_ptr(),
                    N.ptr(scales), *map(N.ptr, parts), x.data_ptr() if want_w else None, _ld(x) if want_w else k, N.ptr(dx),

@@ -11,6 +11,7 @@ the activations are), so decoding, prompts and gradients multiply the same numbe
 from __future__ import annotations
 
 import functools
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -28,14 +29,14 @@ def _ws_bytes(device: int, m: int, n: int, k: int, backward: int) -> int:
     return N.load().usaf_hip_q4_linear_ws_bytes(m, n, k, backward)
 
 
-def _versions(w: Q4Tensor):
-    """Counts of the writes to the scales and zeros (tensors made in inference mode have none)."""
-    return tuple(None if t.is_inference() else t._version for t in (w.s, w.z))
+def _versions(*tensors: torch.Tensor):
+    """Counts of the writes to tensors (those made in inference mode have none)."""
+    return tuple(None if t.is_inference() else t._version for t in tensors)
 
 
 def check_weight(what: str, w: Q4Tensor) -> None:
     """Raise unless w is a 4-bit matrix in the layout that the products read (looked at once for each set of tensors: 5 us)."""
-    parts = (w.q, w.s, w.z, w.shape, w.group_size, *_versions(w))
+    parts = (w.q, w.s, w.z, w.shape, w.group_size, *_versions(w.s, w.z))
     seen = w.__dict__.get("_seen")
     if seen is not None and all(a is b or a == b for a, b in zip(seen[3:], parts[3:])) \
             and all(a is b for a, b in zip(seen[:3], parts[:3])):
@@ -80,6 +81,24 @@ def words(what: str, w: Q4Tensor) -> torch.Tensor:
     return szg
 
 
+class Reading(NamedTuple):
+    """A weight's tensors as a forward reads them, which are what its backward reads, whatever the weight holds by then."""
+    q: torch.Tensor
+    s: torch.Tensor
+    z: torch.Tensor
+    sz: Optional[torch.Tensor]  # words() of s and z, None for a call of no rows
+    versions: Tuple
+
+    @classmethod
+    def of(cls, what: str, w: Q4Tensor, x: torch.Tensor) -> "Reading":
+        return cls(w.q, w.s, w.z, words(what, w) if x.numel() else None, _versions(w.q, w.s, w.z))
+
+    def refuse_written(self, what: str) -> None:
+        """Raise, as for a torch tensor that a backward needs, where these have been written to since."""
+        if _versions(self.q, self.s, self.z) != self.versions:
+            raise RuntimeError(f"{what}: the 4-bit weight's codes, scales or zeros have been written to since the forward")
+
+
 def rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
     """t as rows [M, cols] that start at multiples of 16 bytes, without a copy where they do."""
     t = t if t.dim() == 2 else t.reshape(t.numel() // cols, cols)
@@ -97,30 +116,33 @@ class Q4LinearFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x: torch.Tensor, w: Q4Tensor):
-        ctx.w, ctx.dtype = w, x.dtype
-        return _linear(x, w)
+        read = Reading.of("q4_linear", w, x)
+        if ctx.needs_input_grad[0]:
+            ctx.read, ctx.shape, ctx.dtype = read, w.shape, x.dtype
+        return _linear(x, w.shape, read.q, read.sz)
 
     @staticmethod
     def backward(ctx, dy: torch.Tensor):
         if torch.is_grad_enabled():
             raise RuntimeError("q4_linear has no second derivative (create_graph=True)")
         N.refuse_capture("q4_linear's backward")
-        return _linear(dy if dy.dtype == ctx.dtype else dy.to(ctx.dtype), ctx.w, backward=True), None
+        ctx.read.refuse_written("q4_linear's backward")
+        dy = dy if dy.dtype == ctx.dtype else dy.to(ctx.dtype)
+        return _linear(dy, ctx.shape, ctx.read.q, ctx.read.sz, backward=True), None
 
 
-def _linear(x: torch.Tensor, w: Q4Tensor, backward: bool = False) -> torch.Tensor:
-    n, k = (int(d) for d in w.shape)
+def _linear(x: torch.Tensor, shape, q: torch.Tensor, sz: Optional[torch.Tensor], backward: bool = False) -> torch.Tensor:
+    n, k = (int(d) for d in shape)
     dev, (cols, out_cols) = x.device, (n, k) if backward else (k, n)
     rows = rows_of(x, cols)
     m = rows.shape[0]
     out = torch.empty(m, out_cols, dtype=x.dtype, device=dev)
     if m:
-        sz = words("q4_linear", w)
         with on(dev):
             need = _ws_bytes(dev.index, m, n, k, int(backward))
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
             name, size = ("usaf_hip_q4_linear_bwd", k) if backward else ("usaf_hip_q4_linear", n)
-            N.call(name, rows.data_ptr(), N.dtype_code(x.dtype), m, cols, _ld(rows), w.q.data_ptr(), sz.data_ptr(), size,
+            N.call(name, rows.data_ptr(), N.dtype_code(x.dtype), m, cols, _ld(rows), q.data_ptr(), sz.data_ptr(), size,
                    out.data_ptr(), N.ptr(ws), max(need, 0), N.stream_ptr(dev))
     return out if x.dim() == 2 else out.view(*x.shape[:-1], out_cols)
 
@@ -134,7 +156,9 @@ def q4_linear(x: torch.Tensor, w: Q4Tensor) -> torch.Tensor:
     has written to since are laid out again, but for writes through ``.data`` or by other
     kernels, which torch does not count; those made in inference mode, where it counts
     none, are laid out by every call (two more launches).  A weight is kept, and not written
-    to, until the work that reads it, a graph's replays too, has ended."""
+    to, until the work that reads it, a graph's replays too, has ended.  A backward reads the
+    forward's tensors, also where the weight has been given others since, and raises where
+    torch has counted a write to them."""
     check_weight("q4_linear", w)
     if x.dtype not in ACT:
         raise TypeError(f"q4_linear: activations must be fp16 or bf16, got {x.dtype}")
@@ -145,5 +169,7 @@ def q4_linear(x: torch.Tensor, w: Q4Tensor) -> torch.Tensor:
     if torch.is_grad_enabled() and x.requires_grad:
         N.refuse_capture("q4_linear of activations that want a gradient")
         return Q4LinearFn.apply(x, w)
+    if N.followed(x):
+        return Q4LinearFn.apply(x, w)
     # (the function's own call takes 2 us of the host's time)
-    return Q4LinearFn.apply(x, w) if N.followed(x) else _linear(x, w)
+    return _linear(x, w.shape, w.q, words("q4_linear", w) if x.numel() else None)
