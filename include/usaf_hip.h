@@ -706,6 +706,21 @@ int usaf_hip_gated_bwd(const void* dact, int32_t dtype, int64_t M, int64_t I, in
                        const uint8_t* kept_scales, const uint8_t* q, const uint32_t* sz, const void* w16, const void* x,
                        int64_t ldx, void* dx, void* dw, void* ws, int64_t ws_bytes, void* stream);
 
+/*
+ * Which kernel takes a product of these calls on the current device, for measurements and tests: plan[4] = {kind below,
+ * the tile's rows, the tile's weight rows (gated: gate and up), parts that the contraction is taken in}.  M >= 1.
+ * what as for usaf_hip_gated_ws_bytes (0: a forward that keeps nothing); weight_grad: dw's product, else dx's.
+ */
+enum {
+  USAF_PLAN_ROWS = 0,         /* 16-bit operands, rows along the contraction */
+  USAF_PLAN_CODES = 1,        /* 4-bit codes */
+  USAF_PLAN_FEW_ROWS = 2,     /* 4-bit codes, a few rows */
+  USAF_PLAN_W_TURNED = 3,     /* 16-bit operands, the weight's contraction index first */
+  USAF_PLAN_BOTH_TURNED = 4   /* both operands' */
+};
+int usaf_hip_q4_linear_plan(int64_t M, int64_t N, int64_t K, int32_t backward, int32_t* plan);
+int usaf_hip_gated_plan(int64_t M, int64_t I, int64_t K, int32_t four_bit, int32_t what, int32_t weight_grad, int32_t* plan);
+
 #ifdef __cplusplus
 }
 #endif

@@ -70,6 +70,8 @@ _SIGNATURES: dict[str, list] = {
                            _c_p],
     "usaf_hip_gated_bwd": [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p,
                            _c_p, _c_i64, _c_p],
+    "usaf_hip_q4_linear_plan": [_c_i64, _c_i64, _c_i64, _c_i32, _c_p],
+    "usaf_hip_gated_plan": [_c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_p],
     "usaf_hip_quantize_q4": [_c_p, _c_i32, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p],
     "usaf_hip_pack_scale_zero": [_c_p, _c_p, _c_i64, _c_p, _c_p],
     "usaf_hip_q4_transpose": [_c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p],

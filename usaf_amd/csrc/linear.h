@@ -33,6 +33,7 @@ struct LinPlan {
   int (*launch)(const LinArgs&, int dt, bool gated, hipStream_t) = nullptr;
   int parts = 1;
   double us = 0;
+  int rows = 0, w_rows = 0;  // of the tile: of A, of W
 };
 LinPlan plan_linear_dense(const LinArgs& g, bool gated);
 LinPlan plan_linear_q4(const LinArgs& g, bool gated);

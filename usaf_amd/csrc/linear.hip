@@ -295,14 +295,20 @@ LinArgs product(const void* a, int64_t lda, int64_t M, const void* w, int64_t ld
   return g;
 }
 
+// A forward product's sizes, as the plans read them.
+LinArgs forward_sizes(int64_t M, int64_t N, int64_t K, bool eight_bit) {
+  LinArgs g = product(nullptr, K, M, nullptr, K, N, K, nullptr, 0);
+  static uint8_t kept;  // (not read: that there is one decides which tiles may be taken)
+  if (eight_bit) g.kept = g.kept_s = &kept;
+  return g;
+}
+
 // Whether a 4-bit weight of `rows` rows is multiplied as codes; else its 16-bit values are written once, to the workspace, and
 // multiplied: 2.5 bytes a weight at about 4 TB/s, and a launch.  Measured (us, as codes / written first, bf16): 128, 512, 1,024,
 // 2,048 rows of 4,096 to 4,096 18 / 28, 34 / 39, 46 / 49, 84 / 75; 256, 512, 1,024 of 4,096 to 14,336 44 / 66, 78 / 88,
 // 151 / 127; gated, 512 and 1,000 of 2,048 to 5,632 23.7 / 28.3 and 39.2 / 40.7.
 bool as_codes(int64_t M, int64_t rows, int64_t K, bool gated, bool eight_bit = false) {
-  LinArgs g = product(nullptr, K, M, nullptr, K, gated ? rows / 2 : rows, K, nullptr, 0);
-  static uint8_t kept;  // (not read: that there is one decides which tiles may be taken)
-  if (eight_bit) g.kept = g.kept_s = &kept;
+  const LinArgs g = forward_sizes(M, gated ? rows / 2 : rows, K, eight_bit);
   return plan_linear_q4(g, gated).us <= plan_linear_dense(g, gated).us + (double)rows * (double)K * 2.5 / 4e6 + 3;
 }
 
@@ -512,6 +518,35 @@ static int gated_args(const char* what, int32_t dtype, int64_t M, int64_t I, int
 
 extern "C" int64_t usaf_hip_gated_ws_bytes(int64_t M, int64_t I, int64_t K, int32_t four_bit, int32_t what) {
   return sizes_ok(M, 2 * I, K) && what >= 0 && what <= 4 ? GatedWs(nullptr, M, I, K, four_bit != 0, what).bytes : -1;
+}
+
+// {kind, tile's rows, tile's weight rows, parts of the contraction}
+static int tell(int32_t* to, int kind, const LinPlan& p) {
+  const int32_t v[4] = {kind, p.rows, p.w_rows, p.parts};
+  for (int i = 0; i < 4; ++i) to[i] = v[i];
+  return clear_error();
+}
+static const LinPlan FEW_ROWS{nullptr, 1, 0, 16, 16};
+
+extern "C" int usaf_hip_q4_linear_plan(int64_t M, int64_t N, int64_t K, int32_t backward, int32_t* plan) {
+  if (!sizes_ok(M, N, K) || M == 0 || !plan) return set_error(USAF_ERR_INVALID, "q4_linear_plan: sizes or a null pointer");
+  if (!backward && q4_small_ok(M, N, K)) return tell(plan, USAF_PLAN_FEW_ROWS, FEW_ROWS);
+  const Q4LinearWs w(nullptr, M, N, K, backward != 0);
+  return tell(plan, w.codes ? USAF_PLAN_CODES : USAF_PLAN_ROWS, w.parts.plan);
+}
+
+extern "C" int usaf_hip_gated_plan(int64_t M, int64_t I, int64_t K, int32_t four_bit, int32_t what, int32_t weight_grad,
+                                   int32_t* plan) {
+  const bool forward = what == 0 || what == 4;
+  if (!sizes_ok(M, 2 * I, K) || M == 0 || !plan || what < 0 || what > 4 || (!forward && !(what & (weight_grad ? 2 : 1))))
+    return set_error(USAF_ERR_INVALID, "gated_plan: sizes, what or a null pointer");
+  const GatedWs w(nullptr, M, I, K, four_bit != 0, what);
+  if (!forward)
+    return weight_grad ? tell(plan, w.dw_turned ? USAF_PLAN_BOTH_TURNED : USAF_PLAN_ROWS, w.dw_parts.plan)
+                       : tell(plan, w.dx_turned ? USAF_PLAN_W_TURNED : USAF_PLAN_ROWS, w.dx_parts.plan);
+  if (w.codes && what == 0 && q4_small_ok(M, I, K)) return tell(plan, USAF_PLAN_FEW_ROWS, FEW_ROWS);
+  const LinArgs g = forward_sizes(M, I, w.kp, what == 4);
+  return w.codes ? tell(plan, USAF_PLAN_CODES, plan_linear_q4(g, true)) : tell(plan, USAF_PLAN_ROWS, plan_linear_dense(g, true));
 }
 
 extern "C" int usaf_hip_gated_fwd(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld, const uint8_t* q,

@@ -627,7 +627,7 @@ void consider(LinPlan& best, const LinArgs& g, bool gated) {
   for (int parts = 1; parts <= (gated ? 1 : 16); parts *= 2) {
     if (parts > 1 && g.K / 64 < 4 * parts * S::KW) break;
     const double us = S::us(g, gated, parts);
-    if (best.launch == nullptr || us < best.us) best = {S::launch, parts, us};
+    if (best.launch == nullptr || us < best.us) best = {S::launch, parts, us, S::T::M, S::T::N};
   }
 }
 
