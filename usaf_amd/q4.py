@@ -64,9 +64,9 @@ def words(what: str, w: Q4Tensor) -> torch.Tensor:
     """The scale/zero words by group, int32 [K / 128, rows] (Q4Tensor.scale_zero_by_group's of one matrix): built once and
     kept with the weight, finished when built, so that any stream may read them from then on.  Of scales or zeros made in
     inference mode, whose writes nobody counts, they are the call's own instead, built on its stream, in a capture too."""
-    kept = not (w.s.is_inference() or w.z.is_inference())
-    szg = w._szg if kept else None
+    szg = w._szg
     if szg is None or szg.device != w.device:
+        kept = not (w.s.is_inference() or w.z.is_inference())
         if kept:
             N.refuse_capture(f"{what}: the first call on a weight")
         rows, k = (int(d) for d in w.shape)
