@@ -19,9 +19,9 @@
 // matrix instruction's operand registers: dt(fp16(fp16(q s) + z)), the codec's value bit for bit.
 //
 // What bounds it (bf16).  Large tiles: the matrix instructions and the clock that they leave; 1.27 us of a 256 x 256 x 64 step's
-// 1.6 are theirs alone.  8,192 x 14,336 x 4,096 takes 720 to 770 us (1.25 to 1.34 PFLOP/s; the library's 606).  Smaller tiles:
-// the trip of their lines, so stages count: 2,048 x 2,048 of 16,384 took 182 us with two stages of 128 x 256 tiles and
-// takes 136 to 150 with three.  4-bit weights: the dequantization's vector instructions, 1.20 us a step of 128 x 256 x 64 against 0.90.
+// 1.6 are theirs alone.  8,192 x 14,336 x 4,096 takes 720 to 770 us (1.25 to 1.34 PFLOP/s); the library's product 606, under the
+// same clock.  Smaller tiles: the trip of their lines, so stages count: 2,048 x 2,048 of 16,384 took 182 us with two stages of 128 x 256
+// tiles and takes 136 to 150 with three.  4-bit weights: the dequantization's vector instructions, 1.20 us a step of 128 x 256 x 64 against 0.90.
 #pragma once
 
 #include "dma.h"

@@ -2,8 +2,9 @@
 
 ``q4_linear`` is ``F.linear`` with a ``moe.Q4Tensor`` of shape [N, K], as
 ``quantize_4bit`` makes it (group size 128 along whole rows), beside ``fp8.fp8_linear``:
-a projection or an output head that stays 4-bit in memory, for one token or a
-prompt, differentiable in the activations.  A weight's value is everywhere the
+a projection or an output head that is kept in 4 bits, for one token or a prompt,
+differentiable in the activations.  Calls of a few hundred rows or more, and every
+backward, write the weight's 16-bit values to a workspace of their own.  A weight's value is everywhere the
 codec's in the activations' dtype, ``w.dequantize(x.dtype)`` bit for bit
 (fp16(code * scale) + zero in fp16, usaf/quantization.py:88-132, then bf16 where
 the activations are), so decoding, prompts and gradients multiply the same numbers.
