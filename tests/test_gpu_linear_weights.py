@@ -123,3 +123,19 @@ def test_calls_of_no_rows_need_no_words():
     x = x.clone().requires_grad_()
     (q4_linear(x, w).sum() + gated_linear(x, w).sum()).backward()
     assert x.grad.shape == (0, K) and w._szg is None
+
+
+@pytest.mark.parametrize("call", list(CALLS))
+def test_a_trace_over_a_weight_that_is_written_to(call):
+    """A recorded call reads the weight as a call does."""
+    w, _ = U._weight(N_, K)
+    x = U._x(40, K)
+    traced = torch.jit.trace(lambda t: CALLS[call](t, w), (x,), check_trace=False)
+    before = traced(x)
+    assert torch.equal(before, CALLS[call](x, w))
+    w.s.mul_(2)
+    after = traced(x)
+    assert not torch.equal(before, after) and torch.equal(after, CALLS[call](x, w))
+    w.z = w.z * 2
+    again = traced(x)
+    assert not torch.equal(again, after) and torch.equal(again, CALLS[call](x, w))

@@ -35,6 +35,7 @@ def watched(monkeypatch):
     monkeypatch.setattr(N, "call", call)
     monkeypatch.setattr(N, "stream_ptr", lambda _: None)
     monkeypatch.setattr(N, "refuse_capture", lambda _: None)
+    q4.check_weight("", w)
     words()
     return w, alive
 

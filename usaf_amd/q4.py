@@ -92,6 +92,7 @@ class Reading(NamedTuple):
 
     @classmethod
     def of(cls, what: str, w: Q4Tensor, x: torch.Tensor) -> "Reading":
+        check_weight(what, w)  # (a trace calls the autograd functions by themselves)
         return cls(w.q, w.s, w.z, words(what, w) if x.numel() else None, _versions(w.q, w.s, w.z))
 
     def refuse_written(self, what: str) -> None:
