@@ -139,3 +139,21 @@ def test_a_trace_over_a_weight_that_is_written_to(call):
     w.z = w.z * 2
     again = traced(x)
     assert not torch.equal(again, after) and torch.equal(again, CALLS[call](x, w))
+
+
+def test_a_trace_refuses_what_a_call_refuses():
+    """Other rows than the traced ones are not read past their end or as another type."""
+    w, _ = U._weight(N_, K)
+    dense = U._x(N_, K, seed=3)
+    x = U._x(40, K)
+    for call, weight in ((q4_linear, w), (gated_linear, w), (gated_linear, dense)):
+        traced = torch.jit.trace(lambda t: call(t, weight), (x,), check_trace=False)
+        assert torch.equal(traced(x[:7]), call(x[:7], weight))
+        for bad in (torch.cat([x, x], 1), x[:, :256], x.cpu(), x.float()):
+            with pytest.raises((ValueError, TypeError, RuntimeError)):
+                traced(bad)
+        if weight is dense:
+            with pytest.raises((ValueError, TypeError, RuntimeError)):
+                traced(x.half())
+        else:
+            assert torch.equal(traced(x.half()), call(x.half(), weight))

@@ -43,6 +43,23 @@ def watched(monkeypatch):
 def test_words_live_until_the_launch(watched):
     w, alive = watched
     x = torch.zeros(4, 128, dtype=torch.bfloat16, requires_grad=True)
-    gated.GatedLinearFn.apply(x, None, w, None).sum().backward()
-    q4.Q4LinearFn.apply(x, w).sum().backward()
+    gated.GatedLinearFn.apply(x, None, w, None, True).sum().backward()
+    q4.Q4LinearFn.apply(x, w, True).sum().backward()
     assert alive == [(f"usaf_hip_{name}", True) for name in ("gated_fwd", "gated_bwd", "q4_linear", "q4_linear_bwd")]
+
+
+@pytest.mark.parametrize("call", [q4.q4_linear, gated.gated_linear])
+def test_refusals_of_activations_that_want_a_gradient(call):
+    """The same as without one."""
+    w = Q4Tensor(*O.codes(64, 256), torch.Size((64, 256)))
+    x = torch.zeros(3, 256, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="GPU"):
+        call(x, w)
+    with pytest.raises(ValueError, match="fit"):
+        call(x[:, :128], w)
+    with pytest.raises(ValueError, match="fit"):
+        call(x[0, 0], w)
+    with pytest.raises(TypeError, match="fp16 or bf16"):
+        call(x.float(), w)
+    with pytest.raises(NotImplementedError, match="dequantize"):
+        call(x, Q4Tensor(w.q, w.s, w.z, w.shape, 64))

@@ -23,7 +23,7 @@ import torch
 from . import _native as N
 from .fp8 import on
 from .moe import Q4Tensor
-from .q4 import ACT, Reading, _ld, check_weight, rows_of, words
+from .q4 import Reading, _ld, check_weight, refuse_misfit, rows_of, words
 
 CHECKPOINTS = (None, "fp8")
 
@@ -66,14 +66,20 @@ def _forward(x: torch.Tensor, w, checkpoint: Optional[str], keep: bool, read: Op
 
 
 class GatedLinearFn(torch.autograd.Function):
-    """act = silu(x Wg^T) (x Wu^T) of rows x [M, K]; w is the weight, trained where it is a tensor that wants a gradient."""
+    """act = silu(x Wg^T) (x Wu^T) of rows x [M, K]; w is the weight, trained where it is a tensor that wants a gradient.
+    checked: the caller has looked at them (a trace calls this by itself)."""
 
     @staticmethod
-    def forward(ctx, x: torch.Tensor, weight: Optional[torch.Tensor], q4: Optional[Q4Tensor], checkpoint: Optional[str]):
+    def forward(ctx, x: torch.Tensor, weight: Optional[torch.Tensor], q4: Optional[Q4Tensor], checkpoint: Optional[str],
+                checked: bool):
         keep = any(ctx.needs_input_grad[:2])
+        if not checked:
+            if q4 is not None:
+                check_weight("gated_linear", q4)
+            refuse_misfit("gated_linear", x, weight if q4 is None else q4)
+        read = None if q4 is None else Reading.of("gated_linear", q4, x)
         rows = rows_of(x, x.shape[1])
         w = q4 if weight is None else _dense(weight)
-        read = None if q4 is None else Reading.of("gated_linear", q4, x)
         act, kept, scales = _forward(rows, w, checkpoint, keep, read)
         ctx.dtype, ctx.shape = x.dtype, tuple(w.shape)
         if keep:
@@ -95,7 +101,7 @@ class GatedLinearFn(torch.autograd.Function):
         dx = torch.empty(m, k, dtype=ctx.dtype, device=dev) if want_x else None
         dw = torch.empty(rows, k, dtype=ctx.dtype, device=dev) if want_w else None
         if m == 0:
-            return dx, None if dw is None else dw.zero_(), None, None
+            return dx, None if dw is None else dw.zero_(), None, None, None
         dact = dact.to(ctx.dtype).contiguous()
         # (a saved-tensor hook may have changed what was kept: its layout, its place)
         kept, scales = _dense(kept), None if scales is None else scales.contiguous()
@@ -111,7 +117,7 @@ class GatedLinearFn(torch.autograd.Function):
             N.call("usaf_hip_gated_bwd", dact.data_ptr(), N.dtype_code(ctx.dtype), m, rows // 2, k, kept.data_ptr(),
                    N.ptr(scales), *map(N.ptr, parts), x.data_ptr() if want_w else None, _ld(x) if want_w else k, N.ptr(dx),
                    N.ptr(dw), ws.data_ptr(), ws.numel(), N.stream_ptr(dev))
-        return dx, dw, None, None
+        return dx, dw, None, None, None
 
 
 def gated_linear(x: torch.Tensor, gate_up: Union[Q4Tensor, torch.Tensor], checkpoint: Optional[str] = None) -> torch.Tensor:
@@ -125,29 +131,23 @@ def gated_linear(x: torch.Tensor, gate_up: Union[Q4Tensor, torch.Tensor], checkp
     capture takes calls without a gradient only, of 4-bit weights once they have been used."""
     if checkpoint not in CHECKPOINTS:
         raise ValueError(f"gated_linear: checkpoint must be one of {CHECKPOINTS}, got {checkpoint!r}")
-    if x.dtype not in ACT:
-        raise TypeError(f"gated_linear: activations must be fp16 or bf16, got {x.dtype}")
     four_bit = isinstance(gate_up, Q4Tensor)
     if four_bit:
         check_weight("gated_linear", gate_up)
     elif not isinstance(gate_up, torch.Tensor):
         raise TypeError(f"gated_linear: gate_up must be a Q4Tensor or a tensor, got {type(gate_up).__name__}")
-    elif gate_up.dtype != x.dtype:
-        raise TypeError(f"gated_linear: a 16-bit weight must be of the activations' dtype, got {gate_up.dtype} and {x.dtype}")
     shape = tuple(int(d) for d in gate_up.shape)
     if len(shape) != 2 or shape[0] < 2 or shape[0] % 2 or shape[1] < 1:
         raise ValueError(f"gated_linear: need a weight [2 I, K], got {shape}")
-    if x.dim() < 1 or x.shape[-1] != shape[1]:
-        raise ValueError(f"gated_linear: activations {tuple(x.shape)} do not fit the weight {shape}")
-    if x.device != gate_up.device or not x.is_cuda:
-        raise ValueError(f"gated_linear: activations on {x.device}, weight on {gate_up.device}: both on one GPU")
+    refuse_misfit("gated_linear", x, gate_up)
     rows = x if x.dim() == 2 else x.reshape(x.numel() // shape[1], shape[1])
     grad = torch.is_grad_enabled() and (x.requires_grad or (not four_bit and gate_up.requires_grad))
     if grad:
         N.refuse_capture("gated_linear of tensors that want a gradient")
-    if grad or N.followed(x, *(() if four_bit else (gate_up,))):
+    followed = N.followed(x, *(() if four_bit else (gate_up,)))
+    if grad or followed:
         weight, q4 = (None, gate_up) if four_bit else (gate_up, None)
-        act = GatedLinearFn.apply(rows, weight, q4, checkpoint)
+        act = GatedLinearFn.apply(rows, weight, q4, checkpoint, not followed)
     else:
         act = _forward(rows_of(rows, shape[1]), gate_up if four_bit else _dense(gate_up), checkpoint, False)[0]
     return act if x.dim() == 2 else act.view(*x.shape[:-1], shape[0] // 2)

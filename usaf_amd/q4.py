@@ -82,6 +82,18 @@ def words(what: str, w: Q4Tensor) -> torch.Tensor:
     return szg
 
 
+def refuse_misfit(what: str, x: torch.Tensor, w) -> None:
+    """Raise unless x's rows can be multiplied by a weight [.., K], 4-bit or of x's own type, on its device."""
+    if x.dtype not in ACT:
+        raise TypeError(f"{what}: activations must be fp16 or bf16, got {x.dtype}")
+    if isinstance(w, torch.Tensor) and w.dtype != x.dtype:
+        raise TypeError(f"{what}: a 16-bit weight must be of the activations' dtype, got {w.dtype} and {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"{what}: activations {tuple(x.shape)} do not fit the weight {tuple(w.shape)}")
+    if x.device != w.device or not x.is_cuda:
+        raise ValueError(f"{what}: activations on {x.device}, weight on {w.device}: both on one GPU")
+
+
 class Reading(NamedTuple):
     """A weight's tensors as a forward reads them, which are what its backward reads, whatever the weight holds by then."""
     q: torch.Tensor
@@ -92,7 +104,6 @@ class Reading(NamedTuple):
 
     @classmethod
     def of(cls, what: str, w: Q4Tensor, x: torch.Tensor) -> "Reading":
-        check_weight(what, w)  # (a trace calls the autograd functions by themselves)
         return cls(w.q, w.s, w.z, words(what, w) if x.numel() else None, _versions(w.q, w.s, w.z))
 
     def refuse_written(self, what: str) -> None:
@@ -114,10 +125,13 @@ def _ld(t: torch.Tensor) -> int:
 
 
 class Q4LinearFn(torch.autograd.Function):
-    """y = x W^T; dx = dy W."""
+    """y = x W^T; dx = dy W.  checked: the caller has looked at x and w (a trace calls this by itself)."""
 
     @staticmethod
-    def forward(ctx, x: torch.Tensor, w: Q4Tensor):
+    def forward(ctx, x: torch.Tensor, w: Q4Tensor, checked: bool):
+        if not checked:
+            check_weight("q4_linear", w)
+            refuse_misfit("q4_linear", x, w)
         read = Reading.of("q4_linear", w, x)
         if ctx.needs_input_grad[0]:
             ctx.read, ctx.shape, ctx.dtype = read, w.shape, x.dtype
@@ -130,7 +144,7 @@ class Q4LinearFn(torch.autograd.Function):
         N.refuse_capture("q4_linear's backward")
         ctx.read.refuse_written("q4_linear's backward")
         dy = dy if dy.dtype == ctx.dtype else dy.to(ctx.dtype)
-        return _linear(dy, ctx.shape, ctx.read.q, ctx.read.sz, backward=True), None
+        return _linear(dy, ctx.shape, ctx.read.q, ctx.read.sz, backward=True), None, None
 
 
 def _linear(x: torch.Tensor, shape, q: torch.Tensor, sz: Optional[torch.Tensor], backward: bool = False) -> torch.Tensor:
@@ -162,16 +176,11 @@ def q4_linear(x: torch.Tensor, w: Q4Tensor) -> torch.Tensor:
     forward's tensors, also where the weight has been given others since, and raises where
     torch has counted a write to them."""
     check_weight("q4_linear", w)
-    if x.dtype not in ACT:
-        raise TypeError(f"q4_linear: activations must be fp16 or bf16, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] != w.shape[1]:
-        raise ValueError(f"q4_linear: activations {tuple(x.shape)} do not fit the weight {tuple(w.shape)}")
-    if x.device != w.device or not x.is_cuda:
-        raise ValueError(f"q4_linear: activations on {x.device}, weight on {w.device}: both on one GPU")
-    if torch.is_grad_enabled() and x.requires_grad:
+    refuse_misfit("q4_linear", x, w)
+    grad, followed = torch.is_grad_enabled() and x.requires_grad, N.followed(x)
+    if grad:
         N.refuse_capture("q4_linear of activations that want a gradient")
-        return Q4LinearFn.apply(x, w)
-    if N.followed(x):
-        return Q4LinearFn.apply(x, w)
+    if grad or followed:
+        return Q4LinearFn.apply(x, w, not followed)
     # (the function's own call takes 2 us of the host's time)
     return _linear(x, w.shape, w.q, words("q4_linear", w) if x.numel() else None)
