@@ -157,3 +157,23 @@ def test_a_trace_refuses_what_a_call_refuses():
                 traced(x.half())
         else:
             assert torch.equal(traced(x.half()), call(x.half(), weight))
+
+
+@pytest.mark.parametrize("part", ["q", "s", "z"])
+def test_a_weight_whose_tensors_are_given_other_memory(part):
+    """``t.data = other``: t is the same object, and torch counts no write."""
+    w, (q, s, z) = U._weight(N_, K)
+    x, leaf = U._x(40, K), _leaf(40)
+    U._check(q4_linear(x, w), x, (q, s, z), N_, K, "as made")
+    y = q4_linear(leaf, w)
+    parts = {"q": q, "s": s, "z": z}
+    parts[part] = parts[part].flip(0)
+    getattr(w, part).data = parts[part].cuda()
+    U._check(q4_linear(x, w), x, tuple(parts.values()), N_, K, "other memory")
+    _check_gated(gated_linear(x, w), x, tuple(parts.values()), "gated, other memory")
+    with pytest.raises(RuntimeError, match="written to"):
+        y.float().sum().backward()
+    getattr(w, part).data = parts[part][:-1].cuda()
+    for call in CALLS.values():
+        with pytest.raises(ValueError, match="fit"):
+            call(x, w)

@@ -144,10 +144,9 @@ def gated_linear(x: torch.Tensor, gate_up: Union[Q4Tensor, torch.Tensor], checkp
     grad = torch.is_grad_enabled() and (x.requires_grad or (not four_bit and gate_up.requires_grad))
     if grad:
         N.refuse_capture("gated_linear of tensors that want a gradient")
-    followed = N.followed(x, *(() if four_bit else (gate_up,)))
-    if grad or followed:
+    if grad or N.followed(x, *(() if four_bit else (gate_up,))):
         weight, q4 = (None, gate_up) if four_bit else (gate_up, None)
-        act = GatedLinearFn.apply(rows, weight, q4, checkpoint, not followed)
+        act = GatedLinearFn.apply(rows, weight, q4, checkpoint, grad and not torch.jit.is_tracing())
     else:
         act = _forward(rows_of(rows, shape[1]), gate_up if four_bit else _dense(gate_up), checkpoint, False)[0]
     return act if x.dim() == 2 else act.view(*x.shape[:-1], shape[0] // 2)

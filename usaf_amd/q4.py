@@ -12,7 +12,7 @@ the activations are), so decoding, prompts and gradients multiply the same numbe
 from __future__ import annotations
 
 import functools
-from typing import NamedTuple, Optional, Tuple
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -31,16 +31,15 @@ def _ws_bytes(device: int, m: int, n: int, k: int, backward: int) -> int:
 
 
 def _versions(*tensors: torch.Tensor):
-    """Counts of the writes to tensors (those made in inference mode have none)."""
-    return tuple(None if t.is_inference() else t._version for t in tensors)
+    """Where tensors lie (``t.data = other`` leaves t itself) and counts of the writes to them (None where made in inference
+    mode, which counts none)."""
+    return [(t.data_ptr(), None if t.is_inference() else t._version) for t in tensors]
 
 
 def check_weight(what: str, w: Q4Tensor) -> None:
     """Raise unless w is a 4-bit matrix in the layout that the products read (looked at once for each set of tensors: 5 us)."""
-    parts = (w.q, w.s, w.z, w.shape, w.group_size, *_versions(w.s, w.z))
-    seen = w.__dict__.get("_seen")
-    if seen is not None and all(a is b or a == b for a, b in zip(seen[3:], parts[3:])) \
-            and all(a is b for a, b in zip(seen[:3], parts[:3])):
+    seen, now = w.__dict__.get("_seen"), (w.shape, w.group_size, w.q.data_ptr(), _versions(w.s, w.z))
+    if seen is not None and seen[0] is w.q and seen[1] is w.s and seen[2] is w.z and seen[3] == now:
         return
     if len(w.shape) != 2 or any(int(d) < 1 for d in w.shape):
         raise ValueError(f"{what}: need a 4-bit weight [rows, K], got {tuple(w.shape)}")
@@ -58,7 +57,7 @@ def check_weight(what: str, w: Q4Tensor) -> None:
             or w.s.device != w.q.device or w.z.device != w.q.device:
         raise ValueError(f"{what}: codes, scales and zeros must be contiguous, on one device, the codes 16-byte aligned")
     w._szg = None  # (a copy of a tensor with other parts may have brought its words along)
-    w.__dict__["_seen"] = parts
+    w.__dict__["_seen"] = (w.q, w.s, w.z, now)
 
 
 def words(what: str, w: Q4Tensor) -> torch.Tensor:
@@ -86,7 +85,7 @@ def refuse_misfit(what: str, x: torch.Tensor, w) -> None:
     """Raise unless x's rows can be multiplied by a weight [.., K], 4-bit or of x's own type, on its device."""
     if x.dtype not in ACT:
         raise TypeError(f"{what}: activations must be fp16 or bf16, got {x.dtype}")
-    if isinstance(w, torch.Tensor) and w.dtype != x.dtype:
+    if not isinstance(w, Q4Tensor) and w.dtype != x.dtype:
         raise TypeError(f"{what}: a 16-bit weight must be of the activations' dtype, got {w.dtype} and {x.dtype}")
     if x.dim() < 1 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"{what}: activations {tuple(x.shape)} do not fit the weight {tuple(w.shape)}")
@@ -100,7 +99,7 @@ class Reading(NamedTuple):
     s: torch.Tensor
     z: torch.Tensor
     sz: Optional[torch.Tensor]  # words() of s and z, None for a call of no rows
-    versions: Tuple
+    versions: list
 
     @classmethod
     def of(cls, what: str, w: Q4Tensor, x: torch.Tensor) -> "Reading":
@@ -177,10 +176,10 @@ def q4_linear(x: torch.Tensor, w: Q4Tensor) -> torch.Tensor:
     torch has counted a write to them."""
     check_weight("q4_linear", w)
     refuse_misfit("q4_linear", x, w)
-    grad, followed = torch.is_grad_enabled() and x.requires_grad, N.followed(x)
-    if grad:
+    if torch.is_grad_enabled() and x.requires_grad:
         N.refuse_capture("q4_linear of activations that want a gradient")
-    if grad or followed:
-        return Q4LinearFn.apply(x, w, not followed)
+        return Q4LinearFn.apply(x, w, not torch.jit.is_tracing())
+    if N.followed(x):
+        return Q4LinearFn.apply(x, w, False)
     # (the function's own call takes 2 us of the host's time)
     return _linear(x, w.shape, w.q, words("q4_linear", w) if x.numel() else None)
