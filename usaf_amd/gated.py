@@ -128,7 +128,8 @@ def gated_linear(x: torch.Tensor, gate_up: Union[Q4Tensor, torch.Tensor], checkp
     dtype, which receives a gradient where it wants one.  checkpoint: None keeps gate and up
     in x's dtype for the backward, "fp8" in 8-bit blocks; without a gradient nothing is kept.
     No second or forward-mode derivatives; torch.jit.trace records the call.  A stream
-    capture takes calls without a gradient only, of 4-bit weights once they have been used."""
+    capture takes calls without a gradient only, of 4-bit weights once they have been used.
+    What is said of a weight's writes and lifetime at ``q4_linear`` holds here."""
     if checkpoint not in CHECKPOINTS:
         raise ValueError(f"gated_linear: checkpoint must be one of {CHECKPOINTS}, got {checkpoint!r}")
     four_bit = isinstance(gate_up, Q4Tensor)
